@@ -544,6 +544,64 @@ int mxl_linear_backward(const mxl_linear* p, int parts, const void* dy_bf16, con
                         void* scratch, void* dx_bf16, void* daux, void* dw, uint32_t dw_flags, uint64_t sr_seed,
                         void* stream);
 
+/* ---- around the expert MLP: routing, rows into the experts' order and back ----
+ * The expert MLP takes rows sorted by expert and their probabilities (primus/backends/megatron/core/transformer/experts.py:179-268).
+ * Element types of logits, rows and probabilities: */
+#define MXL_DT_F32 0
+#define MXL_DT_BF16 1
+#define MXL_DT_F16 2
+#define MXL_SCORE_SOFTMAX 0
+#define MXL_SCORE_SIGMOID 1
+
+/* Choice of `topk` experts for every token from logits [tokens, experts] (any MXL_DT_*).
+ *   scores       : softmax over the experts or sigmoid, fp32
+ *   expert_bias  : float[experts] added to the scores for the choice only (NULL: none)
+ *   num_groups   : consecutive groups of experts / num_groups experts (1: no groups, at most 64); the score of a group is the sum of
+ *                  its topk / group_topk largest biased scores, the group_topk best groups take part in the choice
+ *   probs        : float[tokens, topk] = scale * score of the chosen experts, divided by their sum first if renormalize
+ *                  (sigmoid: sum + 1e-20)
+ *   indices      : int64[tokens, topk], best first; ties go to the lower index.  The order is the one of exact scores: fp32
+ *                  scores too near to each other to tell are compared in fp64.  NaN scores are chosen last.  Softmax over
+ *                  nothing but -inf (all of a row, or all that are chosen when renormalised) is 0.
+ *   counts       : int64[experts], tokens of every expert
+ *   token_mask   : uint8[tokens] (NULL: all ones); a token whose byte is 0 gets indices -1 and probs 0 and is not counted
+ * 1 <= topk <= min(32, experts), experts <= 1024; mxl_topk_routing_workspace_bytes gives the workspace.
+ *
+ * mxl_topk_routing_bwd: gradient of probs with respect to the logits (dlogits [tokens, experts], the logits' type), given the
+ * forward's indices; the choice itself has none. */
+int64_t mxl_topk_routing_workspace_bytes(int64_t tokens, int experts);
+int mxl_topk_routing(const void* logits, int dtype, int64_t tokens, int experts, int topk, int score, const float* expert_bias,
+                     int num_groups, int group_topk, int renormalize, float scale, const uint8_t* token_mask, float* probs,
+                     int64_t* indices, int64_t* counts, void* workspace, int64_t workspace_bytes, void* stream);
+int mxl_topk_routing_bwd(const float* dprobs, const void* logits, int dtype, const int64_t* indices, int64_t tokens, int experts,
+                         int topk, int score, int renormalize, float scale, void* dlogits, void* stream);
+
+/* Where the entries of indices [entries] go in a buffer of rows sorted by expert.
+ *   entry i goes to row  off[e_i] + #{j < i : e_j = e_i};  off = prefix sums of the counts rounded up to `align`.
+ *   row_of       : int64[entries], -1 for an entry whose expert is outside [0, num_experts)
+ *   entry_of     : int32[rows], -1 for a row that no entry goes to
+ *   group_lens   : int64[num_experts], the rounded counts; the last one has the rest of the buffer, so they sum to `rows`
+ *   rows         : >= mxl_padded_rows_bound(entries, num_experts, align)
+ *   probs, row_probs : if row_probs is set, row_probs[row_of[i]] = probs[i] (prob_bytes 2 or 4), 0 in the other rows
+ * entries < 2^30, num_experts <= 1024. */
+int64_t mxl_permute_plan_workspace_bytes(int64_t entries, int num_experts);
+int mxl_permute_plan(const int64_t* indices, int64_t entries, int num_experts, int align, int64_t rows, int64_t* row_of,
+                     int32_t* entry_of, int64_t* group_lens, const void* probs, int prob_bytes, void* row_probs, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+/* out[row_of[t, k]] = x[t] for rows of any bytes, zero rows where entry_of is -1; topk <= 32. */
+int mxl_permute_rows(const void* x, int64_t tokens, int64_t row_bytes, const int64_t* row_of, int topk, const int32_t* entry_of,
+                     int64_t rows, void* out, void* stream);
+/* y[t] = sum_k probs[t, k] * rows[row_of[t, k]] (probs NULL: ones), fp32 in the order of k, rounded once; entries of -1 add
+ * nothing.  If row_probs is set, probs_out[t, k] = row_probs[row_of[t, k]] (0 for -1) on the way: together the gradient of
+ * mxl_permute_rows and of the probabilities' move. */
+int mxl_combine_rows(const void* rows_in, int64_t rows, int hidden, int dtype, const int64_t* row_of, int64_t tokens, int topk,
+                     const void* probs, const void* row_probs, void* probs_out, int probs_dtype, void* y, void* stream);
+/* Its gradient with probs: drows[row_of[t, k]] = probs[t, k] * dy[t], zero rows where entry_of is -1;
+ * dprobs[t, k] = <rows[row_of[t, k]], dy[t]>, float (0 for -1).  Either may be NULL: not wanted. */
+int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int hidden, int dtype, const int64_t* row_of,
+                         const int32_t* entry_of, int64_t tokens, int topk, const void* probs, int probs_dtype, void* drows,
+                         float* dprobs, void* stream);
+
 /* ---- calibration (no counterpart in the reference: a measuring aid of this library's benchmark) ----
  *
  * mxl_calibrate_mfma launches a register-only loop of the GEMM kernels' scaled MFMA (32 x 32 x 64; a_fmt / b_fmt:

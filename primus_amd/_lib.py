@@ -34,6 +34,8 @@ GF_ACCUM_F32 = 2                            # wgrad: the output is float32 and t
 GF_B_SHUFFLED = 16                          # forward / dgrad, row-major E2M1: b's codes are in the pre-shuffled byte order
 GF_TILES = {None: 0, "64": 0x100, "64x128": 0x200, "128": 0x300, "256": 0x400}   # output tile of a launch on K-step-major operands
 GF_B_TRANSPOSED = 8                         # forward / dgrad: b's codes are those of the transposed matrices (row-wise weight copy)
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2           # element types of logits, rows and probabilities around the expert MLP
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 BF_B_KN, BF_ACCUM_F32, BF_TILE_128, BF_TILE_256 = 1, 2, 4, 8    # flags of the bf16 grouped GEMMs
 
 EXPORTS = (
@@ -83,6 +85,14 @@ EXPORTS = (
     "mxl_linear_backward",
     "mxl_shuffle_codes",
     "mxl_shuffle_scales",
+    "mxl_topk_routing_workspace_bytes",
+    "mxl_topk_routing",
+    "mxl_topk_routing_bwd",
+    "mxl_permute_plan_workspace_bytes",
+    "mxl_permute_plan",
+    "mxl_permute_rows",
+    "mxl_combine_rows",
+    "mxl_combine_rows_bwd",
     "mxl_calibrate_mfma",
     "mxl_calibrate_mfma_flops",
     "mxl_calibrate_mfma_bf16",
@@ -236,6 +246,23 @@ def load() -> ctypes.CDLL:
         lib.mxl_blockwise_gemm_tile.argtypes = [i32]
         lib.mxl_blockwise_gemm_plan.restype = i32
         lib.mxl_blockwise_gemm_plan.argtypes = [i64, i64, i32, i32, vp, vp]
+        f32 = ctypes.c_float
+        lib.mxl_topk_routing_workspace_bytes.restype = i64
+        lib.mxl_topk_routing_workspace_bytes.argtypes = [i64, i32]
+        lib.mxl_topk_routing.restype = i32
+        lib.mxl_topk_routing.argtypes = [vp, i32, i64, i32, i32, i32, vp, i32, i32, i32, f32, vp, vp, vp, vp, vp, i64, vp]
+        lib.mxl_topk_routing_bwd.restype = i32
+        lib.mxl_topk_routing_bwd.argtypes = [vp, vp, i32, vp, i64, i32, i32, i32, i32, f32, vp, vp]
+        lib.mxl_permute_plan_workspace_bytes.restype = i64
+        lib.mxl_permute_plan_workspace_bytes.argtypes = [i64, i32]
+        lib.mxl_permute_plan.restype = i32
+        lib.mxl_permute_plan.argtypes = [vp, i64, i32, i32, i64, vp, vp, vp, vp, i32, vp, vp, i64, vp]
+        lib.mxl_permute_rows.restype = i32
+        lib.mxl_permute_rows.argtypes = [vp, i64, i64, vp, i32, vp, i64, vp, vp]
+        lib.mxl_combine_rows.restype = i32
+        lib.mxl_combine_rows.argtypes = [vp, i64, i32, i32, vp, i64, i32, vp, vp, vp, i32, vp, vp]
+        lib.mxl_combine_rows_bwd.restype = i32
+        lib.mxl_combine_rows_bwd.argtypes = [vp, vp, i64, i32, i32, vp, vp, i64, i32, vp, i32, vp, vp, vp]
         _lib = lib
     return _lib
 

@@ -1,0 +1,494 @@
+// Routing of tokens to experts and its gradient: what stands in front of the expert MLP
+// (primus/backends/megatron/core/transformer/experts.py:24-268 takes rows that a router has assigned).
+//
+// Per token, from its logits l[E]:
+//   s = softmax(l) or sigmoid(l),  c = s + expert_bias  (the bias takes part in the choice only)
+//   with groups: an expert group's score is the sum of its topk / group_topk largest c; the group_topk best groups stay
+//   indices = the topk largest c, best first, ties to the lower index
+//   probs   = scale * s[indices], renormalised over the chosen ones if asked
+// and over all tokens the number of tokens of every expert.
+//
+// Bound by the logits' bytes where there are many tokens; what it costs beside them is instructions, so a row is held in
+// registers by LPR lanes of a wave, V logits a lane, sorted inside the lane once, and a round of the choice is one maximum over
+// the row's lanes.  Without bias and groups the order of the scores is that of the logits, which are compared as they are.
+// With them the scores are compared in fp32 first; a row in which two neighbours of the result, or the last chosen and the first
+// left out, are nearer to each other than the rounding of fp32 scores allows to tell apart is chosen again from scores in
+// fp64 (about one row in 500 at 256 fp32 sigmoid scores), so the indices are those of the definition and not of a rounding.
+#include "mx_lanes.h"
+
+namespace mxl {
+
+constexpr int RT_MAX_EXPERTS = MXL_MAX_GROUPS;
+constexpr int RT_MAX_TOPK = 32;
+constexpr int RT_MAX_EXPERT_GROUPS = 64;
+
+struct RouteArgs {
+    const void* logits;
+    const float* bias;          // null: none
+    const uint8_t* mask;        // null: every token is routed
+    float* probs;
+    int64_t* indices;
+    int64_t* counts;            // written by the launch itself where it is one workgroup, else
+    int* partial;               // [workgroups, experts], summed by a second launch
+    int64_t tokens;
+    int experts, topk, dtype, sigmoid, renorm;
+    int groups, group_topk, group_size, lanes_per_group, take;
+    float scale;
+};
+
+// Unsigned key in the order of the float: NaN 1 (below -inf), 0 is left for "no element here"; -0 and 0 are the same.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    const uint32_t k = (b >> 31) ? ~b : b | 0x80000000u;
+    return x != x ? 1u : k;
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k); }
+
+// A softmax over nothing but -inf (every expert of the row disabled, or every chosen one) is 0 everywhere.
+__device__ __forceinline__ float finite_top(float top) { return top == -INFINITY ? 0.f : top; }
+__device__ __forceinline__ float some(float sum) { return sum == 0.f ? 1.f : sum; }
+__device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + expf(-x)); }
+
+// (key, index) pairs of a lane in descending order, equal keys by ascending index: Batcher's odd-even merge sort
+template <int V> __device__ __forceinline__ void sort_pairs(uint32_t (&key)[V], uint32_t (&idx)[V]) {
+    auto order = [&](int a, int b) __attribute__((always_inline)) {      // a < b: the better one to a
+        const bool swap = key[b] > key[a] || (key[b] == key[a] && idx[b] < idx[a]);
+        const uint32_t ka = key[a], ia = idx[a];
+        key[a] = swap ? key[b] : ka;
+        idx[a] = swap ? idx[b] : ia;
+        key[b] = swap ? ka : key[b];
+        idx[b] = swap ? ia : idx[b];
+    };
+#pragma unroll
+    for (int p = 1; p < V; p <<= 1)
+#pragma unroll
+        for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+            for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(i + j, i + j + k);
+}
+template <int V> __device__ __forceinline__ void pop_head(uint32_t (&key)[V], uint32_t (&idx)[V], bool take) {
+#pragma unroll
+    for (int v = 0; v + 1 < V; ++v) {
+        key[v] = take ? key[v + 1] : key[v];
+        idx[v] = take ? idx[v + 1] : idx[v];
+    }
+    key[V - 1] = take ? 0u : key[V - 1];
+}
+
+// The choice of one row again, by a whole wave, from scores in fp64 kept in the wave's LDS; lane k < topk returns the k-th index.
+// (Rare: written for few registers.)
+template <int V>
+__device__ __forceinline__ int choose_fp64(const RouteArgs& p, int64_t row, double* c) {
+    const int lane = threadIdx.x & 63;
+    const int sub = lane & (p.lanes_per_group - 1), grp = lane / p.lanes_per_group;
+    const int64_t base = row * p.experts;
+    auto element = [&](int v) {
+        const int j = sub * V + v;
+        return grp < p.groups && j < p.group_size ? grp * p.group_size + j : -1;
+    };
+    auto wave_max = [](double x) {
+        for (int d = 1; d < 64; d <<= 1) x = fmax(x, __shfl_xor(x, d));
+        return x;
+    };
+    double top = -INFINITY, sum = 0.0;
+    if (!p.sigmoid) {
+        _Pragma("unroll 1") for (int v = 0; v < V; ++v) {
+            const int e = element(v);
+            if (e >= 0) top = fmax(top, (double)load_dt(p.logits, p.dtype, base + e));
+        }
+        top = wave_max(top);
+        top = top == -INFINITY ? 0.0 : top;
+        _Pragma("unroll 1") for (int v = 0; v < V; ++v) {
+            const int e = element(v);
+            if (e >= 0) sum += exp((double)load_dt(p.logits, p.dtype, base + e) - top);
+        }
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        sum = sum == 0.0 ? 1.0 : sum;
+    }
+    _Pragma("unroll 1") for (int v = 0; v < V; ++v) {
+        const int e = element(v);
+        double x = -INFINITY;
+        if (e >= 0) {
+            x = (double)load_dt(p.logits, p.dtype, base + e);
+            x = p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum;
+            if (p.bias) x += (double)p.bias[e];
+            if (x != x) x = -INFINITY;
+        }
+        c[v * 64 + lane] = x;
+    }
+    uint32_t left = 0;                          // this lane's elements that are still to be had
+    _Pragma("unroll 1") for (int v = 0; v < V; ++v)
+        if (element(v) >= 0) left |= 1u << v;
+    // the best element left among `lanes` lanes: its value and (lane, v) as one number, smaller = lower index; 0xFFFF: none
+    auto best_of = [&](int lanes, uint32_t have, double& value) {
+        double b = -INFINITY;
+        uint32_t at = 0xFFFFu;
+        _Pragma("unroll 1") for (int v = 0; v < V; ++v)
+            if ((have >> v) & 1) {
+                const double x = c[v * 64 + lane];
+                if (at == 0xFFFFu || x > b) b = x, at = (uint32_t)(lane * V + v);
+            }
+        for (int d = 1; d < lanes; d <<= 1) {
+            const double ob = __shfl_xor(b, d);
+            const uint32_t oat = (uint32_t)__shfl_xor((int)at, d);
+            if (oat != 0xFFFFu && (at == 0xFFFFu || ob > b || (ob == b && oat < at))) b = ob, at = oat;
+        }
+        value = b;
+        return at;
+    };
+    if (p.groups > 1) {
+        uint32_t have = left;
+        double score = 0.0, value;
+        for (int i = 0; i < p.take; ++i) {
+            const uint32_t at = best_of(p.lanes_per_group, have, value);
+            if (at != 0xFFFFu) {
+                score += value;
+                if ((int)(at / V) == lane) have &= ~(1u << (at % V));
+            }
+        }
+        int ahead = 0;
+        for (int g = 0; g < p.groups; ++g) {
+            const double other = __shfl(score, g * p.lanes_per_group);
+            ahead += other > score || (other == score && g < grp);
+        }
+        if (ahead >= p.group_topk) left = 0;
+    }
+    int mine = 0;
+    for (int k = 0; k < p.topk; ++k) {
+        double value;
+        const uint32_t at = best_of(64, left, value);
+        const int wl = (int)(at / V), wv = (int)(at % V);
+        if (wl == lane) left &= ~(1u << wv);
+        if (lane == k && at != 0xFFFFu) mine = (wl / p.lanes_per_group) * p.group_size + (wl & (p.lanes_per_group - 1)) * V + wv;
+    }
+    return mine;
+}
+
+// SCORED: bias or groups, so scores are computed and compared (a row per wave); otherwise the logits are.
+template <int LPR, int V, bool SCORED> constexpr int route_waves() { return !SCORED || V <= 4 ? 16 : 64 / V; }
+
+template <int LPR, int V, bool SCORED>
+__global__ __launch_bounds__((route_waves<LPR, V, SCORED>() * 64)) void route_fwd_kernel(RouteArgs p) {
+    static_assert(!SCORED || LPR == 64, "a scored row is a wave's");
+    constexpr int WAVES = route_waves<LPR, V, SCORED>(), RPW = 64 / LPR;
+    __shared__ int hist[RT_MAX_EXPERTS];
+    __shared__ double spare[SCORED ? WAVES * V * 64 : 1];
+    const int t = threadIdx.x, w = t >> 6, lane = t & 63, lr = lane & (LPR - 1);
+    for (int e = t; e < p.experts; e += WAVES * 64) hist[e] = 0;
+    __syncthreads();
+    // element (lane, v) of a row: expert `first + v`, if v < have.  Lower experts sit in lower lanes.
+    int first, have;
+    if (SCORED) {
+        const int sub = lr & (p.lanes_per_group - 1), g = lr / p.lanes_per_group;
+        first = g * p.group_size + sub * V;
+        have = g < p.groups ? p.group_size - sub * V : 0;
+    } else {
+        first = lr * V;
+        have = p.experts - first;
+    }
+    have = have < 0 ? 0 : have > V ? V : have;
+
+    const int64_t step = (int64_t)gridDim.x * WAVES * RPW;
+    for (int64_t row0 = ((int64_t)blockIdx.x * WAVES + w) * RPW; row0 < p.tokens; row0 += step) {
+        const int64_t row = row0 + lane / LPR;
+        const bool in = row < p.tokens;
+        const int64_t base = (in ? row : p.tokens - 1) * p.experts;
+        float l[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) l[v] = v < have ? load_dt(p.logits, p.dtype, base + first + v) : -INFINITY;
+
+        float top = 0.f, total = 1.f;           // of the row: largest logit, sum of exp(l - top)
+        if (!p.sigmoid && (SCORED || !p.renorm)) {
+            top = -INFINITY;
+#pragma unroll
+            for (int v = 0; v < V; ++v) top = fmaxf(top, l[v]);
+            top = finite_top(lanes_max<LPR>(top));
+            float s = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) s += v < have ? expf(l[v] - top) : 0.f;
+            total = some(lanes_sum<LPR>(s));
+        }
+        uint32_t key[V], idx[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float c = l[v];
+            if (SCORED && v < have) {
+                c = p.sigmoid ? sigmoid_of(l[v]) : expf(l[v] - top) / total;
+                if (p.bias) c += p.bias[first + v];
+            }
+            key[v] = v < have ? order_key(c) : 0u;
+            idx[v] = (uint32_t)(first + v);
+        }
+        sort_pairs<V>(key, idx);
+        bool doubt = false;
+        // What two fp32 scores may be off together: sigmoid, expf, a sum and a quotient, 2^-22 of at most 1 each.  Softmax: a score
+        // s = exp(-x) / total is off by s (x + 40) 2^-24 (the rounding of x, expf, V + 6 additions, the quotient), and neither s nor
+        // s x passes 1 / total.  Without a bias nothing left out has a larger score than what it is compared with: relative there.
+        const float pair_off = p.sigmoid ? 0x1p-21f : 0x1p-17f / total;
+        if (SCORED && p.groups > 1) {
+            uint32_t gk[V], gi[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) gk[v] = key[v], gi[v] = idx[v];
+            float score = 0.f;
+            for (int i = 0; i < p.take; ++i) {
+                const uint32_t best = lanes_reduce<OpMaxU>(gk[0], p.lanes_per_group);
+                const uint32_t who = lanes_reduce<OpMinU>(gk[0] == best ? (uint32_t)lane : 64u, p.lanes_per_group);
+                score += best ? key_value(best) : 0.f;
+                pop_head<V>(gk, gi, who == (uint32_t)lane && best != 0u);
+            }
+            const int grp = lane / p.lanes_per_group;
+            int ahead = 0;
+            for (int g = 0; g < p.groups; ++g) {
+                const float other = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(score), g * p.lanes_per_group));
+                ahead += other > score || (other == score && g < grp);
+            }
+            const bool keep = ahead < p.group_topk, real = grp < p.groups;
+            // the worst group kept and the best one left out, against what fp32 scores and their sums may be off
+            const float in_worst = lanes_min<64>(real && keep ? score : INFINITY), out_best = lanes_max<64>(real && !keep ? score : -INFINITY);
+            if (p.group_topk < p.groups) {
+                const float mag = fabsf(in_worst) + fabsf(out_best);
+                const float off = p.bias || p.sigmoid ? pair_off * (float)p.take : 0x1p-16f * mag;
+                doubt = !(in_worst - out_best > off + 0x1p-22f * (float)p.take * mag);
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) key[v] = keep ? key[v] : 0u;
+        }
+        // the choice, one expert a round; lane k of the row keeps the k-th (a scored row looks one further, to compare with it)
+        int mine = 0;
+        uint32_t mine_key = 0u;
+        const int rounds = p.topk + (SCORED ? 1 : 0);
+        for (int k = 0; k < rounds; ++k) {
+            const uint32_t best = lanes_reduce<OpMaxU, LPR>(key[0]);
+            // equal keys: the lower index is in the lower lane
+            uint32_t who;
+            if constexpr (LPR == 64) who = (uint32_t)__builtin_ctzll(__ballot(key[0] == best));
+            else who = lanes_reduce<OpMinU, LPR>(key[0] == best ? (uint32_t)lane : 64u);
+            uint32_t won;
+            if constexpr (LPR == 64) won = (uint32_t)__builtin_amdgcn_readlane((int)idx[0], (int)who);
+            else won = (uint32_t)__shfl((int)idx[0], (int)who);
+            if (lr == k) mine = (int)won, mine_key = best;
+            pop_head<V>(key, idx, who == (uint32_t)lane);
+        }
+        // lane k < topk: its expert's score
+        const bool chosen = lr < p.topk;
+        float ml = chosen || (SCORED && mine_key) ? load_dt(p.logits, p.dtype, base + mine) : -INFINITY;
+        if (SCORED) {
+            const float s = p.sigmoid ? sigmoid_of(ml) : expf(ml - top) / total;
+            const float c = key_value(mine_key), b = p.bias && (chosen || mine_key) ? p.bias[mine] : 0.f;
+            const float nl = __shfl_down(ml, 1), ns = __shfl_down(s, 1), nc = __shfl_down(c, 1), nb = __shfl_down(b, 1);
+            const uint32_t nk = (uint32_t)__shfl_down((int)mine_key, 1);
+            const float off = (p.bias || p.sigmoid ? pair_off : 0x1p-16f * (s + ns)) + 0x1p-23f * (fabsf(c) + fabsf(nc));
+            // nothing follows, or the same logit and bias (a true tie), or far enough apart: told rightly
+            const bool told = !chosen || nk == 0u || (ml == nl && b == nb) || c - nc > off;
+            doubt = __any(doubt || !told);
+            if (doubt) {
+                const int again = choose_fp64<V>(p, in ? row : p.tokens - 1, spare + w * V * 64);
+                mine = chosen ? again : 0;
+                ml = chosen ? load_dt(p.logits, p.dtype, base + mine) : -INFINITY;
+            }
+        }
+        float prob;
+        if (p.sigmoid) {
+            const float s = chosen ? sigmoid_of(ml) : 0.f;
+            prob = p.renorm ? s / (lanes_sum<LPR>(s) + 1e-20f) : s;
+        } else if (p.renorm) {
+            const float m = finite_top(lanes_max<LPR>(chosen ? ml : -INFINITY));
+            const float s = chosen ? expf(ml - m) : 0.f;
+            prob = s / some(lanes_sum<LPR>(s));
+        } else {
+            prob = expf(ml - top) / total;
+        }
+        if (in && chosen) {
+            const bool live = !p.mask || p.mask[row];
+            p.probs[row * p.topk + lr] = live ? prob * p.scale : 0.f;
+            p.indices[row * p.topk + lr] = live ? mine : -1;
+            if (live) atomicAdd(&hist[mine], 1);
+        }
+    }
+    __syncthreads();
+    if (gridDim.x == 1) {
+        for (int e = t; e < p.experts; e += WAVES * 64) p.counts[e] = hist[e];
+    } else {
+        for (int e = t; e < p.experts; e += WAVES * 64) p.partial[(int64_t)blockIdx.x * p.experts + e] = hist[e];
+    }
+}
+
+// counts[e] = sum over the workgroups: 64 experts by 16 runs of workgroups
+__global__ __launch_bounds__(1024) void route_counts_kernel(const int* partial, int blocks, int experts, int64_t* counts) {
+    __shared__ int part[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+    int n = 0;
+    if (e < experts)
+        for (int b = w; b < blocks; b += 16) n += partial[(int64_t)b * experts + e];
+    part[w][lane] = n;
+    __syncthreads();
+    if (w == 0 && e < experts) {
+        int64_t total = 0;
+        for (int i = 0; i < 16; ++i) total += part[i][lane];
+        counts[e] = total;
+    }
+}
+
+struct RouteBwdArgs {
+    const float* dprobs;
+    const void* logits;
+    const int64_t* indices;
+    void* dlogits;
+    int64_t tokens;
+    int experts, topk, dtype, sigmoid, renorm;
+    float scale;
+};
+
+// g = scale * dprobs, w = the chosen scores' shares.  Renormalised: dl = w (g - sum w g) at the chosen experts (softmax),
+// (g - sum w g) / (S + 1e-20) * s (1 - s) (sigmoid); as they are: softmax s_e ([e chosen] g_e - sum s g) at every expert,
+// sigmoid g s (1 - s).  A wave a row; the chosen experts' gradients meet the row through LDS, which is zero between rows.
+constexpr int RB_WAVES = 8;
+__global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_kernel(RouteBwdArgs p) {
+    __shared__ float rows[RB_WAVES][RT_MAX_EXPERTS];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float* d = rows[w];
+    for (int e = lane; e < p.experts; e += 64) d[e] = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * RB_WAVES + w; row < p.tokens; row += (int64_t)gridDim.x * RB_WAVES) {
+        const int64_t base = row * p.experts;
+        int64_t at = lane < p.topk ? p.indices[row * p.topk + lane] : -1;
+        const bool chosen = at >= 0 && at < p.experts;
+        const float ml = chosen ? load_dt(p.logits, p.dtype, base + at) : -INFINITY;
+        const float g = chosen ? p.dprobs[row * p.topk + lane] * p.scale : 0.f;
+        float mine, all = 0.f, top = 0.f, total = 1.f;
+        const bool dense = !p.sigmoid && !p.renorm;
+        if (p.sigmoid) {
+            const float s = chosen ? sigmoid_of(ml) : 0.f;
+            float ds = g;
+            if (p.renorm) {
+                const float sum = lanes_sum<64>(s) + 1e-20f;
+                ds = (g - lanes_sum<64>(g * (s / sum))) / sum;
+            }
+            mine = ds * s * (chosen ? sigmoid_of(-ml) : 0.f);      // 1 - s without cancellation
+        } else if (p.renorm) {
+            const float m = finite_top(lanes_max<64>(ml));
+            const float e = chosen ? expf(ml - m) : 0.f;
+            const float wgt = e / some(lanes_sum<64>(e));
+            mine = wgt * (g - lanes_sum<64>(wgt * g));
+        } else {
+            top = -INFINITY;
+            for (int e = lane; e < p.experts; e += 64) top = fmaxf(top, load_dt(p.logits, p.dtype, base + e));
+            top = finite_top(lanes_max<64>(top));
+            float sum = 0.f;
+            for (int e = lane; e < p.experts; e += 64) sum += expf(load_dt(p.logits, p.dtype, base + e) - top);
+            total = some(lanes_sum<64>(sum));
+            const float s = chosen ? expf(ml - top) / total : 0.f;
+            all = lanes_sum<64>(s * g);
+            mine = s * g;
+        }
+        const bool live = __any(chosen);
+        if (chosen) atomicAdd(&d[at], mine);      // the same expert twice in a row: its gradients add up
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        for (int e = lane; e < p.experts; e += 64) {
+            float x = d[e];
+            if (dense && live) x -= expf(load_dt(p.logits, p.dtype, base + e) - top) / total * all;
+            store_dt(p.dlogits, p.dtype, base + e, x);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (chosen) d[at] = 0.f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// workgroups of a forward launch: rows for every wave slot of the chip at most
+static int64_t route_blocks(int64_t tokens, int rows_per_block) {
+    int64_t b = (tokens + rows_per_block - 1) / rows_per_block;
+    return b < 512 ? b : 512;
+}
+
+template <int LPR, int V, bool SCORED>
+static int launch_route(const RouteArgs& a, hipStream_t st) {
+    constexpr int WAVES = route_waves<LPR, V, SCORED>();
+    const int64_t blocks = route_blocks(a.tokens, WAVES * (64 / LPR));
+    hipLaunchKernelGGL((route_fwd_kernel<LPR, V, SCORED>), dim3((unsigned)blocks), dim3(WAVES * 64), 0, st, a);
+    if (blocks > 1)
+        hipLaunchKernelGGL(route_counts_kernel, dim3((unsigned)((a.experts + 63) / 64)), dim3(1024), 0, st, a.partial, (int)blocks, a.experts, a.counts);
+    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+}
+
+static bool route_sizes_ok(int64_t tokens, int experts, int topk, int dtype, int score) {
+    return tokens >= 0 && tokens <= 0x7FFFFFFF && experts >= 1 && experts <= RT_MAX_EXPERTS && topk >= 1 && topk <= RT_MAX_TOPK && topk <= experts &&
+           dtype >= MXL_DT_F32 && dtype <= MXL_DT_F16 && (score == MXL_SCORE_SOFTMAX || score == MXL_SCORE_SIGMOID);
+}
+
+__global__ void route_zero_counts_kernel(int64_t* counts, int experts) {
+    for (int e = threadIdx.x; e < experts; e += 256) counts[e] = 0;
+}
+
+}  // namespace mxl
+
+using namespace mxl;
+
+extern "C" int64_t mxl_topk_routing_workspace_bytes(int64_t tokens, int experts) {
+    if (tokens < 0 || experts < 1 || experts > RT_MAX_EXPERTS) return -1;
+    return route_blocks(tokens, 2) * experts * 4;
+}
+
+extern "C" int mxl_topk_routing(const void* logits, int dtype, int64_t tokens, int experts, int topk, int score, const float* expert_bias,
+                                int num_groups, int group_topk, int renormalize, float scale, const uint8_t* token_mask, float* probs,
+                                int64_t* indices, int64_t* counts, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!route_sizes_ok(tokens, experts, topk, dtype, score) || !counts) return MXL_EINVAL;
+    if (num_groups < 1 || num_groups > RT_MAX_EXPERT_GROUPS || experts % num_groups != 0 || group_topk < 1 || group_topk > num_groups ||
+        topk > group_topk * (experts / num_groups))
+        return MXL_EINVAL;
+    if (tokens > 0 && (!logits || !probs || !indices)) return MXL_EINVAL;
+    if (workspace_bytes < mxl_topk_routing_workspace_bytes(tokens, experts) || (tokens > 0 && !workspace)) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    hipStream_t st = (hipStream_t)stream;
+    if (tokens == 0) {
+        hipLaunchKernelGGL(route_zero_counts_kernel, dim3(1), dim3(256), 0, st, counts, experts);
+        return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+    }
+    RouteArgs a{};
+    a.logits = logits, a.bias = expert_bias, a.mask = token_mask, a.probs = probs, a.indices = indices, a.counts = counts;
+    a.partial = (int*)workspace, a.tokens = tokens, a.experts = experts, a.topk = topk, a.dtype = dtype;
+    a.sigmoid = score == MXL_SCORE_SIGMOID, a.renorm = renormalize != 0, a.scale = scale;
+    a.groups = num_groups, a.group_topk = group_topk, a.group_size = experts / num_groups;
+    // the topk / group_topk best of a group make its score
+    a.take = topk / group_topk < 1 ? 1 : topk / group_topk;
+    if (a.take > a.group_size) a.take = a.group_size;
+    if (expert_bias || num_groups > 1) {
+        int pow2 = 1;
+        while (pow2 < num_groups) pow2 *= 2;
+        a.lanes_per_group = 64 / pow2;
+        const int v = (a.group_size + a.lanes_per_group - 1) / a.lanes_per_group;
+        if (v <= 1) return launch_route<64, 1, true>(a, st);
+        if (v <= 2) return launch_route<64, 2, true>(a, st);
+        if (v <= 4) return launch_route<64, 4, true>(a, st);
+        if (v <= 8) return launch_route<64, 8, true>(a, st);
+        if (v <= 16) return launch_route<64, 16, true>(a, st);
+        return launch_route<64, 32, true>(a, st);
+    }
+    a.lanes_per_group = 64;
+    if (topk <= 8 && experts <= 8) return launch_route<8, 1, false>(a, st);
+    if (topk <= 8 && experts <= 16) return launch_route<8, 2, false>(a, st);
+    if (topk <= 8 && experts <= 32) return launch_route<8, 4, false>(a, st);
+    if (topk <= 16 && experts <= 64) return launch_route<16, 4, false>(a, st);
+    if (experts <= 128) return launch_route<32, 4, false>(a, st);
+    if (experts <= 256) return launch_route<64, 4, false>(a, st);
+    if (experts <= 512) return launch_route<64, 8, false>(a, st);
+    return launch_route<64, 16, false>(a, st);
+}
+
+extern "C" int mxl_topk_routing_bwd(const float* dprobs, const void* logits, int dtype, const int64_t* indices, int64_t tokens, int experts,
+                                    int topk, int score, int renormalize, float scale, void* dlogits, void* stream) {
+    if (!route_sizes_ok(tokens, experts, topk, dtype, score)) return MXL_EINVAL;
+    if (tokens == 0) return MXL_OK;
+    if (!dprobs || !logits || !indices || !dlogits) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    RouteBwdArgs a{dprobs, logits, indices, dlogits, tokens, experts, topk, dtype, score == MXL_SCORE_SIGMOID, renormalize != 0, scale};
+    int64_t blocks = (tokens + RB_WAVES - 1) / RB_WAVES;
+    if (blocks > 1024) blocks = 1024;
+    hipLaunchKernelGGL(route_bwd_kernel, dim3((unsigned)blocks), dim3(RB_WAVES * 64), 0, (hipStream_t)stream, a);
+    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+}

@@ -1219,6 +1219,210 @@ def unpad_groups_impl(y, group_lens, align: int, rows: int):
 
 
 # --------------------------------------------------------------------------
+# around the expert MLP: routing, rows into the experts' order and back
+# --------------------------------------------------------------------------
+_DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+ROUTING_MAX_TOPK = 32
+
+
+def _on(device: torch.device):
+    """The tensors' own device as the current one: a launch goes to its stream."""
+    return _NO_HOOK if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _float_type(t: torch.Tensor, what: str) -> int:
+    if t.dtype not in _DT:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return _DT[t.dtype]
+
+
+def _same_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must live on the device of the other operands")
+
+
+def _routing_args(logits, topk, score_function):
+    _require_cuda(logits)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [tokens, experts]")
+    dtype = _float_type(logits, "logits")
+    experts = logits.shape[1]
+    if not 1 <= experts <= _lib.MAX_GROUPS:
+        raise ValueError(f"the number of experts must be in [1, {_lib.MAX_GROUPS}]")
+    if not 1 <= topk <= min(ROUTING_MAX_TOPK, experts):
+        raise ValueError(f"topk must be in [1, {min(ROUTING_MAX_TOPK, experts)}]")
+    if score_function not in _SCORES:
+        raise ValueError(f"score_function must be 'softmax' or 'sigmoid', got {score_function!r}")
+    return dtype, experts, _SCORES[score_function]
+
+
+def topk_routing_impl(logits, topk: int, score_function: str = "softmax", expert_bias: Optional[torch.Tensor] = None,
+                      num_groups: int = 1, group_topk: int = 1, renormalize: bool = True, scaling_factor: float = 1.0,
+                      token_mask: Optional[torch.Tensor] = None):
+    """``(probs [tokens, topk] float32, indices [tokens, topk] int64, tokens_per_expert [experts] int64)``; see
+    ``ops.topk_routing``."""
+    dtype, experts, score = _routing_args(logits, topk, score_function)
+    if not 1 <= num_groups <= 64 or experts % num_groups != 0:
+        raise ValueError("num_groups must divide the number of experts and be at most 64")
+    if not 1 <= group_topk <= num_groups or topk > group_topk * (experts // num_groups):
+        raise ValueError("group_topk must be in [1, num_groups], and its groups must hold topk experts")
+    tokens = logits.shape[0]
+    if expert_bias is not None and (expert_bias.dtype != torch.float32 or tuple(expert_bias.shape) != (experts,)):
+        raise ValueError("expert_bias must be float32 [experts]")
+    if token_mask is not None:
+        if token_mask.dtype not in (torch.bool, torch.uint8) or tuple(token_mask.shape) != (tokens,):
+            raise ValueError("token_mask must be bool or uint8 [tokens]")
+    _require_cuda(expert_bias, token_mask)
+    _same_device(logits.device, expert_bias=expert_bias, token_mask=token_mask)
+    dev = logits.device
+    lib = _lib.load()
+    with _on(dev), _hooked("topk_routing", tokens=tokens, experts=experts, topk=topk):
+        probs = torch.empty((tokens, topk), dtype=torch.float32, device=dev)
+        indices = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
+        counts = torch.empty((experts,), dtype=torch.int64, device=dev)
+        ws = torch.empty((max(int(lib.mxl_topk_routing_workspace_bytes(tokens, experts)), 16),), dtype=torch.uint8, device=dev)
+        rc = lib.mxl_topk_routing(_ptr(logits), dtype, tokens, experts, topk, score, _ptr(expert_bias), num_groups, group_topk,
+                                  int(bool(renormalize)), float(scaling_factor), _ptr(token_mask), _ptr(probs), _ptr(indices),
+                                  _ptr(counts), _ptr(ws), ws.numel(), _stream())
+    _lib.check(rc, "mxl_topk_routing")
+    return probs, indices, counts
+
+
+def topk_routing_bwd_impl(dprobs, logits, indices, score_function: str = "softmax", renormalize: bool = True,
+                          scaling_factor: float = 1.0) -> torch.Tensor:
+    """Gradient of ``topk_routing_impl``'s probabilities with respect to the logits, in their type."""
+    topk = indices.shape[-1]
+    dtype, experts, score = _routing_args(logits, topk, score_function)
+    tokens = logits.shape[0]
+    if dprobs.dtype != torch.float32 or tuple(dprobs.shape) != (tokens, topk):
+        raise ValueError("dprobs must be float32 [tokens, topk]")
+    if indices.dtype != torch.int64 or tuple(indices.shape) != (tokens, topk):
+        raise ValueError("indices must be int64 [tokens, topk]")
+    _require_cuda(dprobs, indices)
+    _same_device(logits.device, dprobs=dprobs, indices=indices)
+    with _on(logits.device), _hooked("topk_routing_bwd", tokens=tokens, experts=experts, topk=topk):
+        dlogits = torch.empty_like(logits)
+        rc = _lib.load().mxl_topk_routing_bwd(_ptr(dprobs), _ptr(logits), dtype, _ptr(indices), tokens, experts, topk, score,
+                                              int(bool(renormalize)), float(scaling_factor), _ptr(dlogits), _stream())
+    _lib.check(rc, "mxl_topk_routing_bwd")
+    return dlogits
+
+
+def permute_plan_impl(indices, num_experts: int, align: int = 1, probs: Optional[torch.Tensor] = None):
+    """``(row_of [tokens, topk] int64, entry_of [rows] int32, group_lens [experts] int64, row_probs [rows] or None)``: where every
+    entry of ``indices`` goes in a buffer of rows sorted by expert; see ``ops.permute_tokens``."""
+    _require_cuda(indices, probs)
+    if indices.dtype != torch.int64 or indices.dim() != 2:
+        raise ValueError("indices must be int64 [tokens, topk]")
+    if not 1 <= num_experts <= _lib.MAX_GROUPS:
+        raise ValueError(f"the number of experts must be in [1, {_lib.MAX_GROUPS}]")
+    if not 1 <= align <= 1 << 20:
+        raise ValueError("align must be in [1, 2^20]")
+    if not 1 <= indices.shape[1] <= ROUTING_MAX_TOPK:
+        raise ValueError(f"topk must be in [1, {ROUTING_MAX_TOPK}]")
+    if indices.numel() > 0x3FFFFFFF:
+        raise ValueError("at most 2^30 - 1 entries")
+    if probs is not None:
+        _float_type(probs, "probs")
+        if probs.shape != indices.shape:
+            raise ValueError("probs must have the shape of indices")
+        _same_device(indices.device, probs=probs)
+    entries = indices.numel()
+    rows = padded_rows_bound(entries, num_experts, align)
+    if rows > 0x7FFFFFFF:
+        raise ValueError("the buffer of rows must have fewer than 2^31 rows")
+    dev = indices.device
+    lib = _lib.load()
+    with _on(dev), _hooked("permute_plan", entries=entries, rows=rows):
+        row_of = torch.empty_like(indices)
+        entry_of = torch.empty((rows,), dtype=torch.int32, device=dev)
+        lens = torch.empty((num_experts,), dtype=torch.int64, device=dev)
+        row_probs = None if probs is None else torch.empty((rows,), dtype=probs.dtype, device=dev)
+        ws = torch.empty((max(int(lib.mxl_permute_plan_workspace_bytes(entries, num_experts)), 16),), dtype=torch.uint8, device=dev)
+        rc = lib.mxl_permute_plan(_ptr(indices), entries, num_experts, align, rows, _ptr(row_of), _ptr(entry_of), _ptr(lens), _ptr(probs),
+                                  0 if probs is None else probs.element_size(), _ptr(row_probs), _ptr(ws), ws.numel(), _stream())
+    _lib.check(rc, "mxl_permute_plan")
+    return row_of, entry_of, lens, row_probs
+
+
+def _row_args(x, row_of, entry_of):
+    _require_cuda(x, row_of, entry_of)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("expected a 2-D tensor of rows that are not empty")
+    _float_type(x, "rows")
+    if row_of.dtype != torch.int64 or row_of.dim() != 2 or not 1 <= row_of.shape[1] <= ROUTING_MAX_TOPK:
+        raise ValueError(f"row_of must be int64 [tokens, topk] with topk in [1, {ROUTING_MAX_TOPK}]")
+    if entry_of.dtype != torch.int32 or entry_of.dim() != 1:
+        raise ValueError("entry_of must be int32 [rows]")
+    _same_device(x.device, row_of=row_of, entry_of=entry_of)
+
+
+def permute_rows_impl(x, row_of, entry_of) -> torch.Tensor:
+    """``rows[row_of[t, k]] = x[t]``, zero rows where ``entry_of`` is -1."""
+    _row_args(x, row_of, entry_of)
+    if x.shape[0] != row_of.shape[0]:
+        raise ValueError("one row of x per token")
+    rows, hidden = entry_of.shape[0], x.shape[1]
+    with _on(x.device), _hooked("permute_rows", tokens=x.shape[0], rows=rows, hidden=hidden):
+        out = torch.empty((rows, hidden), dtype=x.dtype, device=x.device)
+        rc = _lib.load().mxl_permute_rows(_ptr(x), x.shape[0], hidden * x.element_size(), _ptr(row_of), row_of.shape[1], _ptr(entry_of),
+                                          rows, _ptr(out), _stream())
+    _lib.check(rc, "mxl_permute_rows")
+    return out
+
+
+def combine_rows_impl(rows, row_of, entry_of, probs: Optional[torch.Tensor] = None, row_probs: Optional[torch.Tensor] = None):
+    """``(y, probs_out)``: ``y[t] = sum_k probs[t, k] * rows[row_of[t, k]]`` (``probs`` None: ones) in fp32, rounded once, and
+    ``probs_out[t, k] = row_probs[row_of[t, k]]`` (None without ``row_probs``)."""
+    _row_args(rows, row_of, entry_of)
+    _require_cuda(probs, row_probs)
+    _same_device(rows.device, probs=probs, row_probs=row_probs)
+    if rows.shape[0] != entry_of.shape[0]:
+        raise ValueError("rows must be the buffer the permutation was made for")
+    if probs is not None and row_probs is not None:
+        raise ValueError("probs and row_probs exclude each other")
+    if probs is not None and probs.shape != row_of.shape:
+        raise ValueError("probs must be [tokens, topk]")
+    if row_probs is not None and tuple(row_probs.shape) != (rows.shape[0],):
+        raise ValueError("row_probs must be [rows]")
+    p = probs if probs is not None else row_probs
+    pd = _lib.DT_F32 if p is None else _float_type(p, "probs")
+    tokens, topk = row_of.shape
+    with _on(rows.device), _hooked("combine_rows", tokens=tokens, rows=rows.shape[0], hidden=rows.shape[1]):
+        y = torch.empty((tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+        out = None if row_probs is None else torch.empty((tokens, topk), dtype=row_probs.dtype, device=rows.device)
+        # (no rows: _ptr is None for an empty tensor, so the probabilities go the way of zeros)
+        empty = row_probs is not None and row_probs.numel() == 0
+        if empty:
+            out.zero_()
+        rc = _lib.load().mxl_combine_rows(_ptr(rows), rows.shape[0], rows.shape[1], _DT[rows.dtype], _ptr(row_of), tokens, topk, _ptr(probs),
+                                          _ptr(row_probs), None if empty else _ptr(out), pd, _ptr(y), _stream())
+    _lib.check(rc, "mxl_combine_rows")
+    return y, out
+
+
+def combine_rows_bwd_impl(dy, rows, row_of, entry_of, probs, need_rows: bool = True, need_probs: bool = True):
+    """``(drows, dprobs float32)`` of ``combine_rows_impl`` with ``probs``; what is not needed is None."""
+    _row_args(rows, row_of, entry_of)
+    _require_cuda(dy, probs)
+    _same_device(rows.device, dy=dy, probs=probs)
+    tokens, topk = row_of.shape
+    if dy.dtype != rows.dtype or tuple(dy.shape) != (tokens, rows.shape[1]) or rows.shape[0] != entry_of.shape[0]:
+        raise ValueError("dy must be [tokens, hidden] of the rows' type, rows the buffer the permutation was made for")
+    if probs.shape != row_of.shape:
+        raise ValueError("probs must be [tokens, topk]")
+    with _on(rows.device), _hooked("combine_rows_bwd", tokens=tokens, rows=rows.shape[0], hidden=rows.shape[1]):
+        drows = torch.empty_like(rows) if need_rows else None
+        dprobs = torch.empty((tokens, topk), dtype=torch.float32, device=rows.device) if need_probs else None
+        rc = _lib.load().mxl_combine_rows_bwd(_ptr(dy), _ptr(rows), rows.shape[0], rows.shape[1], _DT[rows.dtype], _ptr(row_of), _ptr(entry_of),
+                                              tokens, topk, _ptr(probs), _float_type(probs, "probs"), _ptr(drows), _ptr(dprobs), _stream())
+    _lib.check(rc, "mxl_combine_rows_bwd")
+    return drows, dprobs
+
+
+# --------------------------------------------------------------------------
 # the 128-blockwise FP8 recipe
 # --------------------------------------------------------------------------
 BW_BLOCK = 128

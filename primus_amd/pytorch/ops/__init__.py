@@ -21,9 +21,10 @@ Activations and gradients use 1-D blocks of 32, weights 2-D 32x32 blocks.
 from __future__ import annotations
 
 import contextlib
-from typing import Optional, Union
+from typing import NamedTuple, Optional, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ... import _lib
 from .. import kernels as K
@@ -39,7 +40,8 @@ from ..core.quantized_tensor import QuantizedTensor, QuantizedTensorPair
 __all__ = ["gemm", "grouped_gemm", "gemm_fp8", "gemm_fp4", "grouped_gemm_fp8", "grouped_gemm_fp4", "set_wgrad_overlap",
            "set_dgrad_reads_rowwise_weight",
            "swiglu_with_probs", "geglu_with_probs", "tokens_per_expert_to_mask", "glu_grouped_gemm_fp8",
-           "glu_grouped_gemm_fp4", "manual_sr_seed", "set_kchunk_layout", "rmsnorm", "rmsnorm_gemm_fp8", "rmsnorm_gemm_fp4", "pad_groups", "unpad_groups"]
+           "glu_grouped_gemm_fp4", "manual_sr_seed", "set_kchunk_layout", "rmsnorm", "rmsnorm_gemm_fp8", "rmsnorm_gemm_fp4", "pad_groups", "unpad_groups",
+           "topk_routing", "permute_tokens", "unpermute_tokens", "TokenPermutation"]
 
 # dgrad and wgrad of one linear are independent once dY is quantised, so wgrad may run on a second stream, where its
 # workgroups move in as dgrad's last, partial round of tiles drains.  The default is one stream: _overlaps() names the
@@ -1111,3 +1113,135 @@ def unpad_groups(y: torch.Tensor, group_lens: torch.Tensor, align: int, rows: in
     """The ``rows`` live rows of a buffer made by ``pad_groups`` for the same counts (experts.py:262-264).
     Differentiable in ``y``: padding rows get a zero gradient."""
     return _UnpadGroups.apply(y, group_lens, int(align), int(rows))
+
+
+# ---------------------------------------------------------------------------
+# Around the expert MLP (primus/backends/megatron/core/transformer/experts.py:179-268 takes rows sorted by expert with
+# their probabilities): the router's choice, the rows into the experts' order and back.  Sizes depend on shapes alone and
+# nothing is read back from the device, so the whole of it can be captured in a graph.
+# ---------------------------------------------------------------------------
+class _TopkRouting(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk, score_function, expert_bias, num_groups, group_topk, renormalize, scaling_factor, token_mask):
+        probs, indices, counts = K.topk_routing_impl(logits, topk, score_function, expert_bias, num_groups, group_topk, renormalize,
+                                                     scaling_factor, token_mask)
+        ctx.save_for_backward(logits, indices)
+        ctx.how = (score_function, renormalize, scaling_factor)
+        ctx.mark_non_differentiable(indices, counts)
+        return probs, indices, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dprobs, _, __):
+        logits, indices = ctx.saved_tensors
+        dlogits = K.topk_routing_bwd_impl(dprobs.to(torch.float32).contiguous(), logits, indices, *ctx.how)
+        return dlogits, None, None, None, None, None, None, None, None
+
+
+def topk_routing(logits: torch.Tensor, topk: int, score_function: str = "softmax", expert_bias: Optional[torch.Tensor] = None,
+                 num_groups: Optional[int] = None, group_topk: Optional[int] = None, renormalize: bool = True,
+                 scaling_factor: float = 1.0, token_mask: Optional[torch.Tensor] = None):
+    """``(probs [tokens, topk] float32, indices [tokens, topk] int64, tokens_per_expert [experts] int64)``: the ``topk`` experts of
+    every token from ``logits [tokens, experts]`` (float32, bfloat16 or float16).
+
+    Scores are the softmax over the experts or the sigmoid (``score_function``), in fp32.  ``expert_bias`` (float32
+    ``[experts]``, the load-balancing bias) is added for the choice only.  With ``num_groups`` the experts form that many
+    consecutive groups; a group's score is the sum of its ``topk // group_topk`` largest biased scores (at least one) and only the
+    ``group_topk`` best groups take part.  ``indices`` are best first, ties to the lower index; fp32 scores that are too near to
+    each other to tell are compared in fp64.  ``probs`` are the chosen scores, divided by their sum if ``renormalize`` (sigmoid:
+    by the sum + 1e-20), times ``scaling_factor``.  Tokens whose ``token_mask`` (bool ``[tokens]``) is False get indices -1 and
+    probabilities 0 and are not counted.  Softmax scores of nothing but -inf are 0.  NaN scores are chosen last; the indices are
+    valid and differ from each other whatever the logits hold.  At most 1024 experts, 32 a token, 64 groups.  Differentiable in ``logits``."""
+    if num_groups is None:
+        if group_topk is not None:
+            raise ValueError("group_topk needs num_groups")
+        num_groups = group_topk = 1
+    elif group_topk is None:
+        raise ValueError("num_groups needs group_topk")
+    if expert_bias is not None:
+        expert_bias = expert_bias.detach().contiguous()
+    if token_mask is not None:
+        token_mask = token_mask.contiguous()
+    return _TopkRouting.apply(logits.contiguous(), int(topk), score_function, expert_bias, int(num_groups), int(group_topk),
+                              bool(renormalize), float(scaling_factor), token_mask)
+
+
+class TokenPermutation(NamedTuple):
+    """Where ``permute_tokens`` put every entry: ``row_of [tokens, topk]`` int64 (-1: nowhere) and ``entry_of [rows]`` int32,
+    the entry ``t * topk + k`` of every row (-1: a zero row)."""
+
+    row_of: torch.Tensor
+    entry_of: torch.Tensor
+
+
+class _PermuteTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, indices, num_experts, probs, align):
+        row_of, entry_of, group_lens, row_probs = K.permute_plan_impl(indices, num_experts, align, probs)
+        rows = K.permute_rows_impl(x, row_of, entry_of)
+        ctx.save_for_backward(row_of, entry_of)
+        ctx.dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(group_lens, row_of, entry_of)
+        return rows, row_probs, group_lens, row_of, entry_of
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows, drow_probs, _, __, ___):
+        row_of, entry_of = ctx.saved_tensors
+        dx = dprobs = None
+        if not ctx.needs_input_grad[3]:
+            drow_probs = None
+        if drows is not None and ctx.needs_input_grad[0]:
+            drows = drows.to(ctx.dtype).contiguous()
+            dx, dprobs = K.combine_rows_impl(drows, row_of, entry_of, row_probs=None if drow_probs is None else drow_probs.contiguous())
+        elif drow_probs is not None:
+            dprobs = torch.where(row_of >= 0, drow_probs[row_of.clamp(min=0)], 0.0) if entry_of.numel() else drow_probs.new_zeros(row_of.shape)
+        return dx, None, None, dprobs, None
+
+
+def permute_tokens(x: torch.Tensor, indices: torch.Tensor, num_experts: int, probs: Optional[torch.Tensor] = None, align: int = 1):
+    """``(rows, row_probs, group_lens, permutation)``: the rows of ``x [tokens, hidden]`` in the order of their experts, what the
+    grouped linears and the expert MLP take, for ``indices [tokens, topk]`` as ``topk_routing`` returns them.
+
+    The entries of an expert follow each other in the entries' order (by token, then by k); an entry whose index is outside
+    ``[0, num_experts)`` goes nowhere.  Every expert's rows are padded with zero rows to a multiple of ``align``
+    (the quantisation alignment; ``pad_groups`` does the same to rows that are sorted already).  ``rows`` is sized for the worst
+    case, ``(tokens * topk + num_experts * (align - 1)) // align * align`` rows; the zero rows behind the last expert's count into
+    ``group_lens[-1]``, so ``group_lens`` describes the whole buffer.  ``row_probs [rows]``: ``probs [tokens, topk]`` of the rows, 0 for
+    zero rows (None without ``probs``).  ``permutation`` is what ``unpermute_tokens`` takes.  bfloat16, float16 or float32;
+    differentiable in ``x`` (fp32 sums over the copies, one rounding) and ``probs``."""
+    if x.dim() != 2 or indices.dim() != 2 or x.shape[0] != indices.shape[0]:
+        raise ValueError("x must be [tokens, hidden] and indices [tokens, topk]")
+    if indices.is_floating_point() or indices.dtype == torch.bool:
+        raise ValueError("indices must be integers")
+    rows, row_probs, group_lens, row_of, entry_of = _PermuteTokens.apply(
+        x.contiguous(), indices.to(torch.int64).contiguous(), int(num_experts), None if probs is None else probs.contiguous(), int(align))
+    return rows, row_probs, group_lens, TokenPermutation(row_of, entry_of)
+
+
+class _UnpermuteTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, row_of, entry_of, probs):
+        # without probabilities the gradient is a move of dy's rows: the rows themselves are not kept
+        ctx.save_for_backward(row_of, entry_of, probs, None if probs is None else rows)
+        ctx.dtype = rows.dtype
+        return K.combine_rows_impl(rows, row_of, entry_of, probs)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        row_of, entry_of, probs, rows = ctx.saved_tensors
+        dy = dy.to(ctx.dtype).contiguous()
+        if probs is None:
+            return K.permute_rows_impl(dy, row_of, entry_of), None, None, None
+        drows, dprobs = K.combine_rows_bwd_impl(dy, rows, row_of, entry_of, probs, ctx.needs_input_grad[0], ctx.needs_input_grad[3])
+        return drows, None, None, None if dprobs is None else dprobs.to(probs.dtype)
+
+
+def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, probs: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[t] = sum_k probs[t, k] * rows[row_of[t, k]]`` (``probs`` None: ones, for experts that have applied them already): the
+    experts' outputs back at their tokens, summed in fp32 in the order of k and rounded once.  Entries that went nowhere add
+    nothing; zero rows are ignored.  Differentiable in ``rows`` (rows that no entry went to get zeros) and ``probs``."""
+    row_of, entry_of = permutation
+    return _UnpermuteTokens.apply(rows.contiguous(), row_of, entry_of, None if probs is None else probs.contiguous())

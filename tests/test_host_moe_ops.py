@@ -1,0 +1,105 @@
+"""Refusals of the operators around the expert MLP: every one before a launch, so they are checked without a GPU.  Tensors of a GPU
+are stood in for by a subclass that says it is one; the last check needs none."""
+
+import ctypes
+
+import pytest
+import torch
+
+from primus_amd import _lib
+from primus_amd.pytorch import kernels as K
+from primus_amd.pytorch import ops
+
+
+@pytest.fixture()
+def on_gpu(monkeypatch):
+    """The checks as for tensors on the GPU."""
+    monkeypatch.setattr(K, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(_lib, "load", lambda: pytest.fail("nothing may be launched"))
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(4, 8)
+    for call in (lambda: ops.topk_routing(x, 2), lambda: ops.permute_tokens(x, torch.zeros(4, 2, dtype=torch.int64), 3),
+                 lambda: ops.unpermute_tokens(x, ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)))):
+        with pytest.raises(ValueError, match="GPU only"):
+            call()
+
+
+@pytest.mark.parametrize("why,call", [
+    ("tokens, experts", lambda: ops.topk_routing(torch.randn(2, 3, 4), 2)),
+    ("float32, bfloat16 or float16", lambda: ops.topk_routing(torch.randn(2, 4).double(), 2)),
+    ("topk", lambda: ops.topk_routing(torch.randn(2, 4), 5)),
+    ("topk", lambda: ops.topk_routing(torch.randn(2, 64), 33)),
+    ("topk", lambda: ops.topk_routing(torch.randn(2, 4), 0)),
+    ("number of experts", lambda: ops.topk_routing(torch.randn(2, 1025), 2)),
+    ("number of experts", lambda: ops.topk_routing(torch.randn(2, 0), 1)),
+    ("score_function", lambda: ops.topk_routing(torch.randn(2, 4), 2, score_function="relu")),
+    ("group_topk needs num_groups", lambda: ops.topk_routing(torch.randn(2, 4), 2, group_topk=1)),
+    ("num_groups needs group_topk", lambda: ops.topk_routing(torch.randn(2, 4), 2, num_groups=2)),
+    ("num_groups must divide", lambda: ops.topk_routing(torch.randn(2, 4), 2, num_groups=3, group_topk=1)),
+    ("num_groups must divide", lambda: ops.topk_routing(torch.randn(2, 130), 2, num_groups=65, group_topk=1)),
+    ("group_topk must be in", lambda: ops.topk_routing(torch.randn(2, 4), 2, num_groups=2, group_topk=3)),
+    ("hold topk experts", lambda: ops.topk_routing(torch.randn(2, 8), 3, num_groups=4, group_topk=1)),
+    ("expert_bias", lambda: ops.topk_routing(torch.randn(2, 4), 2, expert_bias=torch.zeros(3))),
+    ("expert_bias", lambda: ops.topk_routing(torch.randn(2, 4), 2, expert_bias=torch.zeros(4).double())),
+    ("token_mask", lambda: ops.topk_routing(torch.randn(2, 4), 2, token_mask=torch.ones(3, dtype=torch.bool))),
+    ("token_mask", lambda: ops.topk_routing(torch.randn(2, 4), 2, token_mask=torch.ones(2))),
+    ("indices", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(3, 2, dtype=torch.int64), 3)),
+    ("integers", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2), 3)),
+    ("integers", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.bool), 3)),
+    ("x must be", lambda: ops.permute_tokens(torch.randn(4), torch.zeros(4, 2, dtype=torch.int64), 3)),
+    ("number of experts", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int64), 0)),
+    ("number of experts", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int64), 1025)),
+    ("align", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int64), 3, align=0)),
+    ("topk must be", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 33, dtype=torch.int64), 3)),
+    ("shape of indices", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int64), 3, probs=torch.zeros(4, 3))),
+    ("probs must be", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int64), 3, probs=torch.zeros(4, 2).double())),
+    ("row_of", lambda: ops.unpermute_tokens(torch.randn(4, 8), ops.TokenPermutation(torch.zeros(4, 2), torch.zeros(4, dtype=torch.int32)))),
+    ("entry_of", lambda: ops.unpermute_tokens(torch.randn(4, 8), ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4)))),
+    ("made for", lambda: ops.unpermute_tokens(torch.randn(4, 8), ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(5, dtype=torch.int32)))),
+    ("probs must be", lambda: ops.unpermute_tokens(torch.randn(4, 8), ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)),
+                                                   probs=torch.zeros(4, 3))),
+    ("not empty", lambda: ops.unpermute_tokens(torch.randn(4, 0), ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)))),
+])
+def test_refusals(on_gpu, why, call):
+    with pytest.raises(ValueError, match=why):
+        call()
+
+
+def test_c_entries_check_before_they_touch_the_device():
+    """Malformed calls are MXL_EINVAL (-1), well-formed ones MXL_ENODEV (-3) on a machine without a GPU."""
+    if torch.cuda.device_count() > 0:
+        pytest.skip("a GPU is present: the well-formed calls would be real launches")
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = ctypes.cast(buf, ctypes.c_void_p)
+    f = ctypes.c_float(1.0)
+    ws = lib.mxl_topk_routing_workspace_bytes(4, 8)
+    route = lambda **k: lib.mxl_topk_routing(*[{**dict(l=p, dt=0, t=4, e=8, k=2, s=0, b=None, g=1, gk=1, r=1, sc=f, m=None, pr=p, i=p, c=p, w=p, wb=ws, st=None), **k}[n]  # noqa: E731
+                                               for n in ("l", "dt", "t", "e", "k", "s", "b", "g", "gk", "r", "sc", "m", "pr", "i", "c", "w", "wb", "st")])
+    assert route() == -3
+    for bad in (dict(l=None), dict(dt=3), dict(t=-1), dict(e=0), dict(e=1025), dict(k=0), dict(k=9), dict(s=2), dict(g=3), dict(g=2, gk=3), dict(g=8, gk=1),
+                dict(pr=None), dict(i=None), dict(c=None), dict(w=None), dict(wb=ws - 1)):
+        assert route(**bad) == -1, bad
+    assert lib.mxl_topk_routing_workspace_bytes(-1, 8) == -1 and lib.mxl_topk_routing_workspace_bytes(1, 0) == -1
+    bwd = lambda **k: lib.mxl_topk_routing_bwd(*[{**dict(d=p, l=p, dt=0, i=p, t=4, e=8, k=2, s=0, r=1, sc=f, o=p, st=None), **k}[n] for n in ("d", "l", "dt", "i", "t", "e", "k", "s", "r", "sc", "o", "st")])  # noqa: E731
+    assert bwd() == -3 and bwd(t=0) == 0
+    for bad in (dict(d=None), dict(o=None), dict(dt=-1), dict(k=33), dict(e=2000)):
+        assert bwd(**bad) == -1, bad
+    pw = lib.mxl_permute_plan_workspace_bytes(8, 4)
+    plan = lambda **k: lib.mxl_permute_plan(*[{**dict(i=p, n=8, e=4, a=1, r=8, ro=p, eo=p, gl=p, pr=None, pb=0, rp=None, w=p, wb=pw, st=None), **k}[n]  # noqa: E731
+                                              for n in ("i", "n", "e", "a", "r", "ro", "eo", "gl", "pr", "pb", "rp", "w", "wb", "st")])
+    assert plan() == -3
+    for bad in (dict(i=None), dict(n=-1), dict(e=0), dict(e=1025), dict(a=0), dict(r=7), dict(ro=None), dict(eo=None), dict(gl=None), dict(pr=p, pb=3, rp=p), dict(pb=4, rp=p),
+                dict(w=None), dict(wb=pw - 1), dict(a=32, r=8)):
+        assert plan(**bad) == -1, bad
+    assert lib.mxl_permute_rows(p, 4, 16, p, 2, p, 8, p, None) == -3
+    assert lib.mxl_permute_rows(p, 4, 0, p, 2, p, 8, p, None) == -1 and lib.mxl_permute_rows(p, 4, 16, p, 33, p, 8, p, None) == -1
+    assert lib.mxl_permute_rows(p, 4, 16, p, 2, None, 8, p, None) == -1 and lib.mxl_permute_rows(None, 4, 16, p, 2, p, 8, p, None) == -1
+    assert lib.mxl_combine_rows(p, 8, 16, 1, p, 4, 2, p, None, None, 0, p, None) == -3
+    assert lib.mxl_combine_rows(p, 8, 16, 1, p, 4, 2, None, p, None, 0, p, None) == -1 and lib.mxl_combine_rows(p, 8, 0, 1, p, 4, 2, p, None, None, 0, p, None) == -1
+    assert lib.mxl_combine_rows(p, 8, 16, 3, p, 4, 2, p, None, None, 0, p, None) == -1 and lib.mxl_combine_rows(p, 8, 16, 1, p, 4, 2, p, None, None, 5, p, None) == -1
+    assert lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, p, 4, 2, p, 0, p, p, None) == -3
+    assert lib.mxl_combine_rows_bwd(None, p, 8, 16, 1, p, p, 4, 2, p, 0, p, p, None) == -1 and lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, p, 4, 2, None, 0, p, p, None) == -1
+    assert lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, None, 4, 2, p, 0, p, p, None) == -1
