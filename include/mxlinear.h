@@ -48,8 +48,15 @@ extern "C" {
 /* gated activations of the expert MLP and the dtype of the router probabilities */
 #define MXL_ACT_SILU 0
 #define MXL_ACT_GELU 1
+#define MXL_ACT_RELU 2   /* dense linear only, as is none */
+#define MXL_ACT_NONE 3
 #define MXL_PROBS_F32 0
 #define MXL_PROBS_BF16 1
+
+/* element types, where an operand may have more than one */
+#define MXL_DT_F32 0
+#define MXL_DT_BF16 1
+#define MXL_DT_F16 2
 
 #define MXL_BLOCK 32      /* MX block size (fp8_utils.py:48, fp4_utils.py:79) */
 #define MXL_SEG_ALIGN 128 /* padding of each expert segment in the transposed layout */
@@ -546,10 +553,7 @@ int mxl_linear_backward(const mxl_linear* p, int parts, const void* dy_bf16, con
 
 /* ---- around the expert MLP: routing, rows into the experts' order and back ----
  * The expert MLP takes rows sorted by expert and their probabilities (primus/backends/megatron/core/transformer/experts.py:179-268).
- * Element types of logits, rows and probabilities: */
-#define MXL_DT_F32 0
-#define MXL_DT_BF16 1
-#define MXL_DT_F16 2
+ * Logits, rows and probabilities are of any MXL_DT_* type. */
 #define MXL_SCORE_SOFTMAX 0
 #define MXL_SCORE_SIGMOID 1
 
@@ -601,6 +605,22 @@ int mxl_combine_rows(const void* rows_in, int64_t rows, int hidden, int dtype, c
 int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int hidden, int dtype, const int64_t* row_of,
                          const int32_t* entry_of, int64_t tokens, int topk, const void* probs, int probs_dtype, void* drows,
                          float* dprobs, void* stream);
+
+/* ---- dense bf16 linear with its epilogue (the route without a recipe,
+ * primus/backends/megatron/core/extensions/primus_turbo.py:1180-1188) ----
+ *   y = act(z) + residual,  z = a . b^T + bias         a [m, k], b [n, k], y, z, residual [m, n] bf16
+ * fp32 from the products to y, which is rounded once; bias (bf16 or float, NULL: none), residual (NULL: none); act MXL_ACT_*.
+ * z_bf16: if not NULL, z rounded to bf16 for the backward.  n and k multiples of 32, n * k * 2 < 2^32, pointers 16-byte aligned.
+ *
+ * Backward: mxl_linear_bf16_dz gives dz = dy * act'(z) (not written, and may be dy itself, for MXL_ACT_NONE) and
+ * dbias = column sums of dz before its rounding (NULL: not wanted); mxl_linear_bf16_dgrad gives da = dz . b;
+ * db = dz^T . a is mxl_grouped_gemm_bf16_wgrad with one group. */
+int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const void* bias, int bias_dtype, int act, const void* residual_bf16, int64_t m,
+                    int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* stream);
+int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* stream);
+int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n);
+int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int act, int64_t m, int64_t n, void* dz_bf16, void* dbias, int dbias_dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- calibration (no counterpart in the reference: a measuring aid of this library's benchmark) ----
  *

@@ -25,7 +25,7 @@ BLOCK = 32
 SEG_ALIGN = 128
 GEMM_K_ALIGN = 128  # the GEMM kernels take the contraction dim in multiples of this
 MAX_GROUPS = 1024
-ACT_SILU, ACT_GELU = 0, 1
+ACT_SILU, ACT_GELU, ACT_RELU, ACT_NONE = 0, 1, 2, 3
 PROBS_F32, PROBS_BF16 = 0, 1
 QF_SR, QF_RHT_COL, QF_KCHUNK, QF_KSTEP, QF_KSTEP128 = 1, 2, 4, 8, 16   # flags of mxl_quantize_ex
 GF_KCHUNK = 1                               # flag of the GEMM _ex entry points: operands are K-chunk-major
@@ -93,6 +93,10 @@ EXPORTS = (
     "mxl_permute_rows",
     "mxl_combine_rows",
     "mxl_combine_rows_bwd",
+    "mxl_linear_bf16",
+    "mxl_linear_bf16_dgrad",
+    "mxl_linear_bf16_dz_workspace_bytes",
+    "mxl_linear_bf16_dz",
     "mxl_calibrate_mfma",
     "mxl_calibrate_mfma_flops",
     "mxl_calibrate_mfma_bf16",
@@ -263,6 +267,14 @@ def load() -> ctypes.CDLL:
         lib.mxl_combine_rows.argtypes = [vp, i64, i32, i32, vp, i64, i32, vp, vp, vp, i32, vp, vp]
         lib.mxl_combine_rows_bwd.restype = i32
         lib.mxl_combine_rows_bwd.argtypes = [vp, vp, i64, i32, i32, vp, vp, i64, i32, vp, i32, vp, vp, vp]
+        lib.mxl_linear_bf16.restype = i32
+        lib.mxl_linear_bf16.argtypes = [vp, vp, vp, i32, i32, vp, i64, i64, i64, vp, vp, vp]
+        lib.mxl_linear_bf16_dgrad.restype = i32
+        lib.mxl_linear_bf16_dgrad.argtypes = [vp, vp, i64, i64, i64, vp, vp]
+        lib.mxl_linear_bf16_dz_workspace_bytes.restype = i64
+        lib.mxl_linear_bf16_dz_workspace_bytes.argtypes = [i64, i64]
+        lib.mxl_linear_bf16_dz.restype = i32
+        lib.mxl_linear_bf16_dz.argtypes = [vp, vp, i32, i64, i64, vp, vp, i32, vp, i64, vp]
         _lib = lib
     return _lib
 

@@ -1,0 +1,466 @@
+// Dense bf16 linear with bias, activation and residual in its epilogue, and its backward: the unquantised linears of a
+// transformer (primus/backends/megatron/core/extensions/primus_turbo.py:1180-1188 is the route without a recipe), whose bias, activation
+// and residual are passes of their own over the output otherwise.
+//
+//   y = act(z) + residual,  z = a . b^T + bias     a [m, k], b [n, k];  fp32 from the products to y, one rounding
+//   backward: dz = dy act'(z),  da = dz . b,  db = dz^T . a,  dbias = column sums of dz
+//
+// The weight gradient, and the products of many rows, run on the grouped kernels' tiles (mx_gemm_bf16.hip) with one group.  This
+// file holds the tiles of 128 x 128 and 64 x 64 for fewer rows, the kernel for a few rows, which is bound by reading b, and
+// the elementwise part of the backward.
+#include "mx_epilogue.h"
+#include "mx_gemm_common.h"
+
+namespace mxl {
+
+typedef __bf16 d8bf __attribute__((ext_vector_type(8)));
+typedef short d4s __attribute__((ext_vector_type(4)));
+
+struct DenseArgs {
+    const uint8_t* a;       // [m, k]
+    const uint8_t* b;       // [n, k], or [k, n] (B_T)
+    uint16_t* c;            // [m, n]
+    int64_t m, n, k;
+    EpilogueArgs epi;
+};
+
+constexpr int DT_KS = 64;       // contraction elements per slot: 128 bytes of a row, four MFMA steps
+
+template <int TM, int TN, int ST> constexpr int dense_lds_bytes() {
+    const int loop = ST * (TM + TN) * DT_KS * 2, out = TM * (TN * 2 + 16);
+    return loop > out ? loop : out;
+}
+
+// ---- tiles: 4 waves (2 x 2), LDS-direct loads into ST stages, one workgroup per tile, two or three of them on a CU so that one's
+// epilogue and waits run under another's MFMAs.  B_T: b is [k, n], read with the transposing LDS read. ----
+template <int TM, int TN, int ST, bool B_T, int ACT>
+__global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
+    constexpr int FM = TM / 64, FN = TN / 64;              // 32 x 32 fragments per wave
+    constexpr int AR = TM / 32, BR = TN / 32, R = AR + BR;  // load rounds of 4 KiB
+    constexpr int A_BYTES = TM * DT_KS * 2, STAGE = A_BYTES + TN * DT_KS * 2;
+    constexpr int BT_PIECES = TN / 8;                       // 16-byte pieces of a staged row of the transposed operand
+    constexpr int BT_SHIFT = TN == 128 ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int t = threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int l = t & 63, lr = l & 31, g = l >> 5;
+    const int wm = w >> 1, wn = w & 1;
+
+    // the tile: each XCD takes one contiguous run of the order, super-rows of 1024 rows
+    const int tiles_m = (int)((p.m + TM - 1) / TM), tiles_n = (int)((p.n + TN - 1) / TN);
+    const int total = tiles_m * tiles_n, per_xcd = (total + 7) >> 3;
+    const int in_xcd = (int)(blockIdx.x >> 3), tile = (int)(blockIdx.x & 7) * per_xcd + in_xcd;
+    if (in_xcd >= per_xcd || tile >= total) return;
+    int pid_m, pid_n;
+    {
+        constexpr int SUPER = 1024 / TM;
+        const int width = SUPER * tiles_n, first = tile / width * SUPER;
+        const int gsz = (tiles_m - first) < SUPER ? (tiles_m - first) : SUPER;
+        pid_m = first + (tile % width) % gsz;
+        pid_n = (tile % width) / gsz;
+    }
+    const int64_t m0 = (int64_t)pid_m * TM, n0 = (int64_t)pid_n * TN;
+    const int m_valid = (int)((p.m - m0) < TM ? p.m - m0 : TM), n_valid = (int)((p.n - n0) < TN ? p.n - n0 : TN);
+    const int slots = (int)((p.k + DT_KS - 1) / DT_KS);
+    const bool odd = (p.k & 32) != 0;       // the last slot's second half is past the contraction: not multiplied
+
+    const int64_t lda = p.k * 2, ldb = B_T ? p.n * 2 : p.k * 2;
+    // the descriptors end with the operands; what is requested past them arrives as zeros
+    const v4i ra = make_rsrc(p.a + m0 * lda, (p.m - m0) * lda);
+    const v4i rb = B_T ? make_rsrc(p.b + n0 * 2, p.k * ldb - n0 * 2) : make_rsrc(p.b + n0 * ldb, (p.n - n0) * ldb);
+    const uint32_t a_step = DT_KS * 2, b_step = (uint32_t)__builtin_amdgcn_readfirstlane(B_T ? (int)(DT_KS * ldb) : DT_KS * 2);
+    uint32_t va[AR], vb[BR];
+#pragma unroll
+    for (int e = 0; e < AR; ++e) {
+        const int row = (t >> 3) + 32 * e;
+        va[e] = (uint32_t)(row * lda + 16 * ((t & 7) ^ ((row >> 1) & 7)));
+    }
+#pragma unroll
+    for (int e = 0; e < BR; ++e) {
+        if constexpr (B_T) {
+            const int row = t / BT_PIECES + (256 / BT_PIECES) * e;
+            vb[e] = (uint32_t)(row * ldb + 16 * ((t % BT_PIECES) ^ ((row & 3) << BT_SHIFT)));
+        } else {
+            const int row = (t >> 3) + 32 * e;
+            vb[e] = (uint32_t)(row * ldb + 16 * ((t & 7) ^ ((row >> 1) & 7)));
+        }
+    }
+    const uint32_t wave_base = (uint32_t)(uintptr_t)smem + (uint32_t)(w * 1024);
+    auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+        const uint32_t base = wave_base + (uint32_t)(stage * STAGE);
+        const bool live = s < slots;        // past the range the requests are dropped, but counted
+        const uint32_t sa = live ? (uint32_t)s * a_step : addr::kDropped, sb = live ? (uint32_t)s * b_step : addr::kDropped;
+        static_for<0, AR>([&](auto e) { dma16_at<decltype(e)::value * 4096>(ra, base, va[decltype(e)::value], sa); });
+        static_for<0, BR>([&](auto e) { dma16_at<A_BYTES + decltype(e)::value * 4096>(rb, base, vb[decltype(e)::value], sb); });
+    };
+
+    // fragment reads: contiguous, row lr, piece 2 ks + g XOR (row / 2) % 8; transposed, this lane addresses row tj of a 4-row
+    // group, 8-byte piece ta4 of its 16-lane block's 16 columns
+    const int lane_c = lr * 128 + 16 * (g ^ ((lr >> 1) & 7));
+    const int tj = (l & 15) >> 2, ta4 = l & 3, tblk = (l >> 4) & 1;
+    auto read_a = [&](uint8_t* st, int i, int ks) __attribute__((always_inline)) {
+        return *(const d8bf*)(st + ((lane_c + wm * (TM / 2) * 128) ^ (32 * ks)) + i * 4096);
+    };
+    auto read_b = [&](uint8_t* st, int j, int ks) __attribute__((always_inline)) {
+        if constexpr (!B_T) {
+            return *(const d8bf*)(st + A_BYTES + ((lane_c + wn * (TN / 2) * 128) ^ (32 * ks)) + j * 4096);
+        } else {
+            d8bf out;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = 16 * ks + 8 * g + 4 * h + tj, byte = 2 * (wn * (TN / 2) + 32 * j) + 32 * tblk + 8 * ta4;
+                uint8_t* ptr = st + A_BYTES + row * (TN * 2) + 16 * ((byte >> 4) ^ ((row & 3) << BT_SHIFT)) + (byte & 15);
+                const d4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) d4s*)ptr);
+                const v4bf q = __builtin_bit_cast(v4bf, v);
+                out[4 * h] = q[0]; out[4 * h + 1] = q[1]; out[4 * h + 2] = q[2]; out[4 * h + 3] = q[3];
+            }
+            return out;
+        }
+    };
+
+    v16f acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    const bool live = __builtin_amdgcn_readfirstlane(wm * (TM / 2) < m_valid);
+
+    for (int s = 0; s < ST - 1; ++s) issue(s, s);
+    int stage = 0;
+    for (int s = 0; s < slots; ++s) {
+        wait_vm<(ST - 2) * R>();        // slot s has landed
+        __syncthreads();                // ... for every wave, and every wave has left the stage of slot s - 1
+        issue(s + ST - 1, stage == 0 ? ST - 1 : stage - 1);
+        uint8_t* st = smem + stage * STAGE;
+        stage = stage == ST - 1 ? 0 : stage + 1;
+        if (!live) continue;
+        const int steps = odd && s == slots - 1 ? 2 : 4;
+        auto step = [&](int ks) __attribute__((always_inline)) {
+            d8bf fa[FM], fb[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = read_b(st, j, ks);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = read_a(st, i, ks);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        };
+        step(0);
+        step(1);
+        if (steps == 4) {
+            step(2);
+            step(3);
+        }
+    }
+    wait_vm<0>();
+    __syncthreads();                    // nothing reads or writes the stages any more
+
+    // ---- epilogue.  Lane (lr, g) of fragment (i, j) holds row 32 i + lr, columns 32 j + 8 q + 4 g .. + 3 in registers 4 q .. + 3.  The
+    // tile passes through LDS as bf16 in rows of 16-byte pieces: z on its way out, the residual on its way in (each lane then
+    // finds its own four columns' values where it puts its results), y on its way out. ----
+    constexpr int PITCH = TN * 2 + 16, LPR = TN / 8, RPI = 256 / LPR;
+    const int rr = t / LPR, cc = (t % LPR) * 8;
+    const int64_t c0 = m0 * p.n + n0;
+    auto spot = [&](int i, int j, int q) __attribute__((always_inline)) {
+        return (uint2*)(smem + (wm * (TM / 2) + i * 32 + lr) * PITCH + (wn * (TN / 2) + j * 32 + 8 * q + 4 * g) * 2);
+    };
+    auto leave = [&](uint16_t* out) __attribute__((always_inline)) {
+        if (cc < n_valid) {
+#pragma unroll
+            for (int u = 0; u < TM / RPI; ++u) {
+                const int row = u * RPI + rr;
+                if (row < m_valid) store16_streaming((uint8_t*)(out + c0 + (int64_t)row * p.n + cc), *(const uint4*)(smem + row * PITCH + cc * 2));
+            }
+        }
+    };
+    if (p.epi.bias) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = wn * (TN / 2) + j * 32 + 8 * q + 4 * g;
+                if (col < n_valid) {        // n is a multiple of 32: four columns are in or out together
+                    const v4f b4 = epi_bias4(p.epi, n0 + col);
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += b4[e];
+                }
+            }
+    }
+    auto quad = [&](int i, int j, int q) __attribute__((always_inline)) {
+        return v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    };
+    if (p.epi.z) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) *spot(i, j, q) = pack4(quad(i, j, q));
+        __syncthreads();
+        leave(p.epi.z);
+        __syncthreads();
+    }
+    if (p.epi.residual) {
+        if (cc < n_valid) {
+#pragma unroll
+            for (int u = 0; u < TM / RPI; ++u) {
+                const int row = u * RPI + rr;
+                if (row < m_valid) *(uint4*)(smem + row * PITCH + cc * 2) = load16_streaming(p.epi.residual + c0 + (int64_t)row * p.n + cc);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v4f y = quad(i, j, q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = epi_act<ACT>(y[e]);
+                if (p.epi.residual) {
+                    const v4f r = unpack4(*spot(i, j, q));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] += r[e];
+                }
+                *spot(i, j, q) = pack4(y);
+            }
+    __syncthreads();
+    leave(p.c);
+}
+
+// ---- a few rows: bound by reading b once.  A workgroup has 16 columns; its 8 waves split the contraction, load b's fragments straight
+// into registers (16 rows of 64 bytes per request, SKINNY_AHEAD requests on their way) and join their sums through LDS. ----
+constexpr int SK_WAVES = 8, SK_AHEAD = 8;
+
+template <int MT, int ACT>
+__global__ __launch_bounds__(SK_WAVES * 64) void dense_few_rows_kernel(DenseArgs p) {
+    __shared__ v4f part[SK_WAVES][MT][64];
+    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63;
+    const int row = l & 15, q = l >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int steps = (int)(p.k / 32), per = (steps + SK_WAVES - 1) / SK_WAVES;
+    const int s0 = w * per, s1 = s0 + per < steps ? s0 + per : steps;
+    const uint8_t* b = p.b + (n0 + row) * p.k * 2 + q * 16;        // n is a multiple of 32: the row exists
+    const uint8_t* a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t r = 16 * i + row < p.m ? 16 * i + row : p.m - 1;      // (a row past the end is some other row's copy, not stored)
+        a[i] = p.a + r * p.k * 2 + q * 16;
+    }
+    v4f acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    int s = s0;
+    for (; s + SK_AHEAD <= s1; s += SK_AHEAD) {
+        d8bf fb[SK_AHEAD];
+#pragma unroll
+        for (int u = 0; u < SK_AHEAD; ++u) fb[u] = __builtin_nontemporal_load((const d8bf*)(b + (int64_t)(s + u) * 64));
+#pragma unroll
+        for (int u = 0; u < SK_AHEAD; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u], *(const d8bf*)(a[i] + (int64_t)(s + u) * 64), acc[i], 0, 0, 0);
+    }
+    for (; s < s1; ++s) {
+        const d8bf fb = *(const d8bf*)(b + (int64_t)s * 64);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, *(const d8bf*)(a[i] + (int64_t)s * 64), acc[i], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[w][i][l] = acc[i];
+    __syncthreads();
+    // lane (row of a = l % 16, columns 4 (l / 16) .. + 3)
+    for (int x = t; x < MT * 64; x += SK_WAVES * 64) {
+        const int i = x >> 6, ll = x & 63;
+        const int64_t r = 16 * i + (ll & 15), col = n0 + 4 * (ll >> 4);
+        v4f z = part[0][i][ll];
+#pragma unroll
+        for (int k = 1; k < SK_WAVES; ++k) z += part[k][i][ll];
+        if (r >= p.m) continue;
+        z += epi_bias4(p.epi, col);
+        if (p.epi.z) *(uint2*)(p.epi.z + r * p.n + col) = pack4(z);
+        v4f y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = epi_act<ACT>(z[e]);
+        if (p.epi.residual) y += unpack4(*(const uint2*)(p.epi.residual + r * p.n + col));
+        *(uint2*)(p.c + r * p.n + col) = pack4(y);
+    }
+}
+
+// ---- the elementwise part of the backward: dz = dy act'(z) (not written without an activation) and column sums of dz.
+// A workgroup has 256 columns (8 a lane) and a run of rows, 8 at a time; its sums go to partial[run][n], which a second launch
+// adds up in order. ----
+struct DzArgs {
+    const uint16_t* dy;
+    const uint16_t* z;
+    uint16_t* dz;
+    float* partial;         // null: no sums wanted
+    int64_t m, n, run;      // rows per workgroup
+};
+template <int ACT>
+__global__ __launch_bounds__(256) void dense_dz_kernel(DzArgs p) {
+    __shared__ float sums[8][32][9];
+    const int lane = threadIdx.x & 31, r8 = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 256 + lane * 8;
+    const int64_t lo = (int64_t)blockIdx.y * p.run, hi = lo + p.run < p.m ? lo + p.run : p.m;
+    float acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    if (col < p.n) {
+        for (int64_t r = lo + r8; r < hi; r += 8) {
+            const uint4 d = ACT == kActNone ? *(const uint4*)(p.dy + r * p.n + col) : load16_streaming(p.dy + r * p.n + col);
+            const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[2 * e] = bf16_lo(dw[e]), x[2 * e + 1] = bf16_hi(dw[e]);
+            if constexpr (ACT != kActNone) {
+                const uint4 zz = load16_streaming(p.z + r * p.n + col);
+                const uint32_t zw[4] = {zz.x, zz.y, zz.z, zz.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[2 * e] *= epi_slope<ACT>(bf16_lo(zw[e]));
+                    x[2 * e + 1] *= epi_slope<ACT>(bf16_hi(zw[e]));
+                }
+                *(uint4*)(p.dz + r * p.n + col) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += x[e];
+        }
+    }
+    if (!p.partial) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[r8][lane][e] = acc[e];
+    __syncthreads();
+    const int c = threadIdx.x;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += sums[i][c >> 3][c & 7];
+    if ((int64_t)blockIdx.x * 256 + c < p.n) p.partial[(int64_t)blockIdx.y * p.n + (int64_t)blockIdx.x * 256 + c] = s;
+}
+
+// dbias[n] = sum of the runs: 64 columns by 4 groups of runs
+__global__ __launch_bounds__(256) void dense_dbias_kernel(const float* partial, int runs, int64_t n, void* dbias, int f32) {
+    __shared__ float part[4][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (col < n)
+        for (int r = w; r < runs; r += 4) s += partial[(int64_t)r * n + col];
+    part[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && col < n) {
+        s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        if (f32) ((float*)dbias)[col] = s;
+        else ((__bf16*)dbias)[col] = (__bf16)s;
+    }
+}
+
+// rows per workgroup of dense_dz_kernel: about 2048 workgroups, a multiple of 8 rows
+static int64_t dz_run(int64_t m, int64_t n) {
+    const int64_t cols = (n + 255) / 256;
+    int64_t runs = 2048 / cols;
+    if (runs < 1) runs = 1;
+    int64_t run = (m + runs - 1) / runs;
+    return (run + 7) / 8 * 8 < 8 ? 8 : (run + 7) / 8 * 8;
+}
+
+template <int TM, int TN, int ST, bool B_T, int ACT>
+static int launch_dense_tile(const DenseArgs& a, hipStream_t st) {
+    constexpr int lds = dense_lds_bytes<TM, TN, ST>();
+    static std::atomic<bool> attr_set[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return MXL_ELAUNCH;
+    auto kern = dense_tile_kernel<TM, TN, ST, B_T, ACT>;
+    if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
+        if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return MXL_ELAUNCH;
+        attr_set[dev & 63].store(true, std::memory_order_release);
+    }
+    const int64_t tiles = ((a.m + TM - 1) / TM) * ((a.n + TN - 1) / TN), grid = (tiles + 7) / 8 * 8;
+    if (grid > 0x7FFFFFFF) return MXL_EINVAL;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, st, a);
+    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+}
+
+template <int ACT>
+static int launch_dense_forward(const DenseArgs& a, hipStream_t st) {
+    const dim3 few((unsigned)(a.n / 16)), threads(SK_WAVES * 64);
+    if (a.m <= 16) hipLaunchKernelGGL((dense_few_rows_kernel<1, ACT>), few, threads, 0, st, a);
+    else if (a.m <= 32) hipLaunchKernelGGL((dense_few_rows_kernel<2, ACT>), few, threads, 0, st, a);
+    else if (a.m <= 64) hipLaunchKernelGGL((dense_few_rows_kernel<4, ACT>), few, threads, 0, st, a);
+    else if (((a.m + 127) / 128) * ((a.n + 127) / 128) >= 256) return launch_dense_tile<128, 128, 2, false, ACT>(a, st);
+    else return launch_dense_tile<64, 64, 3, false, ACT>(a, st);
+    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+}
+
+static bool dense_sizes_ok(int64_t m, int64_t n, int64_t k) {
+    return m >= 0 && m <= 0x7FFFFFFF && n > 0 && n % 32 == 0 && k > 0 && k % 32 == 0 && n <= (1 << 22) && k <= (1 << 22) && n * k * 2 < ((int64_t)1 << 32);
+}
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace mxl
+
+using namespace mxl;
+
+extern "C" int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const void* bias, int bias_dtype, int act, const void* residual_bf16, int64_t m,
+                               int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* stream) {
+    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (bias_dtype != MXL_DT_F32 && bias_dtype != MXL_DT_BF16)) return MXL_EINVAL;
+    if (m == 0) return MXL_OK;
+    if (!a_bf16 || !b_bf16 || !y_bf16) return MXL_EINVAL;
+    if (!aligned16(a_bf16) || !aligned16(b_bf16) || !aligned16(bias) || !aligned16(residual_bf16) || !aligned16(y_bf16) || !aligned16(z_bf16)) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    DenseArgs d{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, (uint16_t*)y_bf16, m, n, k, {bias, (const uint16_t*)residual_bf16, (uint16_t*)z_bf16, bias_dtype == MXL_DT_F32}};
+    hipStream_t st = (hipStream_t)stream;
+    switch (act) {
+        case MXL_ACT_SILU: return launch_dense_forward<kActSilu>(d, st);
+        case MXL_ACT_GELU: return launch_dense_forward<kActGelu>(d, st);
+        case MXL_ACT_RELU: return launch_dense_forward<kActRelu>(d, st);
+        default: return launch_dense_forward<kActNone>(d, st);
+    }
+}
+
+extern "C" int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* stream) {
+    if (!dense_sizes_ok(m, n, k)) return MXL_EINVAL;
+    if (m == 0) return MXL_OK;
+    if (!dz_bf16 || !b_bf16 || !da_bf16 || !aligned16(dz_bf16) || !aligned16(b_bf16) || !aligned16(da_bf16)) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    // da [m, k] = dz [m, n] . b [n, k]: the contraction is over n, b's slow dim
+    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)b_bf16, (uint16_t*)da_bf16, m, k, n, {nullptr, nullptr, nullptr, 0}};
+    hipStream_t st = (hipStream_t)stream;
+    if (((m + 127) / 128) * ((k + 127) / 128) >= 256) return launch_dense_tile<128, 128, 2, true, kActNone>(d, st);
+    return launch_dense_tile<64, 64, 3, true, kActNone>(d, st);
+}
+
+extern "C" int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n) {
+    if (m < 0 || n <= 0) return -1;
+    const int64_t run = dz_run(m, n);
+    return (m + run - 1) / run * n * 4;
+}
+
+extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int act, int64_t m, int64_t n, void* dz_bf16, void* dbias, int dbias_dtype,
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!dense_sizes_ok(m, n, 32) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (dbias_dtype != MXL_DT_F32 && dbias_dtype != MXL_DT_BF16)) return MXL_EINVAL;
+    if (m > 0 && (!dy_bf16 || (act != MXL_ACT_NONE && (!z_bf16 || !dz_bf16)))) return MXL_EINVAL;
+    if (!aligned16(dy_bf16) || !aligned16(z_bf16) || !aligned16(dz_bf16) || !aligned16(workspace)) return MXL_EINVAL;
+    if (dbias && (workspace_bytes < mxl_linear_bf16_dz_workspace_bytes(m, n) || (m > 0 && !workspace))) return MXL_EINVAL;
+    if (!dbias && (act == MXL_ACT_NONE || m == 0)) return MXL_OK;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t run = dz_run(m, n), runs = (m + run - 1) / run;
+    DzArgs d{(const uint16_t*)dy_bf16, (const uint16_t*)z_bf16, (uint16_t*)dz_bf16, dbias ? (float*)workspace : nullptr, m, n, run};
+    const dim3 grid((unsigned)((n + 255) / 256), (unsigned)runs);
+    if (m > 0) {
+        if (act == MXL_ACT_SILU) hipLaunchKernelGGL(dense_dz_kernel<kActSilu>, grid, dim3(256), 0, st, d);
+        else if (act == MXL_ACT_GELU) hipLaunchKernelGGL(dense_dz_kernel<kActGelu>, grid, dim3(256), 0, st, d);
+        else if (act == MXL_ACT_RELU) hipLaunchKernelGGL(dense_dz_kernel<kActRelu>, grid, dim3(256), 0, st, d);
+        else hipLaunchKernelGGL(dense_dz_kernel<kActNone>, grid, dim3(256), 0, st, d);
+    }
+    if (dbias) hipLaunchKernelGGL(dense_dbias_kernel, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, (const float*)workspace, (int)runs, n, dbias, dbias_dtype == MXL_DT_F32);
+    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+}

@@ -1423,6 +1423,112 @@ def combine_rows_bwd_impl(dy, rows, row_of, entry_of, probs, need_rows: bool = T
 
 
 # --------------------------------------------------------------------------
+# the dense bf16 linear with its epilogue
+# --------------------------------------------------------------------------
+_LINEAR_ACTS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
+
+
+def _linear_args(m: int, n: int, k: int, activation):
+    if activation not in _LINEAR_ACTS:
+        raise ValueError(f"activation must be None, 'silu', 'gelu' or 'relu', got {activation!r}")
+    if n < 1 or k < 1 or n % 32 != 0 or k % 32 != 0 or n > 1 << 22 or k > 1 << 22:
+        raise ValueError("the dense bf16 linear needs n and k in multiples of 32 (forward and dgrad contract over them), at most 2^22")
+    if n * k >= 1 << 31:
+        raise ValueError("the weight must be smaller than 4 GiB")
+    if m > 0x7FFFFFFF:
+        raise ValueError("at most 2^31 - 1 rows")
+    return _LINEAR_ACTS[activation]
+
+
+def _bf16_2d(t, what, shape=None):
+    if t.dtype != torch.bfloat16 or t.dim() != 2:
+        raise ValueError(f"{what} must be a 2-D bfloat16 tensor")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must have shape {list(shape)}")
+
+
+def linear_bf16_impl(a, b, bias=None, activation: Optional[str] = None, residual=None, want_z: bool = False):
+    """``(act(a . b^T + bias) + residual, z)`` for bf16 ``a [m, k]``, ``b [n, k]``, ``residual [m, n]`` and a bf16 or float32 ``bias
+    [n]``; ``z`` = the activation's input rounded to bf16, None unless wanted."""
+    _bf16_2d(a, "a")
+    _bf16_2d(b, "b")
+    m, k = a.shape
+    n = b.shape[0]
+    if b.shape[1] != k:
+        raise ValueError("contraction lengths of a and b differ")
+    act = _linear_args(m, n, k, activation)
+    if bias is not None and (bias.dtype not in (torch.bfloat16, torch.float32) or tuple(bias.shape) != (n,)):
+        raise ValueError("bias must be bfloat16 or float32 [n]")
+    if residual is not None:
+        _bf16_2d(residual, "residual", (m, n))
+    _require_cuda(a, b, bias, residual)
+    _same_device(a.device, b=b, bias=bias, residual=residual)
+    with _on(a.device), _hooked("linear_bf16", m=m, n=n, k=k):
+        y = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
+        z = torch.empty_like(y) if want_z else None
+        rc = _lib.load().mxl_linear_bf16(_ptr(a), _ptr(b), _ptr(bias), _lib.DT_BF16 if bias is None else _DT[bias.dtype], act, _ptr(residual), m, n, k,
+                                         _ptr(y), _ptr(z), _stream())
+    _lib.check(rc, "mxl_linear_bf16")
+    return y, z
+
+
+def linear_bf16_dz_impl(dy, z, activation: Optional[str], bias_dtype: Optional[torch.dtype] = None):
+    """``(dz, dbias)``: ``dz = dy * act'(z)`` (``dy`` itself without an activation) and its column sums in ``bias_dtype`` (None: not wanted)."""
+    _bf16_2d(dy, "dy")
+    m, n = dy.shape
+    act = _linear_args(m, n, 32, activation)
+    if act != _lib.ACT_NONE:
+        _bf16_2d(z, "z", (m, n))
+    _require_cuda(dy, z)
+    lib = _lib.load()
+    with _on(dy.device), _hooked("linear_bf16_dz", m=m, n=n):
+        dz = torch.empty_like(dy) if act != _lib.ACT_NONE else dy
+        dbias = ws = None
+        if bias_dtype is not None:
+            dbias = torch.empty((n,), dtype=bias_dtype, device=dy.device)
+            ws = torch.empty((max(int(lib.mxl_linear_bf16_dz_workspace_bytes(m, n)), 16),), dtype=torch.uint8, device=dy.device)
+        rc = lib.mxl_linear_bf16_dz(_ptr(dy), None if act == _lib.ACT_NONE else _ptr(z), act, m, n, None if act == _lib.ACT_NONE else _ptr(dz), _ptr(dbias),
+                                    _lib.DT_BF16 if bias_dtype is None else _DT[bias_dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream())
+    _lib.check(rc, "mxl_linear_bf16_dz")
+    return dz, dbias
+
+
+def linear_bf16_dgrad_impl(dz, b) -> torch.Tensor:
+    """``dz . b`` for bf16 ``dz [m, n]``, ``b [n, k]``."""
+    _bf16_2d(dz, "dz")
+    _bf16_2d(b, "b")
+    m, n = dz.shape
+    k = b.shape[1]
+    if b.shape[0] != n:
+        raise ValueError("contraction lengths of dz and b differ")
+    _linear_args(m, n, k, None)
+    _require_cuda(dz, b)
+    _same_device(dz.device, b=b)
+    with _on(dz.device), _hooked("linear_bf16_dgrad", m=m, n=n, k=k):
+        da = torch.empty((m, k), dtype=torch.bfloat16, device=dz.device)
+        rc = _lib.load().mxl_linear_bf16_dgrad(_ptr(dz), _ptr(b), m, n, k, _ptr(da), _stream())
+    _lib.check(rc, "mxl_linear_bf16_dgrad")
+    return da
+
+
+def linear_bf16_wgrad_impl(dz, a, accum_into: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dz^T . a`` for bf16 ``dz [m, n]``, ``a [m, k]``, or added to the float32 ``accum_into``.  The grouped kernel, whose operands end
+    below 4 GiB: longer ones go through it in runs of rows whose products meet in float32."""
+    _bf16_2d(dz, "dz")
+    _bf16_2d(a, "a")
+    m, n = dz.shape
+    k = a.shape[1]
+    rows = ((1 << 32) - 1) // (2 * max(n, k)) // 64 * 64
+    with _on(dz.device):
+        if m <= rows:
+            return grouped_gemm_bf16_wgrad_impl(dz, a, None, accum_into=accum_into)
+        total = accum_into if accum_into is not None else torch.zeros((1, n, k), dtype=torch.float32, device=dz.device)
+        for lo in range(0, m, rows):
+            grouped_gemm_bf16_wgrad_impl(dz[lo:lo + rows], a[lo:lo + rows], None, accum_into=total)
+        return total if accum_into is not None else total.to(torch.bfloat16)
+
+
+# --------------------------------------------------------------------------
 # the 128-blockwise FP8 recipe
 # --------------------------------------------------------------------------
 BW_BLOCK = 128

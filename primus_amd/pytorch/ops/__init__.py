@@ -41,7 +41,7 @@ __all__ = ["gemm", "grouped_gemm", "gemm_fp8", "gemm_fp4", "grouped_gemm_fp8", "
            "set_dgrad_reads_rowwise_weight",
            "swiglu_with_probs", "geglu_with_probs", "tokens_per_expert_to_mask", "glu_grouped_gemm_fp8",
            "glu_grouped_gemm_fp4", "manual_sr_seed", "set_kchunk_layout", "rmsnorm", "rmsnorm_gemm_fp8", "rmsnorm_gemm_fp4", "pad_groups", "unpad_groups",
-           "topk_routing", "permute_tokens", "unpermute_tokens", "TokenPermutation"]
+           "topk_routing", "permute_tokens", "unpermute_tokens", "TokenPermutation", "gemm_bias_act"]
 
 # dgrad and wgrad of one linear are independent once dY is quantised, so wgrad may run on a second stream, where its
 # workgroups move in as dgrad's last, partial round of tiles drains.  The default is one stream: _overlaps() names the
@@ -967,6 +967,59 @@ def gemm(a, b, trans_a: bool = False, trans_b: bool = True, out_dtype: Optional[
     return out if out_dtype is None else out.to(out_dtype)
 
 
+class _GemmBiasAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, b, bias, residual, activation, accum, need_grad=True):
+        want_z = need_grad and activation is not None and any(ctx.needs_input_grad[:3])
+        y, z = K.linear_bf16_impl(a, b, bias, activation, residual, want_z)
+        if need_grad:
+            ctx.save_for_backward(a, b, z)
+            ctx.activation, ctx.accum, ctx.bias_dtype = activation, accum, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        a, b, z = ctx.saved_tensors
+        need_a, need_b, need_bias, need_residual = ctx.needs_input_grad[:4]
+        dy = _aligned(dy.contiguous() if dy.dtype == torch.bfloat16 else dy.to(torch.bfloat16).contiguous())
+        da = db = dbias = None
+        if need_a or need_b or need_bias:
+            dz, dbias = K.linear_bf16_dz_impl(dy, z, ctx.activation, ctx.bias_dtype if need_bias else None)
+        if need_a:
+            da = K.linear_bf16_dgrad_impl(dz, b)
+        if need_b:
+            fused = ctx.accum is not None and _fusable(ctx.accum[0])
+            gb = K.linear_bf16_wgrad_impl(dz, a, accum_into=ctx.accum[0] if fused else None)
+            db = _finish_wgrad(None if fused else gb, ctx.accum, fused, tuple(b.shape))
+        return da, db, dbias, dy if need_residual else None, None, None, None
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy of it where its storage starts between two 16-byte boundaries."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                  residual: Optional[torch.Tensor] = None, fuse_bgrad_accum_pattern: Optional[str] = None) -> torch.Tensor:
+    """``act(a @ b^T + bias) + residual``: ``gemm`` on bf16 operands with what follows it in its epilogue, computed in fp32 and rounded
+    once.  ``a [..., k]``, ``b [n, k]``, ``bias [n]`` (bfloat16 or float32), ``activation`` None, ``"silu"``, ``"gelu"`` (erf) or ``"relu"``,
+    ``residual [..., n]``.  ``n`` and ``k`` in multiples of 32, the weight below 4 GiB (anything else raises).  Differentiable in the four
+    tensors; the activation's input is kept in bf16 for the backward, whose gradients are those of that rounded value.
+    ``fuse_bgrad_accum_pattern="megatron"`` adds the weight gradient into ``b.main_grad``, as ``gemm`` does."""
+    accum = _accum_from(b, fuse_bgrad_accum_pattern)
+    if a.dim() < 2 or b.dim() != 2:
+        raise ValueError("a must be [..., k] and b [n, k]")
+    shape = a.shape[:-1] + (b.shape[0],)
+    if residual is not None:
+        if residual.shape != shape:
+            raise ValueError(f"residual must have shape {list(shape)}")
+        residual = _aligned(residual.reshape(-1, shape[-1]).contiguous())
+    y = _apply(_GemmBiasAct, _aligned(a.reshape(-1, a.shape[-1]).contiguous()), _aligned(b.contiguous()), None if bias is None else _aligned(bias.contiguous()),
+               residual, activation, accum)
+    return y.view(shape)
+
+
 class _GroupedLinearLibrary(torch.autograd.Function):
     """The same operator for operands the bf16 kernels do not take -- float32 / float16, or tensors in host memory, as
     the host-side module tests use them: a loop of the library GEMM behind ``torch.matmul`` per expert, which reads
@@ -1122,12 +1175,13 @@ def unpad_groups(y: torch.Tensor, group_lens: torch.Tensor, align: int, rows: in
 # ---------------------------------------------------------------------------
 class _TopkRouting(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, topk, score_function, expert_bias, num_groups, group_topk, renormalize, scaling_factor, token_mask):
+    def forward(ctx, logits, topk, score_function, expert_bias, num_groups, group_topk, renormalize, scaling_factor, token_mask, need_grad=True):
         probs, indices, counts = K.topk_routing_impl(logits, topk, score_function, expert_bias, num_groups, group_topk, renormalize,
                                                      scaling_factor, token_mask)
-        ctx.save_for_backward(logits, indices)
-        ctx.how = (score_function, renormalize, scaling_factor)
-        ctx.mark_non_differentiable(indices, counts)
+        if need_grad:
+            ctx.save_for_backward(logits, indices)
+            ctx.how = (score_function, renormalize, scaling_factor)
+            ctx.mark_non_differentiable(indices, counts)
         return probs, indices, counts
 
     @staticmethod
@@ -1135,7 +1189,7 @@ class _TopkRouting(torch.autograd.Function):
     def backward(ctx, dprobs, _, __):
         logits, indices = ctx.saved_tensors
         dlogits = K.topk_routing_bwd_impl(dprobs.to(torch.float32).contiguous(), logits, indices, *ctx.how)
-        return dlogits, None, None, None, None, None, None, None, None
+        return dlogits, None, None, None, None, None, None, None, None, None
 
 
 def topk_routing(logits: torch.Tensor, topk: int, score_function: str = "softmax", expert_bias: Optional[torch.Tensor] = None,
@@ -1162,8 +1216,8 @@ def topk_routing(logits: torch.Tensor, topk: int, score_function: str = "softmax
         expert_bias = expert_bias.detach().contiguous()
     if token_mask is not None:
         token_mask = token_mask.contiguous()
-    return _TopkRouting.apply(logits.contiguous(), int(topk), score_function, expert_bias, int(num_groups), int(group_topk),
-                              bool(renormalize), float(scaling_factor), token_mask)
+    return _apply(_TopkRouting, logits.contiguous(), int(topk), score_function, expert_bias, int(num_groups), int(group_topk),
+                  bool(renormalize), float(scaling_factor), token_mask)
 
 
 class TokenPermutation(NamedTuple):
@@ -1176,13 +1230,14 @@ class TokenPermutation(NamedTuple):
 
 class _PermuteTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, indices, num_experts, probs, align):
+    def forward(ctx, x, indices, num_experts, probs, align, need_grad=True):
         row_of, entry_of, group_lens, row_probs = K.permute_plan_impl(indices, num_experts, align, probs)
         rows = K.permute_rows_impl(x, row_of, entry_of)
-        ctx.save_for_backward(row_of, entry_of)
-        ctx.dtype = x.dtype
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(group_lens, row_of, entry_of)
+        if need_grad:
+            ctx.save_for_backward(row_of, entry_of)
+            ctx.dtype = x.dtype
+            ctx.set_materialize_grads(False)
+            ctx.mark_non_differentiable(group_lens, row_of, entry_of)
         return rows, row_probs, group_lens, row_of, entry_of
 
     @staticmethod
@@ -1197,7 +1252,7 @@ class _PermuteTokens(torch.autograd.Function):
             dx, dprobs = K.combine_rows_impl(drows, row_of, entry_of, row_probs=None if drow_probs is None else drow_probs.contiguous())
         elif drow_probs is not None:
             dprobs = torch.where(row_of >= 0, drow_probs[row_of.clamp(min=0)], 0.0) if entry_of.numel() else drow_probs.new_zeros(row_of.shape)
-        return dx, None, None, dprobs, None
+        return dx, None, None, dprobs, None, None
 
 
 def permute_tokens(x: torch.Tensor, indices: torch.Tensor, num_experts: int, probs: Optional[torch.Tensor] = None, align: int = 1):
@@ -1215,17 +1270,17 @@ def permute_tokens(x: torch.Tensor, indices: torch.Tensor, num_experts: int, pro
         raise ValueError("x must be [tokens, hidden] and indices [tokens, topk]")
     if indices.is_floating_point() or indices.dtype == torch.bool:
         raise ValueError("indices must be integers")
-    rows, row_probs, group_lens, row_of, entry_of = _PermuteTokens.apply(
-        x.contiguous(), indices.to(torch.int64).contiguous(), int(num_experts), None if probs is None else probs.contiguous(), int(align))
+    rows, row_probs, group_lens, row_of, entry_of = _apply(
+        _PermuteTokens, x.contiguous(), indices.to(torch.int64).contiguous(), int(num_experts), None if probs is None else probs.contiguous(), int(align))
     return rows, row_probs, group_lens, TokenPermutation(row_of, entry_of)
 
 
 class _UnpermuteTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, row_of, entry_of, probs):
-        # without probabilities the gradient is a move of dy's rows: the rows themselves are not kept
-        ctx.save_for_backward(row_of, entry_of, probs, None if probs is None else rows)
-        ctx.dtype = rows.dtype
+    def forward(ctx, rows, row_of, entry_of, probs, need_grad=True):
+        if need_grad:       # without probabilities the gradient is a move of dy's rows: the rows themselves are not kept
+            ctx.save_for_backward(row_of, entry_of, probs, None if probs is None else rows)
+            ctx.dtype = rows.dtype
         return K.combine_rows_impl(rows, row_of, entry_of, probs)[0]
 
     @staticmethod
@@ -1234,9 +1289,9 @@ class _UnpermuteTokens(torch.autograd.Function):
         row_of, entry_of, probs, rows = ctx.saved_tensors
         dy = dy.to(ctx.dtype).contiguous()
         if probs is None:
-            return K.permute_rows_impl(dy, row_of, entry_of), None, None, None
+            return K.permute_rows_impl(dy, row_of, entry_of), None, None, None, None
         drows, dprobs = K.combine_rows_bwd_impl(dy, rows, row_of, entry_of, probs, ctx.needs_input_grad[0], ctx.needs_input_grad[3])
-        return drows, None, None, None if dprobs is None else dprobs.to(probs.dtype)
+        return drows, None, None, None if dprobs is None else dprobs.to(probs.dtype), None
 
 
 def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, probs: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -1244,4 +1299,4 @@ def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, probs: O
     experts' outputs back at their tokens, summed in fp32 in the order of k and rounded once.  Entries that went nowhere add
     nothing; zero rows are ignored.  Differentiable in ``rows`` (rows that no entry went to get zeros) and ``probs``."""
     row_of, entry_of = permutation
-    return _UnpermuteTokens.apply(rows.contiguous(), row_of, entry_of, None if probs is None else probs.contiguous())
+    return _apply(_UnpermuteTokens, rows.contiguous(), row_of, entry_of, None if probs is None else probs.contiguous())

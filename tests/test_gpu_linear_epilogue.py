@@ -1,0 +1,208 @@
+"""``ops.gemm_bias_act`` stage by stage against 64-bit arithmetic on the same bf16 inputs, and its gradients against the
+composition of the stages and against differences.
+
+Tolerances.  A product of length k in fp32: (k + 64) 2^-23 of the sum of magnitudes.  bf16 results: half a step, 2^-8 of the value.
+The activations' slopes are at most 1.13 and their fp32 forms are off by at most 2^-18 of the value (hardware exp2 and reciprocal, an
+erfc of 1.2e-7; the exponent's rounding counts z^2 2^-24 with |z| < 16 here) plus 2^-24 |z|; the slopes' by 2^-18 of 1 + |z|.
+Column sums of m values in fp32: (m / 8 + 64) 2^-24 of the sum of magnitudes at most."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ACTS = [None, "silu", "gelu", "relu"]
+
+
+def _act(z, act):
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    if act == "gelu":
+        return 0.5 * z * torch.erfc(-z / math.sqrt(2))
+    return z
+
+
+def _slope(z, act):
+    if act == "relu":
+        return (z > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    if act == "gelu":
+        return 0.5 * torch.erfc(-z / math.sqrt(2)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    return torch.ones_like(z)
+
+
+def _within(got, want, bound):
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound.clamp(min=1e-300)).max())
+
+
+def _inputs(gpu, m, n, k, seed, bias_dtype=torch.bfloat16):
+    gen = torch.Generator(device=gpu).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen, device=gpu)  # noqa: E731
+    return r(m, k).bfloat16(), (r(n, k) * 1.5 * k ** -0.5).bfloat16(), r(n).to(bias_dtype), r(m, n).bfloat16(), r(m, n).bfloat16()
+
+
+# few rows (1, 2 and 4 fragments of 16), 64 x 64 tiles, 128 x 128 tiles, odd halves of a slot, ragged last tiles, long contractions
+SIZES = [(1, 32, 32), (1, 4096, 1056), (7, 96, 4096), (16, 64, 288), (17, 160, 96), (33, 320, 800), (64, 2880, 64), (65, 96, 32), (100, 32, 2080), (127, 224, 160),
+         (129, 416, 64), (300, 512, 1120), (777, 1056, 96), (2051, 2880, 96), (2100, 2080, 160), (4096, 1024, 4096), (1000, 2048, 14336)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_stages(gpu, m, n, k):
+    from primus_amd.pytorch import kernels as K
+    from primus_amd.pytorch import ops
+
+    for x, act in enumerate(ACTS if m * n * k < 1 << 30 else ["gelu"]):
+        with_bias, with_res, bias_dtype = x != 1, x % 2 == 0, torch.float32 if x == 3 else torch.bfloat16
+        a, b, bias, res, dy = _inputs(gpu, m, n, k, m + n + k + x, bias_dtype)
+        bias, res = bias if with_bias else None, res if with_res else None
+        ad, bd = a.double(), b.double()
+        z = ad @ bd.t()
+        mag = a.double().abs() @ bd.abs().t()
+        if with_bias:
+            z, mag = z + bias.double(), mag + bias.double().abs()
+        want = _act(z, act) + (res.double() if with_res else 0.0)
+        ez = (k + 64) * 2.0 ** -23 * mag
+        got, zb = K.linear_bf16_impl(a, b, bias, act, res, want_z=True)
+        _within(zb, z, ez + 2.0 ** -8 * z.abs())
+        ey = 1.13 * ez + 2.0 ** -18 * _act(z, act).abs() + 2.0 ** -23 * (z.abs() + want.abs())
+        _within(got, want, ey + 2.0 ** -8 * (want.abs() + ey))
+        assert torch.equal(K.linear_bf16_impl(a, b, bias, act, res)[0], got)
+
+        dz, dbias = K.linear_bf16_dz_impl(dy, zb, act, bias_dtype)
+        want_dz = dy.double() * _slope(zb.double(), act)
+        e = dy.double().abs() * 2.0 ** -18 * (1 + zb.double().abs()) if act in ("silu", "gelu") else torch.zeros_like(want_dz)
+        _within(dz, want_dz, e + 2.0 ** -8 * want_dz.abs())
+        half = torch.finfo(bias_dtype).eps / 2
+        _within(dbias, want_dz.sum(0), e.sum(0) + (m / 8 + 64) * 2.0 ** -24 * want_dz.abs().sum(0) + half * (want_dz.sum(0).abs() + e.sum(0)) + 1e-30)
+        assert torch.equal(K.linear_bf16_dz_impl(dy, zb, act)[0], dz)
+
+        da = K.linear_bf16_dgrad_impl(dz, b)
+        want_da = dz.double() @ bd
+        _within(da, want_da, (n + 64) * 2.0 ** -23 * (dz.double().abs() @ bd.abs()) + 2.0 ** -8 * want_da.abs() + 1e-30)
+        db = K.linear_bf16_wgrad_impl(dz, a).view(n, k)
+        want_db = dz.double().t() @ ad
+        _within(db, want_db, (m + 64) * 2.0 ** -23 * (dz.double().abs().t() @ ad.abs()) + 2.0 ** -8 * want_db.abs() + 1e-30)
+
+        # the operator is these stages
+        leaves = [None if t is None else t.clone().requires_grad_() for t in (a, b, bias, res)]
+        y = ops.gemm_bias_act(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3])
+        assert torch.equal(y.detach(), got)
+        grads = torch.autograd.grad(y, [t for t in leaves if t is not None], dy)
+        expect = [da, db] + ([dbias] if with_bias else []) + ([dy] if with_res else [])
+        for g, w in zip(grads, expect):
+            assert torch.equal(g, w)
+        with torch.no_grad():
+            assert torch.equal(ops.gemm_bias_act(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3]), got)
+
+
+@pytest.mark.parametrize("m", [3, 40, 150, 1500])
+def test_exact_on_small_integers(gpu, m):
+    from primus_amd.pytorch import ops
+
+    gen = torch.Generator().manual_seed(m)
+    n, k = 1088, 352
+    a, b = (torch.randint(-2, 3, s, generator=gen).bfloat16().to(gpu) for s in ((m, k), (n, k)))
+    bias, res = torch.randint(-9, 9, (n,), generator=gen).float().to(gpu), torch.randint(-9, 9, (m, n), generator=gen).bfloat16().to(gpu)
+    want = (a.double() @ b.double().t() + bias.double()).clamp(min=0) + res.double()
+    assert torch.equal(ops.gemm_bias_act(a, b, bias=bias, activation="relu", residual=res), want.bfloat16())
+
+
+def test_gradients_against_differences(gpu):
+    """In directions of small integers, with a loss in float64: the central difference of the fp64 definition.  The kernel's gradient
+    differs from it by its roundings: dz 2^-8, z 2^-8 |z| through a second derivative of at most 0.8, and the sum; the bound counts them in
+    the direction's 1-norm."""
+    from primus_amd.pytorch import ops
+
+    gen = torch.Generator().manual_seed(1)
+    m, n, k = 6, 64, 32
+    for act in ACTS[1:3]:
+        a, b, bias = torch.randn(m, k, generator=gen).bfloat16(), (torch.randn(n, k, generator=gen) * 0.2).bfloat16(), torch.randn(n, generator=gen).bfloat16()
+        dy = torch.randn(m, n, generator=gen).bfloat16()
+        leaves = [t.to(gpu).requires_grad_() for t in (a, b, bias)]
+        grads = [g.double().cpu() for g in torch.autograd.grad(ops.gemm_bias_act(*leaves, activation=act), leaves, dy.to(gpu))]
+        loss = lambda a, b, c: (_act(a @ b.t() + c, act) * dy.double()).sum()  # noqa: E731
+        z = a.double() @ b.double().t() + bias.double()
+        edz = dy.double().abs() * (0.8 * 2.0 ** -8 * z.abs() + 2.0 ** -8 * _slope(z, act).abs() + 2.0 ** -14)
+        bounds = [edz @ b.double().abs(), edz.t() @ a.double().abs(), edz.sum(0)]
+        for i, t in enumerate((a, b, bias)):
+            d = torch.randint(-1, 2, t.shape, generator=gen).double()
+            x = [a.double(), b.double(), bias.double()]
+            up, down = [list(x), list(x)]
+            up[i], down[i] = x[i] + 1e-5 * d, x[i] - 1e-5 * d
+            diff = (loss(*up) - loss(*down)) / 2e-5
+            off = ((bounds[i] + 2.0 ** -8 * grads[i].abs()) * d.abs()).sum() + 1e-5
+            assert float(((grads[i] * d).sum() - diff).abs()) <= float(off)
+
+
+def test_shapes_strides_and_alignment(gpu):
+    from primus_amd.pytorch import ops
+
+    a, b, bias, res, dy = _inputs(gpu, 60, 96, 64, 5)
+    want = ops.gemm_bias_act(a, b, bias=bias, activation="silu", residual=res)
+    assert torch.equal(ops.gemm_bias_act(a.view(3, 20, 64), b, bias=bias, activation="silu", residual=res.view(3, 20, 96)), want.view(3, 20, 96))
+    shift = lambda t, s: torch.empty(t.numel() + 16, dtype=t.dtype, device=gpu)[s:s + t.numel()].view(t.shape).copy_(t)  # noqa: E731
+    assert torch.equal(ops.gemm_bias_act(shift(a, 1), shift(b, 3), bias=shift(bias, 5), activation="silu", residual=shift(res, 7)), want)
+    assert torch.equal(ops.gemm_bias_act(a.t().contiguous().t(), b.t().contiguous().t(), bias=torch.stack([bias, bias], 1)[:, 0], activation="silu",
+                                         residual=res.t().contiguous().t()), want)
+    assert ops.gemm_bias_act(a[:0], b, bias=bias).shape == (0, 96)
+    x, w, c = a[:0].clone().requires_grad_(), b.clone().requires_grad_(), bias.clone().requires_grad_()
+    grads = torch.autograd.grad(ops.gemm_bias_act(x, w, bias=c, activation="gelu"), [x, w, c], dy[:0])
+    assert grads[0].shape == (0, 64) and not bool(grads[1].any()) and not bool(grads[2].any())
+    # a gradient that is no bf16, and strided
+    x = a.clone().requires_grad_()
+    (g,) = torch.autograd.grad(ops.gemm_bias_act(x, b, activation="relu"), x, dy)
+    (h,) = torch.autograd.grad(ops.gemm_bias_act(x, b, activation="relu").float(), x, dy.float().t().contiguous().t())
+    assert torch.equal(g, h)
+
+
+def test_weight_gradient_into_main_grad(gpu):
+    from primus_amd.pytorch import ops
+
+    a, b, bias, _, dy = _inputs(gpu, 200, 96, 64, 6)
+    w = torch.nn.Parameter(b)
+    (plain,) = torch.autograd.grad(ops.gemm_bias_act(a, w, bias=bias, activation="gelu"), w, dy)
+    w.main_grad = torch.ones(96, 64, device=gpu)
+    w.grad_added_to_main_grad = False
+    ops.gemm_bias_act(a, w, bias=bias, activation="gelu", fuse_bgrad_accum_pattern="megatron").backward(dy)
+    assert w.grad_added_to_main_grad
+    # the product before its rounding, plus one
+    assert bool(((w.main_grad - 1.0 - plain.float()).abs() <= 2.0 ** -8 * plain.float().abs() + 2.0 ** -23 * (2.0 + plain.float().abs())).all())
+
+
+def test_values_that_are_not_finite_stay_in_their_rows(gpu):
+    from primus_amd.pytorch import ops
+
+    for m in (5, 100, 700):
+        a, b, bias, res, _ = _inputs(gpu, m, 2048, 96, 7)
+        want = ops.gemm_bias_act(a, b, bias=bias, activation="relu", residual=res)
+        a[2] = float("nan")
+        a[4, 3] = float("inf")
+        got = ops.gemm_bias_act(a, b, bias=bias, activation="relu", residual=res)
+        keep = [i for i in range(m) if i not in (2, 4)]
+        assert torch.equal(got[keep], want[keep]) and bool(torch.isnan(got[2]).all()) and not bool(torch.isfinite(got[4]).all())
+
+
+def test_operands_past_4_gib(gpu):
+    """Activations of more than 2^32 bytes: offsets past 32 bits, and a weight gradient in runs of rows."""
+    from primus_amd.pytorch import kernels as K
+    from primus_amd.pytorch import ops
+
+    m, n, k = (1 << 17) + 40, 64, 16416
+    gen = torch.Generator(device=gpu).manual_seed(9)
+    a = torch.randint(-1, 2, (m, k), generator=gen, device=gpu, dtype=torch.int8).bfloat16()
+    b = torch.randint(-1, 2, (n, k), generator=gen, device=gpu, dtype=torch.int8).bfloat16()
+    assert a.numel() * 2 > 1 << 32
+    y = ops.gemm_bias_act(a, b)
+    for lo in (0, m - 300):     # fp32 sums of 0, 1 and -1 are exact
+        assert torch.equal(y[lo:lo + 300], (a[lo:lo + 300].float() @ b.float().t()).bfloat16())
+    dz = torch.zeros(m, n, dtype=torch.bfloat16, device=gpu)
+    dz[0, 0] = dz[m - 1, 1] = dz[m // 2, 2] = 1.0
+    db = K.linear_bf16_wgrad_impl(dz, a).view(n, k)
+    assert torch.equal(db[0], a[0]) and torch.equal(db[1], a[m - 1]) and torch.equal(db[2], a[m // 2]) and not bool(db[3:].any())

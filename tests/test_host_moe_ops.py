@@ -18,9 +18,13 @@ def on_gpu(monkeypatch):
     monkeypatch.setattr(_lib, "load", lambda: pytest.fail("nothing may be launched"))
 
 
+def _bf(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
 def test_cpu_tensors_are_refused():
     x = torch.randn(4, 8)
-    for call in (lambda: ops.topk_routing(x, 2), lambda: ops.permute_tokens(x, torch.zeros(4, 2, dtype=torch.int64), 3),
+    for call in (lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32)), lambda: ops.topk_routing(x, 2), lambda: ops.permute_tokens(x, torch.zeros(4, 2, dtype=torch.int64), 3),
                  lambda: ops.unpermute_tokens(x, ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)))):
         with pytest.raises(ValueError, match="GPU only"):
             call()
@@ -60,6 +64,21 @@ def test_cpu_tensors_are_refused():
     ("made for", lambda: ops.unpermute_tokens(torch.randn(4, 8), ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(5, dtype=torch.int32)))),
     ("probs must be", lambda: ops.unpermute_tokens(torch.randn(4, 8), ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)),
                                                    probs=torch.zeros(4, 3))),
+    ("a must be", lambda: ops.gemm_bias_act(_bf(32), _bf(32, 32))),
+    ("a must be", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(1, 32, 32))),
+    ("2-D bfloat16", lambda: ops.gemm_bias_act(torch.randn(4, 32), _bf(32, 32))),
+    ("2-D bfloat16", lambda: ops.gemm_bias_act(_bf(4, 32), torch.randn(32, 32))),
+    ("contraction lengths", lambda: ops.gemm_bias_act(_bf(4, 64), _bf(32, 32))),
+    ("multiples of 32", lambda: ops.gemm_bias_act(_bf(4, 48), _bf(32, 48))),
+    ("multiples of 32", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(40, 32))),
+    ("activation must be", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32), activation="tanh")),
+    ("bias must be", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32), bias=_bf(31))),
+    ("bias must be", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32), bias=_bf(32).half())),
+    ("residual must have", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32), residual=_bf(5, 32))),
+    ("residual must be", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32), residual=torch.randn(4, 32))),
+    ("fuse_bgrad_accum_pattern", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32), fuse_bgrad_accum_pattern="other")),
+    ("main_grad", lambda: ops.gemm_bias_act(_bf(4, 32), _bf(32, 32), fuse_bgrad_accum_pattern="megatron")),
+    ("4 GiB", lambda: ops.gemm_bias_act(_bf(1, 1).expand(1, 1 << 17), _bf(1, 1).expand(1 << 15, 1 << 17))),
     ("not empty", lambda: ops.unpermute_tokens(torch.randn(4, 0), ops.TokenPermutation(torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)))),
 ])
 def test_refusals(on_gpu, why, call):
@@ -103,3 +122,17 @@ def test_c_entries_check_before_they_touch_the_device():
     assert lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, p, 4, 2, p, 0, p, p, None) == -3
     assert lib.mxl_combine_rows_bwd(None, p, 8, 16, 1, p, p, 4, 2, p, 0, p, p, None) == -1 and lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, p, 4, 2, None, 0, p, p, None) == -1
     assert lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, None, 4, 2, p, 0, p, p, None) == -1
+    lin = lambda **k: lib.mxl_linear_bf16(*[{**dict(a=p, b=p, bias=p, bd=1, act=3, r=p, m=4, n=32, k=32, y=p, z=None, st=None), **k}[n]  # noqa: E731
+                                            for n in ("a", "b", "bias", "bd", "act", "r", "m", "n", "k", "y", "z", "st")])
+    odd = ctypes.c_void_p(p.value + 8)
+    assert p.value % 16 == 0 and lin() == -3 and lin(m=0) == 0
+    for bad in (dict(a=None), dict(b=None), dict(y=None), dict(bd=2), dict(act=4), dict(act=-1), dict(m=-1), dict(n=48), dict(k=8), dict(n=0), dict(n=1 << 16, k=1 << 16),
+                dict(a=odd), dict(b=odd), dict(bias=odd), dict(r=odd), dict(y=odd), dict(z=odd)):
+        assert lin(**bad) == -1, bad
+    assert lib.mxl_linear_bf16_dgrad(p, p, 4, 32, 32, p, None) == -3 and lib.mxl_linear_bf16_dgrad(p, p, 4, 32, 33, p, None) == -1
+    assert lib.mxl_linear_bf16_dgrad(None, p, 4, 32, 32, p, None) == -1 and lib.mxl_linear_bf16_dgrad(p, p, 0, 32, 32, p, None) == 0
+    ws = lib.mxl_linear_bf16_dz_workspace_bytes(4, 32)
+    dz = lambda **k: lib.mxl_linear_bf16_dz(*[{**dict(dy=p, z=p, act=1, m=4, n=32, dz=p, db=p, dbd=0, w=p, wb=ws, st=None), **k}[n] for n in ("dy", "z", "act", "m", "n", "dz", "db", "dbd", "w", "wb", "st")])  # noqa: E731
+    assert ws == 128 and dz() == -3 and dz(act=3, db=None) == 0
+    for bad in (dict(dy=None), dict(z=None), dict(dz=None), dict(act=9), dict(n=31), dict(w=None), dict(wb=ws - 1), dict(dbd=2), dict(dy=odd)):
+        assert dz(**bad) == -1, bad
