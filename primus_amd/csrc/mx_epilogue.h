@@ -25,10 +25,24 @@ template <int ACT> __device__ __forceinline__ float epi_slope(float z) {
     if constexpr (ACT == kActNone) return 1.f;
     else if constexpr (ACT == kActRelu) return z != z ? z : (z > 0.f ? 1.f : 0.f);
     else if constexpr (ACT == kActSilu) {
-        const float s = 1.f / (1.f + expf(-z));
+        const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
         return s * (1.f + z * (1.f - s));
     } else {
-        return 0.5f * erfcf(-z * 0.70710678118654752f) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+        // Phi(z) + z phi(z); Phi from the same fit of erfc as act_fwd, t exp(P(t)) exp(-z^2 / 2), whose last factor is phi's too
+        const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.5f * x);
+        float q = 0.17087277f;
+        q = q * t - 0.82215223f;
+        q = q * t + 1.48851587f;
+        q = q * t - 1.13520398f;
+        q = q * t + 0.27886807f;
+        q = q * t - 0.18628806f;
+        q = q * t + 0.09678418f;
+        q = q * t + 0.37409196f;
+        q = q * t + 1.00002368f;
+        q = q * t - 1.26551223f;
+        const float e = __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);
+        const float tail = 0.5f * t * __builtin_amdgcn_exp2f(q * 1.4426950408889634f) * e;
+        return fmaf(z * 0.39894228040143268f, e, z < 0.f ? tail : 1.f - tail);
     }
 }
 

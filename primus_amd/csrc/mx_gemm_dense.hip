@@ -237,9 +237,9 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
 
 // ---- a few rows: bound by reading b once.  A workgroup has 16 columns; its 8 waves split the contraction, load b's fragments straight
 // into registers (16 rows of 64 bytes per request, SKINNY_AHEAD requests on their way) and join their sums through LDS. ----
-constexpr int SK_WAVES = 8, SK_AHEAD = 8;
+constexpr int SK_AHEAD = 8;
 
-template <int MT, int ACT>
+template <int MT, int SK_WAVES, int ACT>
 __global__ __launch_bounds__(SK_WAVES * 64) void dense_few_rows_kernel(DenseArgs p) {
     __shared__ v4f part[SK_WAVES][MT][64];
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63;
@@ -345,18 +345,25 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DzArgs p) {
     if ((int64_t)blockIdx.x * 256 + c < p.n) p.partial[(int64_t)blockIdx.y * p.n + (int64_t)blockIdx.x * 256 + c] = s;
 }
 
-// dbias[n] = sum of the runs: 64 columns by 4 groups of runs
-__global__ __launch_bounds__(256) void dense_dbias_kernel(const float* partial, int runs, int64_t n, void* dbias, int f32) {
-    __shared__ float part[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+// dbias[n] = sum of the runs: 32 columns by 32 groups of runs, four loads on their way
+__global__ __launch_bounds__(1024) void dense_dbias_kernel(const float* partial, int runs, int64_t n, void* dbias, int f32) {
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + lane;       // n is a multiple of 32
     float s = 0.f;
-    if (col < n)
-        for (int r = w; r < runs; r += 4) s += partial[(int64_t)r * n + col];
+    for (int r0 = w; r0 < runs; r0 += 32 * 4) {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = r0 + 32 * u < runs ? partial[(int64_t)(r0 + 32 * u) * n + col] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s += x[u];
+    }
     part[w][lane] = s;
     __syncthreads();
-    if (w == 0 && col < n) {
-        s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    if (w == 0) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += part[i][lane];
         if (f32) ((float*)dbias)[col] = s;
         else ((__bf16*)dbias)[col] = (__bf16)s;
     }
@@ -388,12 +395,18 @@ static int launch_dense_tile(const DenseArgs& a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
 
+template <int MT, int ACT>
+static void launch_few_rows(const DenseArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)(a.n / 16));
+    if (a.n / 16 >= 512) hipLaunchKernelGGL((dense_few_rows_kernel<MT, 4, ACT>), grid, dim3(4 * 64), 0, st, a);
+    else hipLaunchKernelGGL((dense_few_rows_kernel<MT, 8, ACT>), grid, dim3(8 * 64), 0, st, a);
+}
+
 template <int ACT>
 static int launch_dense_forward(const DenseArgs& a, hipStream_t st) {
-    const dim3 few((unsigned)(a.n / 16)), threads(SK_WAVES * 64);
-    if (a.m <= 16) hipLaunchKernelGGL((dense_few_rows_kernel<1, ACT>), few, threads, 0, st, a);
-    else if (a.m <= 32) hipLaunchKernelGGL((dense_few_rows_kernel<2, ACT>), few, threads, 0, st, a);
-    else if (a.m <= 64) hipLaunchKernelGGL((dense_few_rows_kernel<4, ACT>), few, threads, 0, st, a);
+    if (a.m <= 16) launch_few_rows<1, ACT>(a, st);
+    else if (a.m <= 32) launch_few_rows<2, ACT>(a, st);
+    else if (a.m <= 64) launch_few_rows<4, ACT>(a, st);
     else if (((a.m + 127) / 128) * ((a.n + 127) / 128) >= 256) return launch_dense_tile<128, 128, 2, false, ACT>(a, st);
     else return launch_dense_tile<64, 64, 3, false, ACT>(a, st);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
@@ -461,6 +474,6 @@ extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int a
         else if (act == MXL_ACT_RELU) hipLaunchKernelGGL(dense_dz_kernel<kActRelu>, grid, dim3(256), 0, st, d);
         else hipLaunchKernelGGL(dense_dz_kernel<kActNone>, grid, dim3(256), 0, st, d);
     }
-    if (dbias) hipLaunchKernelGGL(dense_dbias_kernel, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, (const float*)workspace, (int)runs, n, dbias, dbias_dtype == MXL_DT_F32);
+    if (dbias) hipLaunchKernelGGL(dense_dbias_kernel, dim3((unsigned)(n / 32)), dim3(1024), 0, st, (const float*)workspace, (int)runs, n, dbias, dbias_dtype == MXL_DT_F32);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }

@@ -140,8 +140,8 @@ __global__ __launch_bounds__(PM_THREADS) void permute_place_kernel(PlanArgs p) {
         }
     }
     // rows that no entry goes to: padding inside the experts' runs, and the rest of the buffer
-    for (int e = (int)blockIdx.x; e < E; e += (int)gridDim.x)
-        for (int r = off[e] + total[e] + t; r < off[e + 1]; r += PM_THREADS) {
+    for (int e = (int)blockIdx.x * PM_THREADS + t; e < E; e += (int)gridDim.x * PM_THREADS)
+        for (int r = off[e] + total[e]; r < off[e + 1]; ++r) {      // fewer than align rows
             p.entry_of[r] = -1;
             if (p.probs) put_prob(p, r, -1);
         }
@@ -281,7 +281,9 @@ __global__ __launch_bounds__(MV_THREADS) void combine_rows_kernel(MoveArgs p) {
 }
 
 // gradient of combine with probabilities: a workgroup takes a token, whose row of dy is scaled into its topk rows of drows and
-// multiplied with their rows for the probabilities' gradients (fp32; the sum's order is fixed by the row length)
+// multiplied with their rows for the probabilities' gradients (fp32; the sum's order is fixed by the row length).  Eight rows at a
+// time, so that a thread has nine loads on their way.
+constexpr int CB_ROWS = 8;
 template <int DT, int N>
 __global__ __launch_bounds__(MV_THREADS) void combine_rows_bwd_kernel(MoveArgs p) {
     constexpr int SIZE = DT == MXL_DT_F32 ? 4 : 2;
@@ -290,31 +292,44 @@ __global__ __launch_bounds__(MV_THREADS) void combine_rows_bwd_kernel(MoveArgs p
     const int64_t vecs = p.hidden / N;
     for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
         const uint8_t* dy = p.dy + t * p.hidden * SIZE;
-        for (int k = 0; k < p.topk; ++k) {
-            const int64_t r = p.row_of[t * p.topk + k];
-            float dot = 0.f;
-            if (r >= 0 && r < p.rows) {
-                const float pr = load_dt(p.probs, p.probs_dtype, t * p.topk + k);
-                const uint8_t* x = p.x + r * p.hidden * SIZE;
-                uint8_t* o = p.out + r * p.hidden * SIZE;
-                for (int64_t v = threadIdx.x; v < vecs; v += MV_THREADS) {
-                    float d[N];
-                    load_n<DT, N>(dy + v * N * SIZE, d);
-                    if (p.dprobs) {
-                        float a[N];
-                        load_n<DT, N>(x + v * N * SIZE, a);
+        for (int k0 = 0; k0 < p.topk; k0 += CB_ROWS) {
+            int64_t at[CB_ROWS];
+            float pr[CB_ROWS], dot[CB_ROWS];
 #pragma unroll
-                        for (int i = 0; i < N; ++i) dot = fmaf(a[i], d[i], dot);
+            for (int k = 0; k < CB_ROWS; ++k) {
+                const int64_t r = k0 + k < p.topk ? p.row_of[t * p.topk + k0 + k] : -1;
+                at[k] = r >= 0 && r < p.rows ? r * p.hidden * SIZE : -1;
+                pr[k] = k0 + k < p.topk ? load_dt(p.probs, p.probs_dtype, t * p.topk + k0 + k) : 0.f;
+                dot[k] = 0.f;
+            }
+            for (int64_t v = threadIdx.x; v < vecs; v += MV_THREADS) {
+                float d[N], a[CB_ROWS][N];
+                load_n<DT, N>(dy + v * N * SIZE, d);
+                if (p.dprobs) {
+#pragma unroll
+                    for (int k = 0; k < CB_ROWS; ++k)
+                        if (at[k] >= 0) load_n<DT, N>(p.x + at[k] + v * N * SIZE, a[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < CB_ROWS; ++k) {
+                    if (at[k] < 0) continue;
+                    if (p.dprobs) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) dot[k] = fmaf(a[k][i], d[i], dot[k]);
                     }
                     if (p.out) {
+                        float o[N];
 #pragma unroll
-                        for (int i = 0; i < N; ++i) d[i] *= pr;
-                        store_n<DT, N>(o + v * N * SIZE, d);
+                        for (int i = 0; i < N; ++i) o[i] = d[i] * pr[k];
+                        store_n<DT, N>(p.out + at[k] + v * N * SIZE, o);
                     }
                 }
-                dot = lanes_sum<64>(dot);
             }
-            if (lane == 0) part[w][k] = dot;
+#pragma unroll
+            for (int k = 0; k < CB_ROWS; ++k) {
+                const float s = lanes_sum<64>(dot[k]);
+                if (lane == 0 && k0 + k < p.topk) part[w][k0 + k] = s;
+            }
         }
         __syncthreads();
         if (p.dprobs && (int)threadIdx.x < p.topk) {

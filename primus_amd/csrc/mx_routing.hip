@@ -48,16 +48,36 @@ __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(
 __device__ __forceinline__ float finite_top(float top) { return top == -INFINITY ? 0.f : top; }
 __device__ __forceinline__ float some(float sum) { return sum == 0.f ? 1.f : sum; }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + expf(-x)); }
+// the same for the choice: hardware exp2 and reciprocal, about 1 ulp each; the product with log2 e adds 1.45 |x| 2^-24
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-x)); }
+__device__ __forceinline__ uint32_t dpp_next_lane(uint32_t v) {        // lane l: lane l + 1's; the last lane 0
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x130, 0xF, 0xF, true);      // wave_shl 1
+}
+__device__ __forceinline__ float dpp_next_lane(float v) { return __uint_as_float(dpp_next_lane(__float_as_uint(v))); }
 
-// (key, index) pairs of a lane in descending order, equal keys by ascending index: Batcher's odd-even merge sort
-template <int V> __device__ __forceinline__ void sort_pairs(uint32_t (&key)[V], uint32_t (&idx)[V]) {
+// One logit of a lane's sorted list: its key, its expert and (where scores are compared) itself
+template <bool SCORED> struct Cand {
+    uint32_t key, idx;
+};
+template <> struct Cand<true> {
+    uint32_t key, idx;
+    float logit;
+};
+template <bool SCORED> __device__ __forceinline__ Cand<SCORED> pick(bool first, const Cand<SCORED>& a, const Cand<SCORED>& b) {
+    Cand<SCORED> r;
+    r.key = first ? a.key : b.key;
+    r.idx = first ? a.idx : b.idx;
+    if constexpr (SCORED) r.logit = first ? a.logit : b.logit;
+    return r;
+}
+// a lane's candidates in descending order, equal keys by ascending index: Batcher's odd-even merge sort
+template <int V, bool SCORED> __device__ __forceinline__ void sort_cands(Cand<SCORED> (&c)[V]) {
     auto order = [&](int a, int b) __attribute__((always_inline)) {      // a < b: the better one to a
-        const bool swap = key[b] > key[a] || (key[b] == key[a] && idx[b] < idx[a]);
-        const uint32_t ka = key[a], ia = idx[a];
-        key[a] = swap ? key[b] : ka;
-        idx[a] = swap ? idx[b] : ia;
-        key[b] = swap ? ka : key[b];
-        idx[b] = swap ? ia : idx[b];
+        const bool keep = c[a].key > c[b].key || (c[a].key == c[b].key && c[a].idx < c[b].idx);
+        const Cand<SCORED> x = pick<SCORED>(keep, c[a], c[b]), y = pick<SCORED>(keep, c[b], c[a]);
+        c[a] = x;
+        c[b] = y;
     };
 #pragma unroll
     for (int p = 1; p < V; p <<= 1)
@@ -69,13 +89,10 @@ template <int V> __device__ __forceinline__ void sort_pairs(uint32_t (&key)[V], 
                 for (int i = 0; i < k; ++i)
                     if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(i + j, i + j + k);
 }
-template <int V> __device__ __forceinline__ void pop_head(uint32_t (&key)[V], uint32_t (&idx)[V], bool take) {
+template <int V, bool SCORED> __device__ __forceinline__ void pop_head(Cand<SCORED> (&c)[V], bool take) {
 #pragma unroll
-    for (int v = 0; v + 1 < V; ++v) {
-        key[v] = take ? key[v + 1] : key[v];
-        idx[v] = take ? idx[v + 1] : idx[v];
-    }
-    key[V - 1] = take ? 0u : key[V - 1];
+    for (int v = 0; v + 1 < V; ++v) c[v] = pick<SCORED>(take, c[v + 1], c[v]);
+    c[V - 1].key = take ? 0u : c[V - 1].key;
 }
 
 // The choice of one row again, by a whole wave, from scores in fp64 kept in the wave's LDS; lane k < topk returns the k-th index.
@@ -168,16 +185,20 @@ __device__ __forceinline__ int choose_fp64(const RouteArgs& p, int64_t row, doub
 }
 
 // SCORED: bias or groups, so scores are computed and compared (a row per wave); otherwise the logits are.
-template <int LPR, int V, bool SCORED> constexpr int route_waves() { return !SCORED || V <= 4 ? 16 : 64 / V; }
+template <int V, bool SCORED> constexpr int route_waves() { return !SCORED || V <= 4 ? 16 : 64 / V; }
 
 template <int LPR, int V, bool SCORED>
-__global__ __launch_bounds__((route_waves<LPR, V, SCORED>() * 64)) void route_fwd_kernel(RouteArgs p) {
+__global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V <= 4 ? 8 : 1)) void route_fwd_kernel(RouteArgs p) {
     static_assert(!SCORED || LPR == 64, "a scored row is a wave's");
-    constexpr int WAVES = route_waves<LPR, V, SCORED>(), RPW = 64 / LPR;
+    constexpr int WAVES = route_waves<V, SCORED>(), RPW = 64 / LPR;
     __shared__ int hist[RT_MAX_EXPERTS];
+    __shared__ float bias[SCORED ? RT_MAX_EXPERTS : 1];
     __shared__ double spare[SCORED ? WAVES * V * 64 : 1];
     const int t = threadIdx.x, w = t >> 6, lane = t & 63, lr = lane & (LPR - 1);
-    for (int e = t; e < p.experts; e += WAVES * 64) hist[e] = 0;
+    for (int e = t; e < p.experts; e += WAVES * 64) {
+        hist[e] = 0;
+        if (SCORED) bias[e] = p.bias ? p.bias[e] : 0.f;
+    }
     __syncthreads();
     // element (lane, v) of a row: expert `first + v`, if v < have.  Lower experts sit in lower lanes.
     int first, have;
@@ -192,13 +213,22 @@ __global__ __launch_bounds__((route_waves<LPR, V, SCORED>() * 64)) void route_fw
     have = have < 0 ? 0 : have > V ? V : have;
 
     const int64_t step = (int64_t)gridDim.x * WAVES * RPW;
-    for (int64_t row0 = ((int64_t)blockIdx.x * WAVES + w) * RPW; row0 < p.tokens; row0 += step) {
-        const int64_t row = row0 + lane / LPR;
-        const bool in = row < p.tokens;
-        const int64_t base = (in ? row : p.tokens - 1) * p.experts;
-        float l[V];
+    auto fetch = [&](int64_t row0, float (&l)[V]) __attribute__((always_inline)) {
+        const int64_t row = row0 + lane / LPR, base = (row < p.tokens ? row : p.tokens - 1) * p.experts;
 #pragma unroll
         for (int v = 0; v < V; ++v) l[v] = v < have ? load_dt(p.logits, p.dtype, base + first + v) : -INFINITY;
+    };
+    int64_t row0 = ((int64_t)blockIdx.x * WAVES + w) * RPW;
+    float next[V];
+    if (row0 < p.tokens) fetch(row0, next);
+    for (; row0 < p.tokens; row0 += step) {
+        const int64_t row = row0 + lane / LPR;
+        const bool in = row < p.tokens;
+        float l[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) l[v] = next[v];
+        if (row0 + step < p.tokens) fetch(row0 + step, next);       // the next row's logits travel while this one's are looked at
+        const bool routed = !p.mask || !in || p.mask[row];
 
         float top = 0.f, total = 1.f;           // of the row: largest logit, sum of exp(l - top)
         if (!p.sigmoid && (SCORED || !p.renorm)) {
@@ -208,36 +238,36 @@ __global__ __launch_bounds__((route_waves<LPR, V, SCORED>() * 64)) void route_fw
             top = finite_top(lanes_max<LPR>(top));
             float s = 0.f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) s += v < have ? expf(l[v] - top) : 0.f;
+            for (int v = 0; v < V; ++v) s += v < have ? exp_fast(l[v] - top) : 0.f;
             total = some(lanes_sum<LPR>(s));
         }
-        uint32_t key[V], idx[V];
+        // What two fp32 scores may be off together: sigmoid, at most 2^-22 each (an exponential, a sum, a reciprocal).  Softmax: a
+        // score s = exp(-x) / total is off by s (1.45 x + 60) 2^-24 (the exponentials, V + 6 additions, the quotient), and neither s
+        // nor 2 s x passes 1 / total.  Without a bias nothing left out has a larger score than what it is compared with: relative there.
+        const float pair_off = p.sigmoid ? 0x1p-21f : 0x1p-17f / total;
+        Cand<SCORED> c[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float c = l[v];
-            if (SCORED && v < have) {
-                c = p.sigmoid ? sigmoid_of(l[v]) : expf(l[v] - top) / total;
-                if (p.bias) c += p.bias[first + v];
+            float x = l[v];
+            if constexpr (SCORED) {
+                c[v].logit = l[v];
+                if (v < have) x = (p.sigmoid ? sigmoid_fast(l[v]) : exp_fast(l[v] - top) / total) + bias[first + v];
             }
-            key[v] = v < have ? order_key(c) : 0u;
-            idx[v] = (uint32_t)(first + v);
+            c[v].key = v < have ? order_key(x) : 0u;
+            c[v].idx = (uint32_t)(first + v);
         }
-        sort_pairs<V>(key, idx);
+        sort_cands<V, SCORED>(c);
         bool doubt = false;
-        // What two fp32 scores may be off together: sigmoid, expf, a sum and a quotient, 2^-22 of at most 1 each.  Softmax: a score
-        // s = exp(-x) / total is off by s (x + 40) 2^-24 (the rounding of x, expf, V + 6 additions, the quotient), and neither s nor
-        // s x passes 1 / total.  Without a bias nothing left out has a larger score than what it is compared with: relative there.
-        const float pair_off = p.sigmoid ? 0x1p-21f : 0x1p-17f / total;
         if (SCORED && p.groups > 1) {
-            uint32_t gk[V], gi[V];
+            Cand<SCORED> q[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) gk[v] = key[v], gi[v] = idx[v];
+            for (int v = 0; v < V; ++v) q[v] = c[v];
             float score = 0.f;
             for (int i = 0; i < p.take; ++i) {
-                const uint32_t best = lanes_reduce<OpMaxU>(gk[0], p.lanes_per_group);
-                const uint32_t who = lanes_reduce<OpMinU>(gk[0] == best ? (uint32_t)lane : 64u, p.lanes_per_group);
+                const uint32_t best = lanes_reduce<OpMaxU>(q[0].key, p.lanes_per_group);
+                const uint32_t who = lanes_reduce<OpMinU>(q[0].key == best ? (uint32_t)lane : 64u, p.lanes_per_group);
                 score += best ? key_value(best) : 0.f;
-                pop_head<V>(gk, gi, who == (uint32_t)lane && best != 0u);
+                pop_head<V, SCORED>(q, who == (uint32_t)lane && best != 0u);
             }
             const int grp = lane / p.lanes_per_group;
             int ahead = 0;
@@ -254,58 +284,69 @@ __global__ __launch_bounds__((route_waves<LPR, V, SCORED>() * 64)) void route_fw
                 doubt = !(in_worst - out_best > off + 0x1p-22f * (float)p.take * mag);
             }
 #pragma unroll
-            for (int v = 0; v < V; ++v) key[v] = keep ? key[v] : 0u;
+            for (int v = 0; v < V; ++v) c[v].key = keep ? c[v].key : 0u;
         }
         // the choice, one expert a round; lane k of the row keeps the k-th (a scored row looks one further, to compare with it)
         int mine = 0;
         uint32_t mine_key = 0u;
+        float ml = -INFINITY;
         const int rounds = p.topk + (SCORED ? 1 : 0);
         for (int k = 0; k < rounds; ++k) {
-            const uint32_t best = lanes_reduce<OpMaxU, LPR>(key[0]);
+            const uint32_t best = lanes_reduce<OpMaxU, LPR>(c[0].key);
             // equal keys: the lower index is in the lower lane
-            uint32_t who;
-            if constexpr (LPR == 64) who = (uint32_t)__builtin_ctzll(__ballot(key[0] == best));
-            else who = lanes_reduce<OpMinU, LPR>(key[0] == best ? (uint32_t)lane : 64u);
-            uint32_t won;
-            if constexpr (LPR == 64) won = (uint32_t)__builtin_amdgcn_readlane((int)idx[0], (int)who);
-            else won = (uint32_t)__shfl((int)idx[0], (int)who);
-            if (lr == k) mine = (int)won, mine_key = best;
-            pop_head<V>(key, idx, who == (uint32_t)lane);
+            if constexpr (LPR == 64) {
+                const int who = __builtin_ctzll(__ballot(c[0].key == best));
+                const int won = __builtin_amdgcn_readlane((int)c[0].idx, who);
+                mine = lr == k ? won : mine;
+                if constexpr (SCORED) {
+                    const float wl = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(c[0].logit), who));
+                    ml = lr == k && best ? wl : ml;
+                    mine_key = lr == k ? best : mine_key;
+                } else {
+                    ml = lr == k ? key_value(best) : ml;
+                }
+                pop_head<V, SCORED>(c, who == lane);
+            } else {
+                const uint32_t won = lanes_reduce<OpMinU, LPR>(c[0].key == best ? c[0].idx : 0xFFFFFFFFu);
+                mine = lr == k ? (int)won : mine;
+                ml = lr == k ? key_value(best) : ml;
+                pop_head<V, SCORED>(c, c[0].key == best && c[0].idx == won);
+            }
         }
-        // lane k < topk: its expert's score
+        // lane k < topk: its expert's score.  (An unscored row's logit is its key's value: exact, but for a NaN, which stays one.)
         const bool chosen = lr < p.topk;
-        float ml = chosen || (SCORED && mine_key) ? load_dt(p.logits, p.dtype, base + mine) : -INFINITY;
-        if (SCORED) {
-            const float s = p.sigmoid ? sigmoid_of(ml) : expf(ml - top) / total;
-            const float c = key_value(mine_key), b = p.bias && (chosen || mine_key) ? p.bias[mine] : 0.f;
-            const float nl = __shfl_down(ml, 1), ns = __shfl_down(s, 1), nc = __shfl_down(c, 1), nb = __shfl_down(b, 1);
-            const uint32_t nk = (uint32_t)__shfl_down((int)mine_key, 1);
-            const float off = (p.bias || p.sigmoid ? pair_off : 0x1p-16f * (s + ns)) + 0x1p-23f * (fabsf(c) + fabsf(nc));
+        if (!chosen && !SCORED) ml = -INFINITY;
+        if constexpr (SCORED) {
+            const float b = bias[mine_key ? mine : 0], s = p.sigmoid ? sigmoid_fast(ml) : exp_fast(ml - top) / total, cc = key_value(mine_key);
+            const float nl = dpp_next_lane(ml), ns = dpp_next_lane(s), nc = dpp_next_lane(cc), nb = dpp_next_lane(b);
+            const uint32_t nk = dpp_next_lane(mine_key);
+            const float off = (p.bias || p.sigmoid ? pair_off : 0x1p-16f * (s + ns)) + 0x1p-23f * (fabsf(cc) + fabsf(nc));
             // nothing follows, or the same logit and bias (a true tie), or far enough apart: told rightly
-            const bool told = !chosen || nk == 0u || (ml == nl && b == nb) || c - nc > off;
+            const bool told = !chosen || nk == 0u || (ml == nl && b == nb) || cc - nc > off;
             doubt = __any(doubt || !told);
             if (doubt) {
-                const int again = choose_fp64<V>(p, in ? row : p.tokens - 1, spare + w * V * 64);
+                const int64_t at = in ? row : p.tokens - 1;
+                const int again = choose_fp64<V>(p, at, spare + w * V * 64);
                 mine = chosen ? again : 0;
-                ml = chosen ? load_dt(p.logits, p.dtype, base + mine) : -INFINITY;
+                ml = chosen ? load_dt(p.logits, p.dtype, at * p.experts + mine) : -INFINITY;
             }
+            ml = chosen ? ml : -INFINITY;
         }
         float prob;
         if (p.sigmoid) {
             const float s = chosen ? sigmoid_of(ml) : 0.f;
             prob = p.renorm ? s / (lanes_sum<LPR>(s) + 1e-20f) : s;
         } else if (p.renorm) {
-            const float m = finite_top(lanes_max<LPR>(chosen ? ml : -INFINITY));
+            const float m = finite_top(lanes_max<LPR>(ml));
             const float s = chosen ? expf(ml - m) : 0.f;
             prob = s / some(lanes_sum<LPR>(s));
         } else {
             prob = expf(ml - top) / total;
         }
         if (in && chosen) {
-            const bool live = !p.mask || p.mask[row];
-            p.probs[row * p.topk + lr] = live ? prob * p.scale : 0.f;
-            p.indices[row * p.topk + lr] = live ? mine : -1;
-            if (live) atomicAdd(&hist[mine], 1);
+            p.probs[row * p.topk + lr] = routed ? prob * p.scale : 0.f;
+            p.indices[row * p.topk + lr] = routed ? mine : -1;
+            if (routed) atomicAdd(&hist[mine], 1);
         }
     }
     __syncthreads();
@@ -316,18 +357,26 @@ __global__ __launch_bounds__((route_waves<LPR, V, SCORED>() * 64)) void route_fw
     }
 }
 
-// counts[e] = sum over the workgroups: 64 experts by 16 runs of workgroups
+// counts[e] = sum over the workgroups: 16 experts by 64 runs of workgroups, 8 loads on their way
 __global__ __launch_bounds__(1024) void route_counts_kernel(const int* partial, int blocks, int experts, int64_t* counts) {
-    __shared__ int part[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+    __shared__ int part[64][17];
+    const int lane = threadIdx.x & 15, run = threadIdx.x >> 4, e = blockIdx.x * 16 + lane;
     int n = 0;
-    if (e < experts)
-        for (int b = w; b < blocks; b += 16) n += partial[(int64_t)b * experts + e];
-    part[w][lane] = n;
+    if (e < experts) {
+        for (int b0 = run; b0 < blocks; b0 += 64 * 8) {
+            int x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = b0 + 64 * u < blocks ? partial[(int64_t)(b0 + 64 * u) * experts + e] : 0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) n += x[u];
+        }
+    }
+    part[run][lane] = n;
     __syncthreads();
-    if (w == 0 && e < experts) {
+    if (run == 0 && e < experts) {
         int64_t total = 0;
-        for (int i = 0; i < 16; ++i) total += part[i][lane];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) total += part[i][lane];
         counts[e] = total;
     }
 }
@@ -408,11 +457,11 @@ static int64_t route_blocks(int64_t tokens, int rows_per_block) {
 
 template <int LPR, int V, bool SCORED>
 static int launch_route(const RouteArgs& a, hipStream_t st) {
-    constexpr int WAVES = route_waves<LPR, V, SCORED>();
+    constexpr int WAVES = route_waves<V, SCORED>();
     const int64_t blocks = route_blocks(a.tokens, WAVES * (64 / LPR));
     hipLaunchKernelGGL((route_fwd_kernel<LPR, V, SCORED>), dim3((unsigned)blocks), dim3(WAVES * 64), 0, st, a);
     if (blocks > 1)
-        hipLaunchKernelGGL(route_counts_kernel, dim3((unsigned)((a.experts + 63) / 64)), dim3(1024), 0, st, a.partial, (int)blocks, a.experts, a.counts);
+        hipLaunchKernelGGL(route_counts_kernel, dim3((unsigned)((a.experts + 15) / 16)), dim3(1024), 0, st, a.partial, (int)blocks, a.experts, a.counts);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
 

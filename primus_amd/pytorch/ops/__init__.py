@@ -1181,6 +1181,7 @@ class _TopkRouting(torch.autograd.Function):
         if need_grad:
             ctx.save_for_backward(logits, indices)
             ctx.how = (score_function, renormalize, scaling_factor)
+            ctx.set_materialize_grads(False)        # (zeros for the indices and the counts are two launches)
             ctx.mark_non_differentiable(indices, counts)
         return probs, indices, counts
 
@@ -1188,6 +1189,8 @@ class _TopkRouting(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dprobs, _, __):
         logits, indices = ctx.saved_tensors
+        if dprobs is None:
+            return (None,) * 10
         dlogits = K.topk_routing_bwd_impl(dprobs.to(torch.float32).contiguous(), logits, indices, *ctx.how)
         return dlogits, None, None, None, None, None, None, None, None, None
 
