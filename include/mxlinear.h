@@ -611,13 +611,17 @@ int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int 
  *   y = act(z) + residual,  z = a . b^T + bias         a [m, k], b [n, k], y, z, residual [m, n] bf16
  * fp32 from the products to y, which is rounded once; bias (bf16 or float, NULL: none), residual (NULL: none); act MXL_ACT_*.
  * z_bf16: if not NULL, z rounded to bf16 for the backward.  n and k multiples of 32, n * k * 2 < 2^32, pointers 16-byte aligned.
+ * Few tiles and a long contraction split it over workgroups, whose sums meet in the caller's workspace:
+ * mxl_linear_bf16_workspace_bytes(m, n, k) bytes for the forward, (m, k, n) for dgrad (0: none, NULL will do).
  *
  * Backward: mxl_linear_bf16_dz gives dz = dy * act'(z) (not written, and may be dy itself, for MXL_ACT_NONE) and
  * dbias = column sums of dz before its rounding (NULL: not wanted); mxl_linear_bf16_dgrad gives da = dz . b;
  * db = dz^T . a is mxl_grouped_gemm_bf16_wgrad with one group. */
+int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const void* bias, int bias_dtype, int act, const void* residual_bf16, int64_t m,
-                    int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* stream);
-int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* stream);
+                    int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* workspace, int64_t workspace_bytes, void* stream);
+int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* workspace,
+                          int64_t workspace_bytes, void* stream);
 int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n);
 int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int act, int64_t m, int64_t n, void* dz_bf16, void* dbias, int dbias_dtype,
                        void* workspace, int64_t workspace_bytes, void* stream);

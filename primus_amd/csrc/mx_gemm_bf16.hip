@@ -18,7 +18,7 @@
 // a + 4, a + 8, a + 12 (in this order).  16-byte pieces are XOR-swizzled on the global side so that both kinds of
 // read are spread over the LDS banks.  The tile list is derived from group_lens by every workgroup; the workgroups
 // are persistent and walk it in rounds.  Both kernels add every output element's products in the same order: the same bits.
-#include "mx_device.h"
+#include "mx_gemm_bf16.h"
 #include "mx_gemm_addr.h"
 
 #include <type_traits>
@@ -35,18 +35,6 @@ constexpr int BF_GROUP_M = 8;              // tile order: super-rows of this man
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-struct Bf16Args {
-    const uint8_t* a;      // forward: activations [total_m, k];   wgrad: p [total_m, m_out]
-    const uint8_t* b;      // forward: weights [G, n, k] or [G, k, n];   wgrad: q [total_m, n_out]
-    void* c;
-    const int64_t* group_lens;
-    int num_groups;
-    int64_t total_m;
-    int64_t m;             // wgrad: m_out
-    int64_t n;             // forward: n;  wgrad: n_out
-    int64_t k;             // forward: contraction length
-};
 
 __device__ __forceinline__ v4i bf_rsrc(const void* base, int64_t bytes) {
     const uint64_t p = (uint64_t)base;
@@ -414,9 +402,12 @@ __device__ __forceinline__ void bf_static_for(F&& f) {
     }
 }
 
-template <bool A_T, bool B_T, bool WGRAD, bool ACCUM>
+// ACT (forward): the output is act(product + bias) + residual, see mx_epilogue.h; kNoEpilogue: the product.
+constexpr int kNoEpilogue = -1;
+template <bool A_T, bool B_T, bool WGRAD, bool ACCUM, int ACT = kNoEpilogue>
 __global__ __launch_bounds__(TL_THREADS, 2) void bf16_gemm_tall_kernel(Bf16Args p) {
     static_assert(!WGRAD || (A_T && B_T), "wgrad contracts over tokens: both operands are token-major");
+    static_assert(ACT == kNoEpilogue || !WGRAD, "the epilogue belongs to the forward");
     static_assert(!ACCUM || WGRAD, "only the weight gradient accumulates");
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     int* pre_tiles = (int*)(smem + TL_OPS * TL_STAGE);
@@ -727,21 +718,8 @@ __global__ __launch_bounds__(TL_THREADS, 2) void bf16_gemm_tall_kernel(Bf16Args 
             // 904 / 901 / 895 -> 890 / 897 / 881.  (Letting them be on their way in the next tile's first slot: +- 0.)
             const uint32_t row_bytes = (uint32_t)p.n * 2;
             const uint32_t at = col < n_valid ? (uint32_t)row0 * row_bytes + (uint32_t)col * 2 : addr::kDropped;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (h) __syncthreads();
-                if (wm == h) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const v4bf o = {(__bf16)acc[i][j][4 * q], (__bf16)acc[i][j][4 * q + 1], (__bf16)acc[i][j][4 * q + 2], (__bf16)acc[i][j][4 * q + 3]};
-                                *(v4bf*)(out + (32 * i + lr) * 512 + 16 * ((8 * wn + 4 * j + q) ^ lr) + 8 * g) = o;
-                            }
-                }
-                __syncthreads();
+            // what stands in the staging area leaves for the rows of half h at `dst`
+            auto leave = [&](uint16_t* dst, int h) __attribute__((always_inline)) {
                 uint4 v[8];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
@@ -752,10 +730,94 @@ __global__ __launch_bounds__(TL_THREADS, 2) void bf16_gemm_tall_kernel(Bf16Args 
                 for (int x = 0; x < 8; ++x) {
                     const int row = h * 128 + x * 16;
                     const int rows = m_valid - row;
-                    const auto rs = __builtin_amdgcn_make_buffer_rsrc(c + (int64_t)row * p.n, 0, rows > 0 ? (rows < 16 ? rows : 16) * (int)row_bytes : 0, 0x00020000);
+                    const auto rs = __builtin_amdgcn_make_buffer_rsrc(dst + (int64_t)row * p.n, 0, rows > 0 ? (rows < 16 ? rows : 16) * (int)row_bytes : 0, 0x00020000);
                     const u32x4 o = {v[x].x, v[x].y, v[x].z, v[x].w};
                     constexpr int kNonTemporal = 2;
                     __builtin_amdgcn_raw_buffer_store_b128(o, rs, (int)at, 0, kNonTemporal);
+                }
+            };
+            auto spot = [&](int i, int j, int q) __attribute__((always_inline)) {
+                return (v4bf*)(out + (32 * i + lr) * 512 + 16 * ((8 * wn + 4 * j + q) ^ lr) + 8 * g);
+            };
+            if constexpr (ACT == kNoEpilogue) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h) __syncthreads();
+                    if (wm == h) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q)
+                                    *spot(i, j, q) = v4bf{(__bf16)acc[i][j][4 * q], (__bf16)acc[i][j][4 * q + 1], (__bf16)acc[i][j][4 * q + 2], (__bf16)acc[i][j][4 * q + 3]};
+                    }
+                    __syncthreads();
+                    leave(c, h);
+                }
+            } else {
+                // z passes through the staging area on its way out and the residual on its way in: a lane finds its four
+                // columns' residual where it puts its results
+                const int64_t c0 = c_row0 * p.n + n0;
+                if (p.epi.bias) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int bc = wn * 64 + 32 * j + 8 * q + 4 * g;
+                            const v4f b4 = bc < n_valid ? epi_bias4(p.epi, n0 + bc) : v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += b4[e];
+                        }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h) __syncthreads();
+                    if (p.epi.z) {
+                        if (wm == h) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q)
+                                        *spot(i, j, q) = v4bf{(__bf16)acc[i][j][4 * q], (__bf16)acc[i][j][4 * q + 1], (__bf16)acc[i][j][4 * q + 2], (__bf16)acc[i][j][4 * q + 3]};
+                        }
+                        __syncthreads();
+                        leave(p.epi.z + c0, h);
+                        __syncthreads();
+                    }
+                    if (p.epi.residual) {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const int row = h * 128 + x * 16, rows = m_valid - row, lrow = x * 16 + row0;
+                            const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.epi.residual + c0 + (int64_t)row * p.n), 0, rows > 0 ? (rows < 16 ? rows : 16) * (int)row_bytes : 0, 0x00020000);
+                            *(u32x4*)(out + lrow * 512 + 16 * ((to & 31) ^ (lrow & 31))) = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)at, 0, 2);
+                        }
+                        __syncthreads();
+                    }
+                    if (wm == h) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    float y[4];
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) y[e] = epi_act<ACT>(acc[i][j][4 * q + e]);
+                                    if (p.epi.residual) {
+                                        const v4bf r = *spot(i, j, q);
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e) y[e] += (float)r[e];
+                                    }
+                                    *spot(i, j, q) = v4bf{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]};
+                                }
+                    }
+                    __syncthreads();
+                    leave(c, h);
                 }
             }
         }
@@ -774,7 +836,7 @@ static int bf16_num_cus(int dev) {
     return pr.multiProcessorCount;
 }
 
-template <int BM, bool A_T, bool B_T, bool WGRAD, bool ACCUM>
+template <int BM, bool A_T, bool B_T, bool WGRAD, bool ACCUM, int ACT = kNoEpilogue>
 static int launch_bf16(const Bf16Args& a, int64_t max_tiles, hipStream_t st) {
     constexpr bool TALL = BM == 256;
     constexpr int lds = TALL ? tall_lds_bytes() : bf16_lds_bytes();
@@ -783,7 +845,7 @@ static int launch_bf16(const Bf16Args& a, int64_t max_tiles, hipStream_t st) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return MXL_ELAUNCH;
     void (*kern)(Bf16Args) = nullptr;
-    if constexpr (TALL) kern = bf16_gemm_tall_kernel<A_T, B_T, WGRAD, ACCUM>;
+    if constexpr (TALL) kern = bf16_gemm_tall_kernel<A_T, B_T, WGRAD, ACCUM, ACT>;
     else kern = bf16_gemm_kernel<A_T, B_T, WGRAD, ACCUM>;
     if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
         if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return MXL_ELAUNCH;
@@ -812,6 +874,16 @@ static bool bf16_tall_tiles(uint32_t flags, int64_t rows_per_group, int64_t thre
     return rows_per_group >= threshold;
 }
 
+int launch_bf16_linear_tall(const Bf16Args& a, int act, hipStream_t st) {
+    const int64_t tiles = ((a.total_m + 255) / 256) * ((a.n + BF_BN - 1) / BF_BN);
+    switch (act) {
+        case kActSilu: return launch_bf16<256, false, false, false, false, kActSilu>(a, tiles, st);
+        case kActGelu: return launch_bf16<256, false, false, false, false, kActGelu>(a, tiles, st);
+        case kActRelu: return launch_bf16<256, false, false, false, false, kActRelu>(a, tiles, st);
+        default: return launch_bf16<256, false, false, false, false, kActNone>(a, tiles, st);
+    }
+}
+
 }  // namespace mxl
 
 using namespace mxl;
@@ -827,7 +899,7 @@ extern "C" int mxl_grouped_gemm_bf16(const void* a_bf16, const void* b_bf16, voi
     if ((((uintptr_t)a_bf16 | (uintptr_t)b_bf16 | (uintptr_t)c_bf16) & 15) != 0) return MXL_EINVAL;
     // offsets inside a tile's operand rows are 32-bit
     if (256 * k * 2 >= ((int64_t)1 << 31) || k * n * 2 >= ((int64_t)1 << 32)) return MXL_EINVAL;
-    Bf16Args a{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, c_bf16, group_lens, num_groups, total_m, 0, n, k};
+    Bf16Args a{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, c_bf16, group_lens, num_groups, total_m, 0, n, k, {}};
     const bool tall = bf16_tall_tiles(flags, total_m / num_groups, 256);
     const int64_t max_tiles = (total_m / (tall ? 256 : 128) + num_groups) * ((n + BF_BN - 1) / BF_BN);
     hipStream_t st = (hipStream_t)stream;
@@ -847,7 +919,7 @@ extern "C" int mxl_grouped_gemm_bf16_wgrad(const void* p_bf16, const void* q_bf1
     if (total_m > 0 && (!p_bf16 || !q_bf16 || (((uintptr_t)p_bf16 | (uintptr_t)q_bf16) & 15) != 0)) return MXL_EINVAL;
     // the K-slot advance inside a group's token range is a 32-bit byte offset
     if (total_m * m_out * 2 >= ((int64_t)1 << 32) || total_m * n_out * 2 >= ((int64_t)1 << 32)) return MXL_EINVAL;
-    Bf16Args a{(const uint8_t*)p_bf16, (const uint8_t*)q_bf16, c, group_lens, num_groups, total_m, m_out, n_out, 0};
+    Bf16Args a{(const uint8_t*)p_bf16, (const uint8_t*)q_bf16, c, group_lens, num_groups, total_m, m_out, n_out, 0, {}};
     // the tiles are cut from the [m_out, n_out] matrix of every group; the contraction runs over the group's tokens
     // (the last K slot may reach 63 tokens past the operand's end, where 32-bit offsets must not wrap around)
     const bool tall = bf16_tall_tiles(flags, total_m / num_groups, 0) && (total_m + 64) * (m_out > n_out ? m_out : n_out) * 2 < ((int64_t)1 << 32);

@@ -8,7 +8,7 @@
 // The weight gradient, and the products of many rows, run on the grouped kernels' tiles (mx_gemm_bf16.hip) with one group.  This
 // file holds the tiles of 128 x 128 and 64 x 64 for fewer rows, the kernel for a few rows, which is bound by reading b, and
 // the elementwise part of the backward.
-#include "mx_epilogue.h"
+#include "mx_gemm_bf16.h"
 #include "mx_gemm_common.h"
 
 namespace mxl {
@@ -22,18 +22,21 @@ struct DenseArgs {
     uint16_t* c;            // [m, n]
     int64_t m, n, k;
     EpilogueArgs epi;
+    float* partial;         // SPLIT: [splits, m, n]
+    int splits, split_slots;
 };
 
 constexpr int DT_KS = 64;       // contraction elements per slot: 128 bytes of a row, four MFMA steps
 
-template <int TM, int TN, int ST> constexpr int dense_lds_bytes() {
-    const int loop = ST * (TM + TN) * DT_KS * 2, out = TM * (TN * 2 + 16);
+template <int TM, int TN, int ST, bool SPLIT> constexpr int dense_lds_bytes() {
+    const int loop = ST * (TM + TN) * DT_KS * 2, out = TM * (TN * (SPLIT ? 4 : 2) + 16);
     return loop > out ? loop : out;
 }
 
 // ---- tiles: 4 waves (2 x 2), LDS-direct loads into ST stages, one workgroup per tile, two or three of them on a CU so that one's
-// epilogue and waits run under another's MFMAs.  B_T: b is [k, n], read with the transposing LDS read. ----
-template <int TM, int TN, int ST, bool B_T, int ACT>
+// epilogue and waits run under another's MFMAs.  B_T: b is [k, n], read with the transposing LDS read.
+// SPLIT: the contraction is cut into `splits` runs of slots, a workgroup each, whose fp32 sums dense_join_kernel adds up. ----
+template <int TM, int TN, int ST, bool B_T, int ACT, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     constexpr int FM = TM / 64, FN = TN / 64;              // 32 x 32 fragments per wave
     constexpr int AR = TM / 32, BR = TN / 32, R = AR + BR;  // load rounds of 4 KiB
@@ -48,9 +51,15 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
 
     // the tile: each XCD takes one contiguous run of the order, super-rows of 1024 rows
     const int tiles_m = (int)((p.m + TM - 1) / TM), tiles_n = (int)((p.n + TN - 1) / TN);
-    const int total = tiles_m * tiles_n, per_xcd = (total + 7) >> 3;
-    const int in_xcd = (int)(blockIdx.x >> 3), tile = (int)(blockIdx.x & 7) * per_xcd + in_xcd;
+    const int total = tiles_m * tiles_n * (SPLIT ? p.splits : 1), per_xcd = (total + 7) >> 3;
+    const int in_xcd = (int)(blockIdx.x >> 3);
+    int tile = (int)(blockIdx.x & 7) * per_xcd + in_xcd;
     if (in_xcd >= per_xcd || tile >= total) return;
+    int split = 0;
+    if (SPLIT) {            // the runs of one split follow each other: their tiles share operands
+        split = tile / (tiles_m * tiles_n);
+        tile -= split * (tiles_m * tiles_n);
+    }
     int pid_m, pid_n;
     {
         constexpr int SUPER = 1024 / TM;
@@ -61,7 +70,8 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     }
     const int64_t m0 = (int64_t)pid_m * TM, n0 = (int64_t)pid_n * TN;
     const int m_valid = (int)((p.m - m0) < TM ? p.m - m0 : TM), n_valid = (int)((p.n - n0) < TN ? p.n - n0 : TN);
-    const int slots = (int)((p.k + DT_KS - 1) / DT_KS);
+    const int all_slots = (int)((p.k + DT_KS - 1) / DT_KS), s_first = SPLIT ? split * p.split_slots : 0;
+    const int slots = SPLIT && s_first + p.split_slots < all_slots ? s_first + p.split_slots : all_slots;      // the run's end
     const bool odd = (p.k & 32) != 0;       // the last slot's second half is past the contraction: not multiplied
 
     const int64_t lda = p.k * 2, ldb = B_T ? p.n * 2 : p.k * 2;
@@ -127,16 +137,16 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     const bool live = __builtin_amdgcn_readfirstlane(wm * (TM / 2) < m_valid);
 
-    for (int s = 0; s < ST - 1; ++s) issue(s, s);
+    for (int s = 0; s < ST - 1; ++s) issue(s_first + s, s);
     int stage = 0;
-    for (int s = 0; s < slots; ++s) {
+    for (int s = s_first; s < slots; ++s) {
         wait_vm<(ST - 2) * R>();        // slot s has landed
         __syncthreads();                // ... for every wave, and every wave has left the stage of slot s - 1
         issue(s + ST - 1, stage == 0 ? ST - 1 : stage - 1);
         uint8_t* st = smem + stage * STAGE;
         stage = stage == ST - 1 ? 0 : stage + 1;
         if (!live) continue;
-        const int steps = odd && s == slots - 1 ? 2 : 4;
+        const int steps = odd && s == all_slots - 1 ? 2 : 4;
         auto step = [&](int ks) __attribute__((always_inline)) {
             d8bf fa[FM], fb[FN];
 #pragma unroll
@@ -157,6 +167,29 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     }
     wait_vm<0>();
     __syncthreads();                    // nothing reads or writes the stages any more
+
+    if constexpr (SPLIT) {
+        constexpr int FP = TN * 4 + 16, FL = TN / 4;        // the fp32 tile through LDS: bytes per row, lanes per row
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(v4f*)(smem + (wm * (TM / 2) + i * 32 + lr) * FP + (wn * (TN / 2) + j * 32 + 8 * q + 4 * g) * 4) =
+                        v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __syncthreads();
+        const int fr = t / FL, fc = (t % FL) * 4;
+        float* out = p.partial + ((int64_t)split * p.m + m0) * p.n + n0 + fc;
+        if (fc < n_valid) {
+#pragma unroll
+            for (int u = 0; u < TM / (256 / FL); ++u) {
+                const int row = u * (256 / FL) + fr;
+                if (row < m_valid) *(v4f*)(out + (int64_t)row * p.n) = *(const v4f*)(smem + row * FP + fc * 4);
+            }
+        }
+        return;
+    }
 
     // ---- epilogue.  Lane (lr, g) of fragment (i, j) holds row 32 i + lr, columns 32 j + 8 q + 4 g .. + 3 in registers 4 q .. + 3.  The
     // tile passes through LDS as bf16 in rows of 16-byte pieces: z on its way out, the residual on its way in (each lane then
@@ -235,55 +268,86 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     leave(p.c);
 }
 
-// ---- a few rows: bound by reading b once.  A workgroup has 16 columns; its 8 waves split the contraction, load b's fragments straight
-// into registers (16 rows of 64 bytes per request, SKINNY_AHEAD requests on their way) and join their sums through LDS. ----
-constexpr int SK_AHEAD = 8;
+// The runs of a split contraction added up in their order, and the epilogue: eight columns of a row per thread.
+template <int ACT>
+__global__ __launch_bounds__(256) void dense_join_kernel(DenseArgs p) {
+    const int64_t mn = p.m * p.n, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (at >= mn) return;
+    const int64_t col = at % p.n;
+    v4f lo = *(const v4f*)(p.partial + at), hi = *(const v4f*)(p.partial + at + 4);
+    for (int s = 1; s < p.splits; ++s) {
+        lo += *(const v4f*)(p.partial + s * mn + at);
+        hi += *(const v4f*)(p.partial + s * mn + at + 4);
+    }
+    lo += epi_bias4(p.epi, col);
+    hi += epi_bias4(p.epi, col + 4);
+    if (p.epi.z) {
+        const uint2 a = pack4(lo), b = pack4(hi);
+        *(uint4*)(p.epi.z + at) = make_uint4(a.x, a.y, b.x, b.y);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lo[e] = epi_act<ACT>(lo[e]), hi[e] = epi_act<ACT>(hi[e]);
+    if (p.epi.residual) {
+        const uint4 r = *(const uint4*)(p.epi.residual + at);
+        lo += unpack4(make_uint2(r.x, r.y));
+        hi += unpack4(make_uint2(r.z, r.w));
+    }
+    const uint2 a = pack4(lo), b = pack4(hi);
+    *(uint4*)(p.c + at) = make_uint4(a.x, a.y, b.x, b.y);
+}
 
-template <int MT, int SK_WAVES, int ACT>
-__global__ __launch_bounds__(SK_WAVES * 64) void dense_few_rows_kernel(DenseArgs p) {
-    __shared__ v4f part[SK_WAVES][MT][64];
+// ---- up to 16 rows: bound by reading b once.  A workgroup has 16 NT columns; its 8 waves split the contraction, load the fragments
+// straight into registers (16 rows of 64 bytes per request, FEW_AHEAD steps on their way) and join their sums through LDS.  b
+// through the caches, although it is read once: weights up to the memory-side cache's size stay there from one token to the next.
+// us, weight cached / from memory: one row by [14336, 4096] 21.5 / 24.9, past the caches 25.4 / 27.4 (the weight alone is 24.6 at the rate of a
+// large copy); [4096, 14336] 19.3 / 24.0, with 8 steps on their way 20.9 / 28.8.  32 columns to a workgroup where that still gives 256 of them, for
+// the rows' sake: 16 rows by [14336, 4096] 31.5 / 39.0 -> 25.2 / 33.7. ----
+constexpr int FEW_AHEAD = 4;
+template <int NT, int ACT>
+__global__ __launch_bounds__(8 * 64) void dense_few_rows_kernel(DenseArgs p) {
+    constexpr int AHEAD = FEW_AHEAD, WAVES = 8;
+    __shared__ v4f part[WAVES][NT][64];
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63;
     const int row = l & 15, q = l >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 16;
-    const int steps = (int)(p.k / 32), per = (steps + SK_WAVES - 1) / SK_WAVES;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);       // n is a multiple of 32: the columns exist
+    const int steps = (int)(p.k / 32), per = (steps + WAVES - 1) / WAVES;
     const int s0 = w * per, s1 = s0 + per < steps ? s0 + per : steps;
-    const uint8_t* b = p.b + (n0 + row) * p.k * 2 + q * 16;        // n is a multiple of 32: the row exists
-    const uint8_t* a[MT];
+    const uint8_t* b = p.b + (n0 + row) * p.k * 2 + q * 16;
+    const uint8_t* a = p.a + (row < p.m ? row : p.m - 1) * p.k * 2 + q * 16;      // (a row past the end is another one's copy, not stored)
+    const int64_t b_tile = p.k * 32;
+    v4f acc[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t r = 16 * i + row < p.m ? 16 * i + row : p.m - 1;      // (a row past the end is some other row's copy, not stored)
-        a[i] = p.a + r * p.k * 2 + q * 16;
-    }
-    v4f acc[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NT; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
     int s = s0;
-    for (; s + SK_AHEAD <= s1; s += SK_AHEAD) {
-        d8bf fb[SK_AHEAD];
+    for (; s + AHEAD <= s1; s += AHEAD) {
+        d8bf fb[AHEAD][NT], fa[AHEAD];
 #pragma unroll
-        for (int u = 0; u < SK_AHEAD; ++u) fb[u] = __builtin_nontemporal_load((const d8bf*)(b + (int64_t)(s + u) * 64));
+        for (int u = 0; u < AHEAD; ++u) {
 #pragma unroll
-        for (int u = 0; u < SK_AHEAD; ++u)
+            for (int j = 0; j < NT; ++j) fb[u][j] = *(const d8bf*)(b + (int64_t)(s + u) * 64 + j * b_tile);
+            fa[u] = *(const d8bf*)(a + (int64_t)(s + u) * 64);
+        }
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u], *(const d8bf*)(a[i] + (int64_t)(s + u) * 64), acc[i], 0, 0, 0);
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][j], fa[u], acc[j], 0, 0, 0);
     }
     for (; s < s1; ++s) {
-        const d8bf fb = *(const d8bf*)(b + (int64_t)s * 64);
+        const d8bf fa = *(const d8bf*)(a + (int64_t)s * 64);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, *(const d8bf*)(a[i] + (int64_t)s * 64), acc[i], 0, 0, 0);
+        for (int j = 0; j < NT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const d8bf*)(b + (int64_t)s * 64 + j * b_tile), fa, acc[j], 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) part[w][i][l] = acc[i];
+    for (int j = 0; j < NT; ++j) part[w][j][l] = acc[j];
     __syncthreads();
     // lane (row of a = l % 16, columns 4 (l / 16) .. + 3)
-    for (int x = t; x < MT * 64; x += SK_WAVES * 64) {
-        const int i = x >> 6, ll = x & 63;
-        const int64_t r = 16 * i + (ll & 15), col = n0 + 4 * (ll >> 4);
-        v4f z = part[0][i][ll];
+    if (t < NT * 64) {
+        const int j = t >> 6;
+        const int64_t r = l & 15, col = n0 + 16 * j + 4 * (l >> 4);
+        v4f z = part[0][j][l];
 #pragma unroll
-        for (int k = 1; k < SK_WAVES; ++k) z += part[k][i][ll];
-        if (r >= p.m) continue;
+        for (int k = 1; k < WAVES; ++k) z += part[k][j][l];
+        if (r >= p.m) return;
         z += epi_bias4(p.epi, col);
         if (p.epi.z) *(uint2*)(p.epi.z + r * p.n + col) = pack4(z);
         v4f y;
@@ -378,38 +442,82 @@ static int64_t dz_run(int64_t m, int64_t n) {
     return (run + 7) / 8 * 8 < 8 ? 8 : (run + 7) / 8 * 8;
 }
 
-template <int TM, int TN, int ST, bool B_T, int ACT>
+template <int TM, int TN, int ST, bool B_T, int ACT, bool SPLIT = false>
 static int launch_dense_tile(const DenseArgs& a, hipStream_t st) {
-    constexpr int lds = dense_lds_bytes<TM, TN, ST>();
+    constexpr int lds = dense_lds_bytes<TM, TN, ST, SPLIT>();
     static std::atomic<bool> attr_set[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return MXL_ELAUNCH;
-    auto kern = dense_tile_kernel<TM, TN, ST, B_T, ACT>;
+    auto kern = dense_tile_kernel<TM, TN, ST, B_T, ACT, SPLIT>;
     if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
         if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return MXL_ELAUNCH;
         attr_set[dev & 63].store(true, std::memory_order_release);
     }
-    const int64_t tiles = ((a.m + TM - 1) / TM) * ((a.n + TN - 1) / TN), grid = (tiles + 7) / 8 * 8;
+    const int64_t tiles = ((a.m + TM - 1) / TM) * ((a.n + TN - 1) / TN) * (SPLIT ? a.splits : 1), grid = (tiles + 7) / 8 * 8;
     if (grid > 0x7FFFFFFF) return MXL_EINVAL;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, st, a);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
 
-template <int MT, int ACT>
-static void launch_few_rows(const DenseArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)(a.n / 16));
-    if (a.n / 16 >= 512) hipLaunchKernelGGL((dense_few_rows_kernel<MT, 4, ACT>), grid, dim3(4 * 64), 0, st, a);
-    else hipLaunchKernelGGL((dense_few_rows_kernel<MT, 8, ACT>), grid, dim3(8 * 64), 0, st, a);
+// How a product runs.  Tiles of 256 x 256 where they fill the chip, then of 128 x 128; below that tiles of 64 x 64, or a contraction
+// that is cut into runs, whichever the figures say: us of a slot of 64 elements with up to one workgroup of 64 x 64 on a CU, two and
+// three 0.31, 0.50, 0.70, of 128 x 128 0.60 and 0.92 with one and two; a split costs the second launch and its fp32 sums' way
+// out and in.
+struct DensePlan {
+    int tile;           // 256, 128, 64
+    int splits;         // 1: none
+    int slots;          // per run
+};
+static DensePlan dense_plan(int64_t m, int64_t n, int64_t k) {
+    auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+    const int slots = (int)((k + DT_KS - 1) / DT_KS);
+    if (tiles(256) >= 256) return {256, 1, slots};
+    if (tiles(128) >= 256) return {128, 1, slots};
+    DensePlan best{64, 1, slots};
+    double least = 1e30;
+    for (int t = 64; t <= 128; t += 64)
+        for (int s = 1; s <= 16; ++s) {
+            const int per = (slots + s - 1) / s;
+            if ((s > 1 && per < 4) || (slots + per - 1) / per != s) continue;
+            const double wgs = (double)(tiles(t) * s), held = t == 64 ? 768 : 512;
+            const double first = t == 64 ? 0.31 : 0.60, more = t == 64 ? 0.195 : 0.32;
+            const double on = wgs < held ? wgs : held;
+            const double slot = first + (on > 256 ? more * (on - 256) / 256 : 0.0);
+            const double rounds = wgs <= held ? 1.0 : wgs / held;
+            const double us = rounds * per * slot + (s > 1 ? 5.0 + (double)s * m * n * 8.0 / 4.5e6 : 0.0);
+            if (us < least) least = us, best = {t, s, per};
+        }
+    return best;
 }
 
+template <bool B_T, int ACT>
+static int launch_dense(DenseArgs a, hipStream_t st) {
+    const DensePlan plan = dense_plan(a.m, a.n, a.k);
+    if (plan.splits == 1) {
+        if (plan.tile == 128) return launch_dense_tile<128, 128, 2, B_T, ACT>(a, st);
+        return launch_dense_tile<64, 64, 3, B_T, ACT>(a, st);
+    }
+    a.splits = plan.splits;
+    a.split_slots = plan.slots;
+    const int rc = plan.tile == 128 ? launch_dense_tile<128, 128, 2, B_T, kActNone, true>(a, st) : launch_dense_tile<64, 64, 3, B_T, kActNone, true>(a, st);
+    if (rc != MXL_OK) return rc;
+    hipLaunchKernelGGL(dense_join_kernel<ACT>, dim3((unsigned)((a.m * a.n / 8 + 255) / 256)), dim3(256), 0, st, a);
+    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+}
+
+constexpr int64_t FEW_ROWS = 16;
 template <int ACT>
 static int launch_dense_forward(const DenseArgs& a, hipStream_t st) {
-    if (a.m <= 16) launch_few_rows<1, ACT>(a, st);
-    else if (a.m <= 32) launch_few_rows<2, ACT>(a, st);
-    else if (a.m <= 64) launch_few_rows<4, ACT>(a, st);
-    else if (((a.m + 127) / 128) * ((a.n + 127) / 128) >= 256) return launch_dense_tile<128, 128, 2, false, ACT>(a, st);
-    else return launch_dense_tile<64, 64, 3, false, ACT>(a, st);
-    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+    if (a.m <= FEW_ROWS) {
+        if (a.n / 32 >= 256) hipLaunchKernelGGL((dense_few_rows_kernel<2, ACT>), dim3((unsigned)(a.n / 32)), dim3(8 * 64), 0, st, a);
+        else hipLaunchKernelGGL((dense_few_rows_kernel<1, ACT>), dim3((unsigned)(a.n / 16)), dim3(8 * 64), 0, st, a);
+        return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+    }
+    if (dense_plan(a.m, a.n, a.k).tile == 256) {
+        const Bf16Args t{a.a, a.b, a.c, nullptr, 1, a.m, 0, a.n, a.k, a.epi};
+        return launch_bf16_linear_tall(t, ACT, st);
+    }
+    return launch_dense<false, ACT>(a, st);
 }
 
 static bool dense_sizes_ok(int64_t m, int64_t n, int64_t k) {
@@ -421,14 +529,23 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 using namespace mxl;
 
+extern "C" int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (!dense_sizes_ok(m, n, k)) return -1;
+    if (m == 0) return 0;
+    const int splits = dense_plan(m, n, k).splits;
+    return splits > 1 ? splits * m * n * 4 : 0;
+}
+
 extern "C" int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const void* bias, int bias_dtype, int act, const void* residual_bf16, int64_t m,
-                               int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* stream) {
+                               int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* workspace, int64_t workspace_bytes, void* stream) {
     if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (bias_dtype != MXL_DT_F32 && bias_dtype != MXL_DT_BF16)) return MXL_EINVAL;
     if (m == 0) return MXL_OK;
     if (!a_bf16 || !b_bf16 || !y_bf16) return MXL_EINVAL;
     if (!aligned16(a_bf16) || !aligned16(b_bf16) || !aligned16(bias) || !aligned16(residual_bf16) || !aligned16(y_bf16) || !aligned16(z_bf16)) return MXL_EINVAL;
+    const int64_t need = mxl_linear_bf16_workspace_bytes(m, n, k);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
-    DenseArgs d{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, (uint16_t*)y_bf16, m, n, k, {bias, (const uint16_t*)residual_bf16, (uint16_t*)z_bf16, bias_dtype == MXL_DT_F32}};
+    DenseArgs d{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, (uint16_t*)y_bf16, m, n, k, {bias, (const uint16_t*)residual_bf16, (uint16_t*)z_bf16, bias_dtype == MXL_DT_F32}, (float*)workspace, 1, 0};
     hipStream_t st = (hipStream_t)stream;
     switch (act) {
         case MXL_ACT_SILU: return launch_dense_forward<kActSilu>(d, st);
@@ -438,16 +555,20 @@ extern "C" int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const voi
     }
 }
 
-extern "C" int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* stream) {
+// da [m, k] = dz [m, n] . b [n, k]: the contraction is over n, b's slow dim
+extern "C" int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
     if (!dense_sizes_ok(m, n, k)) return MXL_EINVAL;
     if (m == 0) return MXL_OK;
     if (!dz_bf16 || !b_bf16 || !da_bf16 || !aligned16(dz_bf16) || !aligned16(b_bf16) || !aligned16(da_bf16)) return MXL_EINVAL;
+    const int64_t need = mxl_linear_bf16_workspace_bytes(m, k, n);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
-    // da [m, k] = dz [m, n] . b [n, k]: the contraction is over n, b's slow dim
-    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)b_bf16, (uint16_t*)da_bf16, m, k, n, {nullptr, nullptr, nullptr, 0}};
+    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)b_bf16, (uint16_t*)da_bf16, m, k, n, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0};
     hipStream_t st = (hipStream_t)stream;
-    if (((m + 127) / 128) * ((k + 127) / 128) >= 256) return launch_dense_tile<128, 128, 2, true, kActNone>(d, st);
-    return launch_dense_tile<64, 64, 3, true, kActNone>(d, st);
+    if (dense_plan(m, k, n).tile == 256)
+        return mxl_grouped_gemm_bf16(dz_bf16, b_bf16, da_bf16, nullptr, 1, m, k, n, MXL_BF_B_KN | MXL_BF_TILE_256, stream);
+    return launch_dense<true, kActNone>(d, st);
 }
 
 extern "C" int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n) {

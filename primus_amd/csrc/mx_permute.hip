@@ -370,7 +370,8 @@ using namespace mxl;
 
 extern "C" int64_t mxl_permute_plan_workspace_bytes(int64_t entries, int num_experts) {
     if (entries < 0 || num_experts < 1 || num_experts > MXL_MAX_GROUPS) return -1;
-    return plan_blocks(entries) * num_experts * 4;
+    const int64_t blocks = plan_blocks(entries);
+    return blocks > 1 ? blocks * num_experts * 4 : 0;
 }
 
 extern "C" int mxl_permute_plan(const int64_t* indices, int64_t entries, int num_experts, int align, int64_t rows, int64_t* row_of,
@@ -380,7 +381,8 @@ extern "C" int mxl_permute_plan(const int64_t* indices, int64_t entries, int num
     if (rows < mxl_padded_rows_bound(entries, num_experts, align) || rows > 0x7FFFFFFF || !group_lens) return MXL_EINVAL;
     if ((entries > 0 && (!indices || !row_of)) || (rows > 0 && !entry_of)) return MXL_EINVAL;
     if (row_probs && ((prob_bytes != 2 && prob_bytes != 4) || (entries > 0 && !probs))) return MXL_EINVAL;
-    if (workspace_bytes < mxl_permute_plan_workspace_bytes(entries, num_experts) || !workspace) return MXL_EINVAL;
+    const int64_t need = mxl_permute_plan_workspace_bytes(entries, num_experts);
+    if (need > 0 && (workspace_bytes < need || !workspace)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     PlanArgs a{};
     a.indices = indices, a.entries = entries, a.rows = rows, a.experts = num_experts, a.align = align;

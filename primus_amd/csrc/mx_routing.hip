@@ -449,8 +449,9 @@ __global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_kernel(RouteBwdArgs p
     }
 }
 
-// workgroups of a forward launch: rows for every wave slot of the chip at most
+// workgroups of a forward launch: rows for every wave slot of the chip at most; a few tokens are one, which writes the counts itself
 static int64_t route_blocks(int64_t tokens, int rows_per_block) {
+    if (tokens <= 16) return 1;
     int64_t b = (tokens + rows_per_block - 1) / rows_per_block;
     return b < 512 ? b : 512;
 }
@@ -480,7 +481,8 @@ using namespace mxl;
 
 extern "C" int64_t mxl_topk_routing_workspace_bytes(int64_t tokens, int experts) {
     if (tokens < 0 || experts < 1 || experts > RT_MAX_EXPERTS) return -1;
-    return route_blocks(tokens, 2) * experts * 4;
+    const int64_t blocks = route_blocks(tokens, 2);        // (two rows at least in any of the kernels)
+    return blocks > 1 ? blocks * experts * 4 : 0;
 }
 
 extern "C" int mxl_topk_routing(const void* logits, int dtype, int64_t tokens, int experts, int topk, int score, const float* expert_bias,
@@ -491,7 +493,8 @@ extern "C" int mxl_topk_routing(const void* logits, int dtype, int64_t tokens, i
         topk > group_topk * (experts / num_groups))
         return MXL_EINVAL;
     if (tokens > 0 && (!logits || !probs || !indices)) return MXL_EINVAL;
-    if (workspace_bytes < mxl_topk_routing_workspace_bytes(tokens, experts) || (tokens > 0 && !workspace)) return MXL_EINVAL;
+    const int64_t need = mxl_topk_routing_workspace_bytes(tokens, experts);
+    if (need > 0 && (workspace_bytes < need || !workspace)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     hipStream_t st = (hipStream_t)stream;
     if (tokens == 0) {

@@ -1231,6 +1231,17 @@ def _on(device: torch.device):
     return _NO_HOOK if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(entry: str, *sizes: int) -> int:
+    return int(getattr(_lib.load(), entry)(*sizes))
+
+
+def _workspace(device, entry: str, *sizes: int):
+    """``(workspace or None, its bytes)`` for an entry point's sizes."""
+    nbytes = _workspace_bytes(entry, *sizes)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes) if nbytes > 0 else (None, 0)
+
+
 def _float_type(t: torch.Tensor, what: str) -> int:
     if t.dtype not in _DT:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
@@ -1268,24 +1279,25 @@ def topk_routing_impl(logits, topk: int, score_function: str = "softmax", expert
         raise ValueError("num_groups must divide the number of experts and be at most 64")
     if not 1 <= group_topk <= num_groups or topk > group_topk * (experts // num_groups):
         raise ValueError("group_topk must be in [1, num_groups], and its groups must hold topk experts")
-    tokens = logits.shape[0]
-    if expert_bias is not None and (expert_bias.dtype != torch.float32 or tuple(expert_bias.shape) != (experts,)):
-        raise ValueError("expert_bias must be float32 [experts]")
+    tokens, dev = logits.shape[0], logits.device
+    if expert_bias is not None:
+        if expert_bias.dtype != torch.float32 or tuple(expert_bias.shape) != (experts,):
+            raise ValueError("expert_bias must be float32 [experts]")
+        _require_cuda(expert_bias)
+        _same_device(dev, expert_bias=expert_bias)
     if token_mask is not None:
         if token_mask.dtype not in (torch.bool, torch.uint8) or tuple(token_mask.shape) != (tokens,):
             raise ValueError("token_mask must be bool or uint8 [tokens]")
-    _require_cuda(expert_bias, token_mask)
-    _same_device(logits.device, expert_bias=expert_bias, token_mask=token_mask)
-    dev = logits.device
-    lib = _lib.load()
+        _require_cuda(token_mask)
+        _same_device(dev, token_mask=token_mask)
     with _on(dev), _hooked("topk_routing", tokens=tokens, experts=experts, topk=topk):
         probs = torch.empty((tokens, topk), dtype=torch.float32, device=dev)
         indices = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
-        counts = torch.empty((experts,), dtype=torch.int64, device=dev)
-        ws = torch.empty((max(int(lib.mxl_topk_routing_workspace_bytes(tokens, experts)), 16),), dtype=torch.uint8, device=dev)
-        rc = lib.mxl_topk_routing(_ptr(logits), dtype, tokens, experts, topk, score, _ptr(expert_bias), num_groups, group_topk,
-                                  int(bool(renormalize)), float(scaling_factor), _ptr(token_mask), _ptr(probs), _ptr(indices),
-                                  _ptr(counts), _ptr(ws), ws.numel(), _stream())
+        counts = torch.empty(experts, dtype=torch.int64, device=dev)
+        ws, nbytes = _workspace(dev, "mxl_topk_routing_workspace_bytes", tokens, experts)
+        rc = _lib.load().mxl_topk_routing(_ptr(logits), dtype, tokens, experts, topk, score, _ptr(expert_bias), num_groups, group_topk,
+                                          renormalize, scaling_factor, _ptr(token_mask), _ptr(probs), _ptr(indices), counts.data_ptr(),
+                                          _ptr(ws), nbytes, _stream())
     _lib.check(rc, "mxl_topk_routing")
     return probs, indices, counts
 
@@ -1334,15 +1346,14 @@ def permute_plan_impl(indices, num_experts: int, align: int = 1, probs: Optional
     if rows > 0x7FFFFFFF:
         raise ValueError("the buffer of rows must have fewer than 2^31 rows")
     dev = indices.device
-    lib = _lib.load()
     with _on(dev), _hooked("permute_plan", entries=entries, rows=rows):
         row_of = torch.empty_like(indices)
-        entry_of = torch.empty((rows,), dtype=torch.int32, device=dev)
-        lens = torch.empty((num_experts,), dtype=torch.int64, device=dev)
-        row_probs = None if probs is None else torch.empty((rows,), dtype=probs.dtype, device=dev)
-        ws = torch.empty((max(int(lib.mxl_permute_plan_workspace_bytes(entries, num_experts)), 16),), dtype=torch.uint8, device=dev)
-        rc = lib.mxl_permute_plan(_ptr(indices), entries, num_experts, align, rows, _ptr(row_of), _ptr(entry_of), _ptr(lens), _ptr(probs),
-                                  0 if probs is None else probs.element_size(), _ptr(row_probs), _ptr(ws), ws.numel(), _stream())
+        entry_of = torch.empty(rows, dtype=torch.int32, device=dev)
+        lens = torch.empty(num_experts, dtype=torch.int64, device=dev)
+        row_probs = None if probs is None else torch.empty(rows, dtype=probs.dtype, device=dev)
+        ws, nbytes = _workspace(dev, "mxl_permute_plan_workspace_bytes", entries, num_experts)
+        rc = _lib.load().mxl_permute_plan(_ptr(indices), entries, num_experts, align, rows, _ptr(row_of), _ptr(entry_of), lens.data_ptr(), _ptr(probs),
+                                          0 if probs is None else probs.element_size(), _ptr(row_probs), _ptr(ws), nbytes, _stream())
     _lib.check(rc, "mxl_permute_plan")
     return row_of, entry_of, lens, row_probs
 
@@ -1466,8 +1477,9 @@ def linear_bf16_impl(a, b, bias=None, activation: Optional[str] = None, residual
     with _on(a.device), _hooked("linear_bf16", m=m, n=n, k=k):
         y = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
         z = torch.empty_like(y) if want_z else None
+        ws, ws_bytes = _workspace(a.device, "mxl_linear_bf16_workspace_bytes", m, n, k)
         rc = _lib.load().mxl_linear_bf16(_ptr(a), _ptr(b), _ptr(bias), _lib.DT_BF16 if bias is None else _DT[bias.dtype], act, _ptr(residual), m, n, k,
-                                         _ptr(y), _ptr(z), _stream())
+                                         _ptr(y), _ptr(z), _ptr(ws), ws_bytes, _stream())
     _lib.check(rc, "mxl_linear_bf16")
     return y, z
 
@@ -1480,15 +1492,14 @@ def linear_bf16_dz_impl(dy, z, activation: Optional[str], bias_dtype: Optional[t
     if act != _lib.ACT_NONE:
         _bf16_2d(z, "z", (m, n))
     _require_cuda(dy, z)
-    lib = _lib.load()
     with _on(dy.device), _hooked("linear_bf16_dz", m=m, n=n):
         dz = torch.empty_like(dy) if act != _lib.ACT_NONE else dy
-        dbias = ws = None
+        dbias, ws, nbytes = None, None, 0
         if bias_dtype is not None:
-            dbias = torch.empty((n,), dtype=bias_dtype, device=dy.device)
-            ws = torch.empty((max(int(lib.mxl_linear_bf16_dz_workspace_bytes(m, n)), 16),), dtype=torch.uint8, device=dy.device)
-        rc = lib.mxl_linear_bf16_dz(_ptr(dy), None if act == _lib.ACT_NONE else _ptr(z), act, m, n, None if act == _lib.ACT_NONE else _ptr(dz), _ptr(dbias),
-                                    _lib.DT_BF16 if bias_dtype is None else _DT[bias_dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream())
+            dbias = torch.empty(n, dtype=bias_dtype, device=dy.device)
+            ws, nbytes = _workspace(dy.device, "mxl_linear_bf16_dz_workspace_bytes", m, n)
+        rc = _lib.load().mxl_linear_bf16_dz(_ptr(dy), None if act == _lib.ACT_NONE else _ptr(z), act, m, n, None if act == _lib.ACT_NONE else _ptr(dz), _ptr(dbias),
+                                    _lib.DT_BF16 if bias_dtype is None else _DT[bias_dtype], _ptr(ws), nbytes, _stream())
     _lib.check(rc, "mxl_linear_bf16_dz")
     return dz, dbias
 
@@ -1506,7 +1517,8 @@ def linear_bf16_dgrad_impl(dz, b) -> torch.Tensor:
     _same_device(dz.device, b=b)
     with _on(dz.device), _hooked("linear_bf16_dgrad", m=m, n=n, k=k):
         da = torch.empty((m, k), dtype=torch.bfloat16, device=dz.device)
-        rc = _lib.load().mxl_linear_bf16_dgrad(_ptr(dz), _ptr(b), m, n, k, _ptr(da), _stream())
+        ws, ws_bytes = _workspace(dz.device, "mxl_linear_bf16_workspace_bytes", m, k, n)
+        rc = _lib.load().mxl_linear_bf16_dgrad(_ptr(dz), _ptr(b), m, n, k, _ptr(da), _ptr(ws), ws_bytes, _stream())
     _lib.check(rc, "mxl_linear_bf16_dgrad")
     return da
 

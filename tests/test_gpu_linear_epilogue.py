@@ -48,9 +48,11 @@ def _inputs(gpu, m, n, k, seed, bias_dtype=torch.bfloat16):
     return r(m, k).bfloat16(), (r(n, k) * 1.5 * k ** -0.5).bfloat16(), r(n).to(bias_dtype), r(m, n).bfloat16(), r(m, n).bfloat16()
 
 
-# few rows (1, 2 and 4 fragments of 16), 64 x 64 tiles, 128 x 128 tiles, odd halves of a slot, ragged last tiles, long contractions
+# few rows (1, 2 and 4 fragments of 16), 64 x 64 tiles, 128 x 128 tiles, 256 x 256 tiles, odd halves of a slot, ragged last tiles, long and
+# split contractions
 SIZES = [(1, 32, 32), (1, 4096, 1056), (7, 96, 4096), (16, 64, 288), (17, 160, 96), (33, 320, 800), (64, 2880, 64), (65, 96, 32), (100, 32, 2080), (127, 224, 160),
-         (129, 416, 64), (300, 512, 1120), (777, 1056, 96), (2051, 2880, 96), (2100, 2080, 160), (4096, 1024, 4096), (1000, 2048, 14336)]
+         (129, 416, 64), (300, 512, 1120), (777, 1056, 96), (2051, 2880, 96), (2100, 2080, 160), (4096, 1024, 4096), (1000, 2048, 14336),
+         (4200, 4128, 32), (4353, 4160, 160), (70, 64, 1056), (130, 128, 4128), (333, 4096, 2048)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)

@@ -94,10 +94,10 @@ def test_c_entries_check_before_they_touch_the_device():
     buf = ctypes.create_string_buffer(1 << 16)
     p = ctypes.cast(buf, ctypes.c_void_p)
     f = ctypes.c_float(1.0)
-    ws = lib.mxl_topk_routing_workspace_bytes(4, 8)
-    route = lambda **k: lib.mxl_topk_routing(*[{**dict(l=p, dt=0, t=4, e=8, k=2, s=0, b=None, g=1, gk=1, r=1, sc=f, m=None, pr=p, i=p, c=p, w=p, wb=ws, st=None), **k}[n]  # noqa: E731
+    ws = lib.mxl_topk_routing_workspace_bytes(40, 8)
+    route = lambda **k: lib.mxl_topk_routing(*[{**dict(l=p, dt=0, t=40, e=8, k=2, s=0, b=None, g=1, gk=1, r=1, sc=f, m=None, pr=p, i=p, c=p, w=p, wb=ws, st=None), **k}[n]  # noqa: E731
                                                for n in ("l", "dt", "t", "e", "k", "s", "b", "g", "gk", "r", "sc", "m", "pr", "i", "c", "w", "wb", "st")])
-    assert route() == -3
+    assert ws > 0 and route() == -3 and lib.mxl_topk_routing_workspace_bytes(16, 8) == 0 and route(t=16, w=None, wb=0) == -3
     for bad in (dict(l=None), dict(dt=3), dict(t=-1), dict(e=0), dict(e=1025), dict(k=0), dict(k=9), dict(s=2), dict(g=3), dict(g=2, gk=3), dict(g=8, gk=1),
                 dict(pr=None), dict(i=None), dict(c=None), dict(w=None), dict(wb=ws - 1)):
         assert route(**bad) == -1, bad
@@ -106,12 +106,12 @@ def test_c_entries_check_before_they_touch_the_device():
     assert bwd() == -3 and bwd(t=0) == 0
     for bad in (dict(d=None), dict(o=None), dict(dt=-1), dict(k=33), dict(e=2000)):
         assert bwd(**bad) == -1, bad
-    pw = lib.mxl_permute_plan_workspace_bytes(8, 4)
-    plan = lambda **k: lib.mxl_permute_plan(*[{**dict(i=p, n=8, e=4, a=1, r=8, ro=p, eo=p, gl=p, pr=None, pb=0, rp=None, w=p, wb=pw, st=None), **k}[n]  # noqa: E731
+    pw = lib.mxl_permute_plan_workspace_bytes(5000, 4)
+    plan = lambda **k: lib.mxl_permute_plan(*[{**dict(i=p, n=5000, e=4, a=1, r=5000, ro=p, eo=p, gl=p, pr=None, pb=0, rp=None, w=p, wb=pw, st=None), **k}[n]  # noqa: E731
                                               for n in ("i", "n", "e", "a", "r", "ro", "eo", "gl", "pr", "pb", "rp", "w", "wb", "st")])
-    assert plan() == -3
-    for bad in (dict(i=None), dict(n=-1), dict(e=0), dict(e=1025), dict(a=0), dict(r=7), dict(ro=None), dict(eo=None), dict(gl=None), dict(pr=p, pb=3, rp=p), dict(pb=4, rp=p),
-                dict(w=None), dict(wb=pw - 1), dict(a=32, r=8)):
+    assert pw > 0 and plan() == -3 and lib.mxl_permute_plan_workspace_bytes(8, 4) == 0 and plan(n=8, w=None, wb=0) == -3
+    for bad in (dict(i=None), dict(n=-1), dict(e=0), dict(e=1025), dict(a=0), dict(r=4999), dict(ro=None), dict(eo=None), dict(gl=None), dict(pr=p, pb=3, rp=p), dict(pb=4, rp=p),
+                dict(w=None), dict(wb=pw - 1), dict(a=32, r=5000)):
         assert plan(**bad) == -1, bad
     assert lib.mxl_permute_rows(p, 4, 16, p, 2, p, 8, p, None) == -3
     assert lib.mxl_permute_rows(p, 4, 0, p, 2, p, 8, p, None) == -1 and lib.mxl_permute_rows(p, 4, 16, p, 33, p, 8, p, None) == -1
@@ -122,15 +122,19 @@ def test_c_entries_check_before_they_touch_the_device():
     assert lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, p, 4, 2, p, 0, p, p, None) == -3
     assert lib.mxl_combine_rows_bwd(None, p, 8, 16, 1, p, p, 4, 2, p, 0, p, p, None) == -1 and lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, p, 4, 2, None, 0, p, p, None) == -1
     assert lib.mxl_combine_rows_bwd(p, p, 8, 16, 1, p, None, 4, 2, p, 0, p, p, None) == -1
-    lin = lambda **k: lib.mxl_linear_bf16(*[{**dict(a=p, b=p, bias=p, bd=1, act=3, r=p, m=4, n=32, k=32, y=p, z=None, st=None), **k}[n]  # noqa: E731
-                                            for n in ("a", "b", "bias", "bd", "act", "r", "m", "n", "k", "y", "z", "st")])
+    lin = lambda **k: lib.mxl_linear_bf16(*[{**dict(a=p, b=p, bias=p, bd=1, act=3, r=p, m=4, n=32, k=32, y=p, z=None, w=None, wb=0, st=None), **k}[n]  # noqa: E731
+                                            for n in ("a", "b", "bias", "bd", "act", "r", "m", "n", "k", "y", "z", "w", "wb", "st")])
     odd = ctypes.c_void_p(p.value + 8)
     assert p.value % 16 == 0 and lin() == -3 and lin(m=0) == 0
     for bad in (dict(a=None), dict(b=None), dict(y=None), dict(bd=2), dict(act=4), dict(act=-1), dict(m=-1), dict(n=48), dict(k=8), dict(n=0), dict(n=1 << 16, k=1 << 16),
-                dict(a=odd), dict(b=odd), dict(bias=odd), dict(r=odd), dict(y=odd), dict(z=odd)):
+                dict(a=odd), dict(b=odd), dict(bias=odd), dict(r=odd), dict(y=odd), dict(z=odd), dict(m=128, n=128, k=4096), dict(m=128, n=128, k=4096, w=p, wb=64)):
         assert lin(**bad) == -1, bad
-    assert lib.mxl_linear_bf16_dgrad(p, p, 4, 32, 32, p, None) == -3 and lib.mxl_linear_bf16_dgrad(p, p, 4, 32, 33, p, None) == -1
-    assert lib.mxl_linear_bf16_dgrad(None, p, 4, 32, 32, p, None) == -1 and lib.mxl_linear_bf16_dgrad(p, p, 0, 32, 32, p, None) == 0
+    need = lib.mxl_linear_bf16_workspace_bytes(128, 128, 4096)
+    assert need > 0 and lin(m=128, n=128, k=4096, w=p, wb=need) == -3 and lib.mxl_linear_bf16_workspace_bytes(4096, 4096, 4096) == 0
+    assert lib.mxl_linear_bf16_workspace_bytes(1, 1, 1) == -1
+    dgrad = lambda a, b, m, n, k, w=None, wb=0: lib.mxl_linear_bf16_dgrad(a, b, m, n, k, p, w, wb, None)  # noqa: E731
+    assert dgrad(p, p, 4, 32, 32) == -3 and dgrad(p, p, 4, 32, 33) == -1 and dgrad(None, p, 4, 32, 32) == -1 and dgrad(p, p, 0, 32, 32) == 0
+    assert dgrad(p, p, 128, 4096, 128) == -1 and dgrad(p, p, 128, 4096, 128, p, need) == -3
     ws = lib.mxl_linear_bf16_dz_workspace_bytes(4, 32)
     dz = lambda **k: lib.mxl_linear_bf16_dz(*[{**dict(dy=p, z=p, act=1, m=4, n=32, dz=p, db=p, dbd=0, w=p, wb=ws, st=None), **k}[n] for n in ("dy", "z", "act", "m", "n", "dz", "db", "dbd", "w", "wb", "st")])  # noqa: E731
     assert ws == 128 and dz() == -3 and dz(act=3, db=None) == 0
