@@ -618,6 +618,9 @@ int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int 
  * dbias = column sums of dz before its rounding (NULL: not wanted); mxl_linear_bf16_dgrad gives da = dz . b;
  * db = dz^T . a is mxl_grouped_gemm_bf16_wgrad with one group. */
 int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t k);
+/* What a product of these sizes runs on, worked out on the host: output tile and runs of the contraction (the forward of up to 16 rows
+ * has a kernel of its own). */
+int mxl_linear_bf16_plan(int64_t m, int64_t n, int64_t k, int* tile_rows, int* tile_cols, int* splits);
 int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const void* bias, int bias_dtype, int act, const void* residual_bf16, int64_t m,
                     int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* workspace, int64_t workspace_bytes, void* stream);
 int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* workspace,

@@ -6,7 +6,7 @@
 //   backward: dz = dy act'(z),  da = dz . b,  db = dz^T . a,  dbias = column sums of dz
 //
 // The weight gradient, and the products of many rows, run on the grouped kernels' tiles (mx_gemm_bf16.hip) with one group.  This
-// file holds the tiles of 128 x 128 and 64 x 64 for fewer rows, the kernel for a few rows, which is bound by reading b, and
+// file holds the tiles of 256 x 128 and 64 x 64 for fewer rows, the kernel for a few rows, which is bound by reading b, and
 // the elementwise part of the backward.
 #include "mx_gemm_bf16.h"
 #include "mx_gemm_common.h"
@@ -33,13 +33,16 @@ template <int TM, int TN, int ST, bool SPLIT> constexpr int dense_lds_bytes() {
     return loop > out ? loop : out;
 }
 
-// ---- tiles: 4 waves (2 x 2), LDS-direct loads into ST stages, one workgroup per tile, two or three of them on a CU so that one's
-// epilogue and waits run under another's MFMAs.  B_T: b is [k, n], read with the transposing LDS read.
+// ---- tiles: WM x 2 waves, LDS-direct loads into three stages.  64 x 64: 4 waves, up to three workgroups on a CU, so that one's epilogue and
+// waits run under another's MFMAs.  256 x 128: 8 waves of 64 x 64, two on a SIMD; a wave reads 1 KiB of LDS per MFMA, which with the
+// fills makes 1375 clocks of LDS for 1024 of MFMAs in a slot.  B_T: b is [k, n], read with the transposing LDS read.
 // SPLIT: the contraction is cut into `splits` runs of slots, a workgroup each, whose fp32 sums dense_join_kernel adds up. ----
-template <int TM, int TN, int ST, bool B_T, int ACT, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
-    constexpr int FM = TM / 64, FN = TN / 64;              // 32 x 32 fragments per wave
-    constexpr int AR = TM / 32, BR = TN / 32, R = AR + BR;  // load rounds of 4 KiB
+template <int TM, int TN, int WM, int ST, bool B_T, int ACT, bool SPLIT>
+__global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
+    constexpr int THREADS = WM * 128, WROWS = TM / WM;     // waves WM x 2; rows of a wave
+    constexpr int FM = WROWS / 32, FN = TN / 64;           // 32 x 32 fragments per wave
+    constexpr int ROUND = THREADS * 16;                    // bytes of a load round
+    constexpr int AR = TM * 128 / ROUND, BR = TN * 128 / ROUND, R = AR + BR;
     constexpr int A_BYTES = TM * DT_KS * 2, STAGE = A_BYTES + TN * DT_KS * 2;
     constexpr int BT_PIECES = TN / 8;                       // 16-byte pieces of a staged row of the transposed operand
     constexpr int BT_SHIFT = TN == 128 ? 2 : 1;
@@ -47,7 +50,7 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     const int t = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int l = t & 63, lr = l & 31, g = l >> 5;
-    const int wm = w >> 1, wn = w & 1;
+    const int wm = WM == 4 ? w & 3 : w >> 1, wn = WM == 4 ? w >> 2 : w & 1;      // the two waves of a SIMD hold the same rows
 
     // the tile: each XCD takes one contiguous run of the order, super-rows of 1024 rows
     const int tiles_m = (int)((p.m + TM - 1) / TM), tiles_n = (int)((p.n + TN - 1) / TN);
@@ -82,34 +85,43 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     uint32_t va[AR], vb[BR];
 #pragma unroll
     for (int e = 0; e < AR; ++e) {
-        const int row = (t >> 3) + 32 * e;
+        const int row = (t >> 3) + THREADS / 8 * e;
         va[e] = (uint32_t)(row * lda + 16 * ((t & 7) ^ ((row >> 1) & 7)));
     }
 #pragma unroll
     for (int e = 0; e < BR; ++e) {
         if constexpr (B_T) {
-            const int row = t / BT_PIECES + (256 / BT_PIECES) * e;
+            const int row = t / BT_PIECES + (THREADS / BT_PIECES) * e;
             vb[e] = (uint32_t)(row * ldb + 16 * ((t % BT_PIECES) ^ ((row & 3) << BT_SHIFT)));
         } else {
-            const int row = (t >> 3) + 32 * e;
+            const int row = (t >> 3) + THREADS / 8 * e;
             vb[e] = (uint32_t)(row * ldb + 16 * ((t & 7) ^ ((row >> 1) & 7)));
         }
     }
     const uint32_t wave_base = (uint32_t)(uintptr_t)smem + (uint32_t)(w * 1024);
-    auto issue = [&](int s, int stage) __attribute__((always_inline)) {
-        const uint32_t base = wave_base + (uint32_t)(stage * STAGE);
-        const bool live = s < slots;        // past the range the requests are dropped, but counted
-        const uint32_t sa = live ? (uint32_t)s * a_step : addr::kDropped, sb = live ? (uint32_t)s * b_step : addr::kDropped;
-        static_for<0, AR>([&](auto e) { dma16_at<decltype(e)::value * 4096>(ra, base, va[decltype(e)::value], sa); });
-        static_for<0, BR>([&](auto e) { dma16_at<A_BYTES + decltype(e)::value * 4096>(rb, base, vb[decltype(e)::value], sb); });
+    // requests of slot s into a stage; past the range they are dropped, but counted
+    struct In {
+        uint32_t base, sa, sb;
+    };
+    auto in_begin = [&](int s, int stage) __attribute__((always_inline)) {
+        const bool in = s < slots;
+        return In{wave_base + (uint32_t)(stage * STAGE), in ? (uint32_t)s * a_step : addr::kDropped, in ? (uint32_t)s * b_step : addr::kDropped};
+    };
+    auto request = [&](auto e_tag, const In& r) __attribute__((always_inline)) {
+        constexpr int e = decltype(e_tag)::value;
+        if constexpr (e < AR) dma16_at<e * ROUND>(ra, r.base, va[e], r.sa);
+        else dma16_at<A_BYTES + (e - AR) * ROUND>(rb, r.base, vb[e - AR], r.sb);
     };
 
     // fragment reads: contiguous, row lr, piece 2 ks + g XOR (row / 2) % 8; transposed, this lane addresses row tj of a 4-row
     // group, 8-byte piece ta4 of its 16-lane block's 16 columns
     const int lane_c = lr * 128 + 16 * (g ^ ((lr >> 1) & 7));
     const int tj = (l & 15) >> 2, ta4 = l & 3, tblk = (l >> 4) & 1;
+    struct Frag {
+        d8bf a[FM], b[FN];
+    };
     auto read_a = [&](uint8_t* st, int i, int ks) __attribute__((always_inline)) {
-        return *(const d8bf*)(st + ((lane_c + wm * (TM / 2) * 128) ^ (32 * ks)) + i * 4096);
+        return *(const d8bf*)(st + ((lane_c + wm * WROWS * 128) ^ (32 * ks)) + i * 4096);
     };
     auto read_b = [&](uint8_t* st, int j, int ks) __attribute__((always_inline)) {
         if constexpr (!B_T) {
@@ -135,34 +147,94 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    const bool live = __builtin_amdgcn_readfirstlane(wm * (TM / 2) < m_valid);
+    const bool live = __builtin_amdgcn_readfirstlane(wm * WROWS < m_valid);
 
-    for (int s = 0; s < ST - 1; ++s) issue(s_first + s, s);
+    static_for<0, ST - 1>([&](auto s) {
+        const In r = in_begin(s_first + decltype(s)::value, decltype(s)::value);
+        static_for<0, R>([&](auto e) { request(e, r); });
+    });
+    // A step's fragments are read behind the MFMAs of the step before (pinned: on its own the compiler reads them in front of their
+    // MFMAs and waits).  A slot's barrier stands one MFMA into its last step: by then every wave holds all its fragments of the
+    // slot, so its stage is free, and the next slot's first fragments and the requests of slot s + ST go out behind the MFMAs
+    // that are left and those of the next step.  (Barrier in front of the slot, its first fragments behind it: 71 us instead of 58 for
+    // [2048, 4096] x 4096, 48 instead of 41 for [2051, 2880] x 2880.)
+    constexpr int NM = FM * FN, NX = FM + FN, NL = NM - 1;      // MFMAs and reads of a step; MFMAs behind the barrier
+    constexpr int Q = NL + NM, E3 = NM == 1 ? R : NL * R / Q;   // places for requests; of them in the last step
+    const int full = slots - s_first - (odd && slots == all_slots ? 1 : 0);      // slots of four steps
     int stage = 0;
-    for (int s = s_first; s < slots; ++s) {
-        wait_vm<(ST - 2) * R>();        // slot s has landed
-        __syncthreads();                // ... for every wave, and every wave has left the stage of slot s - 1
-        issue(s + ST - 1, stage == 0 ? ST - 1 : stage - 1);
-        uint8_t* st = smem + stage * STAGE;
-        stage = stage == ST - 1 ? 0 : stage + 1;
-        if (!live) continue;
-        const int steps = odd && s == all_slots - 1 ? 2 : 4;
-        auto step = [&](int ks) __attribute__((always_inline)) {
-            d8bf fa[FM], fb[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = read_b(st, j, ks);
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = read_a(st, i, ks);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+    In in = in_begin(s_first + ST - 1, ST - 1);
+    if (live) {
+        static_for<0, E3>([&](auto e) { request(e, in); });
+        wait_vm<(ST - 2) * R + E3>();       // the first slot has landed
+        __syncthreads();
+        Frag f[2];
+        auto read = [&](auto x_tag, auto ks_tag, uint8_t* st) __attribute__((always_inline)) {
+            constexpr int x = decltype(x_tag)::value, ks = decltype(ks_tag)::value;
+            if constexpr (x < FN) f[ks & 1].b[x] = read_b(st, x, ks);
+            else f[ks & 1].a[x - FN] = read_a(st, x - FN, ks);
         };
-        step(0);
-        step(1);
-        if (steps == 4) {
-            step(2);
-            step(3);
+        auto multiply = [&](auto m_tag, auto ks_tag) __attribute__((always_inline)) {
+            constexpr int m = decltype(m_tag)::value, ks = decltype(ks_tag)::value, i = m % FM, j = m / FM;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[ks & 1].b[j], f[ks & 1].a[i], acc[i][j], 0, 0, 0);
+        };
+        auto step = [&](auto ks_tag, uint8_t* st) __attribute__((always_inline)) {       // ks 0 .. 2
+            constexpr int ks = decltype(ks_tag)::value;
+            static_for<0, NM>([&](auto m_tag) {
+                constexpr int m = decltype(m_tag)::value;
+                multiply(m_tag, ks_tag);
+                static_for<m * NX / NM, (m + 1) * NX / NM>([&](auto x) { read(x, std::integral_constant<int, ks + 1>{}, st); });
+                if constexpr (ks == 0 && NM > 1) {
+                    constexpr int q = NL + m;
+                    static_for<q * R / Q, (q + 1) * R / Q>([&](auto e) { request(e, in); });
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        constexpr std::integral_constant<int, 0> k0{};
+        constexpr std::integral_constant<int, 3> k3{};
+        static_for<0, NX>([&](auto x) { read(x, k0, smem); });
+        for (int s = 0; s < full; ++s) {
+            uint8_t* st = smem + stage * STAGE;
+            const int nstage = stage == ST - 1 ? 0 : stage + 1;
+            step(k0, st);
+            step(std::integral_constant<int, 1>{}, st);
+            step(std::integral_constant<int, 2>{}, st);
+            multiply(k0, k3);
+            wait_vm<(ST - 2) * R>();        // slot s + 1 has landed
+            __syncthreads();                // ... for every wave, and every wave holds its fragments of slot s
+            in = in_begin(s_first + s + ST, stage);
+            __builtin_amdgcn_sched_barrier(0);
+            uint8_t* nx = smem + nstage * STAGE;
+            if constexpr (NM == 1) {
+                static_for<0, NX>([&](auto x) { read(x, k0, nx); });
+                static_for<0, R>([&](auto e) { request(e, in); });
+            } else {
+                static_for<1, NM>([&](auto m_tag) {
+                    constexpr int m = decltype(m_tag)::value, q = m - 1;
+                    multiply(m_tag, k3);
+                    static_for<(q * NX + NL - 1) / NL, ((q + 1) * NX + NL - 1) / NL>([&](auto x) { read(x, k0, nx); });
+                    static_for<q * R / Q, (q + 1) * R / Q>([&](auto e) { request(e, in); });
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            }
+            stage = nstage;
+        }
+        if (full < slots - s_first) {       // the contraction's last slot of two steps
+            uint8_t* st = smem + stage * STAGE;
+            step(k0, st);
+            static_for<0, NM>([&](auto m_tag) { multiply(m_tag, std::integral_constant<int, 1>{}); });
+        }
+    } else {
+        // none of the tile's rows are this wave's: it only keeps its share of the requests going
+        static_for<0, R>([&](auto e) { request(e, in); });
+        wait_vm<(ST - 1) * R>();
+        __syncthreads();
+        for (int s = 0; s < full; ++s) {
+            wait_vm<(ST - 2) * R>();
+            __syncthreads();
+            in = in_begin(s_first + s + ST, stage);
+            static_for<0, R>([&](auto e) { request(e, in); });
+            stage = stage == ST - 1 ? 0 : stage + 1;
         }
     }
     wait_vm<0>();
@@ -176,15 +248,15 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
             for (int j = 0; j < FN; ++j)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *(v4f*)(smem + (wm * (TM / 2) + i * 32 + lr) * FP + (wn * (TN / 2) + j * 32 + 8 * q + 4 * g) * 4) =
+                    *(v4f*)(smem + (wm * WROWS + i * 32 + lr) * FP + (wn * (TN / 2) + j * 32 + 8 * q + 4 * g) * 4) =
                         v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
         __syncthreads();
         const int fr = t / FL, fc = (t % FL) * 4;
         float* out = p.partial + ((int64_t)split * p.m + m0) * p.n + n0 + fc;
         if (fc < n_valid) {
 #pragma unroll
-            for (int u = 0; u < TM / (256 / FL); ++u) {
-                const int row = u * (256 / FL) + fr;
+            for (int u = 0; u < TM / (THREADS / FL); ++u) {
+                const int row = u * (THREADS / FL) + fr;
                 if (row < m_valid) *(v4f*)(out + (int64_t)row * p.n) = *(const v4f*)(smem + row * FP + fc * 4);
             }
         }
@@ -194,11 +266,11 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     // ---- epilogue.  Lane (lr, g) of fragment (i, j) holds row 32 i + lr, columns 32 j + 8 q + 4 g .. + 3 in registers 4 q .. + 3.  The
     // tile passes through LDS as bf16 in rows of 16-byte pieces: z on its way out, the residual on its way in (each lane then
     // finds its own four columns' values where it puts its results), y on its way out. ----
-    constexpr int PITCH = TN * 2 + 16, LPR = TN / 8, RPI = 256 / LPR;
+    constexpr int PITCH = TN * 2 + 16, LPR = TN / 8, RPI = THREADS / LPR;
     const int rr = t / LPR, cc = (t % LPR) * 8;
     const int64_t c0 = m0 * p.n + n0;
     auto spot = [&](int i, int j, int q) __attribute__((always_inline)) {
-        return (uint2*)(smem + (wm * (TM / 2) + i * 32 + lr) * PITCH + (wn * (TN / 2) + j * 32 + 8 * q + 4 * g) * 2);
+        return (uint2*)(smem + (wm * WROWS + i * 32 + lr) * PITCH + (wn * (TN / 2) + j * 32 + 8 * q + 4 * g) * 2);
     };
     auto leave = [&](uint16_t* out) __attribute__((always_inline)) {
         if (cc < n_valid) {
@@ -442,51 +514,61 @@ static int64_t dz_run(int64_t m, int64_t n) {
     return (run + 7) / 8 * 8 < 8 ? 8 : (run + 7) / 8 * 8;
 }
 
-template <int TM, int TN, int ST, bool B_T, int ACT, bool SPLIT = false>
+template <int TM, int TN, int WM, int ST, bool B_T, int ACT, bool SPLIT = false>
 static int launch_dense_tile(const DenseArgs& a, hipStream_t st) {
     constexpr int lds = dense_lds_bytes<TM, TN, ST, SPLIT>();
     static std::atomic<bool> attr_set[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return MXL_ELAUNCH;
-    auto kern = dense_tile_kernel<TM, TN, ST, B_T, ACT, SPLIT>;
+    auto kern = dense_tile_kernel<TM, TN, WM, ST, B_T, ACT, SPLIT>;
     if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
         if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return MXL_ELAUNCH;
         attr_set[dev & 63].store(true, std::memory_order_release);
     }
     const int64_t tiles = ((a.m + TM - 1) / TM) * ((a.n + TN - 1) / TN) * (SPLIT ? a.splits : 1), grid = (tiles + 7) / 8 * 8;
     if (grid > 0x7FFFFFFF) return MXL_EINVAL;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, st, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(WM * 128), lds, st, a);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
 
-// How a product runs.  Tiles of 256 x 256 where they fill the chip, then of 128 x 128; below that tiles of 64 x 64, or a contraction
-// that is cut into runs, whichever the figures say: us of a slot of 64 elements with up to one workgroup of 64 x 64 on a CU, two and
-// three 0.31, 0.50, 0.70, of 128 x 128 0.60 and 0.92 with one and two; a split costs the second launch and its fp32 sums' way
-// out and in.
+// How a product runs: tiles of 256 x 256 where they fill the chip; below that whichever of the four tiles, with the contraction in one
+// or several runs, these figures make the soonest done.  us of a slot of 64 elements, half with the weight cached and half with it from
+// memory, by the workgroups there are (w, of 256 CUs):
+//   256 x 256  1.12 + 0.42 w / 256                    one on a CU
+//   256 x 128  0.54 + 0.28 (w / 256)^2                one on a CU
+//   64 x 64    0.30 up to 256, 0.45 with two on every CU, 0.63 with three
+// and a split costs 4 us for the second launch and its fp32 sums' way out and in at 7 TB/s.  Forward, us, weight cached / from memory, 256 x 256,
+// 256 x 128 and 64 x 64 unsplit: [2048, 4096] x 4096 88 / 82, 58 / 61, 108 / 118; [1500, 2880] x 2880 55 / 66, 31 / 37, 46 / 51;
+// [4096, 2880] x 2880 77 / 69, 73 / 77, 118 / 121; [1000, 2048] x 2048 41 / 48, 23 / 27, 15 / 18.  256 x 128 in several runs: [333, 14336] x
+// 4096 120 / 133, four 50 / 53 (64 x 64 unsplit 76 / 104); [700, 4096] x 4096 40 / 47, two 34 / 36; [2048, 8192] x 2048 82 / 85, two
+// 68 / 70.  (128 x 128, two workgroups on a CU, is level with 256 x 128 where the weight is cached and behind where it is not: 62 / 70, 34 / 41, 75 / 92
+// for the first three; [333, 14336] x 4096 in four 53 / 65.)
 struct DensePlan {
-    int tile;           // 256, 128, 64
-    int splits;         // 1: none
-    int slots;          // per run
+    int tm, tn;         // output tile
+    int splits;         // runs of the contraction, 1: not split
+    int slots;          // slots per run
 };
 static DensePlan dense_plan(int64_t m, int64_t n, int64_t k) {
-    auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+    auto tiles = [&](int tm, int tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
     const int slots = (int)((k + DT_KS - 1) / DT_KS);
-    if (tiles(256) >= 256) return {256, 1, slots};
-    if (tiles(128) >= 256) return {128, 1, slots};
-    DensePlan best{64, 1, slots};
-    double least = 1e30;
-    for (int t = 64; t <= 128; t += 64)
+    DensePlan best{256, 256, 1, slots};
+    const double tall = (double)tiles(256, 256);
+    if (tall >= 256) return best;
+    double least = slots * (1.12 + 0.42 * tall / 256);
+    auto consider = [&](int tm, int tn, double held, auto us_of) {
         for (int s = 1; s <= 16; ++s) {
             const int per = (slots + s - 1) / s;
             if ((s > 1 && per < 4) || (slots + per - 1) / per != s) continue;
-            const double wgs = (double)(tiles(t) * s), held = t == 64 ? 768 : 512;
-            const double first = t == 64 ? 0.31 : 0.60, more = t == 64 ? 0.195 : 0.32;
-            const double on = wgs < held ? wgs : held;
-            const double slot = first + (on > 256 ? more * (on - 256) / 256 : 0.0);
-            const double rounds = wgs <= held ? 1.0 : wgs / held;
-            const double us = rounds * per * slot + (s > 1 ? 5.0 + (double)s * m * n * 8.0 / 4.5e6 : 0.0);
-            if (us < least) least = us, best = {t, s, per};
+            const double wgs = (double)(tiles(tm, tn) * s), rounds = wgs / held;
+            // workgroups beyond those the chip holds start as others end: between their share of a round and a whole one
+            const double passes = rounds <= 1.0 ? 1.0 : 0.5 * (rounds + (double)(int64_t)(rounds + 0.999999));
+            const double us = passes * per * us_of((rounds < 1.0 ? wgs : held) / 256) + (s > 1 ? 4.0 + (double)s * (double)m * (double)n * 8.0 / 7e6 : 0.0);
+            if (us < least) least = us, best = {tm, tn, s, per};
         }
+    };
+    auto part = [](double x, double lo, double hi) { return x <= lo ? 0.0 : x >= hi ? 1.0 : (x - lo) / (hi - lo); };
+    consider(256, 128, 256, [&](double w) { return 0.54 + 0.28 * w * w; });
+    consider(64, 64, 768, [&](double w) { return 0.30 + 0.15 * part(w, 1.0, 2.0) + 0.18 * part(w, 2.0, 3.0); });
     return best;
 }
 
@@ -494,12 +576,13 @@ template <bool B_T, int ACT>
 static int launch_dense(DenseArgs a, hipStream_t st) {
     const DensePlan plan = dense_plan(a.m, a.n, a.k);
     if (plan.splits == 1) {
-        if (plan.tile == 128) return launch_dense_tile<128, 128, 2, B_T, ACT>(a, st);
-        return launch_dense_tile<64, 64, 3, B_T, ACT>(a, st);
+        if (plan.tm == 256) return launch_dense_tile<256, 128, 4, 3, B_T, ACT>(a, st);
+        return launch_dense_tile<64, 64, 2, 3, B_T, ACT>(a, st);
     }
     a.splits = plan.splits;
     a.split_slots = plan.slots;
-    const int rc = plan.tile == 128 ? launch_dense_tile<128, 128, 2, B_T, kActNone, true>(a, st) : launch_dense_tile<64, 64, 3, B_T, kActNone, true>(a, st);
+    const int rc = plan.tm == 256 ? launch_dense_tile<256, 128, 4, 3, B_T, kActNone, true>(a, st)
+                                 : launch_dense_tile<64, 64, 2, 3, B_T, kActNone, true>(a, st);
     if (rc != MXL_OK) return rc;
     hipLaunchKernelGGL(dense_join_kernel<ACT>, dim3((unsigned)((a.m * a.n / 8 + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
@@ -513,7 +596,7 @@ static int launch_dense_forward(const DenseArgs& a, hipStream_t st) {
         else hipLaunchKernelGGL((dense_few_rows_kernel<1, ACT>), dim3((unsigned)(a.n / 16)), dim3(8 * 64), 0, st, a);
         return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
     }
-    if (dense_plan(a.m, a.n, a.k).tile == 256) {
+    if (dense_plan(a.m, a.n, a.k).tn == 256) {
         const Bf16Args t{a.a, a.b, a.c, nullptr, 1, a.m, 0, a.n, a.k, a.epi};
         return launch_bf16_linear_tall(t, ACT, st);
     }
@@ -534,6 +617,13 @@ extern "C" int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t
     if (m == 0) return 0;
     const int splits = dense_plan(m, n, k).splits;
     return splits > 1 ? splits * m * n * 4 : 0;
+}
+
+extern "C" int mxl_linear_bf16_plan(int64_t m, int64_t n, int64_t k, int* tile_rows, int* tile_cols, int* splits) {
+    if (!dense_sizes_ok(m, n, k) || m == 0 || !tile_rows || !tile_cols || !splits) return MXL_EINVAL;
+    const DensePlan plan = dense_plan(m, n, k);
+    *tile_rows = plan.tm, *tile_cols = plan.tn, *splits = plan.splits;
+    return MXL_OK;
 }
 
 extern "C" int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const void* bias, int bias_dtype, int act, const void* residual_bf16, int64_t m,
@@ -566,7 +656,7 @@ extern "C" int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, in
     if (!device_is_gfx950()) return MXL_ENODEV;
     DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)b_bf16, (uint16_t*)da_bf16, m, k, n, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0};
     hipStream_t st = (hipStream_t)stream;
-    if (dense_plan(m, k, n).tile == 256)
+    if (dense_plan(m, k, n).tn == 256)
         return mxl_grouped_gemm_bf16(dz_bf16, b_bf16, da_bf16, nullptr, 1, m, k, n, MXL_BF_B_KN | MXL_BF_TILE_256, stream);
     return launch_dense<true, kActNone>(d, st);
 }

@@ -48,11 +48,11 @@ def _inputs(gpu, m, n, k, seed, bias_dtype=torch.bfloat16):
     return r(m, k).bfloat16(), (r(n, k) * 1.5 * k ** -0.5).bfloat16(), r(n).to(bias_dtype), r(m, n).bfloat16(), r(m, n).bfloat16()
 
 
-# few rows (1, 2 and 4 fragments of 16), 64 x 64 tiles, 128 x 128 tiles, 256 x 256 tiles, odd halves of a slot, ragged last tiles, long and
-# split contractions
-SIZES = [(1, 32, 32), (1, 4096, 1056), (7, 96, 4096), (16, 64, 288), (17, 160, 96), (33, 320, 800), (64, 2880, 64), (65, 96, 32), (100, 32, 2080), (127, 224, 160),
+# few rows (with 16 and 32 columns to a workgroup), every tile of test_every_way_of_running_is_among_the_sizes, odd halves of a slot,
+# ragged last tiles, long and split contractions
+SIZES = [(1, 32, 32), (13, 8224, 96), (1, 4096, 1056), (7, 96, 4096), (16, 64, 288), (17, 160, 96), (33, 320, 800), (64, 2880, 64), (65, 96, 32), (100, 32, 2080), (127, 224, 160),
          (129, 416, 64), (300, 512, 1120), (777, 1056, 96), (2051, 2880, 96), (2100, 2080, 160), (4096, 1024, 4096), (1000, 2048, 14336),
-         (4200, 4128, 32), (4353, 4160, 160), (70, 64, 1056), (130, 128, 4128), (333, 4096, 2048)]
+         (4200, 4128, 32), (4353, 4160, 160), (70, 64, 1056), (130, 128, 4128), (333, 4096, 2048), (700, 4096, 2080), (1900, 1056, 1184), (2051, 96, 2880), (4200, 32, 4128), (700, 4128, 4128)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -102,6 +102,24 @@ def test_stages(gpu, m, n, k):
             assert torch.equal(g, w)
         with torch.no_grad():
             assert torch.equal(ops.gemm_bias_act(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3]), got)
+
+
+def test_every_way_of_running_is_among_the_sizes():
+    import ctypes
+
+    from primus_amd import _lib
+
+    def plan(m, n, k):
+        t = [ctypes.c_int() for _ in range(3)]
+        assert _lib.load().mxl_linear_bf16_plan(m, n, k, *[ctypes.byref(x) for x in t]) == 0
+        return (t[0].value, t[1].value, t[2].value > 1)
+
+    ways = {(256, 256, False), (256, 128, False), (256, 128, True), (64, 64, False), (64, 64, True)}
+    odd = lambda k: (k // 32) % 2  # noqa: E731
+    assert {plan(*s) for s in SIZES if s[0] > 16} == ways == {plan(m, k, n) for m, n, k in SIZES}
+    for tile in ways:      # and with a contraction that ends half way through a slot
+        assert any(plan(m, n, k) == tile and odd(k) for m, n, k in SIZES if m > 16) and any(plan(m, k, n) == tile and odd(n) for m, n, k in SIZES), tile
+    assert any(m <= 16 and n >= 8192 for m, n, k in SIZES) and any(m <= 16 and n < 8192 for m, n, k in SIZES)
 
 
 @pytest.mark.parametrize("m", [3, 40, 150, 1500])
