@@ -55,29 +55,24 @@ __device__ __forceinline__ uint32_t dpp_next_lane(uint32_t v) {        // lane l
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x130, 0xF, 0xF, true);      // wave_shl 1
 }
 __device__ __forceinline__ float dpp_next_lane(float v) { return __uint_as_float(dpp_next_lane(__float_as_uint(v))); }
-
-// One logit of a lane's sorted list: its key, its expert and (where scores are compared) itself
-template <bool SCORED> struct Cand {
-    uint32_t key, idx;
-};
-template <> struct Cand<true> {
-    uint32_t key, idx;
-    float logit;
-};
-template <bool SCORED> __device__ __forceinline__ Cand<SCORED> pick(bool first, const Cand<SCORED>& a, const Cand<SCORED>& b) {
-    Cand<SCORED> r;
-    r.key = first ? a.key : b.key;
-    r.idx = first ? a.idx : b.idx;
-    if constexpr (SCORED) r.logit = first ? a.logit : b.logit;
-    return r;
+// Largest of the wave's 64 keys as a scalar: inside the rows of 16 lanes, then row 0 into 1 and 2 into 3, 1 into 3; lane 63 has it.
+// (Six instructions; with every lane given the result the last two steps are four each.)
+__device__ __forceinline__ uint32_t wave_max_key(uint32_t v) {
+    v = lanes_reduce<OpMaxU, 16>(v);
+    v = OpMaxU::f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));      // row_bcast 15
+    v = OpMaxU::f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));      // row_bcast 31
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-// a lane's candidates in descending order, equal keys by ascending index: Batcher's odd-even merge sort
-template <int V, bool SCORED> __device__ __forceinline__ void sort_cands(Cand<SCORED> (&c)[V]) {
+
+// (key, expert) pairs of a lane in descending order, equal keys by ascending index: Batcher's odd-even merge sort
+template <int V> __device__ __forceinline__ void sort_pairs(uint32_t (&key)[V], uint32_t (&idx)[V]) {
     auto order = [&](int a, int b) __attribute__((always_inline)) {      // a < b: the better one to a
-        const bool keep = c[a].key > c[b].key || (c[a].key == c[b].key && c[a].idx < c[b].idx);
-        const Cand<SCORED> x = pick<SCORED>(keep, c[a], c[b]), y = pick<SCORED>(keep, c[b], c[a]);
-        c[a] = x;
-        c[b] = y;
+        const bool keep = key[a] > key[b] || (key[a] == key[b] && idx[a] < idx[b]);
+        const uint32_t ka = key[a], ia = idx[a];
+        key[a] = keep ? ka : key[b];
+        idx[a] = keep ? ia : idx[b];
+        key[b] = keep ? key[b] : ka;
+        idx[b] = keep ? idx[b] : ia;
     };
 #pragma unroll
     for (int p = 1; p < V; p <<= 1)
@@ -89,10 +84,13 @@ template <int V, bool SCORED> __device__ __forceinline__ void sort_cands(Cand<SC
                 for (int i = 0; i < k; ++i)
                     if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(i + j, i + j + k);
 }
-template <int V, bool SCORED> __device__ __forceinline__ void pop_head(Cand<SCORED> (&c)[V], bool take) {
+template <int V> __device__ __forceinline__ void pop_head(uint32_t (&key)[V], uint32_t (&idx)[V], bool take) {
 #pragma unroll
-    for (int v = 0; v + 1 < V; ++v) c[v] = pick<SCORED>(take, c[v + 1], c[v]);
-    c[V - 1].key = take ? 0u : c[V - 1].key;
+    for (int v = 0; v + 1 < V; ++v) {
+        key[v] = take ? key[v + 1] : key[v];
+        idx[v] = take ? idx[v + 1] : idx[v];
+    }
+    key[V - 1] = take ? 0u : key[V - 1];
 }
 
 // The choice of one row again, by a whole wave, from scores in fp64 kept in the wave's LDS; lane k < topk returns the k-th index.
@@ -185,16 +183,16 @@ __device__ __forceinline__ int choose_fp64(const RouteArgs& p, int64_t row, doub
 }
 
 // SCORED: bias or groups, so scores are computed and compared (a row per wave); otherwise the logits are.
-template <int V, bool SCORED> constexpr int route_waves() { return !SCORED || V <= 4 ? 16 : 64 / V; }
+template <int V, bool SCORED> constexpr int route_waves() { return !SCORED ? 16 : V <= 8 ? 8 : 64 / V; }
 
 template <int LPR, int V, bool SCORED>
-__global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V <= 4 ? 8 : 1)) void route_fwd_kernel(RouteArgs p) {
+__global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORED ? 6 : 8)) void route_fwd_kernel(RouteArgs p) {
     static_assert(!SCORED || LPR == 64, "a scored row is a wave's");
     constexpr int WAVES = route_waves<V, SCORED>(), RPW = 64 / LPR;
     __shared__ int hist[RT_MAX_EXPERTS];
     __shared__ float bias[SCORED ? RT_MAX_EXPERTS : 1];
     __shared__ double spare[SCORED ? WAVES * V * 64 : 1];
-    const int t = threadIdx.x, w = t >> 6, lane = t & 63, lr = lane & (LPR - 1);
+    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, lr = lane & (LPR - 1);
     for (int e = t; e < p.experts; e += WAVES * 64) {
         hist[e] = 0;
         if (SCORED) bias[e] = p.bias ? p.bias[e] : 0.f;
@@ -214,7 +212,7 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V <= 4 ? 8 : 1)) 
 
     const int64_t step = (int64_t)gridDim.x * WAVES * RPW;
     auto fetch = [&](int64_t row0, float (&l)[V]) __attribute__((always_inline)) {
-        const int64_t row = row0 + lane / LPR, base = (row < p.tokens ? row : p.tokens - 1) * p.experts;
+        const int64_t row = LPR == 64 ? row0 : row0 + lane / LPR, base = (row < p.tokens ? row : p.tokens - 1) * p.experts;
 #pragma unroll
         for (int v = 0; v < V; ++v) l[v] = v < have ? load_dt(p.logits, p.dtype, base + first + v) : -INFINITY;
     };
@@ -222,7 +220,7 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V <= 4 ? 8 : 1)) 
     float next[V];
     if (row0 < p.tokens) fetch(row0, next);
     for (; row0 < p.tokens; row0 += step) {
-        const int64_t row = row0 + lane / LPR;
+        const int64_t row = LPR == 64 ? row0 : row0 + lane / LPR;
         const bool in = row < p.tokens;
         float l[V];
 #pragma unroll
@@ -245,92 +243,85 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V <= 4 ? 8 : 1)) 
         // score s = exp(-x) / total is off by s (1.45 x + 60) 2^-24 (the exponentials, V + 6 additions, the quotient), and neither s
         // nor 2 s x passes 1 / total.  Without a bias nothing left out has a larger score than what it is compared with: relative there.
         const float pair_off = p.sigmoid ? 0x1p-21f : 0x1p-17f / total;
-        Cand<SCORED> c[V];
+        uint32_t key[V], idx[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float x = l[v];
-            if constexpr (SCORED) {
-                c[v].logit = l[v];
-                if (v < have) x = (p.sigmoid ? sigmoid_fast(l[v]) : exp_fast(l[v] - top) / total) + bias[first + v];
-            }
-            c[v].key = v < have ? order_key(x) : 0u;
-            c[v].idx = (uint32_t)(first + v);
+            if (SCORED && v < have) x = (p.sigmoid ? sigmoid_fast(l[v]) : exp_fast(l[v] - top) / total) + bias[first + v];
+            key[v] = v < have ? order_key(x) : 0u;
+            idx[v] = (uint32_t)(first + v);
         }
-        sort_cands<V, SCORED>(c);
+        sort_pairs<V>(key, idx);
         bool doubt = false;
         if (SCORED && p.groups > 1) {
-            Cand<SCORED> q[V];
+            uint32_t gk[V], gi[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) q[v] = c[v];
+            for (int v = 0; v < V; ++v) gk[v] = key[v], gi[v] = 0u;
             float score = 0.f;
             for (int i = 0; i < p.take; ++i) {
-                const uint32_t best = lanes_reduce<OpMaxU>(q[0].key, p.lanes_per_group);
-                const uint32_t who = lanes_reduce<OpMinU>(q[0].key == best ? (uint32_t)lane : 64u, p.lanes_per_group);
+                const uint32_t best = lanes_reduce<OpMaxU>(gk[0], p.lanes_per_group);
+                const uint32_t who = lanes_reduce<OpMinU>(gk[0] == best ? (uint32_t)lane : 64u, p.lanes_per_group);
                 score += best ? key_value(best) : 0.f;
-                pop_head<V, SCORED>(q, who == (uint32_t)lane && best != 0u);
+                pop_head<V>(gk, gi, who == (uint32_t)lane && best != 0u);
             }
-            const int grp = lane / p.lanes_per_group;
             int ahead = 0;
-            for (int g = 0; g < p.groups; ++g) {
-                const float other = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(score), g * p.lanes_per_group));
-                ahead += other > score || (other == score && g < grp);
-            }
-            const bool keep = ahead < p.group_topk, real = grp < p.groups;
-            // the worst group kept and the best one left out, against what fp32 scores and their sums may be off
-            const float in_worst = lanes_min<64>(real && keep ? score : INFINITY), out_best = lanes_max<64>(real && !keep ? score : -INFINITY);
+            for (int g = 0; g < p.groups; ++g)
+                ahead += __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(score), g * p.lanes_per_group)) > score;
+            const bool keep = ahead < p.group_topk, real = lane / p.lanes_per_group < p.groups;
             if (p.group_topk < p.groups) {
+                // the worst group kept and the best one left out, against what fp32 scores and their sums may be off; groups of
+                // the same score, of which too many are kept, are told apart in fp64
+                const int kept = __builtin_popcountll(__ballot(keep && real)) / p.lanes_per_group;
+                const float in_worst = key_value(~wave_max_key(real && keep ? ~order_key(score) : 0u));
+                const float out_best = key_value(wave_max_key(real && !keep ? order_key(score) : 0u));
                 const float mag = fabsf(in_worst) + fabsf(out_best);
                 const float off = p.bias || p.sigmoid ? pair_off * (float)p.take : 0x1p-16f * mag;
-                doubt = !(in_worst - out_best > off + 0x1p-22f * (float)p.take * mag);
+                doubt = kept != p.group_topk || !(in_worst - out_best > off + 0x1p-22f * (float)p.take * mag);
             }
 #pragma unroll
-            for (int v = 0; v < V; ++v) c[v].key = keep ? c[v].key : 0u;
+            for (int v = 0; v < V; ++v) key[v] = keep ? key[v] : 0u;
         }
         // the choice, one expert a round; lane k of the row keeps the k-th (a scored row looks one further, to compare with it)
         int mine = 0;
         uint32_t mine_key = 0u;
-        float ml = -INFINITY;
         const int rounds = p.topk + (SCORED ? 1 : 0);
         for (int k = 0; k < rounds; ++k) {
-            const uint32_t best = lanes_reduce<OpMaxU, LPR>(c[0].key);
-            // equal keys: the lower index is in the lower lane
             if constexpr (LPR == 64) {
-                const int who = __builtin_ctzll(__ballot(c[0].key == best));
-                const int won = __builtin_amdgcn_readlane((int)c[0].idx, who);
-                mine = lr == k ? won : mine;
-                if constexpr (SCORED) {
-                    const float wl = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(c[0].logit), who));
-                    ml = lr == k && best ? wl : ml;
-                    mine_key = lr == k ? best : mine_key;
-                } else {
-                    ml = lr == k ? key_value(best) : ml;
-                }
-                pop_head<V, SCORED>(c, who == lane);
+                const uint32_t best = wave_max_key(key[0]);
+                const uint64_t hit = __ballot(key[0] == best), low = hit & (0 - hit);       // equal keys: the lower index is in the lower lane
+                const int won = __builtin_amdgcn_readlane((int)idx[0], __builtin_ctzll(hit));
+                const bool kth = __builtin_amdgcn_inverse_ballot_w64((uint64_t)1 << k);
+                mine = kth ? won : mine;
+                mine_key = kth ? best : mine_key;
+                pop_head<V>(key, idx, __builtin_amdgcn_inverse_ballot_w64(low));
             } else {
-                const uint32_t won = lanes_reduce<OpMinU, LPR>(c[0].key == best ? c[0].idx : 0xFFFFFFFFu);
+                const uint32_t best = lanes_reduce<OpMaxU, LPR>(key[0]);
+                const uint32_t won = lanes_reduce<OpMinU, LPR>(key[0] == best ? idx[0] : 0xFFFFFFFFu);
                 mine = lr == k ? (int)won : mine;
-                ml = lr == k ? key_value(best) : ml;
-                pop_head<V, SCORED>(c, c[0].key == best && c[0].idx == won);
+                mine_key = lr == k ? best : mine_key;
+                pop_head<V>(key, idx, key[0] == best && idx[0] == won);
             }
         }
-        // lane k < topk: its expert's score.  (An unscored row's logit is its key's value: exact, but for a NaN, which stays one.)
+        // lane k < topk: its expert's logit (an unscored row's is its key's value: exact, but for a NaN, which stays one)
         const bool chosen = lr < p.topk;
-        if (!chosen && !SCORED) ml = -INFINITY;
+        float ml;
         if constexpr (SCORED) {
-            const float b = bias[mine_key ? mine : 0], s = p.sigmoid ? sigmoid_fast(ml) : exp_fast(ml - top) / total, cc = key_value(mine_key);
-            const float nl = dpp_next_lane(ml), ns = dpp_next_lane(s), nc = dpp_next_lane(cc), nb = dpp_next_lane(b);
+            const int64_t at = (in ? row : p.tokens - 1) * p.experts;
+            ml = mine_key ? load_dt(p.logits, p.dtype, at + mine) : -INFINITY;
+            const float b = bias[mine_key ? mine : 0], s = p.sigmoid ? sigmoid_fast(ml) : exp_fast(ml - top) / total, c = key_value(mine_key);
+            const float nl = dpp_next_lane(ml), ns = dpp_next_lane(s), nc = dpp_next_lane(c), nb = dpp_next_lane(b);
             const uint32_t nk = dpp_next_lane(mine_key);
-            const float off = (p.bias || p.sigmoid ? pair_off : 0x1p-16f * (s + ns)) + 0x1p-23f * (fabsf(cc) + fabsf(nc));
+            const float off = (p.bias || p.sigmoid ? pair_off : 0x1p-16f * (s + ns)) + 0x1p-23f * (fabsf(c) + fabsf(nc));
             // nothing follows, or the same logit and bias (a true tie), or far enough apart: told rightly
-            const bool told = !chosen || nk == 0u || (ml == nl && b == nb) || cc - nc > off;
+            const bool told = !chosen || nk == 0u || (ml == nl && b == nb) || c - nc > off;
             doubt = __any(doubt || !told);
             if (doubt) {
-                const int64_t at = in ? row : p.tokens - 1;
-                const int again = choose_fp64<V>(p, at, spare + w * V * 64);
-                mine = chosen ? again : 0;
-                ml = chosen ? load_dt(p.logits, p.dtype, at * p.experts + mine) : -INFINITY;
+                mine = choose_fp64<V>(p, in ? row : p.tokens - 1, spare + w * V * 64);
+                ml = chosen ? load_dt(p.logits, p.dtype, at + mine) : -INFINITY;
             }
             ml = chosen ? ml : -INFINITY;
+        } else {
+            ml = chosen ? key_value(mine_key) : -INFINITY;
         }
         float prob;
         if (p.sigmoid) {
