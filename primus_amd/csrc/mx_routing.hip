@@ -93,91 +93,70 @@ template <int V> __device__ __forceinline__ void pop_head(uint32_t (&key)[V], ui
     key[V - 1] = take ? 0u : key[V - 1];
 }
 
-// The choice of one row again, by a whole wave, from scores in fp64 kept in the wave's LDS; lane k < topk returns the k-th index.
-// (Rare: written for few registers.)
+// The choice of one row again, by a whole wave, from scores in fp64, given the lane's logits (-inf past `have`) and the row's largest;
+// lane k < topk returns the k-th index.  Rare, but the wave that does it is the one the launch waits for: the scores' order keys stand
+// in the wave's LDS, a lane keeps its best one in registers, and a round is two scalar maxima (upper, then lower halves).
 template <int V>
-__device__ __forceinline__ int choose_fp64(const RouteArgs& p, int64_t row, double* c) {
+__device__ __forceinline__ int choose_fp64(const RouteArgs& p, const float (&l)[V], const float* bias, float top, int first, int have, uint64_t* keys) {
     const int lane = threadIdx.x & 63;
-    const int sub = lane & (p.lanes_per_group - 1), grp = lane / p.lanes_per_group;
-    const int64_t base = row * p.experts;
-    auto element = [&](int v) {
-        const int j = sub * V + v;
-        return grp < p.groups && j < p.group_size ? grp * p.group_size + j : -1;
-    };
-    auto wave_max = [](double x) {
-        for (int d = 1; d < 64; d <<= 1) x = fmax(x, __shfl_xor(x, d));
-        return x;
-    };
-    double top = -INFINITY, sum = 0.0;
+    double sum = 0.0;
     if (!p.sigmoid) {
-        _Pragma("unroll 1") for (int v = 0; v < V; ++v) {
-            const int e = element(v);
-            if (e >= 0) top = fmax(top, (double)load_dt(p.logits, p.dtype, base + e));
-        }
-        top = wave_max(top);
-        top = top == -INFINITY ? 0.0 : top;
-        _Pragma("unroll 1") for (int v = 0; v < V; ++v) {
-            const int e = element(v);
-            if (e >= 0) sum += exp((double)load_dt(p.logits, p.dtype, base + e) - top);
-        }
+        _Pragma("unroll 1") for (int v = 0; v < V; ++v) sum += v < have ? exp((double)l[v] - (double)top) : 0.0;
         for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
         sum = sum == 0.0 ? 1.0 : sum;
     }
     _Pragma("unroll 1") for (int v = 0; v < V; ++v) {
-        const int e = element(v);
-        double x = -INFINITY;
-        if (e >= 0) {
-            x = (double)load_dt(p.logits, p.dtype, base + e);
-            x = p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum;
-            if (p.bias) x += (double)p.bias[e];
-            if (x != x) x = -INFINITY;
-        }
-        c[v * 64 + lane] = x;
+        double x = (double)l[v];
+        x = (p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)top) / sum) + (double)bias[v < have ? first + v : 0];
+        const uint64_t bits = (uint64_t)__double_as_longlong(x + 0.0);
+        const uint64_t k = (bits >> 63) ? ~bits : bits | ((uint64_t)1 << 63);
+        keys[v * 64 + lane] = v >= have ? 0 : x != x ? 1 : k;       // 0: no element, 1: NaN, below -inf
     }
-    uint32_t left = 0;                          // this lane's elements that are still to be had
-    _Pragma("unroll 1") for (int v = 0; v < V; ++v)
-        if (element(v) >= 0) left |= 1u << v;
-    // the best element left among `lanes` lanes: its value and (lane, v) as one number, smaller = lower index; 0xFFFF: none
-    auto best_of = [&](int lanes, uint32_t have, double& value) {
-        double b = -INFINITY;
-        uint32_t at = 0xFFFFu;
-        _Pragma("unroll 1") for (int v = 0; v < V; ++v)
-            if ((have >> v) & 1) {
-                const double x = c[v * 64 + lane];
-                if (at == 0xFFFFu || x > b) b = x, at = (uint32_t)(lane * V + v);
-            }
-        for (int d = 1; d < lanes; d <<= 1) {
-            const double ob = __shfl_xor(b, d);
-            const uint32_t oat = (uint32_t)__shfl_xor((int)at, d);
-            if (oat != 0xFFFFu && (at == 0xFFFFu || ob > b || (ob == b && oat < at))) b = ob, at = oat;
+    uint32_t left = have >= 32 ? 0xFFFFFFFFu : (1u << have) - 1u;   // this lane's elements that are still to be had
+    uint64_t best = 0;
+    int at = 0;
+    auto rescan = [&](uint32_t have_bits) {
+        best = 0;
+        _Pragma("unroll 1") for (int v = 0; v < V; ++v) {
+            const uint64_t k = keys[v * 64 + lane];
+            if (((have_bits >> v) & 1) && k > best) best = k, at = v;
         }
-        value = b;
-        return at;
     };
+    rescan(left);
     if (p.groups > 1) {
-        uint32_t have = left;
-        double score = 0.0, value;
+        uint32_t have_bits = left;
+        double score = 0.0;
         for (int i = 0; i < p.take; ++i) {
-            const uint32_t at = best_of(p.lanes_per_group, have, value);
-            if (at != 0xFFFFu) {
-                score += value;
-                if ((int)(at / V) == lane) have &= ~(1u << (at % V));
+            const uint32_t hi = lanes_reduce<OpMaxU>((uint32_t)(best >> 32), p.lanes_per_group);
+            const uint32_t lo = lanes_reduce<OpMaxU>((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u, p.lanes_per_group);
+            const uint64_t k = (uint64_t)hi << 32 | lo;
+            const uint32_t who = lanes_reduce<OpMinU>(best == k ? (uint32_t)lane : 64u, p.lanes_per_group);
+            if (k != 0) score += __longlong_as_double((long long)((k >> 63) ? k & ~((uint64_t)1 << 63) : ~k));
+            if (who == (uint32_t)lane && k != 0) {
+                have_bits &= ~(1u << at);
+                rescan(have_bits);
             }
         }
         int ahead = 0;
+        const int grp = lane / p.lanes_per_group;
         for (int g = 0; g < p.groups; ++g) {
             const double other = __shfl(score, g * p.lanes_per_group);
             ahead += other > score || (other == score && g < grp);
         }
         if (ahead >= p.group_topk) left = 0;
+        rescan(left);
     }
     int mine = 0;
     for (int k = 0; k < p.topk; ++k) {
-        double value;
-        const uint32_t at = best_of(64, left, value);
-        const int wl = (int)(at / V), wv = (int)(at % V);
-        if (wl == lane) left &= ~(1u << wv);
-        if (lane == k && at != 0xFFFFu) mine = (wl / p.lanes_per_group) * p.group_size + (wl & (p.lanes_per_group - 1)) * V + wv;
+        const uint32_t hi = wave_max_key((uint32_t)(best >> 32));
+        const uint32_t lo = wave_max_key((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+        const int who = __builtin_ctzll(__ballot(best == ((uint64_t)hi << 32 | lo)));      // the lower index is in the lower lane
+        const int won = __builtin_amdgcn_readlane(first + at, who);
+        mine = lane == k ? won : mine;
+        if (lane == who) {
+            left &= ~(1u << at);
+            rescan(left);
+        }
     }
     return mine;
 }
@@ -191,7 +170,7 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
     constexpr int WAVES = route_waves<V, SCORED>(), RPW = 64 / LPR;
     __shared__ int hist[RT_MAX_EXPERTS];
     __shared__ float bias[SCORED ? RT_MAX_EXPERTS : 1];
-    __shared__ double spare[SCORED ? WAVES * V * 64 : 1];
+    __shared__ uint64_t spare[SCORED ? WAVES * V * 64 : 1];
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, lr = lane & (LPR - 1);
     for (int e = t; e < p.experts; e += WAVES * 64) {
         hist[e] = 0;
@@ -316,7 +295,7 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
             const bool told = !chosen || nk == 0u || (ml == nl && b == nb) || c - nc > off;
             doubt = __any(doubt || !told);
             if (doubt) {
-                mine = choose_fp64<V>(p, in ? row : p.tokens - 1, spare + w * V * 64);
+                mine = choose_fp64<V>(p, l, bias, top, first, have, spare + w * V * 64);
                 ml = chosen ? load_dt(p.logits, p.dtype, at + mine) : -INFINITY;
             }
             ml = chosen ? ml : -INFINITY;
@@ -444,7 +423,7 @@ __global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_kernel(RouteBwdArgs p
 static int64_t route_blocks(int64_t tokens, int rows_per_block) {
     if (tokens <= 16) return 1;
     int64_t b = (tokens + rows_per_block - 1) / rows_per_block;
-    return b < 512 ? b : 512;
+    return b < 768 ? b : 768;
 }
 
 template <int LPR, int V, bool SCORED>
