@@ -1254,19 +1254,15 @@ def _same_device(device, **tensors) -> None:
             raise ValueError(f"{name} must live on the device of the other operands")
 
 
-def _routing_args(logits, topk, score_function):
-    _require_cuda(logits)
-    if logits.dim() != 2:
-        raise ValueError("logits must be [tokens, experts]")
-    dtype = _float_type(logits, "logits")
-    experts = logits.shape[1]
-    if not 1 <= experts <= _lib.MAX_GROUPS:
-        raise ValueError(f"the number of experts must be in [1, {_lib.MAX_GROUPS}]")
-    if not 1 <= topk <= min(ROUTING_MAX_TOPK, experts):
-        raise ValueError(f"topk must be in [1, {min(ROUTING_MAX_TOPK, experts)}]")
-    if score_function not in _SCORES:
-        raise ValueError(f"score_function must be 'softmax' or 'sigmoid', got {score_function!r}")
-    return dtype, experts, _SCORES[score_function]
+def _gpu_rows(t, what: str) -> int:
+    """The type code of a contiguous 2-D floating tensor on the GPU."""
+    dtype = _DT.get(t.dtype)
+    if dtype is None or t.dim() != 2 or not t.is_cuda or not t.is_contiguous():
+        _require_cuda(t)
+        if t.dim() != 2:
+            raise ValueError(f"{what} must be a 2-D tensor")
+        _float_type(t, what)
+    return dtype
 
 
 def topk_routing_impl(logits, topk: int, score_function: str = "softmax", expert_bias: Optional[torch.Tensor] = None,
@@ -1274,12 +1270,21 @@ def topk_routing_impl(logits, topk: int, score_function: str = "softmax", expert
                       token_mask: Optional[torch.Tensor] = None):
     """``(probs [tokens, topk] float32, indices [tokens, topk] int64, tokens_per_expert [experts] int64)``; see
     ``ops.topk_routing``."""
-    dtype, experts, score = _routing_args(logits, topk, score_function)
-    if not 1 <= num_groups <= 64 or experts % num_groups != 0:
-        raise ValueError("num_groups must divide the number of experts and be at most 64")
-    if not 1 <= group_topk <= num_groups or topk > group_topk * (experts // num_groups):
-        raise ValueError("group_topk must be in [1, num_groups], and its groups must hold topk experts")
-    tokens, dev = logits.shape[0], logits.device
+    dtype = _gpu_rows(logits, "logits [tokens, experts]")
+    tokens, experts = logits.shape
+    if not 1 <= experts <= _lib.MAX_GROUPS:
+        raise ValueError(f"the number of experts must be in [1, {_lib.MAX_GROUPS}]")
+    if not 1 <= topk <= min(ROUTING_MAX_TOPK, experts):
+        raise ValueError(f"topk must be in [1, {min(ROUTING_MAX_TOPK, experts)}]")
+    score = _SCORES.get(score_function)
+    if score is None:
+        raise ValueError(f"score_function must be 'softmax' or 'sigmoid', got {score_function!r}")
+    if num_groups != 1 or group_topk != 1:
+        if not 1 <= num_groups <= 64 or experts % num_groups != 0:
+            raise ValueError("num_groups must divide the number of experts and be at most 64")
+        if not 1 <= group_topk <= num_groups or topk > group_topk * (experts // num_groups):
+            raise ValueError("group_topk must be in [1, num_groups], and its groups must hold topk experts")
+    dev = logits.device
     if expert_bias is not None:
         if expert_bias.dtype != torch.float32 or tuple(expert_bias.shape) != (experts,):
             raise ValueError("expert_bias must be float32 [experts]")
@@ -1290,35 +1295,39 @@ def topk_routing_impl(logits, topk: int, score_function: str = "softmax", expert
             raise ValueError("token_mask must be bool or uint8 [tokens]")
         _require_cuda(token_mask)
         _same_device(dev, token_mask=token_mask)
+    lib = _lib.load()
     with _on(dev), _hooked("topk_routing", tokens=tokens, experts=experts, topk=topk):
         probs = torch.empty((tokens, topk), dtype=torch.float32, device=dev)
         indices = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
         counts = torch.empty(experts, dtype=torch.int64, device=dev)
         ws, nbytes = _workspace(dev, "mxl_topk_routing_workspace_bytes", tokens, experts)
-        rc = _lib.load().mxl_topk_routing(_ptr(logits), dtype, tokens, experts, topk, score, _ptr(expert_bias), num_groups, group_topk,
-                                          renormalize, scaling_factor, _ptr(token_mask), _ptr(probs), _ptr(indices), counts.data_ptr(),
-                                          _ptr(ws), nbytes, _stream())
-    _lib.check(rc, "mxl_topk_routing")
+        rc = lib.mxl_topk_routing(logits.data_ptr() if tokens else None, dtype, tokens, experts, topk, score, _ptr(expert_bias), num_groups, group_topk,
+                                  renormalize, scaling_factor, _ptr(token_mask), _ptr(probs), _ptr(indices), counts.data_ptr(), _ptr(ws), nbytes, _stream())
+    if rc:
+        _lib.check(rc, "mxl_topk_routing")
     return probs, indices, counts
 
 
 def topk_routing_bwd_impl(dprobs, logits, indices, score_function: str = "softmax", renormalize: bool = True,
                           scaling_factor: float = 1.0) -> torch.Tensor:
     """Gradient of ``topk_routing_impl``'s probabilities with respect to the logits, in their type."""
-    topk = indices.shape[-1]
-    dtype, experts, score = _routing_args(logits, topk, score_function)
-    tokens = logits.shape[0]
-    if dprobs.dtype != torch.float32 or tuple(dprobs.shape) != (tokens, topk):
+    dtype = _gpu_rows(logits, "logits [tokens, experts]")
+    if _gpu_rows(dprobs, "dprobs [tokens, topk]") != _lib.DT_F32 or dprobs.shape != indices.shape or dprobs.shape[0] != logits.shape[0]:
         raise ValueError("dprobs must be float32 [tokens, topk]")
-    if indices.dtype != torch.int64 or tuple(indices.shape) != (tokens, topk):
+    if indices.dtype != torch.int64:
         raise ValueError("indices must be int64 [tokens, topk]")
-    _require_cuda(dprobs, indices)
-    _same_device(logits.device, dprobs=dprobs, indices=indices)
-    with _on(logits.device), _hooked("topk_routing_bwd", tokens=tokens, experts=experts, topk=topk):
+    _require_cuda(indices)
+    tokens, experts = logits.shape
+    dev = logits.device
+    if dprobs.device != dev or indices.device != dev:
+        _same_device(dev, dprobs=dprobs, indices=indices)
+    lib = _lib.load()
+    with _on(dev), _hooked("topk_routing_bwd", tokens=tokens, experts=experts, topk=dprobs.shape[1]):
         dlogits = torch.empty_like(logits)
-        rc = _lib.load().mxl_topk_routing_bwd(_ptr(dprobs), _ptr(logits), dtype, _ptr(indices), tokens, experts, topk, score,
-                                              int(bool(renormalize)), float(scaling_factor), _ptr(dlogits), _stream())
-    _lib.check(rc, "mxl_topk_routing_bwd")
+        rc = lib.mxl_topk_routing_bwd(_ptr(dprobs), _ptr(logits), dtype, _ptr(indices), tokens, experts, dprobs.shape[1], _SCORES[score_function],
+                                      renormalize, scaling_factor, _ptr(dlogits), _stream())
+    if rc:
+        _lib.check(rc, "mxl_topk_routing_bwd")
     return dlogits
 
 
@@ -1359,15 +1368,17 @@ def permute_plan_impl(indices, num_experts: int, align: int = 1, probs: Optional
 
 
 def _row_args(x, row_of, entry_of):
-    _require_cuda(x, row_of, entry_of)
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError("expected a 2-D tensor of rows that are not empty")
-    _float_type(x, "rows")
+    dtype = _gpu_rows(x, "rows")
+    if x.shape[1] < 1:
+        raise ValueError("expected rows that are not empty")
     if row_of.dtype != torch.int64 or row_of.dim() != 2 or not 1 <= row_of.shape[1] <= ROUTING_MAX_TOPK:
         raise ValueError(f"row_of must be int64 [tokens, topk] with topk in [1, {ROUTING_MAX_TOPK}]")
     if entry_of.dtype != torch.int32 or entry_of.dim() != 1:
         raise ValueError("entry_of must be int32 [rows]")
-    _same_device(x.device, row_of=row_of, entry_of=entry_of)
+    _require_cuda(row_of, entry_of)
+    if row_of.device != x.device or entry_of.device != x.device:
+        _same_device(x.device, row_of=row_of, entry_of=entry_of)
+    return dtype
 
 
 def permute_rows_impl(x, row_of, entry_of) -> torch.Tensor:

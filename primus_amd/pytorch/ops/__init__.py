@@ -691,6 +691,13 @@ class _NoGradContext:
         pass
 
 
+def _apply_if(needs_grad: bool, fn, *args):
+    """``_apply`` for callers that know which of their tensors may need a gradient."""
+    if (needs_grad and torch.is_grad_enabled()) or torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None:
+        return fn.apply(*args)
+    return fn.forward(_NoGradContext(), *args, need_grad=False)
+
+
 def _apply(fn, *args):
     """``fn.apply(*args)``, or its forward alone when nothing needs a gradient: no graph node, and no copies for a
     backward that cannot come (``requires_grad`` of a leaf says nothing under ``torch.no_grad``).  Inside a function
@@ -1191,8 +1198,9 @@ class _TopkRouting(torch.autograd.Function):
         logits, indices = ctx.saved_tensors
         if dprobs is None:
             return (None,) * 10
-        dlogits = K.topk_routing_bwd_impl(dprobs.to(torch.float32).contiguous(), logits, indices, *ctx.how)
-        return dlogits, None, None, None, None, None, None, None, None, None
+        if dprobs.dtype != torch.float32 or not dprobs.is_contiguous():
+            dprobs = dprobs.to(torch.float32).contiguous()
+        return K.topk_routing_bwd_impl(dprobs, logits, indices, *ctx.how), None, None, None, None, None, None, None, None, None
 
 
 def topk_routing(logits: torch.Tensor, topk: int, score_function: str = "softmax", expert_bias: Optional[torch.Tensor] = None,
@@ -1219,8 +1227,8 @@ def topk_routing(logits: torch.Tensor, topk: int, score_function: str = "softmax
         expert_bias = expert_bias.detach().contiguous()
     if token_mask is not None:
         token_mask = token_mask.contiguous()
-    return _apply(_TopkRouting, logits.contiguous(), int(topk), score_function, expert_bias, int(num_groups), int(group_topk),
-                  bool(renormalize), float(scaling_factor), token_mask)
+    return _apply_if(logits.requires_grad, _TopkRouting, logits.contiguous(), int(topk), score_function, expert_bias, int(num_groups), int(group_topk),
+                     bool(renormalize), float(scaling_factor), token_mask)
 
 
 class TokenPermutation(NamedTuple):
@@ -1273,8 +1281,8 @@ def permute_tokens(x: torch.Tensor, indices: torch.Tensor, num_experts: int, pro
         raise ValueError("x must be [tokens, hidden] and indices [tokens, topk]")
     if indices.is_floating_point() or indices.dtype == torch.bool:
         raise ValueError("indices must be integers")
-    rows, row_probs, group_lens, row_of, entry_of = _apply(
-        _PermuteTokens, x.contiguous(), indices.to(torch.int64).contiguous(), int(num_experts), None if probs is None else probs.contiguous(), int(align))
+    rows, row_probs, group_lens, row_of, entry_of = _apply_if(
+        x.requires_grad or (probs is not None and probs.requires_grad), _PermuteTokens, x.contiguous(), indices.to(torch.int64).contiguous(), int(num_experts), None if probs is None else probs.contiguous(), int(align))
     return rows, row_probs, group_lens, TokenPermutation(row_of, entry_of)
 
 
@@ -1302,4 +1310,4 @@ def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, probs: O
     experts' outputs back at their tokens, summed in fp32 in the order of k and rounded once.  Entries that went nowhere add
     nothing; zero rows are ignored.  Differentiable in ``rows`` (rows that no entry went to get zeros) and ``probs``."""
     row_of, entry_of = permutation
-    return _apply(_UnpermuteTokens, rows.contiguous(), row_of, entry_of, None if probs is None else probs.contiguous())
+    return _apply_if(rows.requires_grad or (probs is not None and probs.requires_grad), _UnpermuteTokens, rows.contiguous(), row_of, entry_of, None if probs is None else probs.contiguous())

@@ -31,7 +31,7 @@ def test_cpu_tensors_are_refused():
 
 
 @pytest.mark.parametrize("why,call", [
-    ("tokens, experts", lambda: ops.topk_routing(torch.randn(2, 3, 4), 2)),
+    ("2-D tensor", lambda: ops.topk_routing(torch.randn(2, 3, 4), 2)),
     ("float32, bfloat16 or float16", lambda: ops.topk_routing(torch.randn(2, 4).double(), 2)),
     ("topk", lambda: ops.topk_routing(torch.randn(2, 4), 5)),
     ("topk", lambda: ops.topk_routing(torch.randn(2, 64), 33)),
