@@ -759,6 +759,16 @@ __global__ __launch_bounds__(TL_THREADS, 2) void bf16_gemm_tall_kernel(Bf16Args 
                 // z passes through the staging area on its way out and the residual on its way in: a lane finds its four
                 // columns' residual where it puts its results
                 const int64_t c0 = c_row0 * p.n + n0;
+                u32x4 rr[8];        // the residual of a half on its way: asked for a phase ahead
+                auto fetch = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int row = h * 128 + x * 16, rows = m_valid - row;
+                        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.epi.residual + c0 + (int64_t)row * p.n), 0, rows > 0 ? (rows < 16 ? rows : 16) * (int)row_bytes : 0, 0x00020000);
+                        rr[x] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)at, 0, 2);
+                    }
+                };
+                if (p.epi.residual) fetch(0);
                 if (p.epi.bias) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
@@ -792,11 +802,11 @@ __global__ __launch_bounds__(TL_THREADS, 2) void bf16_gemm_tall_kernel(Bf16Args 
                     if (p.epi.residual) {
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
-                            const int row = h * 128 + x * 16, rows = m_valid - row, lrow = x * 16 + row0;
-                            const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.epi.residual + c0 + (int64_t)row * p.n), 0, rows > 0 ? (rows < 16 ? rows : 16) * (int)row_bytes : 0, 0x00020000);
-                            *(u32x4*)(out + lrow * 512 + 16 * ((to & 31) ^ (lrow & 31))) = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)at, 0, 2);
+                            const int lrow = x * 16 + row0;
+                            *(u32x4*)(out + lrow * 512 + 16 * ((to & 31) ^ (lrow & 31))) = rr[x];
                         }
                         __syncthreads();
+                        if (h == 0) fetch(1);
                     }
                     if (wm == h) {
 #pragma unroll

@@ -267,7 +267,7 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
     // tile passes through LDS as bf16 in rows of 16-byte pieces: z on its way out, the residual on its way in (each lane then
     // finds its own four columns' values where it puts its results), y on its way out. ----
     constexpr int PITCH = TN * 2 + 16, LPR = TN / 8, RPI = THREADS / LPR;
-    const int rr = t / LPR, cc = (t % LPR) * 8;
+    const int rr0 = t / LPR, cc = (t % LPR) * 8;
     const int64_t c0 = m0 * p.n + n0;
     auto spot = [&](int i, int j, int q) __attribute__((always_inline)) {
         return (uint2*)(smem + (wm * WROWS + i * 32 + lr) * PITCH + (wn * (TN / 2) + j * 32 + 8 * q + 4 * g) * 2);
@@ -276,11 +276,19 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
         if (cc < n_valid) {
 #pragma unroll
             for (int u = 0; u < TM / RPI; ++u) {
-                const int row = u * RPI + rr;
+                const int row = u * RPI + rr0;
                 if (row < m_valid) store16_streaming((uint8_t*)(out + c0 + (int64_t)row * p.n + cc), *(const uint4*)(smem + row * PITCH + cc * 2));
             }
         }
     };
+    uint4 rr[TM / RPI];             // the residual, asked for while z is on its way out
+    if (p.epi.residual && cc < n_valid) {
+#pragma unroll
+        for (int u = 0; u < TM / RPI; ++u) {
+            const int row = u * RPI + rr0;
+            rr[u] = row < m_valid ? load16_streaming(p.epi.residual + c0 + (int64_t)row * p.n + cc) : make_uint4(0, 0, 0, 0);
+        }
+    }
     if (p.epi.bias) {
 #pragma unroll
         for (int j = 0; j < FN; ++j)
@@ -314,8 +322,8 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
         if (cc < n_valid) {
 #pragma unroll
             for (int u = 0; u < TM / RPI; ++u) {
-                const int row = u * RPI + rr;
-                if (row < m_valid) *(uint4*)(smem + row * PITCH + cc * 2) = load16_streaming(p.epi.residual + c0 + (int64_t)row * p.n + cc);
+                const int row = u * RPI + rr0;
+                *(uint4*)(smem + row * PITCH + cc * 2) = rr[u];
             }
         }
         __syncthreads();
