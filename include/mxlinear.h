@@ -629,6 +629,13 @@ int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n);
 int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int act, int64_t m, int64_t n, void* dz_bf16, void* dbias, int dbias_dtype,
                        void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The three of them in one call: da (NULL: not wanted), db [n, k] (NULL: not wanted; MXL_BF_ACCUM_F32: float, added to), dbias (NULL).
+ * m * max(n, k) * 2 < 2^32 where db is wanted.  The workspace holds dz too. */
+int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_dbias);
+int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_bf16, const void* z_bf16, int act, int64_t m, int64_t n, int64_t k,
+                        void* da_bf16, void* db, uint32_t db_flags, void* dbias, int dbias_dtype, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
 /* ---- calibration (no counterpart in the reference: a measuring aid of this library's benchmark) ----
  *
  * mxl_calibrate_mfma launches a register-only loop of the GEMM kernels' scaled MFMA (32 x 32 x 64; a_fmt / b_fmt:

@@ -99,6 +99,8 @@ EXPORTS = (
     "mxl_linear_bf16_dgrad",
     "mxl_linear_bf16_dz_workspace_bytes",
     "mxl_linear_bf16_dz",
+    "mxl_linear_bf16_bwd_workspace_bytes",
+    "mxl_linear_bf16_bwd",
     "mxl_calibrate_mfma",
     "mxl_calibrate_mfma_flops",
     "mxl_calibrate_mfma_bf16",
@@ -281,6 +283,10 @@ def load() -> ctypes.CDLL:
         lib.mxl_linear_bf16_dz_workspace_bytes.argtypes = [i64, i64]
         lib.mxl_linear_bf16_dz.restype = i32
         lib.mxl_linear_bf16_dz.argtypes = [vp, vp, i32, i64, i64, vp, vp, i32, vp, i64, vp]
+        lib.mxl_linear_bf16_bwd_workspace_bytes.restype = i64
+        lib.mxl_linear_bf16_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, i32]
+        lib.mxl_linear_bf16_bwd.restype = i32
+        lib.mxl_linear_bf16_bwd.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, vp, u32, vp, i32, vp, i64, vp]
         _lib = lib
     return _lib
 

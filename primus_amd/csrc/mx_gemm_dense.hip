@@ -696,3 +696,42 @@ extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int a
     if (dbias) hipLaunchKernelGGL(dense_dbias_kernel, dim3((unsigned)(n / 32)), dim3(1024), 0, st, (const float*)workspace, (int)runs, n, dbias, dbias_dtype == MXL_DT_F32);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
+
+// ---- the whole backward in one call ----
+namespace mxl {
+static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+struct BwdSpace {
+    int64_t dz, sums, runs, total;      // bytes: dz (with an activation), dbias's partial sums, dgrad's split sums
+};
+static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int act, bool need_da, bool need_dbias) {
+    BwdSpace s;
+    s.dz = act == MXL_ACT_NONE ? 0 : up256(m * n * 2);
+    s.sums = need_dbias ? up256(mxl_linear_bf16_dz_workspace_bytes(m, n)) : 0;
+    s.runs = need_da ? up256(mxl_linear_bf16_workspace_bytes(m, k, n)) : 0;
+    s.total = s.dz + s.sums + s.runs;
+    return s;
+}
+}  // namespace mxl
+
+extern "C" int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_dbias) {
+    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE) return -1;
+    return bwd_space(m, n, k, act, need_da != 0, need_dbias != 0).total;
+}
+
+extern "C" int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_bf16, const void* z_bf16, int act, int64_t m, int64_t n, int64_t k,
+                                   void* da_bf16, void* db, uint32_t db_flags, void* dbias, int dbias_dtype, void* workspace, int64_t workspace_bytes,
+                                   void* stream) {
+    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (db_flags & ~(uint32_t)MXL_BF_ACCUM_F32)) return MXL_EINVAL;
+    const BwdSpace sp = bwd_space(m, n, k, act, da_bf16 != nullptr, dbias != nullptr);
+    if (sp.total > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < sp.total)) return MXL_EINVAL;
+    if (da_bf16 && m > 0 && !b_bf16) return MXL_EINVAL;
+    uint8_t* at = (uint8_t*)workspace;
+    void* dz = sp.dz ? at : nullptr;
+    int rc = MXL_OK;
+    if (da_bf16 || db || dbias)
+        rc = mxl_linear_bf16_dz(dy_bf16, z_bf16, act, m, n, dz, dbias, dbias_dtype, at + sp.dz, sp.sums, stream);
+    const void* d = sp.dz ? dz : dy_bf16;
+    if (rc == MXL_OK && da_bf16) rc = mxl_linear_bf16_dgrad(d, b_bf16, m, n, k, da_bf16, at + sp.dz + sp.sums, sp.runs, stream);
+    if (rc == MXL_OK && db) rc = mxl_grouped_gemm_bf16_wgrad(d, a_bf16, db, nullptr, 1, m, n, k, db_flags, stream);
+    return rc;
+}

@@ -1451,7 +1451,8 @@ _LINEAR_ACTS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GEL
 
 
 def _linear_args(m: int, n: int, k: int, activation):
-    if activation not in _LINEAR_ACTS:
+    act = _LINEAR_ACTS.get(activation, -1) if activation is None or isinstance(activation, str) else -1
+    if act < 0:
         raise ValueError(f"activation must be None, 'silu', 'gelu' or 'relu', got {activation!r}")
     if n < 1 or k < 1 or n % 32 != 0 or k % 32 != 0 or n > 1 << 22 or k > 1 << 22:
         raise ValueError("the dense bf16 linear needs n and k in multiples of 32 (forward and dgrad contract over them), at most 2^22")
@@ -1459,7 +1460,7 @@ def _linear_args(m: int, n: int, k: int, activation):
         raise ValueError("the weight must be smaller than 4 GiB")
     if m > 0x7FFFFFFF:
         raise ValueError("at most 2^31 - 1 rows")
-    return _LINEAR_ACTS[activation]
+    return act
 
 
 def _bf16_2d(t, what, shape=None):
@@ -1479,20 +1480,67 @@ def linear_bf16_impl(a, b, bias=None, activation: Optional[str] = None, residual
     if b.shape[1] != k:
         raise ValueError("contraction lengths of a and b differ")
     act = _linear_args(m, n, k, activation)
-    if bias is not None and (bias.dtype not in (torch.bfloat16, torch.float32) or tuple(bias.shape) != (n,)):
-        raise ValueError("bias must be bfloat16 or float32 [n]")
+    dev = a.device
+    _require_cuda(a, b)
+    if b.device != dev:
+        _same_device(dev, b=b)
+    bias_ptr, bias_dtype = None, _lib.DT_BF16
+    if bias is not None:
+        if bias.dtype not in (torch.bfloat16, torch.float32) or bias.shape != (n,):
+            raise ValueError("bias must be bfloat16 or float32 [n]")
+        _require_cuda(bias)
+        _same_device(dev, bias=bias)
+        bias_ptr, bias_dtype = bias.data_ptr(), _DT[bias.dtype]
     if residual is not None:
         _bf16_2d(residual, "residual", (m, n))
-    _require_cuda(a, b, bias, residual)
-    _same_device(a.device, b=b, bias=bias, residual=residual)
-    with _on(a.device), _hooked("linear_bf16", m=m, n=n, k=k):
-        y = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
+        _require_cuda(residual)
+        _same_device(dev, residual=residual)
+    lib = _lib.load()
+    with _on(dev), _hooked("linear_bf16", m=m, n=n, k=k):
+        y = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
         z = torch.empty_like(y) if want_z else None
-        ws, ws_bytes = _workspace(a.device, "mxl_linear_bf16_workspace_bytes", m, n, k)
-        rc = _lib.load().mxl_linear_bf16(_ptr(a), _ptr(b), _ptr(bias), _lib.DT_BF16 if bias is None else _DT[bias.dtype], act, _ptr(residual), m, n, k,
-                                         _ptr(y), _ptr(z), _ptr(ws), ws_bytes, _stream())
-    _lib.check(rc, "mxl_linear_bf16")
+        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_workspace_bytes", m, n, k)
+        rc = lib.mxl_linear_bf16(_ptr(a), b.data_ptr(), bias_ptr, bias_dtype, act, _ptr(residual), m, n, k, _ptr(y), _ptr(z), _ptr(ws), ws_bytes, _stream())
+    if rc:
+        _lib.check(rc, "mxl_linear_bf16")
     return y, z
+
+
+def linear_bf16_bwd_impl(dy, a, b, z, activation: Optional[str], need_a: bool = True, need_b: bool = True, bias_dtype: Optional[torch.dtype] = None,
+                         accum_into: Optional[torch.Tensor] = None):
+    """``(da, db, dbias)`` of ``linear_bf16_impl``, what is not needed None: one call for the slope and the bias sums, dgrad and the weight gradient
+    (which is added to the float32 ``accum_into`` if that is given).  Operands too long for the weight gradient's kernel go through the
+    single steps."""
+    _bf16_2d(dy, "dy")
+    _bf16_2d(a, "a")
+    _bf16_2d(b, "b")
+    m, n = dy.shape
+    k = b.shape[1]
+    if a.shape[0] != m or a.shape[1] != k or b.shape[0] != n:
+        raise ValueError("dy [m, n], a [m, k] and b [n, k] do not fit together")
+    act = _linear_args(m, n, k, activation)
+    if act != _lib.ACT_NONE:
+        _bf16_2d(z, "z", (m, n))
+    _require_cuda(dy, a, b, z, accum_into)
+    dev = dy.device
+    if a.device != dev or b.device != dev:
+        _same_device(dev, a=a, b=b)
+    if need_b and m * max(n, k) * 2 >= 1 << 32:
+        dz, dbias = linear_bf16_dz_impl(dy, z, activation, bias_dtype)
+        return linear_bf16_dgrad_impl(dz, b) if need_a else None, linear_bf16_wgrad_impl(dz, a, accum_into=accum_into), dbias
+    if accum_into is not None and (accum_into.dtype != torch.float32 or accum_into.numel() != n * k):
+        raise ValueError("accum_into must be a contiguous float32 buffer of the weight's size")
+    lib = _lib.load()
+    with _on(dev), _hooked("linear_bf16_bwd", m=m, n=n, k=k):
+        da = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_a else None
+        db = None if not need_b else accum_into if accum_into is not None else torch.empty((n, k), dtype=torch.bfloat16, device=dev)
+        dbias = torch.empty(n, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
+        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_bwd_workspace_bytes", m, n, k, act, int(need_a), int(dbias is not None))
+        rc = lib.mxl_linear_bf16_bwd(_ptr(dy), _ptr(a), b.data_ptr(), _ptr(z), act, m, n, k, _ptr(da), _ptr(db), _lib.BF_ACCUM_F32 if accum_into is not None else 0,
+                                     _ptr(dbias), _lib.DT_BF16 if bias_dtype is None else _DT[bias_dtype], _ptr(ws), ws_bytes, _stream())
+    if rc:
+        _lib.check(rc, "mxl_linear_bf16_bwd")
+    return da, db, dbias
 
 
 def linear_bf16_dz_impl(dy, z, activation: Optional[str], bias_dtype: Optional[torch.dtype] = None):

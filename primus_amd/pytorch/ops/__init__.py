@@ -989,16 +989,18 @@ class _GemmBiasAct(torch.autograd.Function):
     def backward(ctx, dy):
         a, b, z = ctx.saved_tensors
         need_a, need_b, need_bias, need_residual = ctx.needs_input_grad[:4]
-        dy = _aligned(dy.contiguous() if dy.dtype == torch.bfloat16 else dy.to(torch.bfloat16).contiguous())
+        if dy.dtype != torch.bfloat16:
+            dy = dy.to(torch.bfloat16)
+        dy = _aligned(dy.contiguous())
         da = db = dbias = None
         if need_a or need_b or need_bias:
-            dz, dbias = K.linear_bf16_dz_impl(dy, z, ctx.activation, ctx.bias_dtype if need_bias else None)
-        if need_a:
-            da = K.linear_bf16_dgrad_impl(dz, b)
-        if need_b:
-            fused = ctx.accum is not None and _fusable(ctx.accum[0])
-            gb = K.linear_bf16_wgrad_impl(dz, a, accum_into=ctx.accum[0] if fused else None)
-            db = _finish_wgrad(None if fused else gb, ctx.accum, fused, tuple(b.shape))
+            fused = need_b and ctx.accum is not None and _fusable(ctx.accum[0])
+            da, db, dbias = K.linear_bf16_bwd_impl(dy, a, b, z, ctx.activation, need_a, need_b, ctx.bias_dtype if need_bias else None,
+                                                   ctx.accum[0] if fused else None)
+            if need_b and ctx.accum is not None:
+                db = _finish_wgrad(None if fused else db, ctx.accum, fused, tuple(b.shape))
+            elif need_b:
+                db = db.view(b.shape)
         return da, db, dbias, dy if need_residual else None, None, None, None
 
 
@@ -1014,17 +1016,20 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     ``residual [..., n]``.  ``n`` and ``k`` in multiples of 32, the weight below 4 GiB (anything else raises).  Differentiable in the four
     tensors; the activation's input is kept in bf16 for the backward, whose gradients are those of that rounded value.
     ``fuse_bgrad_accum_pattern="megatron"`` adds the weight gradient into ``b.main_grad``, as ``gemm`` does."""
-    accum = _accum_from(b, fuse_bgrad_accum_pattern)
+    accum = None if fuse_bgrad_accum_pattern is None else _accum_from(b, fuse_bgrad_accum_pattern)
     if a.dim() < 2 or b.dim() != 2:
         raise ValueError("a must be [..., k] and b [n, k]")
     shape = a.shape[:-1] + (b.shape[0],)
+    flat = a.dim() == 2
     if residual is not None:
         if residual.shape != shape:
             raise ValueError(f"residual must have shape {list(shape)}")
-        residual = _aligned(residual.reshape(-1, shape[-1]).contiguous())
-    y = _apply(_GemmBiasAct, _aligned(a.reshape(-1, a.shape[-1]).contiguous()), _aligned(b.contiguous()), None if bias is None else _aligned(bias.contiguous()),
-               residual, activation, accum)
-    return y.view(shape)
+        residual = _aligned((residual if flat else residual.reshape(-1, shape[-1])).contiguous())
+    if bias is not None:
+        bias = _aligned(bias.contiguous())
+    a2 = _aligned((a if flat else a.reshape(-1, a.shape[-1])).contiguous())
+    y = _apply(_GemmBiasAct, a2, _aligned(b.contiguous()), bias, residual, activation, accum)
+    return y if flat else y.view(shape)
 
 
 class _GroupedLinearLibrary(torch.autograd.Function):

@@ -225,4 +225,7 @@ def test_operands_past_4_gib(gpu):
     dz = torch.zeros(m, n, dtype=torch.bfloat16, device=gpu)
     dz[0, 0] = dz[m - 1, 1] = dz[m // 2, 2] = 1.0
     db = K.linear_bf16_wgrad_impl(dz, a).view(n, k)
+    w = b.clone().requires_grad_()
+    (g,) = torch.autograd.grad(ops.gemm_bias_act(a, w), w, dz)
+    assert torch.equal(g, db)
     assert torch.equal(db[0], a[0]) and torch.equal(db[1], a[m - 1]) and torch.equal(db[2], a[m // 2]) and not bool(db[3:].any())
