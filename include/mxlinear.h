@@ -610,7 +610,7 @@ int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int 
  * primus/backends/megatron/core/extensions/primus_turbo.py:1180-1188) ----
  *   y = act(z) + residual,  z = a . b^T + bias         a [m, k], b [n, k], y, z, residual [m, n] bf16
  * fp32 from the products to y, which is rounded once; bias (bf16 or float, NULL: none), residual (NULL: none); act MXL_ACT_*.
- * z_bf16: if not NULL, z rounded to bf16 for the backward.  n and k multiples of 32, n * k * 2 < 2^32, pointers 16-byte aligned.
+ * z_bf16: if not NULL, z rounded to bf16 for the backward.  n and k multiples of 32 up to 2^21, n * k * 2 < 2^32, pointers 16-byte aligned.
  * Few tiles and a long contraction split it over workgroups, whose sums meet in the caller's workspace:
  * mxl_linear_bf16_workspace_bytes(m, n, k) bytes for the forward, (m, k, n) for dgrad (0: none, NULL will do).
  *

@@ -611,8 +611,9 @@ static int launch_dense_forward(const DenseArgs& a, hipStream_t st) {
     return launch_dense<false, ACT>(a, st);
 }
 
+// (offsets inside a tile's operand rows are 32-bit: 256 rows of k or n stay below 2^31 bytes)
 static bool dense_sizes_ok(int64_t m, int64_t n, int64_t k) {
-    return m >= 0 && m <= 0x7FFFFFFF && n > 0 && n % 32 == 0 && k > 0 && k % 32 == 0 && n <= (1 << 22) && k <= (1 << 22) && n * k * 2 < ((int64_t)1 << 32);
+    return m >= 0 && m <= 0x7FFFFFFF && n > 0 && n % 32 == 0 && k > 0 && k % 32 == 0 && n <= (1 << 21) && k <= (1 << 21) && n * k * 2 < ((int64_t)1 << 32);
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

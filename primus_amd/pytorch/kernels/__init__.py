@@ -1454,8 +1454,8 @@ def _linear_args(m: int, n: int, k: int, activation):
     act = _LINEAR_ACTS.get(activation, -1) if activation is None or isinstance(activation, str) else -1
     if act < 0:
         raise ValueError(f"activation must be None, 'silu', 'gelu' or 'relu', got {activation!r}")
-    if n < 1 or k < 1 or n % 32 != 0 or k % 32 != 0 or n > 1 << 22 or k > 1 << 22:
-        raise ValueError("the dense bf16 linear needs n and k in multiples of 32 (forward and dgrad contract over them), at most 2^22")
+    if n < 1 or k < 1 or n % 32 != 0 or k % 32 != 0 or n > 1 << 21 or k > 1 << 21:
+        raise ValueError("the dense bf16 linear needs n and k in multiples of 32 (forward and dgrad contract over them), at most 2^21")
     if n * k >= 1 << 31:
         raise ValueError("the weight must be smaller than 4 GiB")
     if m > 0x7FFFFFFF:

@@ -1013,7 +1013,7 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
                   residual: Optional[torch.Tensor] = None, fuse_bgrad_accum_pattern: Optional[str] = None) -> torch.Tensor:
     """``act(a @ b^T + bias) + residual``: ``gemm`` on bf16 operands with what follows it in its epilogue, computed in fp32 and rounded
     once.  ``a [..., k]``, ``b [n, k]``, ``bias [n]`` (bfloat16 or float32), ``activation`` None, ``"silu"``, ``"gelu"`` (erf) or ``"relu"``,
-    ``residual [..., n]``.  ``n`` and ``k`` in multiples of 32, the weight below 4 GiB (anything else raises).  Differentiable in the four
+    ``residual [..., n]``.  ``n`` and ``k`` in multiples of 32 up to 2^21, the weight below 4 GiB (anything else raises).  Differentiable in the four
     tensors; the activation's input is kept in bf16 for the backward, whose gradients are those of that rounded value.
     ``fuse_bgrad_accum_pattern="megatron"`` adds the weight gradient into ``b.main_grad``, as ``gemm`` does."""
     accum = None if fuse_bgrad_accum_pattern is None else _accum_from(b, fuse_bgrad_accum_pattern)
@@ -1286,6 +1286,7 @@ def permute_tokens(x: torch.Tensor, indices: torch.Tensor, num_experts: int, pro
         raise ValueError("x must be [tokens, hidden] and indices [tokens, topk]")
     if indices.is_floating_point() or indices.dtype == torch.bool:
         raise ValueError("indices must be integers")
+    K._float_type(x, "x")
     rows, row_probs, group_lens, row_of, entry_of = _apply_if(
         x.requires_grad or (probs is not None and probs.requires_grad), _PermuteTokens, x.contiguous(), indices.to(torch.int64).contiguous(), int(num_experts), None if probs is None else probs.contiguous(), int(align))
     return rows, row_probs, group_lens, TokenPermutation(row_of, entry_of)

@@ -52,6 +52,8 @@ def test_cpu_tensors_are_refused():
     ("indices", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(3, 2, dtype=torch.int64), 3)),
     ("integers", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2), 3)),
     ("integers", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.bool), 3)),
+    ("x must be float32", lambda: ops.permute_tokens(torch.randn(4, 8).double(), torch.zeros(4, 2, dtype=torch.int64), 3)),
+    ("2.21", lambda: ops.gemm_bias_act(_bf(1, 1).expand(1, 32), _bf(1, 1).expand((1 << 21) + 32, 32))),
     ("x must be", lambda: ops.permute_tokens(torch.randn(4), torch.zeros(4, 2, dtype=torch.int64), 3)),
     ("number of experts", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int64), 0)),
     ("number of experts", lambda: ops.permute_tokens(torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int64), 1025)),
