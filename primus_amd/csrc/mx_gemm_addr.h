@@ -125,6 +125,19 @@ MXL_HD uint32_t tall_cols_lane(int t, int e, int64_t ld) {
 // The L2 request, one dword per 128-byte line: line 0 .. 255 of a slot of the operand.
 MXL_HD uint32_t tall_l2_lane(int line, bool cols, int64_t ld) { return (uint32_t)(cols ? (line >> 2) * ld + (line & 3) * 128 : line * ld); }
 
+// ---------------- dense bf16 linear's tiles (dense_tile_kernel) ----------------
+// `threads` lanes fetch 16-byte pieces of a slot of 64 contraction elements.  Rows whose contraction is contiguous: descriptor as
+// tall_rows_desc, thread t takes a piece of row t / 8 + (threads / 8) e.  Rows that are contraction rows, tn columns of them: descriptor as
+// tall_cols_desc from the matrix's first row, thread t takes a piece of row t / (tn / 8) + (threads / (tn / 8)) e.
+MXL_HD uint32_t dense_rows_lane(int t, int e, int threads, int64_t ld) {
+    const int row = (t >> 3) + threads / 8 * e;
+    return (uint32_t)(row * ld + 16 * ((t & 7) ^ ((row >> 1) & 7)));
+}
+MXL_HD uint32_t dense_cols_lane(int t, int e, int threads, int tn, int64_t ld) {
+    const int pieces = tn / 8, row = t / pieces + threads / pieces * e;
+    return (uint32_t)(row * ld + 16 * ((t % pieces) ^ ((row & 3) << (tn == 128 ? 2 : 1))));
+}
+
 // A scalar offset no request survives: operands end below 4 GiB and are a multiple of 32 bytes, so num_records is at most
 // 2^32 - 32 and the sum of the offsets (no wrap-around) is past it.
 constexpr uint32_t kDropped = 0xFFFFFFF0u;

@@ -44,7 +44,6 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
     constexpr int ROUND = THREADS * 16;                    // bytes of a load round
     constexpr int AR = TM * 128 / ROUND, BR = TN * 128 / ROUND, R = AR + BR;
     constexpr int A_BYTES = TM * DT_KS * 2, STAGE = A_BYTES + TN * DT_KS * 2;
-    constexpr int BT_PIECES = TN / 8;                       // 16-byte pieces of a staged row of the transposed operand
     constexpr int BT_SHIFT = TN == 128 ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int t = threadIdx.x;
@@ -79,25 +78,15 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
 
     const int64_t lda = p.k * 2, ldb = B_T ? p.n * 2 : p.k * 2;
     // the descriptors end with the operands; what is requested past them arrives as zeros
-    const v4i ra = make_rsrc(p.a + m0 * lda, (p.m - m0) * lda);
-    const v4i rb = B_T ? make_rsrc(p.b + n0 * 2, p.k * ldb - n0 * 2) : make_rsrc(p.b + n0 * ldb, (p.n - n0) * ldb);
+    const addr::Desc da = addr::tall_rows_desc(p.m, m0, lda);
+    const addr::Desc db = B_T ? addr::tall_cols_desc(0, p.k, ldb, n0 * 2) : addr::tall_rows_desc(p.n, n0, ldb);
+    const v4i ra = make_rsrc(p.a + da.base, da.records), rb = make_rsrc(p.b + db.base, db.records);
     const uint32_t a_step = DT_KS * 2, b_step = (uint32_t)__builtin_amdgcn_readfirstlane(B_T ? (int)(DT_KS * ldb) : DT_KS * 2);
     uint32_t va[AR], vb[BR];
 #pragma unroll
-    for (int e = 0; e < AR; ++e) {
-        const int row = (t >> 3) + THREADS / 8 * e;
-        va[e] = (uint32_t)(row * lda + 16 * ((t & 7) ^ ((row >> 1) & 7)));
-    }
+    for (int e = 0; e < AR; ++e) va[e] = addr::dense_rows_lane(t, e, THREADS, lda);
 #pragma unroll
-    for (int e = 0; e < BR; ++e) {
-        if constexpr (B_T) {
-            const int row = t / BT_PIECES + (THREADS / BT_PIECES) * e;
-            vb[e] = (uint32_t)(row * ldb + 16 * ((t % BT_PIECES) ^ ((row & 3) << BT_SHIFT)));
-        } else {
-            const int row = (t >> 3) + THREADS / 8 * e;
-            vb[e] = (uint32_t)(row * ldb + 16 * ((t & 7) ^ ((row >> 1) & 7)));
-        }
-    }
+    for (int e = 0; e < BR; ++e) vb[e] = B_T ? addr::dense_cols_lane(t, e, THREADS, TN, ldb) : addr::dense_rows_lane(t, e, THREADS, ldb);
     const uint32_t wave_base = (uint32_t)(uintptr_t)smem + (uint32_t)(w * 1024);
     // requests of slot s into a stage; past the range they are dropped, but counted
     struct In {

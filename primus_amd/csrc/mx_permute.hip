@@ -11,7 +11,10 @@
 //                                                                              dp[t, k] = <rows[row_of[t, k]], dy[t]>
 //
 // All of them are bound by the rows' bytes.  They go by tokens, not by rows of the permuted buffer: a token's row is read (or
-// written) once and its topk copies come out of (or go into) registers, which is the least there is to move.
+// written) once and its topk copies come out of (or go into) registers, which is the least there is to move.  us (TB/s): 16384 tokens of
+// 4096, two rows each, permute 76 (5.3), combine 85 (4.7), counting and placing 3.8 + 7.9; 8192 of 7168, eight each with probabilities,
+// combine 193 (5.5), its gradient 406 (4.9; a row at a time 536); 32 tokens of 2880, four each, 3.7 and 3.6 for placing.  A large copy
+// reaches 4.8-5.1 TB/s.
 #include "mx_lanes.h"
 
 namespace mxl {
