@@ -97,6 +97,8 @@ EXPORTS = (
     "mxl_linear_bf16_plan",
     "mxl_linear_bf16",
     "mxl_linear_bf16_dgrad",
+    "mxl_linear_bf16_wgrad_workspace_bytes",
+    "mxl_linear_bf16_wgrad",
     "mxl_linear_bf16_dz_workspace_bytes",
     "mxl_linear_bf16_dz",
     "mxl_linear_bf16_bwd_workspace_bytes",
@@ -274,7 +276,7 @@ def load() -> ctypes.CDLL:
         lib.mxl_linear_bf16.restype = i32
         lib.mxl_linear_bf16.argtypes = [vp, vp, vp, i32, i32, vp, i64, i64, i64, vp, vp, vp, i64, vp]
         lib.mxl_linear_bf16_plan.restype = i32
-        lib.mxl_linear_bf16_plan.argtypes = [i64, i64, i64, vp, vp, vp]
+        lib.mxl_linear_bf16_plan.argtypes = [i64, i64, i64, i32, vp, vp, vp]
         lib.mxl_linear_bf16_workspace_bytes.restype = i64
         lib.mxl_linear_bf16_workspace_bytes.argtypes = [i64, i64, i64]
         lib.mxl_linear_bf16_dgrad.restype = i32
@@ -284,7 +286,11 @@ def load() -> ctypes.CDLL:
         lib.mxl_linear_bf16_dz.restype = i32
         lib.mxl_linear_bf16_dz.argtypes = [vp, vp, i32, i64, i64, vp, vp, i32, vp, i64, vp]
         lib.mxl_linear_bf16_bwd_workspace_bytes.restype = i64
-        lib.mxl_linear_bf16_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, i32]
+        lib.mxl_linear_bf16_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, i32, i32]
+        lib.mxl_linear_bf16_wgrad_workspace_bytes.restype = i64
+        lib.mxl_linear_bf16_wgrad_workspace_bytes.argtypes = [i64, i64, i64]
+        lib.mxl_linear_bf16_wgrad.restype = i32
+        lib.mxl_linear_bf16_wgrad.argtypes = [vp, vp, i64, i64, i64, vp, u32, vp, i64, vp]
         lib.mxl_linear_bf16_bwd.restype = i32
         lib.mxl_linear_bf16_bwd.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, vp, u32, vp, i32, vp, i64, vp]
         _lib = lib

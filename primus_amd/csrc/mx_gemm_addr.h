@@ -135,7 +135,7 @@ MXL_HD uint32_t dense_rows_lane(int t, int e, int threads, int64_t ld) {
 }
 MXL_HD uint32_t dense_cols_lane(int t, int e, int threads, int tn, int64_t ld) {
     const int pieces = tn / 8, row = t / pieces + threads / pieces * e;
-    return (uint32_t)(row * ld + 16 * ((t % pieces) ^ ((row & 3) << (tn == 128 ? 2 : 1))));
+    return (uint32_t)(row * ld + 16 * ((t % pieces) ^ ((row & 3) << (tn >= 128 ? 2 : 1))));
 }
 
 // A scalar offset no request survives: operands end below 4 GiB and are a multiple of 32 bytes, so num_records is at most

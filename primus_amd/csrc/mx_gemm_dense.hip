@@ -5,7 +5,7 @@
 //   y = act(z) + residual,  z = a . b^T + bias     a [m, k], b [n, k];  fp32 from the products to y, one rounding
 //   backward: dz = dy act'(z),  da = dz . b,  db = dz^T . a,  dbias = column sums of dz
 //
-// The weight gradient, and the products of many rows, run on the grouped kernels' tiles (mx_gemm_bf16.hip) with one group.  This
+// Products with enough of them run on the grouped kernels' 256 x 256 tiles (mx_gemm_bf16.hip) with one group.  This
 // file holds the tiles of 256 x 128 and 64 x 64 for fewer rows, the kernel for a few rows, which is bound by reading b, and
 // the elementwise part of the backward.
 #include "mx_gemm_bf16.h"
@@ -17,7 +17,7 @@ typedef __bf16 d8bf __attribute__((ext_vector_type(8)));
 typedef short d4s __attribute__((ext_vector_type(4)));
 
 struct DenseArgs {
-    const uint8_t* a;       // [m, k]
+    const uint8_t* a;       // [m, k], or [k, m] (A_T)
     const uint8_t* b;       // [n, k], or [k, n] (B_T)
     uint16_t* c;            // [m, n]
     int64_t m, n, k;
@@ -35,16 +35,15 @@ template <int TM, int TN, int ST, bool SPLIT> constexpr int dense_lds_bytes() {
 
 // ---- tiles: WM x 2 waves, LDS-direct loads into three stages.  64 x 64: 4 waves, up to three workgroups on a CU, so that one's epilogue and
 // waits run under another's MFMAs.  256 x 128: 8 waves of 64 x 64, two on a SIMD; a wave reads 1 KiB of LDS per MFMA, which with the
-// fills makes 1375 clocks of LDS for 1024 of MFMAs in a slot.  B_T: b is [k, n], read with the transposing LDS read.
+// fills makes 1375 clocks of LDS for 1024 of MFMAs in a slot.  A_T, B_T: the operand is [k, m], [k, n], read with the transposing LDS read.
 // SPLIT: the contraction is cut into `splits` runs of slots, a workgroup each, whose fp32 sums dense_join_kernel adds up. ----
-template <int TM, int TN, int WM, int ST, bool B_T, int ACT, bool SPLIT>
+template <int TM, int TN, int WM, int ST, bool A_T, bool B_T, int ACT, bool SPLIT>
 __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
     constexpr int THREADS = WM * 128, WROWS = TM / WM;     // waves WM x 2; rows of a wave
     constexpr int FM = WROWS / 32, FN = TN / 64;           // 32 x 32 fragments per wave
     constexpr int ROUND = THREADS * 16;                    // bytes of a load round
     constexpr int AR = TM * 128 / ROUND, BR = TN * 128 / ROUND, R = AR + BR;
     constexpr int A_BYTES = TM * DT_KS * 2, STAGE = A_BYTES + TN * DT_KS * 2;
-    constexpr int BT_SHIFT = TN == 128 ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int t = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -74,17 +73,19 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
     const int m_valid = (int)((p.m - m0) < TM ? p.m - m0 : TM), n_valid = (int)((p.n - n0) < TN ? p.n - n0 : TN);
     const int all_slots = (int)((p.k + DT_KS - 1) / DT_KS), s_first = SPLIT ? split * p.split_slots : 0;
     const int slots = SPLIT && s_first + p.split_slots < all_slots ? s_first + p.split_slots : all_slots;      // the run's end
-    const bool odd = (p.k & 32) != 0;       // the last slot's second half is past the contraction: not multiplied
+    // the last slot's second half may be past the contraction, in the next row: not multiplied.  (Contraction rows past the end are zeros.)
+    const bool odd = !A_T && (p.k & 32) != 0;
 
-    const int64_t lda = p.k * 2, ldb = B_T ? p.n * 2 : p.k * 2;
+    const int64_t lda = A_T ? p.m * 2 : p.k * 2, ldb = B_T ? p.n * 2 : p.k * 2;
     // the descriptors end with the operands; what is requested past them arrives as zeros
-    const addr::Desc da = addr::tall_rows_desc(p.m, m0, lda);
+    const addr::Desc da = A_T ? addr::tall_cols_desc(0, p.k, lda, m0 * 2) : addr::tall_rows_desc(p.m, m0, lda);
     const addr::Desc db = B_T ? addr::tall_cols_desc(0, p.k, ldb, n0 * 2) : addr::tall_rows_desc(p.n, n0, ldb);
     const v4i ra = make_rsrc(p.a + da.base, da.records), rb = make_rsrc(p.b + db.base, db.records);
-    const uint32_t a_step = DT_KS * 2, b_step = (uint32_t)__builtin_amdgcn_readfirstlane(B_T ? (int)(DT_KS * ldb) : DT_KS * 2);
+    const uint32_t a_step = (uint32_t)__builtin_amdgcn_readfirstlane(A_T ? (int)(DT_KS * lda) : DT_KS * 2);
+    const uint32_t b_step = (uint32_t)__builtin_amdgcn_readfirstlane(B_T ? (int)(DT_KS * ldb) : DT_KS * 2);
     uint32_t va[AR], vb[BR];
 #pragma unroll
-    for (int e = 0; e < AR; ++e) va[e] = addr::dense_rows_lane(t, e, THREADS, lda);
+    for (int e = 0; e < AR; ++e) va[e] = A_T ? addr::dense_cols_lane(t, e, THREADS, TM, lda) : addr::dense_rows_lane(t, e, THREADS, lda);
 #pragma unroll
     for (int e = 0; e < BR; ++e) vb[e] = B_T ? addr::dense_cols_lane(t, e, THREADS, TN, ldb) : addr::dense_rows_lane(t, e, THREADS, ldb);
     const uint32_t wave_base = (uint32_t)(uintptr_t)smem + (uint32_t)(w * 1024);
@@ -109,24 +110,27 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
     struct Frag {
         d8bf a[FM], b[FN];
     };
+    // 8 contraction elements of 32 columns from col0 on, of an operand staged as [contraction row][columns] with `pitch` bytes a row
+    auto read_trans = [&](uint8_t* base, int pitch, int col0, int ks) __attribute__((always_inline)) {
+        const int shift = pitch >= 256 ? 2 : 1;
+        d8bf out;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = 16 * ks + 8 * g + 4 * h + tj, byte = 2 * col0 + 32 * tblk + 8 * ta4;
+            uint8_t* ptr = base + row * pitch + 16 * ((byte >> 4) ^ ((row & 3) << shift)) + (byte & 15);
+            const d4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) d4s*)ptr);
+            const v4bf q = __builtin_bit_cast(v4bf, v);
+            out[4 * h] = q[0]; out[4 * h + 1] = q[1]; out[4 * h + 2] = q[2]; out[4 * h + 3] = q[3];
+        }
+        return out;
+    };
     auto read_a = [&](uint8_t* st, int i, int ks) __attribute__((always_inline)) {
-        return *(const d8bf*)(st + ((lane_c + wm * WROWS * 128) ^ (32 * ks)) + i * 4096);
+        if constexpr (A_T) return read_trans(st, TM * 2, wm * WROWS + 32 * i, ks);
+        else return *(const d8bf*)(st + ((lane_c + wm * WROWS * 128) ^ (32 * ks)) + i * 4096);
     };
     auto read_b = [&](uint8_t* st, int j, int ks) __attribute__((always_inline)) {
-        if constexpr (!B_T) {
-            return *(const d8bf*)(st + A_BYTES + ((lane_c + wn * (TN / 2) * 128) ^ (32 * ks)) + j * 4096);
-        } else {
-            d8bf out;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = 16 * ks + 8 * g + 4 * h + tj, byte = 2 * (wn * (TN / 2) + 32 * j) + 32 * tblk + 8 * ta4;
-                uint8_t* ptr = st + A_BYTES + row * (TN * 2) + 16 * ((byte >> 4) ^ ((row & 3) << BT_SHIFT)) + (byte & 15);
-                const d4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) d4s*)ptr);
-                const v4bf q = __builtin_bit_cast(v4bf, v);
-                out[4 * h] = q[0]; out[4 * h + 1] = q[1]; out[4 * h + 2] = q[2]; out[4 * h + 3] = q[3];
-            }
-            return out;
-        }
+        if constexpr (B_T) return read_trans(st + A_BYTES, TN * 2, wn * (TN / 2) + 32 * j, ks);
+        else return *(const d8bf*)(st + A_BYTES + ((lane_c + wn * (TN / 2) * 128) ^ (32 * ks)) + j * 4096);
     };
 
     v16f acc[FM][FN];
@@ -511,13 +515,13 @@ static int64_t dz_run(int64_t m, int64_t n) {
     return (run + 7) / 8 * 8 < 8 ? 8 : (run + 7) / 8 * 8;
 }
 
-template <int TM, int TN, int WM, int ST, bool B_T, int ACT, bool SPLIT = false>
+template <int TM, int TN, int WM, int ST, bool A_T, bool B_T, int ACT, bool SPLIT = false>
 static int launch_dense_tile(const DenseArgs& a, hipStream_t st) {
     constexpr int lds = dense_lds_bytes<TM, TN, ST, SPLIT>();
     static std::atomic<bool> attr_set[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return MXL_ELAUNCH;
-    auto kern = dense_tile_kernel<TM, TN, WM, ST, B_T, ACT, SPLIT>;
+    auto kern = dense_tile_kernel<TM, TN, WM, ST, A_T, B_T, ACT, SPLIT>;
     if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
         if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return MXL_ELAUNCH;
         attr_set[dev & 63].store(true, std::memory_order_release);
@@ -532,7 +536,7 @@ static int launch_dense_tile(const DenseArgs& a, hipStream_t st) {
 // or several runs, these figures make the soonest done.  us of a slot of 64 elements, half with the weight cached and half with it from
 // memory, by the workgroups there are (w, of 256 CUs):
 //   256 x 256  1.12 + 0.42 w / 256                    one on a CU
-//   256 x 128  0.54 + 0.28 (w / 256)^2                one on a CU
+//   256 x 128  0.54 + 0.28 (w / 256)^2                one on a CU; 0.52 (w / 256)^2 for the weight gradient, which reads both operands transposed
 //   64 x 64    0.30 up to 256, 0.45 with two on every CU, 0.63 with three
 // and a split costs 4 us for the second launch and its fp32 sums' way out and in at 7 TB/s.  Forward, us, weight cached / from memory, 256 x 256,
 // 256 x 128 and 64 x 64 unsplit: [2048, 4096] x 4096 88 / 82, 58 / 61, 108 / 118; [1500, 2880] x 2880 55 / 66, 31 / 37, 46 / 51;
@@ -540,12 +544,15 @@ static int launch_dense_tile(const DenseArgs& a, hipStream_t st) {
 // 4096 120 / 133, four 50 / 53 (64 x 64 unsplit 76 / 104); [700, 4096] x 4096 40 / 47, two 34 / 36; [2048, 8192] x 2048 82 / 85, two
 // 68 / 70.  (128 x 128, two workgroups on a CU, is level with 256 x 128 where the weight is cached and behind where it is not: 62 / 70, 34 / 41, 75 / 92
 // for the first three; [333, 14336] x 4096 in four 53 / 65.)
+// Weight gradient [m, n]^T . [m, k], us, 256 x 256 (the grouped kernel with one group) / 256 x 128 / 64 x 64, unsplit, best split: 2051, 2880, 2880
+// 50 / 54 / 60; 1000, 2048, 2048 23 / 15 / 17; 4096, 1024, 4096 70 / 44 / 65, two runs 43; 8192, 2048, 1024 137 / 75 / 59, four runs of
+// 256 x 128 43; 8192, 256, 512 131 / 72 / 33, eight runs of 64 x 64 12; 300, 512, 1120 11 / - / 4.
 struct DensePlan {
     int tm, tn;         // output tile
     int splits;         // runs of the contraction, 1: not split
     int slots;          // slots per run
 };
-static DensePlan dense_plan(int64_t m, int64_t n, int64_t k) {
+static DensePlan dense_plan(int64_t m, int64_t n, int64_t k, bool a_by_columns = false) {
     auto tiles = [&](int tm, int tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
     const int slots = (int)((k + DT_KS - 1) / DT_KS);
     DensePlan best{256, 256, 1, slots};
@@ -564,22 +571,22 @@ static DensePlan dense_plan(int64_t m, int64_t n, int64_t k) {
         }
     };
     auto part = [](double x, double lo, double hi) { return x <= lo ? 0.0 : x >= hi ? 1.0 : (x - lo) / (hi - lo); };
-    consider(256, 128, 256, [&](double w) { return 0.54 + 0.28 * w * w; });
+    consider(256, 128, 256, [&](double w) { return 0.54 + (a_by_columns ? 0.52 : 0.28) * w * w; });
     consider(64, 64, 768, [&](double w) { return 0.30 + 0.15 * part(w, 1.0, 2.0) + 0.18 * part(w, 2.0, 3.0); });
     return best;
 }
 
-template <bool B_T, int ACT>
+template <bool A_T, bool B_T, int ACT>
 static int launch_dense(DenseArgs a, hipStream_t st) {
-    const DensePlan plan = dense_plan(a.m, a.n, a.k);
+    const DensePlan plan = dense_plan(a.m, a.n, a.k, A_T);
     if (plan.splits == 1) {
-        if (plan.tm == 256) return launch_dense_tile<256, 128, 4, 3, B_T, ACT>(a, st);
-        return launch_dense_tile<64, 64, 2, 3, B_T, ACT>(a, st);
+        if (plan.tm == 256) return launch_dense_tile<256, 128, 4, 3, A_T, B_T, ACT>(a, st);
+        return launch_dense_tile<64, 64, 2, 3, A_T, B_T, ACT>(a, st);
     }
     a.splits = plan.splits;
     a.split_slots = plan.slots;
-    const int rc = plan.tm == 256 ? launch_dense_tile<256, 128, 4, 3, B_T, kActNone, true>(a, st)
-                                 : launch_dense_tile<64, 64, 2, 3, B_T, kActNone, true>(a, st);
+    const int rc = plan.tm == 256 ? launch_dense_tile<256, 128, 4, 3, A_T, B_T, kActNone, true>(a, st)
+                                  : launch_dense_tile<64, 64, 2, 3, A_T, B_T, kActNone, true>(a, st);
     if (rc != MXL_OK) return rc;
     hipLaunchKernelGGL(dense_join_kernel<ACT>, dim3((unsigned)((a.m * a.n / 8 + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
@@ -597,13 +604,15 @@ static int launch_dense_forward(const DenseArgs& a, hipStream_t st) {
         const Bf16Args t{a.a, a.b, a.c, nullptr, 1, a.m, 0, a.n, a.k, a.epi};
         return launch_bf16_linear_tall(t, ACT, st);
     }
-    return launch_dense<false, ACT>(a, st);
+    return launch_dense<false, false, ACT>(a, st);
 }
 
 // (offsets inside a tile's operand rows are 32-bit: 256 rows of k or n stay below 2^31 bytes)
 static bool dense_sizes_ok(int64_t m, int64_t n, int64_t k) {
     return m >= 0 && m <= 0x7FFFFFFF && n > 0 && n % 32 == 0 && k > 0 && k % 32 == 0 && n <= (1 << 21) && k <= (1 << 21) && n * k * 2 < ((int64_t)1 << 32);
 }
+// the weight gradient contracts over the m rows, whose number is free; its operands end below 4 GiB
+static bool dense_wgrad_ok(int64_t m, int64_t n, int64_t k) { return dense_sizes_ok(m, n, k) && m * (n > k ? n : k) * 2 < ((int64_t)1 << 32); }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace mxl
@@ -617,9 +626,9 @@ extern "C" int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t
     return splits > 1 ? splits * m * n * 4 : 0;
 }
 
-extern "C" int mxl_linear_bf16_plan(int64_t m, int64_t n, int64_t k, int* tile_rows, int* tile_cols, int* splits) {
-    if (!dense_sizes_ok(m, n, k) || m == 0 || !tile_rows || !tile_cols || !splits) return MXL_EINVAL;
-    const DensePlan plan = dense_plan(m, n, k);
+extern "C" int mxl_linear_bf16_plan(int64_t m, int64_t n, int64_t k, int a_by_columns, int* tile_rows, int* tile_cols, int* splits) {
+    if (!dense_sizes_ok(m, n, 32) || m == 0 || k <= 0 || k > 0x7FFFFFFF || !tile_rows || !tile_cols || !splits) return MXL_EINVAL;
+    const DensePlan plan = dense_plan(m, n, k, a_by_columns != 0);
     *tile_rows = plan.tm, *tile_cols = plan.tn, *splits = plan.splits;
     return MXL_OK;
 }
@@ -656,7 +665,29 @@ extern "C" int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, in
     hipStream_t st = (hipStream_t)stream;
     if (dense_plan(m, k, n).tn == 256)
         return mxl_grouped_gemm_bf16(dz_bf16, b_bf16, da_bf16, nullptr, 1, m, k, n, MXL_BF_B_KN | MXL_BF_TILE_256, stream);
-    return launch_dense<true, kActNone>(d, st);
+    return launch_dense<false, true, kActNone>(d, st);
+}
+
+extern "C" int64_t mxl_linear_bf16_wgrad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (!dense_wgrad_ok(m, n, k)) return -1;
+    if (m == 0) return 0;
+    const int splits = dense_plan(n, k, m, true).splits;
+    return splits > 1 ? splits * n * k * 4 : 0;
+}
+
+// db [n, k] = dz [m, n]^T . a [m, k]
+extern "C" int mxl_linear_bf16_wgrad(const void* dz_bf16, const void* a_bf16, int64_t m, int64_t n, int64_t k, void* db, uint32_t flags, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+    if (!dense_wgrad_ok(m, n, k) || (flags & ~(uint32_t)MXL_BF_ACCUM_F32)) return MXL_EINVAL;
+    // added to a float buffer, without rows, or with enough large tiles: the grouped kernel with one group
+    if ((flags & MXL_BF_ACCUM_F32) || m == 0 || dense_plan(n, k, m, true).tn == 256)
+        return mxl_grouped_gemm_bf16_wgrad(dz_bf16, a_bf16, db, nullptr, 1, m, n, k, flags, stream);
+    if (!dz_bf16 || !a_bf16 || !db || !aligned16(dz_bf16) || !aligned16(a_bf16) || !aligned16(db)) return MXL_EINVAL;
+    const int64_t need = mxl_linear_bf16_wgrad_workspace_bytes(m, n, k);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)a_bf16, (uint16_t*)db, n, k, m, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0};
+    return launch_dense<true, true, kActNone>(d, (hipStream_t)stream);
 }
 
 extern "C" int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n) {
@@ -691,28 +722,33 @@ extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int a
 namespace mxl {
 static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 struct BwdSpace {
-    int64_t dz, sums, runs, total;      // bytes: dz (with an activation), dbias's partial sums, dgrad's split sums
+    int64_t dz, sums, runs, total;      // bytes: dz (with an activation), dbias's partial sums, the split sums of dgrad, then of the weight gradient
 };
-static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int act, bool need_da, bool need_dbias) {
+static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int act, bool need_da, bool need_db, bool need_dbias) {
     BwdSpace s;
     s.dz = act == MXL_ACT_NONE ? 0 : up256(m * n * 2);
     s.sums = need_dbias ? up256(mxl_linear_bf16_dz_workspace_bytes(m, n)) : 0;
-    s.runs = need_da ? up256(mxl_linear_bf16_workspace_bytes(m, k, n)) : 0;
+    const int64_t da = need_da ? mxl_linear_bf16_workspace_bytes(m, k, n) : 0, db = need_db ? mxl_linear_bf16_wgrad_workspace_bytes(m, n, k) : 0;
+    s.runs = up256(da > db ? da : db);
     s.total = s.dz + s.sums + s.runs;
     return s;
 }
 }  // namespace mxl
 
-extern "C" int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_dbias) {
-    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE) return -1;
-    return bwd_space(m, n, k, act, need_da != 0, need_dbias != 0).total;
+extern "C" int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_db,
+                                                       int need_dbias) {
+    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (need_db && !dense_wgrad_ok(m, n, k))) return -1;
+    return bwd_space(m, n, k, act, need_da != 0, need_db != 0, need_dbias != 0).total;
 }
 
 extern "C" int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_bf16, const void* z_bf16, int act, int64_t m, int64_t n, int64_t k,
                                    void* da_bf16, void* db, uint32_t db_flags, void* dbias, int dbias_dtype, void* workspace, int64_t workspace_bytes,
                                    void* stream) {
-    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (db_flags & ~(uint32_t)MXL_BF_ACCUM_F32)) return MXL_EINVAL;
-    const BwdSpace sp = bwd_space(m, n, k, act, da_bf16 != nullptr, dbias != nullptr);
+    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (db_flags & ~(uint32_t)MXL_BF_ACCUM_F32) ||
+        (db && !dense_wgrad_ok(m, n, k)))
+        return MXL_EINVAL;
+    const bool small_db = db && !(db_flags & MXL_BF_ACCUM_F32);
+    const BwdSpace sp = bwd_space(m, n, k, act, da_bf16 != nullptr, small_db, dbias != nullptr);
     if (sp.total > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < sp.total)) return MXL_EINVAL;
     if (da_bf16 && m > 0 && !b_bf16) return MXL_EINVAL;
     uint8_t* at = (uint8_t*)workspace;
@@ -722,6 +758,6 @@ extern "C" int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, cons
         rc = mxl_linear_bf16_dz(dy_bf16, z_bf16, act, m, n, dz, dbias, dbias_dtype, at + sp.dz, sp.sums, stream);
     const void* d = sp.dz ? dz : dy_bf16;
     if (rc == MXL_OK && da_bf16) rc = mxl_linear_bf16_dgrad(d, b_bf16, m, n, k, da_bf16, at + sp.dz + sp.sums, sp.runs, stream);
-    if (rc == MXL_OK && db) rc = mxl_grouped_gemm_bf16_wgrad(d, a_bf16, db, nullptr, 1, m, n, k, db_flags, stream);
+    if (rc == MXL_OK && db) rc = mxl_linear_bf16_wgrad(d, a_bf16, m, n, k, db, db_flags, at + sp.dz + sp.sums, sp.runs, stream);
     return rc;
 }

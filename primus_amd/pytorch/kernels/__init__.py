@@ -1535,7 +1535,8 @@ def linear_bf16_bwd_impl(dy, a, b, z, activation: Optional[str], need_a: bool = 
         da = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_a else None
         db = None if not need_b else accum_into if accum_into is not None else torch.empty((n, k), dtype=torch.bfloat16, device=dev)
         dbias = torch.empty(n, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
-        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_bwd_workspace_bytes", m, n, k, act, int(need_a), int(dbias is not None))
+        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_bwd_workspace_bytes", m, n, k, act, int(need_a), int(need_b and accum_into is None),
+                                  int(dbias is not None))
         rc = lib.mxl_linear_bf16_bwd(_ptr(dy), _ptr(a), b.data_ptr(), _ptr(z), act, m, n, k, _ptr(da), _ptr(db), _lib.BF_ACCUM_F32 if accum_into is not None else 0,
                                      _ptr(dbias), _lib.DT_BF16 if bias_dtype is None else _DT[bias_dtype], _ptr(ws), ws_bytes, _stream())
     if rc:
@@ -1583,20 +1584,34 @@ def linear_bf16_dgrad_impl(dz, b) -> torch.Tensor:
 
 
 def linear_bf16_wgrad_impl(dz, a, accum_into: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``dz^T . a`` for bf16 ``dz [m, n]``, ``a [m, k]``, or added to the float32 ``accum_into``.  The grouped kernel, whose operands end
-    below 4 GiB: longer ones go through it in runs of rows whose products meet in float32."""
+    """``dz^T . a`` for bf16 ``dz [m, n]``, ``a [m, k]``, or added to the float32 ``accum_into``.  The kernels' operands end below 4 GiB:
+    longer ones go through them in runs of rows whose products meet in float32."""
     _bf16_2d(dz, "dz")
     _bf16_2d(a, "a")
     m, n = dz.shape
     k = a.shape[1]
+    if a.shape[0] != m:
+        raise ValueError("dz and a must have the same rows")
+    _linear_args(m, n, k, None)
+    if accum_into is not None and (accum_into.dtype != torch.float32 or accum_into.numel() != n * k):
+        raise ValueError("accum_into must be a contiguous float32 buffer of the weight's size")
+    _require_cuda(dz, a, accum_into)
+    dev = dz.device
+    _same_device(dev, a=a, accum_into=accum_into)
     rows = ((1 << 32) - 1) // (2 * max(n, k)) // 64 * 64
-    with _on(dz.device):
-        if m <= rows:
-            return grouped_gemm_bf16_wgrad_impl(dz, a, None, accum_into=accum_into)
-        total = accum_into if accum_into is not None else torch.zeros((1, n, k), dtype=torch.float32, device=dz.device)
+    if m > rows:
+        total = accum_into if accum_into is not None else torch.zeros((n, k), dtype=torch.float32, device=dev)
         for lo in range(0, m, rows):
-            grouped_gemm_bf16_wgrad_impl(dz[lo:lo + rows], a[lo:lo + rows], None, accum_into=total)
+            linear_bf16_wgrad_impl(dz[lo:lo + rows], a[lo:lo + rows], accum_into=total)
         return total if accum_into is not None else total.to(torch.bfloat16)
+    with _on(dev), _hooked("linear_bf16_wgrad", m=m, n=n, k=k):
+        db = accum_into if accum_into is not None else torch.empty((n, k), dtype=torch.bfloat16, device=dev)
+        ws, ws_bytes = (None, 0) if accum_into is not None else _workspace(dev, "mxl_linear_bf16_wgrad_workspace_bytes", m, n, k)
+        rc = _lib.load().mxl_linear_bf16_wgrad(_ptr(dz), _ptr(a), m, n, k, db.data_ptr(), _lib.BF_ACCUM_F32 if accum_into is not None else 0, _ptr(ws), ws_bytes,
+                                               _stream())
+    if rc:
+        _lib.check(rc, "mxl_linear_bf16_wgrad")
+    return db
 
 
 # --------------------------------------------------------------------------

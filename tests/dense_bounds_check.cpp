@@ -40,7 +40,7 @@ static void cols(int tile, int threads, int64_t k, int64_t n, int64_t col0) {
     for (int64_t s = 0; s < slots + 3; ++s)
         for (int e = 0; e < tile * 128 / (threads * 16); ++e)
             for (int t = 0; t < threads; ++t) {
-                const int row = t / pieces + threads / pieces * e, piece = (t % pieces) ^ ((row & 3) << (tile == 128 ? 2 : 1));
+                const int row = t / pieces + threads / pieces * e, piece = (t % pieces) ^ ((row & 3) << (tile >= 128 ? 2 : 1));
                 const bool live = s < slots;
                 if (piece < 0 || piece >= pieces || row >= 64) std::exit(2);
                 request(d, dense_cols_lane(t, e, threads, tile, ld), live ? (uint32_t)(s * 64 * ld) : kDropped, k * ld, live && s * 64 + row < k && col0 + piece * 8 < n);
@@ -58,6 +58,13 @@ int main() {
         for (int64_t k : std::initializer_list<int64_t>{32, 64, 96, 224}) {
             for (int64_t c = 0; c < n; c += 64) cols(64, 256, k, n, c);
             for (int64_t c = 0; c < n; c += 128) cols(128, 512, k, n, c);
+        }
+    // the weight gradient: contraction rows in any number, 256 columns of the first operand
+    for (int64_t n : std::initializer_list<int64_t>{32, 96, 256, 288, 544})
+        for (int64_t k : std::initializer_list<int64_t>{1, 17, 63, 64, 65, 130}) {
+            for (int64_t c = 0; c < n; c += 64) cols(64, 256, k, n, c);
+            for (int64_t c = 0; c < n; c += 128) cols(128, 512, k, n, c);
+            for (int64_t c = 0; c < n; c += 256) cols(256, 512, k, n, c);
         }
     // the largest operands: one row, and a tile's last rows, of 2^21 elements; a matrix of almost 4 GiB
     rows(256, 512, 256, 1 << 21, 0);

@@ -52,7 +52,8 @@ def _inputs(gpu, m, n, k, seed, bias_dtype=torch.bfloat16):
 # ragged last tiles, long and split contractions
 SIZES = [(1, 32, 32), (13, 8224, 96), (1, 4096, 1056), (7, 96, 4096), (16, 64, 288), (17, 160, 96), (33, 320, 800), (64, 2880, 64), (65, 96, 32), (100, 32, 2080), (127, 224, 160),
          (129, 416, 64), (300, 512, 1120), (777, 1056, 96), (2051, 2880, 96), (2100, 2080, 160), (4096, 1024, 4096), (1000, 2048, 14336),
-         (4200, 4128, 32), (4353, 4160, 160), (70, 64, 1056), (130, 128, 4128), (333, 4096, 2048), (700, 4096, 2080), (1900, 1056, 1184), (2051, 96, 2880), (4200, 32, 4128), (700, 4128, 4128)]
+         (4200, 4128, 32), (4353, 4160, 160), (70, 64, 1056), (130, 128, 4128), (333, 4096, 2048), (700, 4096, 2080), (1900, 1056, 1184), (2051, 96, 2880), (4200, 32, 4128), (700, 4128, 4128),
+         (5003, 1088, 1056)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -109,9 +110,9 @@ def test_every_way_of_running_is_among_the_sizes():
 
     from primus_amd import _lib
 
-    def plan(m, n, k):
+    def plan(m, n, k, by_columns=0):
         t = [ctypes.c_int() for _ in range(3)]
-        assert _lib.load().mxl_linear_bf16_plan(m, n, k, *[ctypes.byref(x) for x in t]) == 0
+        assert _lib.load().mxl_linear_bf16_plan(m, n, k, by_columns, *[ctypes.byref(x) for x in t]) == 0
         return (t[0].value, t[1].value, t[2].value > 1)
 
     ways = {(256, 256, False), (256, 128, False), (256, 128, True), (64, 64, False), (64, 64, True)}
@@ -119,6 +120,10 @@ def test_every_way_of_running_is_among_the_sizes():
     assert {plan(*s) for s in SIZES if s[0] > 16} == ways == {plan(m, k, n) for m, n, k in SIZES}
     for tile in ways:      # and with a contraction that ends half way through a slot
         assert any(plan(m, n, k) == tile and odd(k) for m, n, k in SIZES if m > 16) and any(plan(m, k, n) == tile and odd(n) for m, n, k in SIZES), tile
+    # the weight gradient, whose contraction is over the rows and ends anywhere in a slot
+    assert {plan(n, k, m, 1) for m, n, k in SIZES} == ways
+    for tile in ways:
+        assert any(plan(n, k, m, 1) == tile and m % 64 for m, n, k in SIZES), tile
     assert any(m <= 16 and n >= 8192 for m, n, k in SIZES) and any(m <= 16 and n < 8192 for m, n, k in SIZES)
 
 
