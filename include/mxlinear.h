@@ -612,8 +612,8 @@ int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int 
  * fp32 from the products to y, which is rounded once; bias (bf16 or float, NULL: none), residual (NULL: none); act MXL_ACT_*.
  * z_bf16: if not NULL, z rounded to bf16 for the backward.  n and k multiples of 32 up to 2^21, n * k * 2 < 2^32, pointers 16-byte aligned.
  * Few tiles and a long contraction split it over workgroups, whose sums meet in the caller's workspace:
- * mxl_linear_bf16_workspace_bytes(m, n, k) bytes for the forward, (m, k, n) for dgrad, mxl_linear_bf16_wgrad_workspace_bytes(m, n, k) for the
- * weight gradient (0: none, NULL will do).
+ * mxl_linear_bf16_workspace_bytes(m, n, k) bytes for the forward, (m, k, n) for dgrad, mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, flags) for
+ * the weight gradient (0: none, NULL will do).
  *
  * Backward: mxl_linear_bf16_dz gives dz = dy * act'(z) (not written, and may be dy itself, for MXL_ACT_NONE) and
  * dbias = column sums of dz before its rounding (NULL: not wanted); mxl_linear_bf16_dgrad gives da = dz . b;
@@ -626,7 +626,7 @@ int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const void* bias, in
                     int64_t n, int64_t k, void* y_bf16, void* z_bf16, void* workspace, int64_t workspace_bytes, void* stream);
 int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* workspace,
                           int64_t workspace_bytes, void* stream);
-int64_t mxl_linear_bf16_wgrad_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int64_t mxl_linear_bf16_wgrad_workspace_bytes(int64_t m, int64_t n, int64_t k, uint32_t flags);
 int mxl_linear_bf16_wgrad(const void* dz_bf16, const void* a_bf16, int64_t m, int64_t n, int64_t k, void* db, uint32_t flags, void* workspace,
                           int64_t workspace_bytes, void* stream);
 int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n);
@@ -635,7 +635,8 @@ int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int act, int64_t
 
 /* The three of them in one call: da (NULL: not wanted), db [n, k] (NULL: not wanted; MXL_BF_ACCUM_F32: float, added to), dbias (NULL).
  * m * max(n, k) * 2 < 2^32 where db is wanted.  The workspace holds dz too. */
-int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_db, int need_dbias);
+int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_db, uint32_t db_flags,
+                                            int need_dbias);
 int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_bf16, const void* z_bf16, int act, int64_t m, int64_t n, int64_t k,
                         void* da_bf16, void* db, uint32_t db_flags, void* dbias, int dbias_dtype, void* workspace, int64_t workspace_bytes,
                         void* stream);

@@ -286,9 +286,9 @@ def load() -> ctypes.CDLL:
         lib.mxl_linear_bf16_dz.restype = i32
         lib.mxl_linear_bf16_dz.argtypes = [vp, vp, i32, i64, i64, vp, vp, i32, vp, i64, vp]
         lib.mxl_linear_bf16_bwd_workspace_bytes.restype = i64
-        lib.mxl_linear_bf16_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, i32, i32]
+        lib.mxl_linear_bf16_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, i32, u32, i32]
         lib.mxl_linear_bf16_wgrad_workspace_bytes.restype = i64
-        lib.mxl_linear_bf16_wgrad_workspace_bytes.argtypes = [i64, i64, i64]
+        lib.mxl_linear_bf16_wgrad_workspace_bytes.argtypes = [i64, i64, i64, u32]
         lib.mxl_linear_bf16_wgrad.restype = i32
         lib.mxl_linear_bf16_wgrad.argtypes = [vp, vp, i64, i64, i64, vp, u32, vp, i64, vp]
         lib.mxl_linear_bf16_bwd.restype = i32

@@ -24,6 +24,7 @@ struct DenseArgs {
     EpilogueArgs epi;
     float* partial;         // SPLIT: [splits, m, n]
     int splits, split_slots;
+    float* sum;             // the join adds to this float [m, n] (the weight gradient into main_grad) instead of writing c
 };
 
 constexpr int DT_KS = 64;       // contraction elements per slot: 128 bytes of a row, four MFMA steps
@@ -341,7 +342,8 @@ __global__ __launch_bounds__(WM * 128, 2) void dense_tile_kernel(DenseArgs p) {
     leave(p.c);
 }
 
-// The runs of a split contraction added up in their order, and the epilogue: eight columns of a row per thread.
+// The runs of a split contraction added up in their order, and the epilogue, or the addition to a float buffer: eight columns of a row per
+// thread.
 template <int ACT>
 __global__ __launch_bounds__(256) void dense_join_kernel(DenseArgs p) {
     const int64_t mn = p.m * p.n, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
@@ -351,6 +353,11 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseArgs p) {
     for (int s = 1; s < p.splits; ++s) {
         lo += *(const v4f*)(p.partial + s * mn + at);
         hi += *(const v4f*)(p.partial + s * mn + at + 4);
+    }
+    if (p.sum) {
+        *(v4f*)(p.sum + at) += lo;
+        *(v4f*)(p.sum + at + 4) += hi;
+        return;
     }
     lo += epi_bias4(p.epi, col);
     hi += epi_bias4(p.epi, col + 4);
@@ -579,7 +586,7 @@ static DensePlan dense_plan(int64_t m, int64_t n, int64_t k, bool a_by_columns =
 template <bool A_T, bool B_T, int ACT>
 static int launch_dense(DenseArgs a, hipStream_t st) {
     const DensePlan plan = dense_plan(a.m, a.n, a.k, A_T);
-    if (plan.splits == 1) {
+    if (plan.splits == 1 && !a.sum) {
         if (plan.tm == 256) return launch_dense_tile<256, 128, 4, 3, A_T, B_T, ACT>(a, st);
         return launch_dense_tile<64, 64, 2, 3, A_T, B_T, ACT>(a, st);
     }
@@ -613,6 +620,10 @@ static bool dense_sizes_ok(int64_t m, int64_t n, int64_t k) {
 }
 // the weight gradient contracts over the m rows, whose number is free; its operands end below 4 GiB
 static bool dense_wgrad_ok(int64_t m, int64_t n, int64_t k) { return dense_sizes_ok(m, n, k) && m * (n > k ? n : k) * 2 < ((int64_t)1 << 32); }
+// It runs on this file's tiles unless it has enough large ones, or no rows, or offsets that pass 32 bits in the 63 rows behind the last one
+static bool dense_wgrad_here(int64_t m, int64_t n, int64_t k) {
+    return m > 0 && (m + 64) * (n > k ? n : k) * 2 < ((int64_t)1 << 32) && dense_plan(n, k, m, true).tn != 256;
+}
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace mxl
@@ -642,7 +653,7 @@ extern "C" int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const voi
     const int64_t need = mxl_linear_bf16_workspace_bytes(m, n, k);
     if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
-    DenseArgs d{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, (uint16_t*)y_bf16, m, n, k, {bias, (const uint16_t*)residual_bf16, (uint16_t*)z_bf16, bias_dtype == MXL_DT_F32}, (float*)workspace, 1, 0};
+    DenseArgs d{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, (uint16_t*)y_bf16, m, n, k, {bias, (const uint16_t*)residual_bf16, (uint16_t*)z_bf16, bias_dtype == MXL_DT_F32}, (float*)workspace, 1, 0, nullptr};
     hipStream_t st = (hipStream_t)stream;
     switch (act) {
         case MXL_ACT_SILU: return launch_dense_forward<kActSilu>(d, st);
@@ -661,32 +672,33 @@ extern "C" int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, in
     const int64_t need = mxl_linear_bf16_workspace_bytes(m, k, n);
     if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
-    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)b_bf16, (uint16_t*)da_bf16, m, k, n, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0};
+    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)b_bf16, (uint16_t*)da_bf16, m, k, n, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0, nullptr};
     hipStream_t st = (hipStream_t)stream;
     if (dense_plan(m, k, n).tn == 256)
         return mxl_grouped_gemm_bf16(dz_bf16, b_bf16, da_bf16, nullptr, 1, m, k, n, MXL_BF_B_KN | MXL_BF_TILE_256, stream);
     return launch_dense<false, true, kActNone>(d, st);
 }
 
-extern "C" int64_t mxl_linear_bf16_wgrad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    if (!dense_wgrad_ok(m, n, k)) return -1;
-    if (m == 0) return 0;
+extern "C" int64_t mxl_linear_bf16_wgrad_workspace_bytes(int64_t m, int64_t n, int64_t k, uint32_t flags) {
+    if (!dense_wgrad_ok(m, n, k) || (flags & ~(uint32_t)MXL_BF_ACCUM_F32)) return -1;
+    const bool accum = (flags & MXL_BF_ACCUM_F32) != 0;
+    if (!dense_wgrad_here(m, n, k)) return 0;
     const int splits = dense_plan(n, k, m, true).splits;
-    return splits > 1 ? splits * n * k * 4 : 0;
+    return splits > 1 || accum ? splits * n * k * 4 : 0;
 }
 
 // db [n, k] = dz [m, n]^T . a [m, k]
 extern "C" int mxl_linear_bf16_wgrad(const void* dz_bf16, const void* a_bf16, int64_t m, int64_t n, int64_t k, void* db, uint32_t flags, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
     if (!dense_wgrad_ok(m, n, k) || (flags & ~(uint32_t)MXL_BF_ACCUM_F32)) return MXL_EINVAL;
-    // added to a float buffer, without rows, or with enough large tiles: the grouped kernel with one group
-    if ((flags & MXL_BF_ACCUM_F32) || m == 0 || dense_plan(n, k, m, true).tn == 256)
+    if (!dense_wgrad_here(m, n, k))      // the grouped kernel with one group
         return mxl_grouped_gemm_bf16_wgrad(dz_bf16, a_bf16, db, nullptr, 1, m, n, k, flags, stream);
     if (!dz_bf16 || !a_bf16 || !db || !aligned16(dz_bf16) || !aligned16(a_bf16) || !aligned16(db)) return MXL_EINVAL;
-    const int64_t need = mxl_linear_bf16_wgrad_workspace_bytes(m, n, k);
+    const bool accum = (flags & MXL_BF_ACCUM_F32) != 0;
+    const int64_t need = mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, flags);
     if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
-    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)a_bf16, (uint16_t*)db, n, k, m, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0};
+    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)a_bf16, accum ? nullptr : (uint16_t*)db, n, k, m, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0, accum ? (float*)db : nullptr};
     return launch_dense<true, true, kActNone>(d, (hipStream_t)stream);
 }
 
@@ -724,21 +736,23 @@ static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 struct BwdSpace {
     int64_t dz, sums, runs, total;      // bytes: dz (with an activation), dbias's partial sums, the split sums of dgrad, then of the weight gradient
 };
-static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int act, bool need_da, bool need_db, bool need_dbias) {
+static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int act, bool need_da, bool need_db, uint32_t db_flags, bool need_dbias) {
     BwdSpace s;
     s.dz = act == MXL_ACT_NONE ? 0 : up256(m * n * 2);
     s.sums = need_dbias ? up256(mxl_linear_bf16_dz_workspace_bytes(m, n)) : 0;
-    const int64_t da = need_da ? mxl_linear_bf16_workspace_bytes(m, k, n) : 0, db = need_db ? mxl_linear_bf16_wgrad_workspace_bytes(m, n, k) : 0;
+    const int64_t da = need_da ? mxl_linear_bf16_workspace_bytes(m, k, n) : 0, db = need_db ? mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, db_flags) : 0;
     s.runs = up256(da > db ? da : db);
     s.total = s.dz + s.sums + s.runs;
     return s;
 }
 }  // namespace mxl
 
-extern "C" int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_db,
+extern "C" int64_t mxl_linear_bf16_bwd_workspace_bytes(int64_t m, int64_t n, int64_t k, int act, int need_da, int need_db, uint32_t db_flags,
                                                        int need_dbias) {
-    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (need_db && !dense_wgrad_ok(m, n, k))) return -1;
-    return bwd_space(m, n, k, act, need_da != 0, need_db != 0, need_dbias != 0).total;
+    if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (need_db && !dense_wgrad_ok(m, n, k)) ||
+        (db_flags & ~(uint32_t)MXL_BF_ACCUM_F32))
+        return -1;
+    return bwd_space(m, n, k, act, need_da != 0, need_db != 0, db_flags, need_dbias != 0).total;
 }
 
 extern "C" int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_bf16, const void* z_bf16, int act, int64_t m, int64_t n, int64_t k,
@@ -747,8 +761,7 @@ extern "C" int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, cons
     if (!dense_sizes_ok(m, n, k) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (db_flags & ~(uint32_t)MXL_BF_ACCUM_F32) ||
         (db && !dense_wgrad_ok(m, n, k)))
         return MXL_EINVAL;
-    const bool small_db = db && !(db_flags & MXL_BF_ACCUM_F32);
-    const BwdSpace sp = bwd_space(m, n, k, act, da_bf16 != nullptr, small_db, dbias != nullptr);
+    const BwdSpace sp = bwd_space(m, n, k, act, da_bf16 != nullptr, db != nullptr, db_flags, dbias != nullptr);
     if (sp.total > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < sp.total)) return MXL_EINVAL;
     if (da_bf16 && m > 0 && !b_bf16) return MXL_EINVAL;
     uint8_t* at = (uint8_t*)workspace;

@@ -1535,8 +1535,8 @@ def linear_bf16_bwd_impl(dy, a, b, z, activation: Optional[str], need_a: bool = 
         da = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_a else None
         db = None if not need_b else accum_into if accum_into is not None else torch.empty((n, k), dtype=torch.bfloat16, device=dev)
         dbias = torch.empty(n, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
-        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_bwd_workspace_bytes", m, n, k, act, int(need_a), int(need_b and accum_into is None),
-                                  int(dbias is not None))
+        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_bwd_workspace_bytes", m, n, k, act, int(need_a), int(need_b),
+                                  _lib.BF_ACCUM_F32 if accum_into is not None else 0, int(dbias is not None))
         rc = lib.mxl_linear_bf16_bwd(_ptr(dy), _ptr(a), b.data_ptr(), _ptr(z), act, m, n, k, _ptr(da), _ptr(db), _lib.BF_ACCUM_F32 if accum_into is not None else 0,
                                      _ptr(dbias), _lib.DT_BF16 if bias_dtype is None else _DT[bias_dtype], _ptr(ws), ws_bytes, _stream())
     if rc:
@@ -1606,9 +1606,9 @@ def linear_bf16_wgrad_impl(dz, a, accum_into: Optional[torch.Tensor] = None) -> 
         return total if accum_into is not None else total.to(torch.bfloat16)
     with _on(dev), _hooked("linear_bf16_wgrad", m=m, n=n, k=k):
         db = accum_into if accum_into is not None else torch.empty((n, k), dtype=torch.bfloat16, device=dev)
-        ws, ws_bytes = (None, 0) if accum_into is not None else _workspace(dev, "mxl_linear_bf16_wgrad_workspace_bytes", m, n, k)
-        rc = _lib.load().mxl_linear_bf16_wgrad(_ptr(dz), _ptr(a), m, n, k, db.data_ptr(), _lib.BF_ACCUM_F32 if accum_into is not None else 0, _ptr(ws), ws_bytes,
-                                               _stream())
+        flags = _lib.BF_ACCUM_F32 if accum_into is not None else 0
+        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_wgrad_workspace_bytes", m, n, k, flags)
+        rc = _lib.load().mxl_linear_bf16_wgrad(_ptr(dz), _ptr(a), m, n, k, db.data_ptr(), flags, _ptr(ws), ws_bytes, _stream())
     if rc:
         _lib.check(rc, "mxl_linear_bf16_wgrad")
     return db

@@ -201,6 +201,19 @@ def test_weight_gradient_into_main_grad(gpu):
     assert bool(((w.main_grad - 1.0 - plain.float()).abs() <= 2.0 ** -8 * plain.float().abs() + 2.0 ** -23 * (2.0 + plain.float().abs())).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(200, 96, 64), (1, 32, 32), (777, 1056, 96), (4200, 4128, 32), (1000, 2048, 1056), (5003, 1088, 1056), (700, 4128, 4128), (0, 64, 32)])
+def test_weight_gradient_added_to_a_float_buffer(gpu, m, n, k):
+    """Integers, whose sums are exact in float32: what was there plus the product, before any rounding to bf16."""
+    from primus_amd.pytorch import kernels as K
+
+    gen = torch.Generator().manual_seed(m + n)
+    dz, a = (torch.randint(-2, 3, s, generator=gen).bfloat16().to(gpu) for s in ((m, n), (m, k)))
+    total = torch.randint(-9, 9, (n, k), generator=gen).float().to(gpu)
+    want = total.double() + dz.double().t() @ a.double()
+    assert K.linear_bf16_wgrad_impl(dz, a, accum_into=total) is total and torch.equal(total.double(), want)
+    assert torch.equal(K.linear_bf16_wgrad_impl(dz, a), (dz.double().t() @ a.double()).bfloat16())
+
+
 def test_values_that_are_not_finite_stay_in_their_rows(gpu):
     from primus_amd.pytorch import ops
 

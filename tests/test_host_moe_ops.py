@@ -142,16 +142,16 @@ def test_c_entries_check_before_they_touch_the_device():
     assert ws == 128 and dz() == -3 and dz(act=3, db=None) == 0
     for bad in (dict(dy=None), dict(z=None), dict(dz=None), dict(act=9), dict(n=31), dict(w=None), dict(wb=ws - 1), dict(dbd=2), dict(dy=odd)):
         assert dz(**bad) == -1, bad
-    need = lib.mxl_linear_bf16_bwd_workspace_bytes(100, 64, 32, 1, 1, 1, 1)
-    assert need > 0 and lib.mxl_linear_bf16_bwd_workspace_bytes(100, 64, 32, 3, 0, 0, 0) == 0 and lib.mxl_linear_bf16_bwd_workspace_bytes(1, 1, 1, 3, 0, 0, 0) == -1
+    need = lib.mxl_linear_bf16_bwd_workspace_bytes(100, 64, 32, 1, 1, 1, 0, 1)
+    assert need > 0 and lib.mxl_linear_bf16_bwd_workspace_bytes(100, 64, 32, 3, 0, 0, 0, 0) == 0 and lib.mxl_linear_bf16_bwd_workspace_bytes(1, 1, 1, 3, 0, 0, 0, 0) == -1
     bwd = lambda **k: lib.mxl_linear_bf16_bwd(*[{**dict(dy=p, a=p, b=p, z=p, act=1, m=100, n=64, k=32, da=p, db=p, f=0, dbias=p, dbd=0, w=p, wb=need, st=None), **k}[n]  # noqa: E731
                                                 for n in ("dy", "a", "b", "z", "act", "m", "n", "k", "da", "db", "f", "dbias", "dbd", "w", "wb", "st")])
     assert bwd() == -3 and bwd(act=3, da=None, db=None, dbias=None, w=None, wb=0) == 0
     for bad in (dict(dy=None), dict(b=None), dict(z=None), dict(act=7), dict(n=33), dict(f=1), dict(dbd=2), dict(w=None), dict(wb=need - 1)):
         assert bwd(**bad) == -1, bad
-    need = lib.mxl_linear_bf16_wgrad_workspace_bytes(4096, 64, 64)
+    need = lib.mxl_linear_bf16_wgrad_workspace_bytes(4096, 64, 64, 0)
     wgrad = lambda dz, a, m, n, k, db, f=0, w=None, wb=0: lib.mxl_linear_bf16_wgrad(dz, a, m, n, k, db, f, w, wb, None)  # noqa: E731
-    assert need > 0 and wgrad(p, p, 4096, 64, 64, p, 0, p, need) == -3 and wgrad(p, p, 7, 32, 32, p) == -3 and wgrad(p, p, 7, 32, 32, p, 2) == -3
-    for bad in ((None, p, 7, 32, 32, p), (p, None, 7, 32, 32, p), (p, p, 7, 32, 32, None), (p, p, 7, 33, 32, p), (p, p, 7, 32, 32, p, 1), (p, p, 4096, 64, 64, p),
+    assert need > 0 and wgrad(p, p, 4096, 64, 64, p, 0, p, need) == -3 and wgrad(p, p, 7, 32, 32, p) == -3 and wgrad(p, p, 7, 32, 32, p, 2, p, 4096) == -3
+    for bad in ((None, p, 7, 32, 32, p), (p, None, 7, 32, 32, p), (p, p, 7, 32, 32, None), (p, p, 7, 33, 32, p), (p, p, 7, 32, 32, p, 1), (p, p, 7, 32, 32, p, 2), (p, p, 7, 32, 32, p, 2, p, 4095), (p, p, 4096, 64, 64, p),
                 (p, p, 4096, 64, 64, p, 0, p, need - 1), (p, p, 1 << 20, 4096, 4096, p), (odd, p, 7, 32, 32, p)):
         assert wgrad(*bad) == -1, bad
