@@ -595,6 +595,10 @@ int mxl_permute_plan(const int64_t* indices, int64_t entries, int num_experts, i
 /* out[row_of[t, k]] = x[t] for rows of any bytes, zero rows where entry_of is -1; topk <= 32. */
 int mxl_permute_rows(const void* x, int64_t tokens, int64_t row_bytes, const int64_t* row_of, int topk, const int32_t* entry_of,
                      int64_t rows, void* out, void* stream);
+/* mxl_permute_plan for indices [tokens, topk], then mxl_permute_rows of x: one call, and the plan's workspace. */
+int mxl_permute_tokens(const void* x, int64_t tokens, int64_t row_bytes, const int64_t* indices, int topk, int num_experts, int align,
+                       int64_t rows, int64_t* row_of, int32_t* entry_of, int64_t* group_lens, const void* probs, int prob_bytes,
+                       void* row_probs, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 /* y[t] = sum_k probs[t, k] * rows[row_of[t, k]] (probs NULL: ones), fp32 in the order of k, rounded once; entries of -1 add
  * nothing.  If row_probs is set, probs_out[t, k] = row_probs[row_of[t, k]] (0 for -1) on the way: together the gradient of
  * mxl_permute_rows and of the probabilities' move. */

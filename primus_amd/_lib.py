@@ -90,6 +90,7 @@ EXPORTS = (
     "mxl_topk_routing_bwd",
     "mxl_permute_plan_workspace_bytes",
     "mxl_permute_plan",
+    "mxl_permute_tokens",
     "mxl_permute_rows",
     "mxl_combine_rows",
     "mxl_combine_rows_bwd",
@@ -265,6 +266,8 @@ def load() -> ctypes.CDLL:
         lib.mxl_topk_routing_bwd.argtypes = [vp, vp, i32, vp, i64, i32, i32, i32, i32, f32, vp, vp]
         lib.mxl_permute_plan_workspace_bytes.restype = i64
         lib.mxl_permute_plan_workspace_bytes.argtypes = [i64, i32]
+        lib.mxl_permute_tokens.restype = i32
+        lib.mxl_permute_tokens.argtypes = [vp, i64, i64, vp, i32, i32, i32, i64, vp, vp, vp, vp, i32, vp, vp, vp, i64, vp]
         lib.mxl_permute_plan.restype = i32
         lib.mxl_permute_plan.argtypes = [vp, i64, i32, i32, i64, vp, vp, vp, vp, i32, vp, vp, i64, vp]
         lib.mxl_permute_rows.restype = i32

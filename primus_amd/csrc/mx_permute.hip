@@ -433,6 +433,15 @@ extern "C" int mxl_permute_rows(const void* x, int64_t tokens, int64_t row_bytes
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
 
+extern "C" int mxl_permute_tokens(const void* x, int64_t tokens, int64_t row_bytes, const int64_t* indices, int topk, int num_experts, int align,
+                                  int64_t rows, int64_t* row_of, int32_t* entry_of, int64_t* group_lens, const void* probs, int prob_bytes,
+                                  void* row_probs, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!move_sizes_ok(tokens, topk, rows) || row_bytes < 1 || row_bytes > (1 << 24) || (tokens > 0 && !x) || (rows > 0 && !out)) return MXL_EINVAL;
+    const int rc = mxl_permute_plan(indices, tokens * topk, num_experts, align, rows, row_of, entry_of, group_lens, probs, prob_bytes, row_probs,
+                                    workspace, workspace_bytes, stream);
+    return rc != MXL_OK ? rc : mxl_permute_rows(x, tokens, row_bytes, row_of, topk, entry_of, rows, out, stream);
+}
+
 // launches `kernel<DT, N>` for a type and whether rows are made of aligned 16-byte pieces
 #define MXL_BY_TYPE(kernel, wide, grid, st, a)                                                                                \
     do {                                                                                                                      \

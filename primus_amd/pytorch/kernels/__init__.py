@@ -1331,40 +1331,48 @@ def topk_routing_bwd_impl(dprobs, logits, indices, score_function: str = "softma
     return dlogits
 
 
-def permute_plan_impl(indices, num_experts: int, align: int = 1, probs: Optional[torch.Tensor] = None):
-    """``(row_of [tokens, topk] int64, entry_of [rows] int32, group_lens [experts] int64, row_probs [rows] or None)``: where every
-    entry of ``indices`` goes in a buffer of rows sorted by expert; see ``ops.permute_tokens``."""
+def permute_tokens_impl(x, indices, num_experts: int, align: int = 1, probs: Optional[torch.Tensor] = None):
+    """``(out [rows, hidden], row_of [tokens, topk] int64, entry_of [rows] int32, group_lens [experts] int64, row_probs [rows] or None)``:
+    where every entry of ``indices`` goes in a buffer of rows sorted by expert, and that buffer; see ``ops.permute_tokens``."""
+    _gpu_rows(x, "rows")
     _require_cuda(indices, probs)
-    if indices.dtype != torch.int64 or indices.dim() != 2:
-        raise ValueError("indices must be int64 [tokens, topk]")
+    if x.shape[1] < 1:
+        raise ValueError("expected rows that are not empty")
+    if indices.dtype != torch.int64 or indices.dim() != 2 or indices.shape[0] != x.shape[0]:
+        raise ValueError("indices must be int64 [tokens, topk] with one row per row of x")
+    tokens, topk = indices.shape
     if not 1 <= num_experts <= _lib.MAX_GROUPS:
         raise ValueError(f"the number of experts must be in [1, {_lib.MAX_GROUPS}]")
     if not 1 <= align <= 1 << 20:
         raise ValueError("align must be in [1, 2^20]")
-    if not 1 <= indices.shape[1] <= ROUTING_MAX_TOPK:
+    if not 1 <= topk <= ROUTING_MAX_TOPK:
         raise ValueError(f"topk must be in [1, {ROUTING_MAX_TOPK}]")
-    if indices.numel() > 0x3FFFFFFF:
+    entries = tokens * topk
+    if entries > 0x3FFFFFFF:
         raise ValueError("at most 2^30 - 1 entries")
+    dev = x.device
     if probs is not None:
         _float_type(probs, "probs")
         if probs.shape != indices.shape:
             raise ValueError("probs must have the shape of indices")
-        _same_device(indices.device, probs=probs)
-    entries = indices.numel()
-    rows = padded_rows_bound(entries, num_experts, align)
+    if indices.device != dev or (probs is not None and probs.device != dev):
+        _same_device(dev, indices=indices, probs=probs)
+    rows, hidden = padded_rows_bound(entries, num_experts, align), x.shape[1]
     if rows > 0x7FFFFFFF:
         raise ValueError("the buffer of rows must have fewer than 2^31 rows")
-    dev = indices.device
-    with _on(dev), _hooked("permute_plan", entries=entries, rows=rows):
-        row_of = torch.empty_like(indices)
+    with _on(dev), _hooked("permute_tokens", tokens=tokens, rows=rows, hidden=hidden):
+        out = torch.empty((rows, hidden), dtype=x.dtype, device=dev)
+        row_of = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
         entry_of = torch.empty(rows, dtype=torch.int32, device=dev)
         lens = torch.empty(num_experts, dtype=torch.int64, device=dev)
         row_probs = None if probs is None else torch.empty(rows, dtype=probs.dtype, device=dev)
         ws, nbytes = _workspace(dev, "mxl_permute_plan_workspace_bytes", entries, num_experts)
-        rc = _lib.load().mxl_permute_plan(_ptr(indices), entries, num_experts, align, rows, _ptr(row_of), _ptr(entry_of), lens.data_ptr(), _ptr(probs),
-                                          0 if probs is None else probs.element_size(), _ptr(row_probs), _ptr(ws), nbytes, _stream())
-    _lib.check(rc, "mxl_permute_plan")
-    return row_of, entry_of, lens, row_probs
+        rc = _lib.load().mxl_permute_tokens(_ptr(x), tokens, hidden * x.element_size(), _ptr(indices), topk, num_experts, align, rows, _ptr(row_of),
+                                            _ptr(entry_of), lens.data_ptr(), _ptr(probs), 0 if probs is None else probs.element_size(), _ptr(row_probs),
+                                            _ptr(out), _ptr(ws), nbytes, _stream())
+    if rc:
+        _lib.check(rc, "mxl_permute_tokens")
+    return out, row_of, entry_of, lens, row_probs
 
 
 def _row_args(x, row_of, entry_of):

@@ -1247,8 +1247,7 @@ class TokenPermutation(NamedTuple):
 class _PermuteTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, indices, num_experts, probs, align, need_grad=True):
-        row_of, entry_of, group_lens, row_probs = K.permute_plan_impl(indices, num_experts, align, probs)
-        rows = K.permute_rows_impl(x, row_of, entry_of)
+        rows, row_of, entry_of, group_lens, row_probs = K.permute_tokens_impl(x, indices, num_experts, align, probs)
         if need_grad:
             ctx.save_for_backward(row_of, entry_of)
             ctx.dtype = x.dtype

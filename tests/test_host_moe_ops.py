@@ -115,6 +115,12 @@ def test_c_entries_check_before_they_touch_the_device():
     for bad in (dict(i=None), dict(n=-1), dict(e=0), dict(e=1025), dict(a=0), dict(r=4999), dict(ro=None), dict(eo=None), dict(gl=None), dict(pr=p, pb=3, rp=p), dict(pb=4, rp=p),
                 dict(w=None), dict(wb=pw - 1), dict(a=32, r=5000)):
         assert plan(**bad) == -1, bad
+    both = lambda **k: lib.mxl_permute_tokens(*[{**dict(x=p, t=2500, rb=16, i=p, k=2, e=4, a=1, r=5000, ro=p, eo=p, gl=p, pr=None, pb=0, rp=None, o=p, w=p, wb=pw, st=None), **k}[n]  # noqa: E731
+                                                for n in ("x", "t", "rb", "i", "k", "e", "a", "r", "ro", "eo", "gl", "pr", "pb", "rp", "o", "w", "wb", "st")])
+    assert both() == -3
+    for bad in (dict(x=None), dict(t=-1), dict(rb=0), dict(rb=(1 << 24) + 1), dict(i=None), dict(k=0), dict(k=33), dict(e=0), dict(a=0), dict(r=4999), dict(ro=None), dict(eo=None), dict(gl=None),
+                dict(pr=p, pb=3, rp=p), dict(o=None), dict(w=None), dict(wb=pw - 1)):
+        assert both(**bad) == -1, bad
     assert lib.mxl_permute_rows(p, 4, 16, p, 2, p, 8, p, None) == -3
     assert lib.mxl_permute_rows(p, 4, 0, p, 2, p, 8, p, None) == -1 and lib.mxl_permute_rows(p, 4, 16, p, 33, p, 8, p, None) == -1
     assert lib.mxl_permute_rows(p, 4, 16, p, 2, None, 8, p, None) == -1 and lib.mxl_permute_rows(None, 4, 16, p, 2, p, 8, p, None) == -1
