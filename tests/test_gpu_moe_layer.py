@@ -194,3 +194,23 @@ def test_expert_mlp_of_the_megatron_side(gpu):
         pt.PrimusTurboLowPrecisionGlobalStateManager.reset()
         runtime.set_args()
         runtime.set_num_microbatches(1)
+
+
+def test_a_second_derivative_is_refused(gpu):
+    """The gradients are kernels' outputs with no graph behind them: what depends on them through a second backward raises."""
+    from primus_amd.pytorch import ops
+
+    logits = torch.randn(40, 8, device=gpu, requires_grad=True)
+    x = torch.randn(40, 64, device=gpu).bfloat16().requires_grad_()
+    w = torch.randn(96, 64, device=gpu).bfloat16().requires_grad_()
+    probs, idx, _ = ops.topk_routing(logits, 2)
+    rows, _, _, order = ops.permute_tokens(x, idx, 8)
+    outputs = [(probs, logits), (rows, x), (ops.unpermute_tokens(rows.detach().requires_grad_(), order, probs), logits),
+               (ops.gemm_bias_act(x, w, activation="gelu"), x)]
+    for y, leaf in outputs:
+        dy = torch.ones_like(y).requires_grad_()
+        (plain,) = torch.autograd.grad(y, leaf, dy.detach(), retain_graph=True)
+        (g,) = torch.autograd.grad(y, leaf, dy, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
