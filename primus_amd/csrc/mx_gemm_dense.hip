@@ -445,9 +445,15 @@ struct DzArgs {
     const uint16_t* dy;
     const uint16_t* z;
     uint16_t* dz;
-    float* partial;         // null: no sums wanted
+    float* partial;         // [runs, n]; null: no sums wanted, or one run, which writes dbias itself
     int64_t m, n, run;      // rows per workgroup
+    void* dbias;
+    int f32;
 };
+__device__ __forceinline__ void put_dbias(void* dbias, int f32, int64_t col, float s) {
+    if (f32) ((float*)dbias)[col] = s;
+    else ((__bf16*)dbias)[col] = (__bf16)s;
+}
 template <int ACT>
 __global__ __launch_bounds__(256) void dense_dz_kernel(DzArgs p) {
     __shared__ float sums[8][32][9];
@@ -478,7 +484,7 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DzArgs p) {
             for (int e = 0; e < 8; ++e) acc[e] += x[e];
         }
     }
-    if (!p.partial) return;
+    if (!p.partial && !p.dbias) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[r8][lane][e] = acc[e];
     __syncthreads();
@@ -486,7 +492,10 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DzArgs p) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += sums[i][c >> 3][c & 7];
-    if ((int64_t)blockIdx.x * 256 + c < p.n) p.partial[(int64_t)blockIdx.y * p.n + (int64_t)blockIdx.x * 256 + c] = s;
+    const int64_t at = (int64_t)blockIdx.x * 256 + c;
+    if (at >= p.n) return;
+    if (p.partial) p.partial[(int64_t)blockIdx.y * p.n + at] = s;
+    else put_dbias(p.dbias, p.f32, at, s);
 }
 
 // dbias[n] = sum of the runs: 32 columns by 32 groups of runs, four loads on their way
@@ -508,13 +517,14 @@ __global__ __launch_bounds__(1024) void dense_dbias_kernel(const float* partial,
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) s += part[i][lane];
-        if (f32) ((float*)dbias)[col] = s;
-        else ((__bf16*)dbias)[col] = (__bf16)s;
+        put_dbias(dbias, f32, col, s);
     }
 }
 
-// rows per workgroup of dense_dz_kernel: about 2048 workgroups, a multiple of 8 rows
+// rows per workgroup of dense_dz_kernel: about 2048 workgroups, a multiple of 8 rows.  Up to 64 rows are one run, whose workgroups write the
+// bias gradient themselves: eight rounds of loads instead of a second launch.
 static int64_t dz_run(int64_t m, int64_t n) {
+    if (m <= 64) return 64;
     const int64_t cols = (n + 255) / 256;
     int64_t runs = 2048 / cols;
     if (runs < 1) runs = 1;
@@ -704,8 +714,8 @@ extern "C" int mxl_linear_bf16_wgrad(const void* dz_bf16, const void* a_bf16, in
 
 extern "C" int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n) {
     if (m < 0 || n <= 0) return -1;
-    const int64_t run = dz_run(m, n);
-    return (m + run - 1) / run * n * 4;
+    const int64_t run = dz_run(m, n), runs = (m + run - 1) / run;
+    return runs > 1 ? runs * n * 4 : 0;
 }
 
 extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int act, int64_t m, int64_t n, void* dz_bf16, void* dbias, int dbias_dtype,
@@ -713,12 +723,13 @@ extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int a
     if (!dense_sizes_ok(m, n, 32) || act < MXL_ACT_SILU || act > MXL_ACT_NONE || (dbias_dtype != MXL_DT_F32 && dbias_dtype != MXL_DT_BF16)) return MXL_EINVAL;
     if (m > 0 && (!dy_bf16 || (act != MXL_ACT_NONE && (!z_bf16 || !dz_bf16)))) return MXL_EINVAL;
     if (!aligned16(dy_bf16) || !aligned16(z_bf16) || !aligned16(dz_bf16) || !aligned16(workspace)) return MXL_EINVAL;
-    if (dbias && (workspace_bytes < mxl_linear_bf16_dz_workspace_bytes(m, n) || (m > 0 && !workspace))) return MXL_EINVAL;
+    const int64_t need = dbias ? mxl_linear_bf16_dz_workspace_bytes(m, n) : 0;
+    if (need > 0 && (!workspace || workspace_bytes < need)) return MXL_EINVAL;
     if (!dbias && (act == MXL_ACT_NONE || m == 0)) return MXL_OK;
     if (!device_is_gfx950()) return MXL_ENODEV;
     hipStream_t st = (hipStream_t)stream;
     const int64_t run = dz_run(m, n), runs = (m + run - 1) / run;
-    DzArgs d{(const uint16_t*)dy_bf16, (const uint16_t*)z_bf16, (uint16_t*)dz_bf16, dbias ? (float*)workspace : nullptr, m, n, run};
+    DzArgs d{(const uint16_t*)dy_bf16, (const uint16_t*)z_bf16, (uint16_t*)dz_bf16, need > 0 ? (float*)workspace : nullptr, m, n, run, dbias, dbias_dtype == MXL_DT_F32};
     const dim3 grid((unsigned)((n + 255) / 256), (unsigned)runs);
     if (m > 0) {
         if (act == MXL_ACT_SILU) hipLaunchKernelGGL(dense_dz_kernel<kActSilu>, grid, dim3(256), 0, st, d);
@@ -726,7 +737,7 @@ extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int a
         else if (act == MXL_ACT_RELU) hipLaunchKernelGGL(dense_dz_kernel<kActRelu>, grid, dim3(256), 0, st, d);
         else hipLaunchKernelGGL(dense_dz_kernel<kActNone>, grid, dim3(256), 0, st, d);
     }
-    if (dbias) hipLaunchKernelGGL(dense_dbias_kernel, dim3((unsigned)(n / 32)), dim3(1024), 0, st, (const float*)workspace, (int)runs, n, dbias, dbias_dtype == MXL_DT_F32);
+    if (dbias && runs != 1) hipLaunchKernelGGL(dense_dbias_kernel, dim3((unsigned)(n / 32)), dim3(1024), 0, st, (const float*)workspace, (int)runs, n, dbias, dbias_dtype == MXL_DT_F32);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
 

@@ -143,9 +143,9 @@ def test_c_entries_check_before_they_touch_the_device():
     dgrad = lambda a, b, m, n, k, w=None, wb=0: lib.mxl_linear_bf16_dgrad(a, b, m, n, k, p, w, wb, None)  # noqa: E731
     assert dgrad(p, p, 4, 32, 32) == -3 and dgrad(p, p, 4, 32, 33) == -1 and dgrad(None, p, 4, 32, 32) == -1 and dgrad(p, p, 0, 32, 32) == 0
     assert dgrad(p, p, 128, 4096, 128) == -1 and dgrad(p, p, 128, 4096, 128, p, need) == -3
-    ws = lib.mxl_linear_bf16_dz_workspace_bytes(4, 32)
-    dz = lambda **k: lib.mxl_linear_bf16_dz(*[{**dict(dy=p, z=p, act=1, m=4, n=32, dz=p, db=p, dbd=0, w=p, wb=ws, st=None), **k}[n] for n in ("dy", "z", "act", "m", "n", "dz", "db", "dbd", "w", "wb", "st")])  # noqa: E731
-    assert ws == 128 and dz() == -3 and dz(act=3, db=None) == 0
+    ws = lib.mxl_linear_bf16_dz_workspace_bytes(80, 32)
+    dz = lambda **k: lib.mxl_linear_bf16_dz(*[{**dict(dy=p, z=p, act=1, m=80, n=32, dz=p, db=p, dbd=0, w=p, wb=ws, st=None), **k}[n] for n in ("dy", "z", "act", "m", "n", "dz", "db", "dbd", "w", "wb", "st")])  # noqa: E731
+    assert ws == 10 * 32 * 4 and lib.mxl_linear_bf16_dz_workspace_bytes(64, 32) == 0 and dz(m=64, w=None, wb=0) == -3 and dz() == -3 and dz(act=3, db=None) == 0
     for bad in (dict(dy=None), dict(z=None), dict(dz=None), dict(act=9), dict(n=31), dict(w=None), dict(wb=ws - 1), dict(dbd=2), dict(dy=odd)):
         assert dz(**bad) == -1, bad
     need = lib.mxl_linear_bf16_bwd_workspace_bytes(100, 64, 32, 1, 1, 1, 0, 1)
