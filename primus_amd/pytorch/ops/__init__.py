@@ -1005,7 +1005,7 @@ class _GemmBiasAct(torch.autograd.Function):
         dy = _aligned(dy.contiguous())
         da = db = dbias = None
         if need_a or need_b or need_bias:
-            fused = need_b and ctx.accum is not None and _fusable(ctx.accum[0])
+            fused = need_b and ctx.accum is not None and _fusable(ctx.accum[0]) and ctx.accum[0].data_ptr() % 16 == 0
             da, db, dbias = K.linear_bf16_bwd_impl(dy, a, b, z, ctx.activation, need_a, need_b, ctx.bias_dtype if need_bias else None,
                                                    ctx.accum[0] if fused else None)
             if need_b and ctx.accum is not None:

@@ -197,6 +197,12 @@ def test_weight_gradient_into_main_grad(gpu):
     w.grad_added_to_main_grad = False
     ops.gemm_bias_act(a, w, bias=bias, activation="gelu", fuse_bgrad_accum_pattern="megatron").backward(dy)
     assert w.grad_added_to_main_grad
+    # a buffer that starts between two 16-byte boundaries is added to from outside the kernel
+    other = torch.nn.Parameter(b)
+    other.main_grad = torch.ones(96 * 64 + 1, device=gpu)[1:].view(96, 64)
+    other.grad_added_to_main_grad = False
+    ops.gemm_bias_act(a, other, bias=bias, activation="gelu", fuse_bgrad_accum_pattern="megatron").backward(dy)
+    assert other.grad_added_to_main_grad and torch.equal(other.main_grad, 1.0 + plain.float())
     # the product before its rounding, plus one
     assert bool(((w.main_grad - 1.0 - plain.float()).abs() <= 2.0 ** -8 * plain.float().abs() + 2.0 ** -23 * (2.0 + plain.float().abs())).all())
 

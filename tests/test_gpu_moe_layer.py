@@ -214,3 +214,29 @@ def test_a_second_derivative_is_refused(gpu):
         assert torch.equal(g, plain)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.sum().backward()
+
+
+def test_saved_tensors_through_host_memory_and_with_other_strides(gpu):
+    """What autograd kept may come back from hooks: the same values give the same gradients, other strides are refused."""
+    from primus_amd.pytorch import ops
+
+    gen = torch.Generator().manual_seed(11)
+    logits, x, w = torch.randn(50, 8, generator=gen).to(gpu), torch.randn(50, 64, generator=gen).bfloat16().to(gpu), torch.randn(96, 64, generator=gen).bfloat16().to(gpu)
+    with torch.no_grad():
+        _, idx, _ = ops.topk_routing(logits, 2)
+        probs = torch.rand(50, 2, generator=gen).to(gpu)
+        rows, _, _, order = ops.permute_tokens(x, idx, 8, align=32)
+    leaves = [t.clone().requires_grad_() for t in (logits, x, rows, probs, w)]
+    runs = [(lambda: ops.topk_routing(leaves[0], 2)[0], leaves[:1]), (lambda: ops.permute_tokens(leaves[1], idx, 8)[0], leaves[1:2]),
+            (lambda: ops.unpermute_tokens(leaves[2], order, leaves[3]), leaves[2:4]), (lambda: ops.gemm_bias_act(leaves[1], leaves[4], activation="silu"), [leaves[1], leaves[4]])]
+    for run, inputs in runs:
+        y = run()
+        dy = torch.randn(y.shape, generator=gen).to(gpu).to(y.dtype)
+        want = torch.autograd.grad(y, inputs, dy)
+        with torch.autograd.graph.save_on_cpu():
+            y = run()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, inputs, dy), want))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.t().contiguous(), lambda t: t.t()):
+            y = run()
+        with pytest.raises(ValueError):
+            torch.autograd.grad(y, inputs, dy)
