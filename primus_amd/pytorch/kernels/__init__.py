@@ -1297,8 +1297,8 @@ def topk_routing_impl(logits, topk: int, score_function: str = "softmax", expert
         _same_device(dev, token_mask=token_mask)
     lib = _lib.load()
     with _on(dev), _hooked("topk_routing", tokens=tokens, experts=experts, topk=topk):
-        probs = torch.empty((tokens, topk), dtype=torch.float32, device=dev)
-        indices = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
+        probs = torch.empty(tokens, topk, dtype=torch.float32, device=dev)
+        indices = torch.empty(tokens, topk, dtype=torch.int64, device=dev)
         counts = torch.empty(experts, dtype=torch.int64, device=dev)
         ws, nbytes = _workspace(dev, "mxl_topk_routing_workspace_bytes", tokens, experts)
         rc = lib.mxl_topk_routing(logits.data_ptr() if tokens else None, dtype, tokens, experts, topk, score, _ptr(expert_bias), num_groups, group_topk,
@@ -1361,8 +1361,8 @@ def permute_tokens_impl(x, indices, num_experts: int, align: int = 1, probs: Opt
     if rows > 0x7FFFFFFF:
         raise ValueError("the buffer of rows must have fewer than 2^31 rows")
     with _on(dev), _hooked("permute_tokens", tokens=tokens, rows=rows, hidden=hidden):
-        out = torch.empty((rows, hidden), dtype=x.dtype, device=dev)
-        row_of = torch.empty((tokens, topk), dtype=torch.int64, device=dev)
+        out = torch.empty(rows, hidden, dtype=x.dtype, device=dev)
+        row_of = torch.empty(tokens, topk, dtype=torch.int64, device=dev)
         entry_of = torch.empty(rows, dtype=torch.int32, device=dev)
         lens = torch.empty(num_experts, dtype=torch.int64, device=dev)
         row_probs = None if probs is None else torch.empty(rows, dtype=probs.dtype, device=dev)
@@ -1396,7 +1396,7 @@ def permute_rows_impl(x, row_of, entry_of) -> torch.Tensor:
         raise ValueError("one row of x per token")
     rows, hidden = entry_of.shape[0], x.shape[1]
     with _on(x.device), _hooked("permute_rows", tokens=x.shape[0], rows=rows, hidden=hidden):
-        out = torch.empty((rows, hidden), dtype=x.dtype, device=x.device)
+        out = torch.empty(rows, hidden, dtype=x.dtype, device=x.device)
         rc = _lib.load().mxl_permute_rows(_ptr(x), x.shape[0], hidden * x.element_size(), _ptr(row_of), row_of.shape[1], _ptr(entry_of),
                                           rows, _ptr(out), _stream())
     _lib.check(rc, "mxl_permute_rows")
@@ -1421,8 +1421,8 @@ def combine_rows_impl(rows, row_of, entry_of, probs: Optional[torch.Tensor] = No
     pd = _lib.DT_F32 if p is None else _float_type(p, "probs")
     tokens, topk = row_of.shape
     with _on(rows.device), _hooked("combine_rows", tokens=tokens, rows=rows.shape[0], hidden=rows.shape[1]):
-        y = torch.empty((tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-        out = None if row_probs is None else torch.empty((tokens, topk), dtype=row_probs.dtype, device=rows.device)
+        y = torch.empty(tokens, rows.shape[1], dtype=rows.dtype, device=rows.device)
+        out = None if row_probs is None else torch.empty(tokens, topk, dtype=row_probs.dtype, device=rows.device)
         # (no rows: _ptr is None for an empty tensor, so the probabilities go the way of zeros)
         empty = row_probs is not None and row_probs.numel() == 0
         if empty:
@@ -1445,7 +1445,7 @@ def combine_rows_bwd_impl(dy, rows, row_of, entry_of, probs, need_rows: bool = T
         raise ValueError("probs must be [tokens, topk]")
     with _on(rows.device), _hooked("combine_rows_bwd", tokens=tokens, rows=rows.shape[0], hidden=rows.shape[1]):
         drows = torch.empty_like(rows) if need_rows else None
-        dprobs = torch.empty((tokens, topk), dtype=torch.float32, device=rows.device) if need_probs else None
+        dprobs = torch.empty(tokens, topk, dtype=torch.float32, device=rows.device) if need_probs else None
         rc = _lib.load().mxl_combine_rows_bwd(_ptr(dy), _ptr(rows), rows.shape[0], rows.shape[1], _DT[rows.dtype], _ptr(row_of), _ptr(entry_of),
                                               tokens, topk, _ptr(probs), _float_type(probs, "probs"), _ptr(drows), _ptr(dprobs), _stream())
     _lib.check(rc, "mxl_combine_rows_bwd")
@@ -1505,7 +1505,7 @@ def linear_bf16_impl(a, b, bias=None, activation: Optional[str] = None, residual
         _same_device(dev, residual=residual)
     lib = _lib.load()
     with _on(dev), _hooked("linear_bf16", m=m, n=n, k=k):
-        y = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+        y = torch.empty(m, n, dtype=torch.bfloat16, device=dev)
         z = torch.empty_like(y) if want_z else None
         ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_workspace_bytes", m, n, k)
         rc = lib.mxl_linear_bf16(_ptr(a), b.data_ptr(), bias_ptr, bias_dtype, act, _ptr(residual), m, n, k, _ptr(y), _ptr(z), _ptr(ws), ws_bytes, _stream())
@@ -1540,8 +1540,8 @@ def linear_bf16_bwd_impl(dy, a, b, z, activation: Optional[str], need_a: bool = 
         raise ValueError("accum_into must be a contiguous float32 buffer of the weight's size")
     lib = _lib.load()
     with _on(dev), _hooked("linear_bf16_bwd", m=m, n=n, k=k):
-        da = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_a else None
-        db = None if not need_b else accum_into if accum_into is not None else torch.empty((n, k), dtype=torch.bfloat16, device=dev)
+        da = torch.empty(m, k, dtype=torch.bfloat16, device=dev) if need_a else None
+        db = None if not need_b else accum_into if accum_into is not None else torch.empty(n, k, dtype=torch.bfloat16, device=dev)
         dbias = torch.empty(n, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
         ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_bwd_workspace_bytes", m, n, k, act, int(need_a), int(need_b),
                                   _lib.BF_ACCUM_F32 if accum_into is not None else 0, int(dbias is not None))
@@ -1584,7 +1584,7 @@ def linear_bf16_dgrad_impl(dz, b) -> torch.Tensor:
     _require_cuda(dz, b)
     _same_device(dz.device, b=b)
     with _on(dz.device), _hooked("linear_bf16_dgrad", m=m, n=n, k=k):
-        da = torch.empty((m, k), dtype=torch.bfloat16, device=dz.device)
+        da = torch.empty(m, k, dtype=torch.bfloat16, device=dz.device)
         ws, ws_bytes = _workspace(dz.device, "mxl_linear_bf16_workspace_bytes", m, k, n)
         rc = _lib.load().mxl_linear_bf16_dgrad(_ptr(dz), _ptr(b), m, n, k, _ptr(da), _ptr(ws), ws_bytes, _stream())
     _lib.check(rc, "mxl_linear_bf16_dgrad")
@@ -1613,7 +1613,7 @@ def linear_bf16_wgrad_impl(dz, a, accum_into: Optional[torch.Tensor] = None) -> 
             linear_bf16_wgrad_impl(dz[lo:lo + rows], a[lo:lo + rows], accum_into=total)
         return total if accum_into is not None else total.to(torch.bfloat16)
     with _on(dev), _hooked("linear_bf16_wgrad", m=m, n=n, k=k):
-        db = accum_into if accum_into is not None else torch.empty((n, k), dtype=torch.bfloat16, device=dev)
+        db = accum_into if accum_into is not None else torch.empty(n, k, dtype=torch.bfloat16, device=dev)
         flags = _lib.BF_ACCUM_F32 if accum_into is not None else 0
         ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_wgrad_workspace_bytes", m, n, k, flags)
         rc = _lib.load().mxl_linear_bf16_wgrad(_ptr(dz), _ptr(a), m, n, k, db.data_ptr(), flags, _ptr(ws), ws_bytes, _stream())
