@@ -423,9 +423,12 @@ __global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_kernel(RouteBwdArgs p
     }
 }
 
-// workgroups of a forward launch: rows for every wave slot of the chip at most; a few tokens are one, which writes the counts itself
-static int64_t route_blocks(int64_t tokens, int rows_per_block) {
-    if (tokens <= 16) return 1;
+// workgroups of a forward launch: rows for every wave slot of the chip at most; a few tokens are one, which writes the counts itself.  Where
+// a wave takes several rows that is up to two rounds of rows, on the GPU / host, against two launches: 64 tokens of 128 experts 6.8 / 12.2
+// and 6.8 / 14.7 us, 256 of 8 3.5 / 12.3 and 4.6 / 14.8; a third and fourth round cost more than the launch (128 of 128 11.7 and 6.9), and so does a
+// second one of rows that are a wave's (32 of 256 9.2 and 8.0).
+static int64_t route_blocks(int64_t tokens, int rows_per_block, int rows_per_wave = 1) {
+    if (tokens <= 16 || (rows_per_wave > 1 && tokens <= 2 * rows_per_block)) return 1;
     int64_t b = (tokens + rows_per_block - 1) / rows_per_block;
     return b < 768 ? b : 768;
 }
@@ -433,7 +436,7 @@ static int64_t route_blocks(int64_t tokens, int rows_per_block) {
 template <int LPR, int V, bool SCORED>
 static int launch_route(const RouteArgs& a, hipStream_t st) {
     constexpr int WAVES = route_waves<V, SCORED>();
-    const int64_t blocks = route_blocks(a.tokens, WAVES * (64 / LPR));
+    const int64_t blocks = route_blocks(a.tokens, WAVES * (64 / LPR), 64 / LPR);
     hipLaunchKernelGGL((route_fwd_kernel<LPR, V, SCORED>), dim3((unsigned)blocks), dim3(WAVES * 64), 0, st, a);
     if (blocks > 1)
         hipLaunchKernelGGL(route_counts_kernel, dim3((unsigned)((a.experts + 15) / 16)), dim3(1024), 0, st, a.partial, (int)blocks, a.experts, a.counts);

@@ -227,7 +227,7 @@ def test_rows_that_are_not_finite_keep_valid_indices(gpu, score, bias, groups):
     assert bool((idx[~mask.to(gpu)] == -1).all()) and int(counts.sum()) == 59 * 6
 
 
-@pytest.mark.parametrize("t", [0, 1, 4097, 50000])
+@pytest.mark.parametrize("t", [0, 1, 128, 256, 257, 4097, 50000])
 def test_counts_over_one_and_many_workgroups(gpu, t):
     from primus_amd.pytorch import ops
 
