@@ -5,8 +5,8 @@
 //   y = act(z) + residual,  z = a . b^T + bias     a [m, k], b [n, k];  fp32 from the products to y, one rounding
 //   backward: dz = dy act'(z),  da = dz . b,  db = dz^T . a,  dbias = column sums of dz
 //
-// Products with enough of them run on the grouped kernels' 256 x 256 tiles (mx_gemm_bf16.hip) with one group.  This
-// file holds the tiles of 256 x 128 and 64 x 64 for fewer rows, the kernel for a few rows, which is bound by reading b, and
+// A product with enough tiles of 256 x 256 runs on the grouped kernels' (mx_gemm_bf16.hip) with one group.  This
+// file holds the tiles of 256 x 128 and 64 x 64 for the others, the kernel for a few rows, which is bound by reading b, and
 // the elementwise part of the backward.
 #include "mx_gemm_bf16.h"
 #include "mx_gemm_common.h"

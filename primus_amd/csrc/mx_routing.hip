@@ -15,8 +15,8 @@
 // left out, are nearer to each other than the rounding of fp32 scores allows to tell apart is chosen again from scores in
 // fp64 (one row in 2000 at 256 fp32 scores), so the indices are those of the definition and not of a rounding.
 //
-// us: 8 tokens of 128 experts, top 4, 2.7; 16384 of 8, top 2, 3.9 and 2.2 for adding up the counts, gradient 7.0; 5003 of 160, top 6, 9.6 + 3.3,
-// 7.4; 16384 of 256, sigmoid, bias, 4 of 8 groups, top 8, 28 + 4.0, 9.6 (the logits alone are 3.3 at the rate of a large copy).  The last one's forward
+// us: 8 tokens of 128 experts, top 4, 2.7; 16384 of 8, top 2, 3.9 and 2.2 for adding up the counts, gradient 3.5; 5003 of 160, top 6, 9.6 + 3.3,
+// 7.4; 16384 of 256, sigmoid, bias, 4 of 8 groups, top 8, 28 + 4.0, 6.9 (the logits alone are 3.3 at the rate of a large copy).  The last one's forward
 // without the fp64 rows is 22-26, with one round instead of nine 17.
 #include "mx_lanes.h"
 
@@ -367,8 +367,73 @@ struct RouteBwdArgs {
 
 // g = scale * dprobs, w = the chosen scores' shares.  Renormalised: dl = w (g - sum w g) at the chosen experts (softmax),
 // (g - sum w g) / (S + 1e-20) * s (1 - s) (sigmoid); as they are: softmax s_e ([e chosen] g_e - sum s g) at every expert,
-// sigmoid g s (1 - s).  A wave a row; the chosen experts' gradients meet the row through LDS, which is zero between rows.
+// sigmoid g s (1 - s).  The chosen experts' gradients meet their rows through LDS, which is zero between rows.
 constexpr int RB_WAVES = 8;
+// All but the plain softmax: the other experts' gradients are zero.  LPR lanes a row, so that 64 / LPR rows wait for their indices and
+// logits together; the rows leave as one run of memory, four elements a lane and request (VEC).  Bound by that one wait and, with many
+// experts, by the rows' bytes.  us with a wave a row, two rows, eight rows: 16384 tokens of 8 experts, top 2, 5.8 / 4.4 / 2.9, of 64, top 6, 6.2 / 4.8 / 3.8, of 256, top 8,
+// 8.7 / 6.1 / 6.5, of 1024 16.2 / 13.6 / 16.2; 8192 of 64 4.5 / 3.6 / 3.4; 1024 of 64 2.8 / 2.8 / 3.2, of 256 3.3 / 3.1 / 4.0.  So eight rows for many tokens of few
+// experts, else two.
+template <int LPR, bool VEC>
+__global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_chosen_kernel(RouteBwdArgs p) {
+    constexpr int RPW = 64 / LPR;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & (LPR - 1), sub = lane / LPR;
+    const int size = RPW * p.experts;
+    float* d = lds + w * ((size + 3) & ~3);
+    for (int e = lane * 4; e < size; e += 256) *(v4f*)(d + e) = v4f{0.f, 0.f, 0.f, 0.f};      // (a wave's part is a multiple of four long)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int64_t row0 = ((int64_t)blockIdx.x * RB_WAVES + w) * RPW; row0 < p.tokens; row0 += (int64_t)gridDim.x * RB_WAVES * RPW) {
+        const int64_t row = row0 + sub;
+        const int64_t at = row < p.tokens && lr < p.topk ? p.indices[row * p.topk + lr] : -1;
+        const bool chosen = at >= 0 && at < p.experts;
+        const float g = chosen ? p.dprobs[row * p.topk + lr] * p.scale : 0.f;
+        const float ml = chosen ? load_dt(p.logits, p.dtype, row * p.experts + at) : -INFINITY;
+        float mine;
+        if (p.sigmoid) {
+            const float s = chosen ? sigmoid_of(ml) : 0.f;
+            float ds = g;
+            if (p.renorm) {
+                const float sum = lanes_sum<LPR>(s) + 1e-20f;
+                ds = (g - lanes_sum<LPR>(g * (s / sum))) / sum;
+            }
+            mine = ds * s * (chosen ? sigmoid_of(-ml) : 0.f);      // 1 - s without cancellation
+        } else {
+            const float m = finite_top(lanes_max<LPR>(ml));
+            const float e = chosen ? expf(ml - m) : 0.f;
+            const float wgt = e / some(lanes_sum<LPR>(e));
+            mine = wgt * (g - lanes_sum<LPR>(wgt * g));
+        }
+        float* mine_at = d + sub * p.experts + (chosen ? (int)at : 0);
+        if (chosen) atomicAdd(mine_at, mine);      // the same expert twice in a row: its gradients add up
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int n = (int)((p.tokens - row0 < RPW ? p.tokens - row0 : RPW) * p.experts), whole = VEC ? n & ~3 : 0;
+        const int64_t base = row0 * p.experts;
+        if constexpr (VEC) {
+            for (int e = lane * 4; e < whole; e += 256) {
+                const v4f x = *(const v4f*)(d + e);
+                if (p.dtype == MXL_DT_F32) {
+                    *(v4f*)((float*)p.dlogits + base + e) = x;
+                } else {
+                    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+                    const h4 h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+                    const uint2 b = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+                    *(uint2*)((uint16_t*)p.dlogits + base + e) = p.dtype == MXL_DT_BF16 ? b : __builtin_bit_cast(uint2, h);
+                }
+            }
+        }
+        for (int e = whole + lane; e < n; e += 64) store_dt(p.dlogits, p.dtype, base + e, d[e]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (chosen) *mine_at = 0.f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The plain softmax: a wave a row, whose logits are read again
 __global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_kernel(RouteBwdArgs p) {
     __shared__ float rows[RB_WAVES][RT_MAX_EXPERTS];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -376,43 +441,23 @@ __global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_kernel(RouteBwdArgs p
     for (int e = lane; e < p.experts; e += 64) d[e] = 0.f;
     for (int64_t row = (int64_t)blockIdx.x * RB_WAVES + w; row < p.tokens; row += (int64_t)gridDim.x * RB_WAVES) {
         const int64_t base = row * p.experts;
-        int64_t at = lane < p.topk ? p.indices[row * p.topk + lane] : -1;
+        const int64_t at = lane < p.topk ? p.indices[row * p.topk + lane] : -1;
         const bool chosen = at >= 0 && at < p.experts;
         const float ml = chosen ? load_dt(p.logits, p.dtype, base + at) : -INFINITY;
         const float g = chosen ? p.dprobs[row * p.topk + lane] * p.scale : 0.f;
-        float mine, all = 0.f, top = 0.f, total = 1.f;
-        const bool dense = !p.sigmoid && !p.renorm;
-        if (p.sigmoid) {
-            const float s = chosen ? sigmoid_of(ml) : 0.f;
-            float ds = g;
-            if (p.renorm) {
-                const float sum = lanes_sum<64>(s) + 1e-20f;
-                ds = (g - lanes_sum<64>(g * (s / sum))) / sum;
-            }
-            mine = ds * s * (chosen ? sigmoid_of(-ml) : 0.f);      // 1 - s without cancellation
-        } else if (p.renorm) {
-            const float m = finite_top(lanes_max<64>(ml));
-            const float e = chosen ? expf(ml - m) : 0.f;
-            const float wgt = e / some(lanes_sum<64>(e));
-            mine = wgt * (g - lanes_sum<64>(wgt * g));
-        } else {
-            top = -INFINITY;
-            for (int e = lane; e < p.experts; e += 64) top = fmaxf(top, load_dt(p.logits, p.dtype, base + e));
-            top = finite_top(lanes_max<64>(top));
-            float sum = 0.f;
-            for (int e = lane; e < p.experts; e += 64) sum += expf(load_dt(p.logits, p.dtype, base + e) - top);
-            total = some(lanes_sum<64>(sum));
-            const float s = chosen ? expf(ml - top) / total : 0.f;
-            all = lanes_sum<64>(s * g);
-            mine = s * g;
-        }
+        float top = -INFINITY, sum = 0.f;
+        for (int e = lane; e < p.experts; e += 64) top = fmaxf(top, load_dt(p.logits, p.dtype, base + e));
+        top = finite_top(lanes_max<64>(top));
+        for (int e = lane; e < p.experts; e += 64) sum += expf(load_dt(p.logits, p.dtype, base + e) - top);
+        const float total = some(lanes_sum<64>(sum));
+        const float s = chosen ? expf(ml - top) / total : 0.f, all = lanes_sum<64>(s * g);
         const bool live = __any(chosen);
-        if (chosen) atomicAdd(&d[at], mine);      // the same expert twice in a row: its gradients add up
+        if (chosen) atomicAdd(&d[at], s * g);      // the same expert twice in a row: its gradients add up
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         for (int e = lane; e < p.experts; e += 64) {
             float x = d[e];
-            if (dense && live) x -= expf(load_dt(p.logits, p.dtype, base + e) - top) / total * all;
+            if (live) x -= expf(load_dt(p.logits, p.dtype, base + e) - top) / total * all;
             store_dt(p.dlogits, p.dtype, base + e, x);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -421,6 +466,18 @@ __global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_kernel(RouteBwdArgs p
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
+}
+
+template <int LPR> static void launch_route_bwd_chosen(const RouteBwdArgs& a, hipStream_t st) {
+    constexpr int RPW = 64 / LPR;
+    const int lds = RB_WAVES * ((RPW * a.experts + 3) & ~3) * 4;       // at most 64 KiB: two rows of 1024, or eight of 64, a wave
+    int64_t blocks = (a.tokens + RB_WAVES * RPW - 1) / (RB_WAVES * RPW);
+    if (blocks > 4096) blocks = 4096;
+    // a wave's rows start at a multiple of four elements
+    const bool vec = RPW * a.experts % 4 == 0 && ((uintptr_t)a.dlogits & (a.dtype == MXL_DT_F32 ? 15 : 7)) == 0;
+    const dim3 grid((unsigned)blocks), block(RB_WAVES * 64);
+    if (vec) hipLaunchKernelGGL((route_bwd_chosen_kernel<LPR, true>), grid, block, (unsigned)lds, st, a);
+    else hipLaunchKernelGGL((route_bwd_chosen_kernel<LPR, false>), grid, block, (unsigned)lds, st, a);
 }
 
 // workgroups of a forward launch: rows for every wave slot of the chip at most; a few tokens are one, which writes the counts itself.  Where
@@ -516,8 +573,13 @@ extern "C" int mxl_topk_routing_bwd(const float* dprobs, const void* logits, int
     if (!dprobs || !logits || !indices || !dlogits) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     RouteBwdArgs a{dprobs, logits, indices, dlogits, tokens, experts, topk, dtype, score == MXL_SCORE_SIGMOID, renormalize != 0, scale};
-    int64_t blocks = (tokens + RB_WAVES - 1) / RB_WAVES;
-    if (blocks > 1024) blocks = 1024;
-    hipLaunchKernelGGL(route_bwd_kernel, dim3((unsigned)blocks), dim3(RB_WAVES * 64), 0, (hipStream_t)stream, a);
+    if (score == MXL_SCORE_SIGMOID || renormalize) {
+        if (topk <= 8 && experts <= 64 && tokens >= 8192) launch_route_bwd_chosen<8>(a, (hipStream_t)stream);
+        else launch_route_bwd_chosen<32>(a, (hipStream_t)stream);
+    } else {
+        int64_t blocks = (tokens + RB_WAVES - 1) / RB_WAVES;
+        if (blocks > 1024) blocks = 1024;
+        hipLaunchKernelGGL(route_bwd_kernel, dim3((unsigned)blocks), dim3(RB_WAVES * 64), 0, (hipStream_t)stream, a);
+    }
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }

@@ -96,7 +96,7 @@ def _inputs(gpu, t, e, k, dtype, seed):
     return logits, bias, dprobs, mask
 
 
-SIZES = [(1, 1, 1), (1, 2, 1), (3, 7, 7), (65, 8, 2), (130, 16, 3), (33, 20, 12), (70, 32, 4), (9, 33, 32), (50, 64, 6), (21, 64, 17),
+SIZES = [(8200, 8, 2), (8193, 63, 7), (1, 1, 1), (1, 2, 1), (3, 7, 7), (65, 8, 2), (130, 16, 3), (33, 20, 12), (70, 32, 4), (9, 33, 32), (50, 64, 6), (21, 64, 17),
          (40, 100, 5), (77, 128, 4), (200, 160, 6), (37, 256, 8), (1, 257, 2), (20, 512, 10), (11, 1000, 32), (5, 1024, 1)]
 
 
