@@ -291,7 +291,7 @@ template <int DT, int N>
 __global__ __launch_bounds__(MV_THREADS) void combine_rows_bwd_kernel(MoveArgs p) {
     constexpr int SIZE = DT == MXL_DT_F32 ? 4 : 2;
     __shared__ float part[MV_WAVES][PM_MAX_TOPK];
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, threads = (int)blockDim.x, block_waves = threads >> 6;
     const int64_t vecs = p.hidden / N;
     for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
         const uint8_t* dy = p.dy + t * p.hidden * SIZE;
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(MV_THREADS) void combine_rows_bwd_kernel(MoveArgs p
                 pr[k] = k0 + k < p.topk ? load_dt(p.probs, p.probs_dtype, t * p.topk + k0 + k) : 0.f;
                 dot[k] = 0.f;
             }
-            for (int64_t v = threadIdx.x; v < vecs; v += MV_THREADS) {
+            for (int64_t v = threadIdx.x; v < vecs; v += threads) {
                 float d[N], a[CB_ROWS][N];
                 load_n<DT, N>(dy + v * N * SIZE, d);
                 if (p.dprobs) {
@@ -337,19 +337,18 @@ __global__ __launch_bounds__(MV_THREADS) void combine_rows_bwd_kernel(MoveArgs p
         __syncthreads();
         if (p.dprobs && (int)threadIdx.x < p.topk) {
             float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < MV_WAVES; ++i) s += part[i][threadIdx.x];
+            for (int i = 0; i < block_waves; ++i) s += part[i][threadIdx.x];
             p.dprobs[t * p.topk + threadIdx.x] = s;
         }
         __syncthreads();
     }
     if (!p.out) return;
-    const int64_t wave = (int64_t)blockIdx.x * MV_WAVES + w;
+    const int64_t wave = (int64_t)blockIdx.x * block_waves + w;
     if constexpr (N == 1) {
-        if constexpr (SIZE == 2) zero_rows<uint16_t>(p, wave, (int64_t)gridDim.x * MV_WAVES);
-        else zero_rows<uint32_t>(p, wave, (int64_t)gridDim.x * MV_WAVES);
+        if constexpr (SIZE == 2) zero_rows<uint16_t>(p, wave, (int64_t)gridDim.x * block_waves);
+        else zero_rows<uint32_t>(p, wave, (int64_t)gridDim.x * block_waves);
     } else {
-        zero_rows<m32x4>(p, wave, (int64_t)gridDim.x * MV_WAVES);
+        zero_rows<m32x4>(p, wave, (int64_t)gridDim.x * block_waves);
     }
 }
 
@@ -443,17 +442,17 @@ extern "C" int mxl_permute_tokens(const void* x, int64_t tokens, int64_t row_byt
 }
 
 // launches `kernel<DT, N>` for a type and whether rows are made of aligned 16-byte pieces
-#define MXL_BY_TYPE(kernel, wide, grid, st, a)                                                                                \
+#define MXL_BY_TYPE(kernel, wide, grid, threads, st, a)                                                                       \
     do {                                                                                                                      \
         if (a.dtype == MXL_DT_F32) {                                                                                          \
-            if (wide) hipLaunchKernelGGL((kernel<MXL_DT_F32, 4>), grid, dim3(MV_THREADS), 0, st, a);                          \
-            else hipLaunchKernelGGL((kernel<MXL_DT_F32, 1>), grid, dim3(MV_THREADS), 0, st, a);                               \
+            if (wide) hipLaunchKernelGGL((kernel<MXL_DT_F32, 4>), grid, dim3(threads), 0, st, a);                             \
+            else hipLaunchKernelGGL((kernel<MXL_DT_F32, 1>), grid, dim3(threads), 0, st, a);                                  \
         } else if (a.dtype == MXL_DT_BF16) {                                                                                  \
-            if (wide) hipLaunchKernelGGL((kernel<MXL_DT_BF16, 8>), grid, dim3(MV_THREADS), 0, st, a);                         \
-            else hipLaunchKernelGGL((kernel<MXL_DT_BF16, 1>), grid, dim3(MV_THREADS), 0, st, a);                              \
+            if (wide) hipLaunchKernelGGL((kernel<MXL_DT_BF16, 8>), grid, dim3(threads), 0, st, a);                            \
+            else hipLaunchKernelGGL((kernel<MXL_DT_BF16, 1>), grid, dim3(threads), 0, st, a);                                 \
         } else {                                                                                                              \
-            if (wide) hipLaunchKernelGGL((kernel<MXL_DT_F16, 8>), grid, dim3(MV_THREADS), 0, st, a);                          \
-            else hipLaunchKernelGGL((kernel<MXL_DT_F16, 1>), grid, dim3(MV_THREADS), 0, st, a);                               \
+            if (wide) hipLaunchKernelGGL((kernel<MXL_DT_F16, 8>), grid, dim3(threads), 0, st, a);                             \
+            else hipLaunchKernelGGL((kernel<MXL_DT_F16, 1>), grid, dim3(threads), 0, st, a);                                  \
         }                                                                                                                     \
     } while (0)
 
@@ -474,7 +473,7 @@ extern "C" int mxl_combine_rows(const void* rows_in, int64_t rows, int hidden, i
     const bool wide = (((uintptr_t)rows_in | (uintptr_t)y | (uintptr_t)((int64_t)hidden * size)) & 15) == 0;
     const int64_t pieces = (hidden / (wide ? 16 / size : 1) + 63) / 64;
     const dim3 grid((unsigned)move_blocks(tokens * pieces));
-    MXL_BY_TYPE(combine_rows_kernel, wide, grid, (hipStream_t)stream, a);
+    MXL_BY_TYPE(combine_rows_kernel, wide, grid, MV_THREADS, (hipStream_t)stream, a);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
 
@@ -493,6 +492,8 @@ extern "C" int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t
     int64_t blocks = tokens > (rows + 255) / 256 ? tokens : (rows + 255) / 256;
     if (blocks > 256 * 8) blocks = 256 * 8;
     const dim3 grid((unsigned)(blocks < 1 ? 1 : blocks));
-    MXL_BY_TYPE(combine_rows_bwd_kernel, wide, grid, (hipStream_t)stream, a);
+    // rows of up to 128 vectors: half the threads (20000 tokens of 512, two each, 77 -> 46 us; 16384 of 4096 136 with all, 138 with half)
+    const int threads = hidden / (wide ? 16 / size : 1) <= MV_THREADS / 2 ? MV_THREADS / 2 : MV_THREADS;
+    MXL_BY_TYPE(combine_rows_bwd_kernel, wide, grid, threads, (hipStream_t)stream, a);
     return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
 }
