@@ -594,8 +594,7 @@ static DensePlan dense_plan(int64_t m, int64_t n, int64_t k, bool a_by_columns =
 }
 
 template <bool A_T, bool B_T, int ACT>
-static int launch_dense(DenseArgs a, hipStream_t st) {
-    const DensePlan plan = dense_plan(a.m, a.n, a.k, A_T);
+static int launch_dense(DenseArgs a, const DensePlan& plan, hipStream_t st) {
     if (plan.splits == 1 && !a.sum) {
         if (plan.tm == 256) return launch_dense_tile<256, 128, 4, 3, A_T, B_T, ACT>(a, st);
         return launch_dense_tile<64, 64, 2, 3, A_T, B_T, ACT>(a, st);
@@ -611,17 +610,17 @@ static int launch_dense(DenseArgs a, hipStream_t st) {
 
 constexpr int64_t FEW_ROWS = 16;
 template <int ACT>
-static int launch_dense_forward(const DenseArgs& a, hipStream_t st) {
+static int launch_dense_forward(const DenseArgs& a, const DensePlan& plan, hipStream_t st) {
     if (a.m <= FEW_ROWS) {
         if (a.n / 32 >= 256) hipLaunchKernelGGL((dense_few_rows_kernel<2, ACT>), dim3((unsigned)(a.n / 32)), dim3(8 * 64), 0, st, a);
         else hipLaunchKernelGGL((dense_few_rows_kernel<1, ACT>), dim3((unsigned)(a.n / 16)), dim3(8 * 64), 0, st, a);
         return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
     }
-    if (dense_plan(a.m, a.n, a.k).tn == 256) {
+    if (plan.tn == 256) {
         const Bf16Args t{a.a, a.b, a.c, nullptr, 1, a.m, 0, a.n, a.k, a.epi};
         return launch_bf16_linear_tall(t, ACT, st);
     }
-    return launch_dense<false, false, ACT>(a, st);
+    return launch_dense<false, false, ACT>(a, plan, st);
 }
 
 // (offsets inside a tile's operand rows are 32-bit: 256 rows of k or n stay below 2^31 bytes)
@@ -630,9 +629,15 @@ static bool dense_sizes_ok(int64_t m, int64_t n, int64_t k) {
 }
 // the weight gradient contracts over the m rows, whose number is free; its operands end below 4 GiB
 static bool dense_wgrad_ok(int64_t m, int64_t n, int64_t k) { return dense_sizes_ok(m, n, k) && m * (n > k ? n : k) * 2 < ((int64_t)1 << 32); }
-// It runs on this file's tiles unless it has enough large ones, or no rows, or offsets that pass 32 bits in the 63 rows behind the last one
-static bool dense_wgrad_here(int64_t m, int64_t n, int64_t k) {
-    return m > 0 && (m + 64) * (n > k ? n : k) * 2 < ((int64_t)1 << 32) && dense_plan(n, k, m, true).tn != 256;
+// fp32 sums of a product's runs [m, n] (a product that is added to a float buffer goes through them with one run too)
+static int64_t runs_bytes(const DensePlan& plan, int64_t m, int64_t n, bool accum = false) {
+    return plan.splits > 1 || (accum && plan.tn != 256) ? plan.splits * m * n * 4 : 0;
+}
+// The weight gradient runs on this file's tiles unless it has enough large ones, or no rows, or offsets that pass 32 bits in the 63 rows
+// behind the last one
+static DensePlan wgrad_plan(int64_t m, int64_t n, int64_t k) {
+    if (m == 0 || (m + 64) * (n > k ? n : k) * 2 >= ((int64_t)1 << 32)) return {256, 256, 1, 0};
+    return dense_plan(n, k, m, true);
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -642,9 +647,7 @@ using namespace mxl;
 
 extern "C" int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t k) {
     if (!dense_sizes_ok(m, n, k)) return -1;
-    if (m == 0) return 0;
-    const int splits = dense_plan(m, n, k).splits;
-    return splits > 1 ? splits * m * n * 4 : 0;
+    return m == 0 ? 0 : runs_bytes(dense_plan(m, n, k), m, n);
 }
 
 extern "C" int mxl_linear_bf16_plan(int64_t m, int64_t n, int64_t k, int a_by_columns, int* tile_rows, int* tile_cols, int* splits) {
@@ -660,56 +663,62 @@ extern "C" int mxl_linear_bf16(const void* a_bf16, const void* b_bf16, const voi
     if (m == 0) return MXL_OK;
     if (!a_bf16 || !b_bf16 || !y_bf16) return MXL_EINVAL;
     if (!aligned16(a_bf16) || !aligned16(b_bf16) || !aligned16(bias) || !aligned16(residual_bf16) || !aligned16(y_bf16) || !aligned16(z_bf16)) return MXL_EINVAL;
-    const int64_t need = mxl_linear_bf16_workspace_bytes(m, n, k);
+    const DensePlan plan = m > FEW_ROWS ? dense_plan(m, n, k) : DensePlan{};
+    const int64_t need = m > FEW_ROWS ? runs_bytes(plan, m, n) : 0;
     if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     DenseArgs d{(const uint8_t*)a_bf16, (const uint8_t*)b_bf16, (uint16_t*)y_bf16, m, n, k, {bias, (const uint16_t*)residual_bf16, (uint16_t*)z_bf16, bias_dtype == MXL_DT_F32}, (float*)workspace, 1, 0, nullptr};
     hipStream_t st = (hipStream_t)stream;
     switch (act) {
-        case MXL_ACT_SILU: return launch_dense_forward<kActSilu>(d, st);
-        case MXL_ACT_GELU: return launch_dense_forward<kActGelu>(d, st);
-        case MXL_ACT_RELU: return launch_dense_forward<kActRelu>(d, st);
-        default: return launch_dense_forward<kActNone>(d, st);
+        case MXL_ACT_SILU: return launch_dense_forward<kActSilu>(d, plan, st);
+        case MXL_ACT_GELU: return launch_dense_forward<kActGelu>(d, plan, st);
+        case MXL_ACT_RELU: return launch_dense_forward<kActRelu>(d, plan, st);
+        default: return launch_dense_forward<kActNone>(d, plan, st);
     }
 }
 
+namespace mxl {
 // da [m, k] = dz [m, n] . b [n, k]: the contraction is over n, b's slow dim
+static int run_dgrad(const DensePlan& plan, const void* dz, const void* b, int64_t m, int64_t n, int64_t k, void* da, void* workspace, int64_t workspace_bytes,
+                     void* stream) {
+    if (!dz || !b || !da || !aligned16(dz) || !aligned16(b) || !aligned16(da)) return MXL_EINVAL;
+    const int64_t need = runs_bytes(plan, m, k);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    if (plan.tn == 256) return mxl_grouped_gemm_bf16(dz, b, da, nullptr, 1, m, k, n, MXL_BF_B_KN | MXL_BF_TILE_256, stream);
+    DenseArgs d{(const uint8_t*)dz, (const uint8_t*)b, (uint16_t*)da, m, k, n, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0, nullptr};
+    return launch_dense<false, true, kActNone>(d, plan, (hipStream_t)stream);
+}
+// db [n, k] = dz [m, n]^T . a [m, k]
+static int run_wgrad(const DensePlan& plan, const void* dz, const void* a, int64_t m, int64_t n, int64_t k, void* db, uint32_t flags, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+    if (plan.tn == 256) return mxl_grouped_gemm_bf16_wgrad(dz, a, db, nullptr, 1, m, n, k, flags, stream);      // one group
+    if (!dz || !a || !db || !aligned16(dz) || !aligned16(a) || !aligned16(db)) return MXL_EINVAL;
+    const bool accum = (flags & MXL_BF_ACCUM_F32) != 0;
+    const int64_t need = runs_bytes(plan, n, k, accum);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    DenseArgs d{(const uint8_t*)dz, (const uint8_t*)a, accum ? nullptr : (uint16_t*)db, n, k, m, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0, accum ? (float*)db : nullptr};
+    return launch_dense<true, true, kActNone>(d, plan, (hipStream_t)stream);
+}
+}  // namespace mxl
+
 extern "C" int mxl_linear_bf16_dgrad(const void* dz_bf16, const void* b_bf16, int64_t m, int64_t n, int64_t k, void* da_bf16, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
     if (!dense_sizes_ok(m, n, k)) return MXL_EINVAL;
     if (m == 0) return MXL_OK;
-    if (!dz_bf16 || !b_bf16 || !da_bf16 || !aligned16(dz_bf16) || !aligned16(b_bf16) || !aligned16(da_bf16)) return MXL_EINVAL;
-    const int64_t need = mxl_linear_bf16_workspace_bytes(m, k, n);
-    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
-    if (!device_is_gfx950()) return MXL_ENODEV;
-    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)b_bf16, (uint16_t*)da_bf16, m, k, n, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0, nullptr};
-    hipStream_t st = (hipStream_t)stream;
-    if (dense_plan(m, k, n).tn == 256)
-        return mxl_grouped_gemm_bf16(dz_bf16, b_bf16, da_bf16, nullptr, 1, m, k, n, MXL_BF_B_KN | MXL_BF_TILE_256, stream);
-    return launch_dense<false, true, kActNone>(d, st);
+    return run_dgrad(dense_plan(m, k, n), dz_bf16, b_bf16, m, n, k, da_bf16, workspace, workspace_bytes, stream);
 }
 
 extern "C" int64_t mxl_linear_bf16_wgrad_workspace_bytes(int64_t m, int64_t n, int64_t k, uint32_t flags) {
     if (!dense_wgrad_ok(m, n, k) || (flags & ~(uint32_t)MXL_BF_ACCUM_F32)) return -1;
-    const bool accum = (flags & MXL_BF_ACCUM_F32) != 0;
-    if (!dense_wgrad_here(m, n, k)) return 0;
-    const int splits = dense_plan(n, k, m, true).splits;
-    return splits > 1 || accum ? splits * n * k * 4 : 0;
+    return runs_bytes(wgrad_plan(m, n, k), n, k, (flags & MXL_BF_ACCUM_F32) != 0);
 }
 
-// db [n, k] = dz [m, n]^T . a [m, k]
 extern "C" int mxl_linear_bf16_wgrad(const void* dz_bf16, const void* a_bf16, int64_t m, int64_t n, int64_t k, void* db, uint32_t flags, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
     if (!dense_wgrad_ok(m, n, k) || (flags & ~(uint32_t)MXL_BF_ACCUM_F32)) return MXL_EINVAL;
-    if (!dense_wgrad_here(m, n, k))      // the grouped kernel with one group
-        return mxl_grouped_gemm_bf16_wgrad(dz_bf16, a_bf16, db, nullptr, 1, m, n, k, flags, stream);
-    if (!dz_bf16 || !a_bf16 || !db || !aligned16(dz_bf16) || !aligned16(a_bf16) || !aligned16(db)) return MXL_EINVAL;
-    const bool accum = (flags & MXL_BF_ACCUM_F32) != 0;
-    const int64_t need = mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, flags);
-    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MXL_EINVAL;
-    if (!device_is_gfx950()) return MXL_ENODEV;
-    DenseArgs d{(const uint8_t*)dz_bf16, (const uint8_t*)a_bf16, accum ? nullptr : (uint16_t*)db, n, k, m, {nullptr, nullptr, nullptr, 0}, (float*)workspace, 1, 0, accum ? (float*)db : nullptr};
-    return launch_dense<true, true, kActNone>(d, (hipStream_t)stream);
+    return run_wgrad(wgrad_plan(m, n, k), dz_bf16, a_bf16, m, n, k, db, flags, workspace, workspace_bytes, stream);
 }
 
 extern "C" int64_t mxl_linear_bf16_dz_workspace_bytes(int64_t m, int64_t n) {
@@ -745,13 +754,16 @@ extern "C" int mxl_linear_bf16_dz(const void* dy_bf16, const void* z_bf16, int a
 namespace mxl {
 static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 struct BwdSpace {
+    DensePlan dgrad, wgrad;
     int64_t dz, sums, runs, total;      // bytes: dz (with an activation), dbias's partial sums, the split sums of dgrad, then of the weight gradient
 };
 static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int act, bool need_da, bool need_db, uint32_t db_flags, bool need_dbias) {
-    BwdSpace s;
+    BwdSpace s{};
     s.dz = act == MXL_ACT_NONE ? 0 : up256(m * n * 2);
     s.sums = need_dbias ? up256(mxl_linear_bf16_dz_workspace_bytes(m, n)) : 0;
-    const int64_t da = need_da ? mxl_linear_bf16_workspace_bytes(m, k, n) : 0, db = need_db ? mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, db_flags) : 0;
+    int64_t da = 0, db = 0;
+    if (need_da && m > 0) s.dgrad = dense_plan(m, k, n), da = runs_bytes(s.dgrad, m, k);
+    if (need_db) s.wgrad = wgrad_plan(m, n, k), db = runs_bytes(s.wgrad, n, k, (db_flags & MXL_BF_ACCUM_F32) != 0);
     s.runs = up256(da > db ? da : db);
     s.total = s.dz + s.sums + s.runs;
     return s;
@@ -781,7 +793,7 @@ extern "C" int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, cons
     if (da_bf16 || db || dbias)
         rc = mxl_linear_bf16_dz(dy_bf16, z_bf16, act, m, n, dz, dbias, dbias_dtype, at + sp.dz, sp.sums, stream);
     const void* d = sp.dz ? dz : dy_bf16;
-    if (rc == MXL_OK && da_bf16) rc = mxl_linear_bf16_dgrad(d, b_bf16, m, n, k, da_bf16, at + sp.dz + sp.sums, sp.runs, stream);
-    if (rc == MXL_OK && db) rc = mxl_linear_bf16_wgrad(d, a_bf16, m, n, k, db, db_flags, at + sp.dz + sp.sums, sp.runs, stream);
+    if (rc == MXL_OK && da_bf16 && m > 0) rc = run_dgrad(sp.dgrad, d, b_bf16, m, n, k, da_bf16, at + sp.dz + sp.sums, sp.runs, stream);
+    if (rc == MXL_OK && db) rc = run_wgrad(sp.wgrad, d, a_bf16, m, n, k, db, db_flags, at + sp.dz + sp.sums, sp.runs, stream);
     return rc;
 }
