@@ -11,9 +11,10 @@
 // Bound by instructions and, for few tokens, by one row's chain of them: a row is held in registers by LPR lanes of a wave, V logits a
 // lane, sorted inside the lane once (V = 4: five comparisons), and a round of the choice is one maximum over the row's lanes and a step
 // in one lane's list, 27 instructions.  Without bias and groups the order of the scores is that of the logits, which are compared as they are.
-// With them the scores are compared in fp32 first; a row in which two neighbours of the result, or the last chosen and the first
-// left out, are nearer to each other than the rounding of fp32 scores allows to tell apart is chosen again from scores in
-// fp64 (one row in 2000 at 256 fp32 scores), so the indices are those of the definition and not of a rounding.
+// With them the scores are compared in fp32 first; a row in which two neighbours of the result, or the last chosen and the best
+// left out that is no true tie of it (same logit, same bias), are nearer to each other than the rounding of fp32 scores allows to tell apart is
+// chosen again from scores in fp64 (one row in 2000 at 256 fp32 scores), so the indices are those of the definition and not of a rounding.
+// A tie at that border costs its row a pass over the registers: 16384 rows of 256 zeros 21.0 us with the counts, 19.2 without the comparison.
 //
 // us: 8 tokens of 128 experts, top 4, 2.7; 16384 of 8, top 2, 3.9 and 2.2 for adding up the counts, gradient 3.5; 5003 of 160, top 6, 9.6 + 3.3,
 // 7.4; 16384 of 256, sigmoid, bias, 4 of 8 groups, top 8, 28 + 4.0, 6.9 (the logits alone are 3.3 at the rate of a large copy).  The last one's forward
@@ -235,7 +236,7 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
             idx[v] = (uint32_t)(first + v);
         }
         sort_pairs<V>(key, idx);
-        bool doubt = false;
+        bool doubt = false, keep = true;
         if (SCORED && p.groups > 1) {
             uint32_t gk[V], gi[V];
 #pragma unroll
@@ -250,7 +251,8 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
             int ahead = 0;
             for (int g = 0; g < p.groups; ++g)
                 ahead += __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(score), g * p.lanes_per_group)) > score;
-            const bool keep = ahead < p.group_topk, real = lane / p.lanes_per_group < p.groups;
+            keep = ahead < p.group_topk;
+            const bool real = lane / p.lanes_per_group < p.groups;
             if (p.group_topk < p.groups) {
                 // the worst group kept and the best one left out, against what fp32 scores and their sums may be off; groups of
                 // the same score, of which too many are kept, are told apart in fp64
@@ -294,9 +296,29 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
             const float b = bias[mine_key ? mine : 0], s = p.sigmoid ? sigmoid_fast(ml) : exp_fast(ml - top) / total, c = key_value(mine_key);
             const float nl = dpp_next_lane(ml), ns = dpp_next_lane(s), nc = dpp_next_lane(c), nb = dpp_next_lane(b);
             const uint32_t nk = dpp_next_lane(mine_key);
-            const float off = (p.bias || p.sigmoid ? pair_off : 0x1p-16f * (s + ns)) + 0x1p-23f * (fabsf(c) + fabsf(nc));
+            auto off_of = [&](float both, float c1, float c2) __attribute__((always_inline)) {
+                return (p.bias || p.sigmoid ? pair_off : 0x1p-16f * both) + 0x1p-23f * (fabsf(c1) + fabsf(c2));
+            };
             // nothing follows, or the same logit and bias (a true tie), or far enough apart: told rightly
-            const bool told = !chosen || nk == 0u || (ml == nl && b == nb) || c - nc > off;
+            const bool tie = nk != 0u && ml == nl && b == nb;
+            const bool told = !chosen || nk == 0u || tie || c - nc > off_of(s + ns, c, nc);
+            // The last one chosen and the first left out are a true tie: the best one left out that is none of their kind has to be told from
+            // them too.  True ties have the same fp32 key; whether anything else has it, the numbers of both say.
+            if (__ballot(tie) >> (p.topk - 1) & 1) {
+                auto of_last = [&](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), p.topk - 1)); };
+                const uint32_t key_t = (uint32_t)__builtin_amdgcn_readlane((int)mine_key, p.topk - 1);
+                const float l_t = of_last(ml), b_t = of_last(b), c_t = of_last(c);
+                uint32_t behind = 0u;
+                int others = mine_key == key_t;         // chosen or left out, with that key, less the ties
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    behind = key[v] < key_t && key[v] > behind ? key[v] : behind;
+                    others += (key[v] == key_t) - (v < have && keep && l[v] == l_t && bias[first + v] == b_t);
+                }
+                behind = wave_max_key(behind);
+                const float z = key_value(behind);      // (the score itself where there is no bias)
+                doubt |= lanes_sum<64>((float)others) != 0.f || (behind != 0u && !(c_t - z > off_of(c_t + z, c_t, z)));
+            }
             doubt = __any(doubt || !told);
             if (doubt) {
                 mine = choose_fp64<V>(p, l, bias, top, first, have, spare + w * V * 64);
