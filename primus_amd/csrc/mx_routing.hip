@@ -241,11 +241,12 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
             uint32_t gk[V], gi[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) gk[v] = key[v], gi[v] = 0u;
-            float score = 0.f;
+            float score = 0.f, terms = 0.f;         // the group's sum, and its terms' magnitudes
             for (int i = 0; i < p.take; ++i) {
                 const uint32_t best = lanes_reduce<OpMaxU>(gk[0], p.lanes_per_group);
                 const uint32_t who = lanes_reduce<OpMinU>(gk[0] == best ? (uint32_t)lane : 64u, p.lanes_per_group);
                 score += best ? key_value(best) : 0.f;
+                terms += best ? fabsf(key_value(best)) : 0.f;
                 pop_head<V>(gk, gi, who == (uint32_t)lane && best != 0u);
             }
             int ahead = 0;
@@ -254,14 +255,16 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
             keep = ahead < p.group_topk;
             const bool real = lane / p.lanes_per_group < p.groups;
             if (p.group_topk < p.groups) {
-                // the worst group kept and the best one left out, against what fp32 scores and their sums may be off; groups of
-                // the same score, of which too many are kept, are told apart in fp64
+                // The worst that any group kept may be and the best that any left out may be; groups of the same score, of which too many
+                // are kept, are told apart in fp64.  A sum of n = take terms is off by what its scores are, and by n roundings at most
+                // where biases are added and as many in the sum, each up to 2^-24 of the terms' magnitudes together (biased terms may
+                // cancel: the sum says nothing of them).  Infinite sums are exact.
+                const float sum_off = (p.bias || p.sigmoid ? 0.5f * pair_off * (float)p.take : 0x1p-16f * score) + 0x1p-22f * (float)p.take * terms;
+                const float off = fabsf(score) == INFINITY ? 0.f : sum_off;
                 const int kept = __builtin_popcountll(__ballot(keep && real)) / p.lanes_per_group;
-                const float in_worst = key_value(~wave_max_key(real && keep ? ~order_key(score) : 0u));
-                const float out_best = key_value(wave_max_key(real && !keep ? order_key(score) : 0u));
-                const float mag = fabsf(in_worst) + fabsf(out_best);
-                const float off = p.bias || p.sigmoid ? pair_off * (float)p.take : 0x1p-16f * mag;
-                doubt = kept != p.group_topk || !(in_worst - out_best > off + 0x1p-22f * (float)p.take * mag);
+                const float in_worst = key_value(~wave_max_key(real && keep ? ~order_key(score - off) : 0u));
+                const float out_best = key_value(wave_max_key(real && !keep ? order_key(score + off) : 0u));
+                doubt = kept != p.group_topk || !(in_worst > out_best);
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) key[v] = keep ? key[v] : 0u;
