@@ -258,8 +258,9 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
                 // The worst that any group kept may be and the best that any left out may be; groups of the same score, of which too many
                 // are kept, are told apart in fp64.  A sum of n = take terms is off by what its scores are, and by n roundings at most
                 // where biases are added and as many in the sum, each up to 2^-24 of the terms' magnitudes together (biased terms may
-                // cancel: the sum says nothing of them).  Infinite sums are exact.
-                const float sum_off = (p.bias || p.sigmoid ? 0.5f * pair_off * (float)p.take : 0x1p-16f * score) + 0x1p-22f * (float)p.take * terms;
+                // cancel: the sum says nothing of them).  Of a softmax without a bias terms below 2^-126 may be 0, at most 32 of them.  Infinite
+                // sums are exact.
+                const float sum_off = (p.bias || p.sigmoid ? 0.5f * pair_off * (float)p.take : fmaf(0x1p-16f, score, 0x1p-121f)) + 0x1p-22f * (float)p.take * terms;
                 const float off = fabsf(score) == INFINITY ? 0.f : sum_off;
                 const int kept = __builtin_popcountll(__ballot(keep && real)) / p.lanes_per_group;
                 const float in_worst = key_value(~wave_max_key(real && keep ? ~order_key(score - off) : 0u));

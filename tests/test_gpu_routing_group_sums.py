@@ -33,3 +33,15 @@ def test_terms_that_cancel(gpu, score, size):
     _, idx, _ = ops.topk_routing(logits.to(gpu), topk, score_function=score, expert_bias=bias.to(gpu), num_groups=groups, group_topk=group_topk)
     wrong = (idx.cpu() != want).any(1) & clear
     assert not bool(wrong.any()), (int(wrong.sum()), int(clear.sum()))
+
+
+def test_scores_below_the_smallest_normal_number(gpu):
+    """One expert has all of the softmax but 2^-28: of the other groups, one with an expert above and one below 2^-126 beats one with
+    both just above."""
+    from primus_amd.pytorch import ops
+
+    row = torch.tensor([0.0, -20.0, -87.300, -87.340, -87.325, -87.325, -95.0, -95.0])
+    p = torch.softmax(row.double(), 0)
+    assert p[3] < 2.0 ** -126 < p[5] < p[2] and float(p[2] + p[3]) > 1.004 * float(p[4] + p[5])
+    _, idx, _ = ops.topk_routing(row[None].repeat(3, 1).to(gpu), 4, num_groups=4, group_topk=2)
+    assert idx.tolist() == [[0, 1, 2, 3]] * 3
