@@ -565,7 +565,7 @@ int mxl_linear_backward(const mxl_linear* p, int parts, const void* dy_bf16, con
  *   probs        : float[tokens, topk] = scale * score of the chosen experts, divided by their sum first if renormalize
  *                  (sigmoid: sum + 1e-20)
  *   indices      : int64[tokens, topk], best first; ties go to the lower index.  The order is the one of exact scores: fp32
- *                  scores too near to each other to tell are compared in fp64.  NaN scores are chosen last.  Softmax over
+ *                  scores too near to each other to tell are compared in fp64.  NaN scores are chosen last, groups of a NaN score stay last.  Softmax over
  *                  nothing but -inf (all of a row, or all that are chosen when renormalised) is 0.
  *   counts       : int64[experts], tokens of every expert
  *   token_mask   : uint8[tokens] (NULL: all ones); a token whose byte is 0 gets indices -1 and probs 0 and is not counted

@@ -142,11 +142,12 @@ __device__ __forceinline__ int choose_fp64(const RouteArgs& p, const float (&l)[
                 rescan(have_bits);
             }
         }
+        const bool nan = score != score;        // behind every score that is none
         int ahead = 0;
         const int grp = lane / p.lanes_per_group;
         for (int g = 0; g < p.groups; ++g) {
             const double other = __shfl(score, g * p.lanes_per_group);
-            ahead += other > score || (other == score && g < grp);
+            ahead += other > score || (nan ? g < grp || other == other : other == score && g < grp);
         }
         if (ahead >= p.group_topk) left = 0;
         rescan(left);
@@ -255,8 +256,8 @@ __global__ __launch_bounds__((route_waves<V, SCORED>() * 64), (V > 4 ? 1 : SCORE
             keep = ahead < p.group_topk;
             const bool real = lane / p.lanes_per_group < p.groups;
             if (p.group_topk < p.groups) {
-                // The worst that any group kept may be and the best that any left out may be; groups of the same score, of which too many
-                // are kept, are told apart in fp64.  A sum of n = take terms is off by what its scores are, and by n roundings at most
+                // The worst that any group kept may be and the best that any left out may be; groups of the same score and groups that are
+                // NaN, of which too many are kept, are told apart in fp64.  A sum of n = take terms is off by what its scores are, and by n roundings at most
                 // where biases are added and as many in the sum, each up to 2^-24 of the terms' magnitudes together (biased terms may
                 // cancel: the sum says nothing of them).  Of a softmax without a bias terms below 2^-126 may be 0, at most 32 of them.  Infinite
                 // sums are exact.

@@ -1231,8 +1231,8 @@ def topk_routing(logits: torch.Tensor, topk: int, score_function: str = "softmax
     ``group_topk`` best groups take part.  ``indices`` are best first, ties to the lower index; fp32 scores that are too near to
     each other to tell are compared in fp64.  ``probs`` are the chosen scores, divided by their sum if ``renormalize`` (sigmoid:
     by the sum + 1e-20), times ``scaling_factor``.  Tokens whose ``token_mask`` (bool ``[tokens]``) is False get indices -1 and
-    probabilities 0 and are not counted.  Softmax scores of nothing but -inf are 0.  NaN scores are chosen last; the indices are
-    valid and differ from each other whatever the logits hold.  At most 1024 experts, 32 a token, 64 groups.  Differentiable in ``logits``."""
+    probabilities 0 and are not counted.  Softmax scores of nothing but -inf are 0.  NaN scores are chosen last, and a
+    group whose score is NaN comes last; the indices are valid and differ from each other whatever the logits hold.  At most 1024 experts, 32 a token, 64 groups.  Differentiable in ``logits``."""
     if num_groups is None:
         if group_topk is not None:
             raise ValueError("group_topk needs num_groups")
