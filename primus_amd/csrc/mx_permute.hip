@@ -462,9 +462,9 @@ static bool move_types_ok(int hidden, int dtype, int probs_dtype) {
 
 extern "C" int mxl_combine_rows(const void* rows_in, int64_t rows, int hidden, int dtype, const int64_t* row_of, int64_t tokens, int topk,
                                 const void* probs, const void* row_probs, void* probs_out, int probs_dtype, void* y, void* stream) {
-    if (!move_sizes_ok(tokens, topk, rows) || !move_types_ok(hidden, dtype, probs_dtype) || (row_probs != nullptr) != (probs_out != nullptr)) return MXL_EINVAL;
-    if (tokens == 0) return MXL_OK;
-    if ((rows > 0 && !rows_in) || !row_of || !y) return MXL_EINVAL;
+    if (!move_sizes_ok(tokens, topk, rows) || !move_types_ok(hidden, dtype, probs_dtype)) return MXL_EINVAL;
+    if (tokens == 0) return MXL_OK;         // (empty outputs, which may have no address, beside rows that are there)
+    if ((row_probs != nullptr) != (probs_out != nullptr) || (rows > 0 && !rows_in) || !row_of || !y) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     MoveArgs a{};
     a.x = (const uint8_t*)rows_in, a.out = (uint8_t*)y, a.row_of = row_of, a.probs = probs, a.row_probs = row_probs, a.probs_out = probs_out;
