@@ -601,7 +601,7 @@ int mxl_permute_tokens(const void* x, int64_t tokens, int64_t row_bytes, const i
                        void* row_probs, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 /* y[t] = sum_k probs[t, k] * rows[row_of[t, k]] (probs NULL: ones), fp32 in the order of k, rounded once; entries of -1 add
  * nothing.  If row_probs is set, probs_out[t, k] = row_probs[row_of[t, k]] (0 for -1) on the way: together the gradient of
- * mxl_permute_rows and of the probabilities' move. */
+ * mxl_permute_rows and of the probabilities' move.  y NULL: probs_out alone (rows_in and probs are not looked at). */
 int mxl_combine_rows(const void* rows_in, int64_t rows, int hidden, int dtype, const int64_t* row_of, int64_t tokens, int topk,
                      const void* probs, const void* row_probs, void* probs_out, int probs_dtype, void* y, void* stream);
 /* Its gradient with probs: drows[row_of[t, k]] = probs[t, k] * dy[t], zero rows where entry_of is -1;

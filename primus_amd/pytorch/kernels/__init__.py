@@ -1433,6 +1433,22 @@ def combine_rows_impl(rows, row_of, entry_of, probs: Optional[torch.Tensor] = No
     return y, out
 
 
+def entry_probs_impl(row_probs, row_of) -> torch.Tensor:
+    """``row_probs[row_of[t, k]]`` (0 where ``row_of`` is -1) in ``row_probs``' type: the part of ``combine_rows_impl`` that is left when no
+    rows are wanted."""
+    pd = _float_type(row_probs, "row_probs")
+    if row_probs.dim() != 1 or row_of.dtype != torch.int64 or row_of.dim() != 2 or not 1 <= row_of.shape[1] <= ROUTING_MAX_TOPK:
+        raise ValueError(f"row_probs must be [rows] and row_of int64 [tokens, topk] with topk in [1, {ROUTING_MAX_TOPK}]")
+    _require_cuda(row_probs, row_of)
+    _same_device(row_probs.device, row_of=row_of)
+    tokens, topk = row_of.shape
+    with _on(row_probs.device), _hooked("entry_probs", tokens=tokens, rows=row_probs.shape[0]):
+        out = torch.empty(tokens, topk, dtype=row_probs.dtype, device=row_probs.device)
+        rc = _lib.load().mxl_combine_rows(None, row_probs.shape[0], 1, pd, _ptr(row_of), tokens, topk, None, _ptr(row_probs), _ptr(out), pd, None, _stream())
+    _lib.check(rc, "mxl_combine_rows")
+    return out
+
+
 def combine_rows_bwd_impl(dy, rows, row_of, entry_of, probs, need_rows: bool = True, need_probs: bool = True):
     """``(drows, dprobs float32)`` of ``combine_rows_impl`` with ``probs``; what is not needed is None."""
     _row_args(rows, row_of, entry_of)

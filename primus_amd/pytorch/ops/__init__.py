@@ -1277,7 +1277,7 @@ class _PermuteTokens(torch.autograd.Function):
             drows = drows.to(ctx.dtype).contiguous()
             dx, dprobs = K.combine_rows_impl(drows, row_of, entry_of, row_probs=None if drow_probs is None else drow_probs.contiguous())
         elif drow_probs is not None:
-            dprobs = torch.where(row_of >= 0, drow_probs[row_of.clamp(min=0)], 0.0) if entry_of.numel() else drow_probs.new_zeros(row_of.shape)
+            dprobs = K.entry_probs_impl(drow_probs.contiguous(), row_of)
         return dx, None, None, dprobs, None, None
 
 
