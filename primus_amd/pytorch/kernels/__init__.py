@@ -1547,8 +1547,8 @@ def linear_bf16_bwd_impl(dy, a, b, z, activation: Optional[str], need_a: bool = 
         _bf16_2d(z, "z", (m, n))
     _require_cuda(dy, a, b, z, accum_into)
     dev = dy.device
-    if a.device != dev or b.device != dev:
-        _same_device(dev, a=a, b=b)
+    if a.device != dev or b.device != dev or (z is not None and z.device != dev) or (accum_into is not None and accum_into.device != dev):
+        _same_device(dev, a=a, b=b, z=z, accum_into=accum_into)
     if need_b and m * max(n, k) * 2 >= 1 << 32:
         dz, dbias = linear_bf16_dz_impl(dy, z, activation, bias_dtype)
         return linear_bf16_dgrad_impl(dz, b) if need_a else None, linear_bf16_wgrad_impl(dz, a, accum_into=accum_into), dbias
@@ -1576,6 +1576,7 @@ def linear_bf16_dz_impl(dy, z, activation: Optional[str], bias_dtype: Optional[t
     if act != _lib.ACT_NONE:
         _bf16_2d(z, "z", (m, n))
     _require_cuda(dy, z)
+    _same_device(dy.device, z=z)
     with _on(dy.device), _hooked("linear_bf16_dz", m=m, n=n):
         dz = torch.empty_like(dy) if act != _lib.ACT_NONE else dy
         dbias, ws, nbytes = None, None, 0
