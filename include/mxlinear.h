@@ -616,12 +616,14 @@ int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int 
  * fp32 from the products to y, which is rounded once; bias (bf16 or float, NULL: none), residual (NULL: none); act MXL_ACT_*.
  * z_bf16: if not NULL, z rounded to bf16 for the backward.  n and k multiples of 32 up to 2^21, n * k * 2 < 2^32, pointers 16-byte aligned.
  * Few tiles and a long contraction split it over workgroups, whose sums meet in the caller's workspace:
- * mxl_linear_bf16_workspace_bytes(m, n, k) bytes for the forward, (m, k, n) for dgrad, mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, flags) for
- * the weight gradient (0: none, NULL will do).
+ * mxl_linear_bf16_forward_workspace_bytes(m, n, k) bytes for the forward (none up to 16 rows, which have a kernel of their own),
+ * mxl_linear_bf16_workspace_bytes(m, k, n) for dgrad, mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, flags) for the weight gradient
+ * (0: none, NULL will do).  mxl_linear_bf16_workspace_bytes(m, n, k) is what a product [m, k] . [k, n] takes on tiles: enough for the forward too.
  *
  * Backward: mxl_linear_bf16_dz gives dz = dy * act'(z) (not written, and may be dy itself, for MXL_ACT_NONE) and
  * dbias = column sums of dz before its rounding (NULL: not wanted); mxl_linear_bf16_dgrad gives da = dz . b;
  * mxl_linear_bf16_wgrad db = dz^T . a [n, k], bf16 or (MXL_BF_ACCUM_F32) added to a float buffer, m * max(n, k) * 2 < 2^32. */
+int64_t mxl_linear_bf16_forward_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t k);
 /* What a product of these sizes runs on, worked out on the host: output tile and runs of the contraction, of any length (the forward of
  * up to 16 rows has a kernel of its own).  dgrad's are (m, k, n), the weight gradient's (n, k, m) with a_by_columns 1. */

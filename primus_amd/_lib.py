@@ -94,6 +94,7 @@ EXPORTS = (
     "mxl_permute_rows",
     "mxl_combine_rows",
     "mxl_combine_rows_bwd",
+    "mxl_linear_bf16_forward_workspace_bytes",
     "mxl_linear_bf16_workspace_bytes",
     "mxl_linear_bf16_plan",
     "mxl_linear_bf16",
@@ -280,6 +281,8 @@ def load() -> ctypes.CDLL:
         lib.mxl_linear_bf16.argtypes = [vp, vp, vp, i32, i32, vp, i64, i64, i64, vp, vp, vp, i64, vp]
         lib.mxl_linear_bf16_plan.restype = i32
         lib.mxl_linear_bf16_plan.argtypes = [i64, i64, i64, i32, vp, vp, vp]
+        lib.mxl_linear_bf16_forward_workspace_bytes.restype = i64
+        lib.mxl_linear_bf16_forward_workspace_bytes.argtypes = [i64, i64, i64]
         lib.mxl_linear_bf16_workspace_bytes.restype = i64
         lib.mxl_linear_bf16_workspace_bytes.argtypes = [i64, i64, i64]
         lib.mxl_linear_bf16_dgrad.restype = i32

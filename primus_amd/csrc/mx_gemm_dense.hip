@@ -650,6 +650,11 @@ extern "C" int64_t mxl_linear_bf16_workspace_bytes(int64_t m, int64_t n, int64_t
     return m == 0 ? 0 : runs_bytes(dense_plan(m, n, k), m, n);
 }
 
+extern "C" int64_t mxl_linear_bf16_forward_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (!dense_sizes_ok(m, n, k)) return -1;
+    return m <= FEW_ROWS ? 0 : runs_bytes(dense_plan(m, n, k), m, n);
+}
+
 extern "C" int mxl_linear_bf16_plan(int64_t m, int64_t n, int64_t k, int a_by_columns, int* tile_rows, int* tile_cols, int* splits) {
     if (!dense_sizes_ok(m, n, 32) || m == 0 || k <= 0 || k > 0x7FFFFFFF || !tile_rows || !tile_cols || !splits) return MXL_EINVAL;
     const DensePlan plan = dense_plan(m, n, k, a_by_columns != 0);

@@ -1523,7 +1523,7 @@ def linear_bf16_impl(a, b, bias=None, activation: Optional[str] = None, residual
     with _on(dev), _hooked("linear_bf16", m=m, n=n, k=k):
         y = torch.empty(m, n, dtype=torch.bfloat16, device=dev)
         z = torch.empty_like(y) if want_z else None
-        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_workspace_bytes", m, n, k)
+        ws, ws_bytes = _workspace(dev, "mxl_linear_bf16_forward_workspace_bytes", m, n, k)
         rc = lib.mxl_linear_bf16(_ptr(a), b.data_ptr(), bias_ptr, bias_dtype, act, _ptr(residual), m, n, k, _ptr(y), _ptr(z), _ptr(ws), ws_bytes, _stream())
     if rc:
         _lib.check(rc, "mxl_linear_bf16")
