@@ -28,20 +28,10 @@ template <int ACT> __device__ __forceinline__ float epi_slope(float z) {
         const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
         return s * (1.f + z * (1.f - s));
     } else {
-        // Phi(z) + z phi(z); Phi from the same fit of erfc as act_fwd, t exp(P(t)) exp(-z^2 / 2), whose last factor is phi's too
+        // Phi(z) + z phi(z); Phi from erfc_fit as in act_fwd, t exp(P(t)) exp(-z^2 / 2), whose last factor is phi's too
         const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.5f * x);
-        float q = 0.17087277f;
-        q = q * t - 0.82215223f;
-        q = q * t + 1.48851587f;
-        q = q * t - 1.13520398f;
-        q = q * t + 0.27886807f;
-        q = q * t - 0.18628806f;
-        q = q * t + 0.09678418f;
-        q = q * t + 0.37409196f;
-        q = q * t + 1.00002368f;
-        q = q * t - 1.26551223f;
         const float e = __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);
-        const float tail = 0.5f * t * __builtin_amdgcn_exp2f(q * 1.4426950408889634f) * e;
+        const float tail = 0.5f * t * __builtin_amdgcn_exp2f(erfc_fit(t) * 1.4426950408889634f) * e;
         return fmaf(z * 0.39894228040143268f, e, z < 0.f ? tail : 1.f - tail);
     }
 }

@@ -23,9 +23,6 @@ struct OpMinU {
 struct OpMaxF {
     __device__ static __forceinline__ uint32_t f(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
 };
-struct OpMinF {
-    __device__ static __forceinline__ uint32_t f(uint32_t a, uint32_t b) { return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b))); }
-};
 struct OpAddF {
     __device__ static __forceinline__ uint32_t f(uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }
 };
@@ -49,7 +46,6 @@ template <class OP> __device__ __forceinline__ uint32_t lanes_reduce(uint32_t v,
     return v;
 }
 template <int LANES> __device__ __forceinline__ float lanes_max(float v) { return __uint_as_float(lanes_reduce<OpMaxF, LANES>(__float_as_uint(v))); }
-template <int LANES> __device__ __forceinline__ float lanes_min(float v) { return __uint_as_float(lanes_reduce<OpMinF, LANES>(__float_as_uint(v))); }
 template <int LANES> __device__ __forceinline__ float lanes_sum(float v) { return __uint_as_float(lanes_reduce<OpAddF, LANES>(__float_as_uint(v))); }
 
 // element i of an array of MXL_DT_* type
