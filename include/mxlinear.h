@@ -620,7 +620,7 @@ int mxl_combine_rows_bwd(const void* dy, const void* rows_in, int64_t rows, int 
  * mxl_linear_bf16_workspace_bytes(m, k, n) for dgrad, mxl_linear_bf16_wgrad_workspace_bytes(m, n, k, flags) for the weight gradient
  * (0: none, NULL will do).  mxl_linear_bf16_workspace_bytes(m, n, k) is what a product [m, k] . [k, n] takes on tiles: enough for the forward too.
  *
- * Backward: mxl_linear_bf16_dz gives dz = dy * act'(z) (not written, and may be dy itself, for MXL_ACT_NONE) and
+ * Backward: mxl_linear_bf16_dz gives dz = dy * act'(z), rounded to bf16 (not written, and may be dy itself, for MXL_ACT_NONE) and
  * dbias = column sums of dz before its rounding (NULL: not wanted); mxl_linear_bf16_dgrad gives da = dz . b;
  * mxl_linear_bf16_wgrad db = dz^T . a [n, k], bf16 or (MXL_BF_ACCUM_F32) added to a float buffer, m * max(n, k) * 2 < 2^32. */
 int64_t mxl_linear_bf16_forward_workspace_bytes(int64_t m, int64_t n, int64_t k);

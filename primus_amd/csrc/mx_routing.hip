@@ -16,8 +16,8 @@
 // chosen again from scores in fp64 (one row in 2000 at 256 fp32 scores), so the indices are those of the definition and not of a rounding.
 // A tie at that border costs its row a pass over the registers: 16384 rows of 256 zeros 21.0 us with the counts, 19.2 without the comparison.
 //
-// us: 8 tokens of 128 experts, top 4, 2.7; 16384 of 8, top 2, 3.9 and 2.2 for adding up the counts, gradient 3.5; 5003 of 160, top 6, 9.6 + 3.3,
-// 7.4; 16384 of 256, sigmoid, bias, 4 of 8 groups, top 8, 28 + 4.0, 6.9 (the logits alone are 3.3 at the rate of a large copy).  The last one's forward
+// us in a trace: 8 tokens of 128 experts, top 4, 2.9; 16384 of 8, top 2, 3.6 and 2.3 for adding up the counts, gradient 3.6; 5003 of 160, top 6,
+// 9.4 + 3.3, 7.2; 16384 of 256, sigmoid, bias, 4 of 8 groups, top 8, 29 + 3.9, 7.0 (the logits alone are 3.3 at the rate of a large copy).  The last one's forward
 // without the fp64 rows is 22-26, with one round instead of nine 17.
 #include "mx_lanes.h"
 
@@ -398,8 +398,9 @@ struct RouteBwdArgs {
 constexpr int RB_WAVES = 8;
 // All but the plain softmax: the other experts' gradients are zero.  LPR lanes a row, so that 64 / LPR rows wait for their indices and
 // logits together; the rows leave as one run of memory, four elements a lane and request (VEC).  Bound by that one wait and, with many
-// experts, by the rows' bytes.  us with a wave a row, two rows, eight rows: 16384 tokens of 8 experts, top 2, 5.8 / 4.4 / 2.9, of 64, top 6, 6.2 / 4.8 / 3.8, of 256, top 8,
-// 8.7 / 6.1 / 6.5, of 1024 16.2 / 13.6 / 16.2; 8192 of 64 4.5 / 3.6 / 3.4; 1024 of 64 2.8 / 2.8 / 3.2, of 256 3.3 / 3.1 / 4.0.  So eight rows for many tokens of few
+// experts, by the rows' bytes.  us from launch to launch of a replayed graph (a trace has 0.5 to 1 us more for a launch) with a wave a row, two
+// rows, eight rows: 16384 tokens of 8 experts, top 2, 5.8 / 4.4 / 2.9, of 64, top 6, 6.2 / 4.8 / 3.8, of 256, top 8, 8.7 / 6.1 / 6.5, of
+// 1024 16.2 / 13.6 / 16.2; 8192 of 64 4.5 / 3.6 / 3.4; 1024 of 64 2.8 / 2.8 / 3.2, of 256 3.3 / 3.1 / 4.0.  So eight rows for many tokens of few
 // experts, else two.
 template <int LPR, bool VEC>
 __global__ __launch_bounds__(RB_WAVES * 64) void route_bwd_chosen_kernel(RouteBwdArgs p) {

@@ -1025,7 +1025,8 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     """``act(a @ b^T + bias) + residual``: ``gemm`` on bf16 operands with what follows it in its epilogue, computed in fp32 and rounded
     once.  ``a [..., k]``, ``b [n, k]``, ``bias [n]`` (bfloat16 or float32), ``activation`` None, ``"silu"``, ``"gelu"`` (erf) or ``"relu"``,
     ``residual [..., n]``.  ``n`` and ``k`` in multiples of 32 up to 2^21, the weight below 4 GiB (anything else raises).  Differentiable in the four
-    tensors; the activation's input is kept in bf16 for the backward, whose gradients are those of that rounded value.
+    tensors; the activation's input is kept in bf16 for the backward, whose gradients are those of that rounded value, and the gradient before the
+    activation is rounded to bf16 for the products that make those of ``a`` and ``b`` (the bias gradient is summed before that rounding).
     ``fuse_bgrad_accum_pattern="megatron"`` adds the weight gradient into ``b.main_grad``, as ``gemm`` does."""
     accum = None if fuse_bgrad_accum_pattern is None else _accum_from(b, fuse_bgrad_accum_pattern)
     if a.dim() < 2 or b.dim() != 2:
