@@ -647,6 +647,44 @@ int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_b
                         void* da_bf16, void* db, uint32_t db_flags, void* dbias, int dbias_dtype, void* workspace, int64_t workspace_bytes,
                         void* stream);
 
+/* ---- norms where blocks meet: residual add, gate and residual scale (the reference normalises in front of its linears,
+ * primus/backends/megatron/core/extensions/primus_turbo.py:1689-1700) ----
+ *   n = x * rp * post_weight,  rp = 1 / sqrt(mean_j x^2 + post_eps)       (post_weight NULL: n = x)
+ *   h = residual + scale * gate * n                                       (gate NULL: 1)
+ *   y = h * r * weight,        r = 1 / sqrt(mean_j h^2 + eps)             (weight NULL: no y)
+ * x, y [rows, k], weights [k] and gate of type `dtype`, residual and h [rows, k] of stream_dtype (the same, or MXL_DT_F32); fp32 from the inputs to
+ * y and h, one rounding each (y is the norm of the unrounded h).  gate: [gate_mod, gate_cols], gate_cols 1 or k; row r has gate row
+ * r / gate_div % gate_mod, and gate_div * gate_mod divides rows.  post_rstd, rstd: float[rows], what the backward takes (NULL: not
+ * wanted).  k <= 16384, any; at least one of the weights.
+ *
+ * mxl_block_norm_bwd: gradients given those of y (dy; not looked at without weight) and of h (dh, stream_dtype; NULL: zero).  Any output may be
+ * NULL: not wanted.  dresidual is written in stream_dtype; without weight it is dh itself, which is left to the caller (written all the same
+ * if asked for).  x is looked at with post_weight or dgate, h with weight.  mxl_block_norm_bwd_workspace_bytes: has_weight, has_post_weight:
+ * whether dweight, dpost_weight are wanted, gate_cols 0: dgate is not. */
+int mxl_block_norm(const void* x, const void* residual, int64_t rows, int64_t k, int dtype, int stream_dtype, const void* post_weight,
+                   float post_eps, const void* gate, int64_t gate_div, int64_t gate_mod, int64_t gate_cols, float scale, const void* weight,
+                   float eps, void* y, void* h, float* post_rstd, float* rstd, void* stream);
+int64_t mxl_block_norm_bwd_workspace_bytes(int64_t rows, int64_t k, int has_weight, int has_post_weight, int64_t gate_div, int64_t gate_mod,
+                                           int64_t gate_cols);
+int mxl_block_norm_bwd(const void* dy, const void* dh, const void* x, const void* h, int64_t rows, int64_t k, int dtype, int stream_dtype,
+                       const void* post_weight, const float* post_rstd, const void* gate, int64_t gate_div, int64_t gate_mod, int64_t gate_cols,
+                       float scale, const void* weight, const float* rstd, void* dx, void* dresidual, void* dweight, void* dpost_weight,
+                       void* dgate, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- the global norm of many gradients, and clipping ----
+ * grads, sizes (elements), dtypes (MXL_DT_*): host arrays of `count` tensors, each a run of elements without gaps at any element's address.
+ * mxl_grad_norm: *norm (device) = sqrt of the sum of all squares (MXL_NORM_L2) or the largest magnitude (MXL_NORM_MAX; NaN if there is one);
+ * fp64 sums in an order that the sizes decide; 0 for no elements.
+ * mxl_clip_grads: out = grad * min(1, max_norm / (*norm + 1e-6)), NaN for a norm of NaN; outs[i] may be grads[i] (same type): with a factor of 1 those
+ * are left untouched.  No byte that is written may belong to another tensor of the lists. */
+#define MXL_NORM_L2 0
+#define MXL_NORM_MAX 1
+int64_t mxl_grad_norm_workspace_bytes(int count);
+int mxl_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int count, int kind, float* norm, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+int mxl_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* dtypes, const int32_t* out_dtypes, int count,
+                   double max_norm, const float* norm, void* stream);
+
 /* ---- calibration (no counterpart in the reference: a measuring aid of this library's benchmark) ----
  *
  * mxl_calibrate_mfma launches a register-only loop of the GEMM kernels' scaled MFMA (32 x 32 x 64; a_fmt / b_fmt:

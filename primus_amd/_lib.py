@@ -36,6 +36,7 @@ GF_TILES = {None: 0, "64": 0x100, "64x128": 0x200, "128": 0x300, "256": 0x400}  
 GF_B_TRANSPOSED = 8                         # forward / dgrad: b's codes are those of the transposed matrices (row-wise weight copy)
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2           # element types of logits, rows and probabilities around the expert MLP
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+NORM_L2, NORM_MAX = 0, 1
 BF_B_KN, BF_ACCUM_F32, BF_TILE_128, BF_TILE_256 = 1, 2, 4, 8    # flags of the bf16 grouped GEMMs
 
 EXPORTS = (
@@ -105,6 +106,12 @@ EXPORTS = (
     "mxl_linear_bf16_dz",
     "mxl_linear_bf16_bwd_workspace_bytes",
     "mxl_linear_bf16_bwd",
+    "mxl_block_norm",
+    "mxl_block_norm_bwd_workspace_bytes",
+    "mxl_block_norm_bwd",
+    "mxl_grad_norm_workspace_bytes",
+    "mxl_grad_norm",
+    "mxl_clip_grads",
     "mxl_calibrate_mfma",
     "mxl_calibrate_mfma_flops",
     "mxl_calibrate_mfma_bf16",
@@ -299,6 +306,18 @@ def load() -> ctypes.CDLL:
         lib.mxl_linear_bf16_wgrad.argtypes = [vp, vp, i64, i64, i64, vp, u32, vp, i64, vp]
         lib.mxl_linear_bf16_bwd.restype = i32
         lib.mxl_linear_bf16_bwd.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, vp, u32, vp, i32, vp, i64, vp]
+        lib.mxl_block_norm.restype = i32
+        lib.mxl_block_norm.argtypes = [vp, vp, i64, i64, i32, i32, vp, f32, vp, i64, i64, i64, f32, vp, f32, vp, vp, vp, vp, vp]
+        lib.mxl_block_norm_bwd_workspace_bytes.restype = i64
+        lib.mxl_block_norm_bwd_workspace_bytes.argtypes = [i64, i64, i32, i32, i64, i64, i64]
+        lib.mxl_block_norm_bwd.restype = i32
+        lib.mxl_block_norm_bwd.argtypes = [vp, vp, vp, vp, i64, i64, i32, i32, vp, vp, vp, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.mxl_grad_norm_workspace_bytes.restype = i64
+        lib.mxl_grad_norm_workspace_bytes.argtypes = [i32]
+        lib.mxl_grad_norm.restype = i32
+        lib.mxl_grad_norm.argtypes = [vp, vp, vp, i32, i32, vp, vp, i64, vp]
+        lib.mxl_clip_grads.restype = i32
+        lib.mxl_clip_grads.argtypes = [vp, vp, vp, vp, vp, i32, ctypes.c_double, vp, vp]
         _lib = lib
     return _lib
 

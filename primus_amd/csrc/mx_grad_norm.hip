@@ -1,0 +1,362 @@
+// The global norm of many tensors, and their clipping by it:
+//
+//   norm = sqrt(sum over tensors and elements of g^2)   or   max |g|          g *= min(1, max_norm / (norm + 1e-6))
+//
+// The tensors' addresses and sizes travel in the kernels' arguments, GN_TENSORS a launch: nothing is copied to the device and a
+// captured launch keeps its own table.  A launch's tensors are cut into chunks, which its workgroups take in turn.
+//
+// Squares and sums are fp64: a float's square is exact there and neither overflows nor underflows, whatever the gradients' scale.
+// Every workgroup leaves one sum, one workgroup adds them up in their order: the result depends on the sizes alone, and no atomics.
+#include <math.h>
+#include <stdlib.h>
+
+#include "mx_lanes.h"
+
+namespace mxl {
+
+constexpr int GN_TENSORS = 160;             // a launch: 20 bytes each, the arguments stay below 4 KB
+constexpr int GN_THREADS = 256;
+constexpr int GN_LOADS = 8;                 // 16-byte loads a lane asks for at once
+constexpr int GN_CHUNK = GN_THREADS * GN_LOADS * 16;        // bytes
+constexpr int GN_BLOCKS = 2048;
+constexpr int GN_JOIN_THREADS = 1024;
+
+typedef uint32_t gn_u32x4 __attribute__((ext_vector_type(4)));
+
+struct NormTable {
+    const void* p[GN_TENSORS];
+    int64_t n[GN_TENSORS];                  // elements; the type code in the upper bits
+    uint32_t end[GN_TENSORS];               // chunks up to and with this tensor's
+    int count;
+};
+constexpr int GN_TYPE_SHIFT = 56;
+static_assert(sizeof(NormTable) <= 4032, "kernel arguments");
+
+__device__ __forceinline__ float half_lo(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(v & 0xFFFFu)); }
+__device__ __forceinline__ float half_hi(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16)); }
+
+// a sum of squares, or the largest magnitude's bits (those of a NaN are above those of every number)
+template <bool MAX> struct Stat;
+template <> struct Stat<false> {
+    double a = 0., b = 0.;
+    __device__ __forceinline__ void add(float x, float y) {
+        a = fma((double)x, (double)x, a);
+        b = fma((double)y, (double)y, b);
+    }
+    __device__ __forceinline__ void join(const Stat& o) { a += o.a, b += o.b; }
+};
+template <> struct Stat<true> {
+    uint32_t a = 0;
+    __device__ __forceinline__ void add(float x, float y) {
+        const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu, v = __float_as_uint(y) & 0x7FFFFFFFu, m = u > v ? u : v;
+        a = a > m ? a : m;
+    }
+};
+template <int DT, bool MAX> __device__ __forceinline__ void add_vec(Stat<MAX>& s, const gn_u32x4& v) {
+#pragma unroll
+    for (int i = 0; i < 4; i += DT == MXL_DT_F32 ? 2 : 1) {
+        if (DT == MXL_DT_F32) s.add(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        else if (DT == MXL_DT_BF16) s.add(bf16_lo(v[i]), bf16_hi(v[i]));
+        else s.add(half_lo(v[i]), half_hi(v[i]));
+    }
+}
+
+// Elements [lo, hi) of a tensor: up to where 16-byte pieces begin, the pieces, and the rest.
+template <int DT, bool MAX> __device__ __forceinline__ void chunk_stat(Stat<MAX>& s, const void* base, int64_t lo, int64_t hi) {
+    constexpr int SIZE = DT == MXL_DT_F32 ? 4 : 2;
+    const uintptr_t a = (uintptr_t)base + lo * SIZE, z = (uintptr_t)base + hi * SIZE;
+    const uintptr_t a16 = (a + 15) & ~(uintptr_t)15;
+    if (a16 >= z) {         // fewer than 16 bytes
+        const int n = (int)(hi - lo);
+        if ((int)threadIdx.x < n) s.add(load_dt(base, DT, lo + threadIdx.x), 0.f);
+        return;
+    }
+    const int head = (int)(a16 - a) / SIZE, vecs = (int)((z - a16) / 16);
+    const int tail = (int)(z - a16 - (uintptr_t)vecs * 16) / SIZE;
+    if ((int)threadIdx.x < head) s.add(load_dt(base, DT, lo + threadIdx.x), 0.f);
+    const gn_u32x4* v = (const gn_u32x4*)a16;
+    gn_u32x4 r[GN_LOADS];
+#pragma unroll
+    for (int u = 0; u < GN_LOADS; ++u) {
+        const int i = u * GN_THREADS + (int)threadIdx.x;
+        r[u] = gn_u32x4{0, 0, 0, 0};
+        if (i < vecs) r[u] = __builtin_nontemporal_load(v + i);
+    }
+#pragma unroll
+    for (int u = 0; u < GN_LOADS; ++u) add_vec<DT, MAX>(s, r[u]);
+    if ((int)threadIdx.x < tail) s.add(load_dt(base, DT, hi - tail + threadIdx.x), 0.f);
+}
+
+__device__ __forceinline__ double lanes_sum_f64(double v) {
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
+    return v;
+}
+template <int THREADS> __device__ __forceinline__ double block_stat(double v, bool max) {     // thread 0 gets it
+    __shared__ double part[THREADS / 64];
+    if (max) {
+        // (bits of a float as a double: whole numbers, in order)
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) v = fmax(v, __shfl_xor(v, m));
+    } else {
+        v = lanes_sum_f64(v);
+    }
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = part[0];
+    if (threadIdx.x == 0)
+        for (int i = 1; i < THREADS / 64; ++i) s = max ? fmax(s, part[i]) : s + part[i];
+    return s;
+}
+__device__ __forceinline__ float norm_of(double total, bool max) { return max ? __uint_as_float((uint32_t)total) : (float)sqrt(total); }
+
+// `out` set: the launch's only workgroup writes the norm itself.
+template <bool MAX> __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(NormTable t, double* partial, float* out) {
+    Stat<MAX> s;
+    const uint32_t chunks = t.end[t.count - 1];
+    int at = 0;
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        while (t.end[at] <= c) ++at;
+        const uint32_t first = at ? t.end[at - 1] : 0;
+        const int64_t packed = t.n[at], n = packed & (((int64_t)1 << GN_TYPE_SHIFT) - 1);
+        const int type = (int)(packed >> GN_TYPE_SHIFT);
+        const int64_t per = type == MXL_DT_F32 ? GN_CHUNK / 4 : GN_CHUNK / 2, lo = (int64_t)(c - first) * per, hi = lo + per < n ? lo + per : n;
+        if (type == MXL_DT_F32) chunk_stat<MXL_DT_F32, MAX>(s, t.p[at], lo, hi);
+        else if (type == MXL_DT_BF16) chunk_stat<MXL_DT_BF16, MAX>(s, t.p[at], lo, hi);
+        else chunk_stat<MXL_DT_F16, MAX>(s, t.p[at], lo, hi);
+    }
+    double v;
+    if constexpr (MAX) v = (double)s.a;
+    else v = s.a + s.b;
+    v = block_stat<GN_THREADS>(v, MAX);
+    if (threadIdx.x == 0) {
+        if (out) *out = norm_of(v, MAX);
+        else partial[blockIdx.x] = v;
+    }
+}
+
+__global__ __launch_bounds__(GN_JOIN_THREADS) void grad_norm_join_kernel(const double* partial, int64_t n, int max, float* out) {
+    double v = 0.;
+    for (int64_t i = threadIdx.x; i < n; i += GN_JOIN_THREADS) v = max ? fmax(v, partial[i]) : v + partial[i];
+    v = block_stat<GN_JOIN_THREADS>(v, max != 0);
+    if (threadIdx.x == 0) *out = norm_of(v, max != 0);
+}
+
+// ---- clipping ----
+constexpr int GC_TENSORS = 128;
+struct ClipTable {
+    const void* p[GC_TENSORS];
+    void* out[GC_TENSORS];
+    int64_t n[GC_TENSORS];                  // elements; the type codes, out's above the gradient's
+    uint32_t end[GC_TENSORS];
+    int count;
+};
+static_assert(sizeof(ClipTable) <= 4032, "kernel arguments");
+constexpr int GC_PER = GN_THREADS * 32;     // elements of a chunk
+
+// The product is rounded once: a float's is made in fp64; of the 16-bit types it is exact but for the coefficient's 24 bits.
+template <int DT> __device__ __forceinline__ float scaled(float g, double c, float cf) { return DT == MXL_DT_F32 ? (float)((double)g * c) : g * cf; }
+
+template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void* src, void* dst, int64_t lo, int64_t hi, double c, float cf) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+    constexpr int IN = DT == MXL_DT_F32 ? 2 : 1, OUT = DO == MXL_DT_F32 ? 2 : 1;    // 16-byte pieces of eight elements
+    constexpr int UNROLL = 4;
+    const uint8_t* s = (const uint8_t*)src + lo * (IN * 2);
+    uint8_t* d = (uint8_t*)dst + lo * (OUT * 2);
+    const int n = (int)(hi - lo), eights = n / 8;
+#pragma unroll
+    for (int u0 = 0; u0 < GC_PER / 8 / GN_THREADS; u0 += UNROLL) {
+        uint32_t r[UNROLL][4 * IN];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int i = (u0 + u) * GN_THREADS + (int)threadIdx.x;
+            if (i < eights) {
+#pragma unroll
+                for (int q = 0; q < IN; ++q) {
+                    const u32x4 v = __builtin_nontemporal_load((const u32x4*)(s + (int64_t)i * 16 * IN) + q);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r[u][4 * q + j] = v[j];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int i = (u0 + u) * GN_THREADS + (int)threadIdx.x;
+            if (i >= eights) continue;
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (DT == MXL_DT_F32) f[j] = __uint_as_float(r[u][j % (4 * IN)]);
+                else if (DT == MXL_DT_BF16) f[j] = j & 1 ? bf16_hi(r[u][j / 2]) : bf16_lo(r[u][j / 2]);
+                else f[j] = j & 1 ? half_hi(r[u][j / 2]) : half_lo(r[u][j / 2]);
+                f[j] = scaled<DT>(f[j], c, cf);
+            }
+            uint32_t o[4 * OUT];
+            if (DO == MXL_DT_F32) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j % (4 * OUT)] = __float_as_uint(f[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (DO == MXL_DT_BF16) o[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
+                    else o[j] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j + 1]) << 16);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < OUT; ++q) {
+                const u32x4 v = {o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]};
+                __builtin_nontemporal_store(v, (u32x4*)(d + (int64_t)i * 16 * OUT) + q);
+            }
+        }
+    }
+    const int rest = n - eights * 8;
+    if ((int)threadIdx.x < rest) {
+        const int64_t i = hi - rest + threadIdx.x;
+        store_dt(dst, DO, i, scaled<DT>(load_dt(src, DT, i), c, cf));
+    }
+}
+
+__global__ __launch_bounds__(GN_THREADS) void clip_kernel(ClipTable t, const float* norm, double max_norm) {
+    const double raw = max_norm / ((double)*norm + 1e-6);
+    const bool within = raw >= 1.;          // (a NaN is not)
+    const double c = within ? 1. : raw;
+    const float cf = (float)c;
+    const uint32_t chunks = t.end[t.count - 1];
+    int at = 0;
+    for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
+        while (t.end[at] <= i) ++at;
+        const void* src = t.p[at];
+        void* dst = t.out[at];
+        const int64_t packed = t.n[at], n = packed & (((int64_t)1 << GN_TYPE_SHIFT) - 1);
+        const int types = (int)(packed >> GN_TYPE_SHIFT), in = types & 3, out = types >> 2;
+        if (within && src == dst) continue;
+        const uint32_t first = at ? t.end[at - 1] : 0;
+        const int64_t lo = (int64_t)(i - first) * GC_PER, hi = lo + GC_PER < n ? lo + GC_PER : n;
+#define MXL_CLIP(DT, DO) clip_chunk<DT, DO>(src, dst, lo, hi, c, cf)
+        switch (in * 4 + out) {
+            case MXL_DT_F32 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_F32, MXL_DT_F32); break;
+            case MXL_DT_F32 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_F32, MXL_DT_BF16); break;
+            case MXL_DT_F32 * 4 + MXL_DT_F16: MXL_CLIP(MXL_DT_F32, MXL_DT_F16); break;
+            case MXL_DT_BF16 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_BF16, MXL_DT_F32); break;
+            case MXL_DT_BF16 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_BF16, MXL_DT_BF16); break;
+            case MXL_DT_BF16 * 4 + MXL_DT_F16: MXL_CLIP(MXL_DT_BF16, MXL_DT_F16); break;
+            case MXL_DT_F16 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_F16, MXL_DT_F32); break;
+            case MXL_DT_F16 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_F16, MXL_DT_BF16); break;
+            default: MXL_CLIP(MXL_DT_F16, MXL_DT_F16); break;
+        }
+#undef MXL_CLIP
+    }
+}
+
+static bool gn_list_ok(const void* const* p, const int64_t* n, const int32_t* dtypes, int count) {
+    if (count < 0 || (count > 0 && (!p || !n || !dtypes))) return false;
+    for (int i = 0; i < count; ++i)
+        if (n[i] < 0 || n[i] >= ((int64_t)1 << 40) || dtypes[i] < MXL_DT_F32 || dtypes[i] > MXL_DT_F16 || (n[i] > 0 && !p[i])) return false;
+    return true;
+}
+static int gn_size(int dtype) { return dtype == MXL_DT_F32 ? 4 : 2; }
+
+struct Span {
+    uintptr_t lo, hi;
+    int written;
+};
+static int span_order(const void* a, const void* b) {
+    const Span *x = (const Span*)a, *y = (const Span*)b;
+    return x->lo < y->lo ? -1 : x->lo > y->lo;
+}
+// Whether what is written shares no byte with anything else that is read or written (a gradient that is its own output is one span).
+static int clip_spans_apart(const void* const* p, void* const* out, const int64_t* n, const int32_t* dtypes, const int32_t* out_dtypes, int count) {
+    Span* s = (Span*)malloc((size_t)(2 * (int64_t)count + 1) * sizeof(Span));
+    if (!s) return 0;
+    int64_t m = 0;
+    for (int i = 0; i < count; ++i) {
+        if (n[i] == 0) continue;
+        const bool same = p[i] == out[i] && dtypes[i] == out_dtypes[i];
+        if (!same) s[m++] = {(uintptr_t)p[i], (uintptr_t)p[i] + (uintptr_t)n[i] * gn_size(dtypes[i]), 0};
+        s[m++] = {(uintptr_t)out[i], (uintptr_t)out[i] + (uintptr_t)n[i] * gn_size(out_dtypes[i]), 1};
+    }
+    qsort(s, (size_t)m, sizeof(Span), span_order);
+    uintptr_t read_end = 0, write_end = 0;
+    int apart = 1;
+    for (int64_t i = 0; i < m && apart; ++i) {
+        if (s[i].lo < write_end || (s[i].written && s[i].lo < read_end)) apart = 0;
+        uintptr_t& end = s[i].written ? write_end : read_end;
+        if (s[i].hi > end) end = s[i].hi;
+    }
+    free(s);
+    return apart;
+}
+
+}  // namespace mxl
+
+using namespace mxl;
+
+extern "C" int64_t mxl_grad_norm_workspace_bytes(int count) {
+    if (count < 0) return -1;
+    return ((int64_t)count + GN_TENSORS - 1) / GN_TENSORS * GN_BLOCKS * 8;
+}
+
+extern "C" int mxl_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int count, int kind, float* norm, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+    if (!gn_list_ok(grads, sizes, dtypes, count) || (kind != MXL_NORM_L2 && kind != MXL_NORM_MAX) || !norm) return MXL_EINVAL;
+    if (workspace_bytes < mxl_grad_norm_workspace_bytes(count) || (count > 0 && (!workspace || ((uintptr_t)workspace & 7) != 0))) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    hipStream_t st = (hipStream_t)stream;
+    const bool max = kind == MXL_NORM_MAX;
+    double* partial = (double*)workspace;
+    int64_t partials = 0;
+    int i = 0;
+    while (i < count) {
+        NormTable t;
+        t.count = 0;
+        uint32_t chunks = 0;
+        for (; i < count && t.count < GN_TENSORS; ++i) {
+            if (sizes[i] == 0) continue;
+            const int64_t per = GN_CHUNK / gn_size(dtypes[i]), more = (sizes[i] + per - 1) / per;
+            if (more + chunks > 0x7FFFFFFF) break;
+            chunks += (uint32_t)more;
+            t.p[t.count] = grads[i];
+            t.n[t.count] = sizes[i] | ((int64_t)dtypes[i] << GN_TYPE_SHIFT);
+            t.end[t.count++] = chunks;
+        }
+        if (t.count == 0) break;
+        const int blocks = (int)(chunks < (uint32_t)GN_BLOCKS ? chunks : (uint32_t)GN_BLOCKS);
+        float* out = i == count && partials == 0 && blocks == 1 ? norm : nullptr;
+        if (max) hipLaunchKernelGGL(grad_norm_kernel<true>, dim3((unsigned)blocks), dim3(GN_THREADS), 0, st, t, partial + partials, out);
+        else hipLaunchKernelGGL(grad_norm_kernel<false>, dim3((unsigned)blocks), dim3(GN_THREADS), 0, st, t, partial + partials, out);
+        if (hipGetLastError() != hipSuccess) return MXL_ELAUNCH;
+        if (out) return MXL_OK;
+        partials += blocks;
+    }
+    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(GN_JOIN_THREADS), 0, st, partial, partials, (int)max, norm);
+    return hipGetLastError() == hipSuccess ? MXL_OK : MXL_ELAUNCH;
+}
+
+extern "C" int mxl_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* dtypes, const int32_t* out_dtypes,
+                              int count, double max_norm, const float* norm, void* stream) {
+    if (!gn_list_ok(grads, sizes, dtypes, count) || !gn_list_ok(outs, sizes, out_dtypes, count) || !norm || !(max_norm >= 0.)) return MXL_EINVAL;
+    if (!clip_spans_apart(grads, outs, sizes, dtypes, out_dtypes, count)) return MXL_EINVAL;
+    if (!device_is_gfx950()) return MXL_ENODEV;
+    hipStream_t st = (hipStream_t)stream;
+    int i = 0;
+    while (i < count) {
+        ClipTable t;
+        t.count = 0;
+        uint32_t chunks = 0;
+        for (; i < count && t.count < GC_TENSORS; ++i) {
+            if (sizes[i] == 0) continue;
+            const int64_t more = (sizes[i] + GC_PER - 1) / GC_PER;
+            if (more + chunks > 0x7FFFFFFF) break;
+            chunks += (uint32_t)more;
+            t.p[t.count] = grads[i];
+            t.out[t.count] = outs[i];
+            t.n[t.count] = sizes[i] | ((int64_t)(dtypes[i] | (out_dtypes[i] << 2)) << GN_TYPE_SHIFT);
+            t.end[t.count++] = chunks;
+        }
+        if (t.count == 0) break;
+        const int blocks = (int)(chunks < (uint32_t)GN_BLOCKS ? chunks : (uint32_t)GN_BLOCKS);
+        hipLaunchKernelGGL(clip_kernel, dim3((unsigned)blocks), dim3(GN_THREADS), 0, st, t, norm, max_norm);
+        if (hipGetLastError() != hipSuccess) return MXL_ELAUNCH;
+    }
+    return MXL_OK;
+}

@@ -10,8 +10,10 @@ stream, allocates only its outputs and never reads device data from the host.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -1466,6 +1468,194 @@ def combine_rows_bwd_impl(dy, rows, row_of, entry_of, probs, need_rows: bool = T
                                               tokens, topk, _ptr(probs), _float_type(probs, "probs"), _ptr(drows), _ptr(dprobs), _stream())
     _lib.check(rc, "mxl_combine_rows_bwd")
     return drows, dprobs
+
+
+# --------------------------------------------------------------------------
+# norms where blocks meet, the global gradient norm and clipping
+# --------------------------------------------------------------------------
+@functools.lru_cache(maxsize=1024)
+def _gate_rows(shape, gate_shape) -> Tuple[int, int, int]:
+    """``(div, mod, cols)``: row r of ``shape`` has row ``r // div % mod`` of a gate ``[mod, cols]``."""
+    k, lead = shape[-1], shape[:-1]
+    if len(gate_shape) <= len(shape):
+        full = (1,) * (len(shape) - len(gate_shape)) + tuple(gate_shape)
+        kept = [d for d, n in enumerate(full[:-1]) if n != 1]
+        if full[-1] in (1, k) and all(full[d] == lead[d] for d in kept):
+            if not kept:
+                return max(1, math.prod(lead)), 1, full[-1]
+            first, last = kept[0], kept[-1]
+            if all(full[d] == lead[d] for d in range(first, last + 1)):
+                return math.prod(lead[last + 1:]), math.prod(lead[first:last + 1]), full[-1]
+    raise ValueError(f"gate {list(gate_shape)} must broadcast to {list(shape)}, over leading or trailing dimensions of its rows, the last one, or none")
+
+
+def _block_norm_args(x, residual, weight, post_weight, gate):
+    """``(rows, k, type codes of x and residual, the gate's rows)``."""
+    dtype = _DT.get(x.dtype)
+    if dtype is None:
+        _float_type(x, "x")
+    if x.dim() < 1 or residual.shape != x.shape:
+        raise ValueError("x [..., hidden] and residual must have one shape")
+    if residual.dtype != x.dtype and residual.dtype != torch.float32:
+        raise ValueError("residual must have the type of x or be float32")
+    k = x.shape[-1]
+    if not 1 <= k <= RMSNORM_MAX_K:
+        raise ValueError(f"the normalised dim ({k}) must be in [1, {RMSNORM_MAX_K}]")
+    dev = x.device
+    if not x.is_cuda or residual.device != dev:
+        _require_cuda(x, residual)
+        _same_device(dev, residual=residual)
+    for name, t in (("weight", weight), ("post_weight", post_weight)):
+        if t is not None:
+            if t.dtype != x.dtype or t.shape != (k,):
+                raise ValueError(f"{name} must be a vector of the normalised length, of the type of x")
+            if t.device != dev:
+                _same_device(dev, **{name: t})
+    how = (1, 1, 0)
+    if gate is not None:
+        if gate.dtype != x.dtype:
+            raise ValueError("gate must have the type of x")
+        if gate.device != dev:
+            _same_device(dev, gate=gate)
+        how = _gate_rows(x.shape, gate.shape)
+    return x.numel() // k, k, dtype, _DT[residual.dtype], how
+
+
+def block_norm_impl(x, residual, weight, eps: float, post_weight, post_eps: float, gate, scale: float, want_rstd: bool = True):
+    """``(y, h, rstd, post_rstd)``: ``h = residual + scale * gate * n``, ``n`` = ``x``, normalised with ``post_weight`` if there is one, and
+    ``y`` = ``h`` normalised with ``weight`` (None without); see ``ops.add_rmsnorm``."""
+    rows, k, dtype, stream_dtype, (div, mod, cols) = _block_norm_args(x, residual, weight, post_weight, gate)
+    if rows > 0x7FFFFFFF:
+        raise ValueError("at most 2^31 - 1 rows")
+    if weight is None and post_weight is None:
+        raise ValueError("a norm needs its weight")
+    if not (eps >= 0 and post_eps >= 0):
+        raise ValueError("eps must not be negative")
+    for t in (x, residual, weight, post_weight, gate):
+        if t is not None and not t.is_contiguous():
+            raise ValueError("operands must be contiguous")
+    dev = x.device
+    lib = _lib.load()
+    with _on(dev), _hooked("block_norm", rows=rows, k=k):
+        h = torch.empty_like(residual)
+        y = rstd = post_rstd = None
+        if weight is not None:
+            y = torch.empty_like(x)
+            if want_rstd:
+                rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+        if post_weight is not None and want_rstd:
+            post_rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+        rc = lib.mxl_block_norm(x.data_ptr(), residual.data_ptr(), rows, k, dtype, stream_dtype, None if post_weight is None else post_weight.data_ptr(), post_eps,
+                                None if gate is None else gate.data_ptr(), div, mod, cols, scale, None if weight is None else weight.data_ptr(), eps,
+                                None if y is None else y.data_ptr(), h.data_ptr(), None if post_rstd is None else post_rstd.data_ptr(),
+                                None if rstd is None else rstd.data_ptr(), _stream())
+    if rc:
+        _lib.check(rc, "mxl_block_norm")
+    return y, h, rstd, post_rstd
+
+
+def block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate, scale: float, need_x: bool = True, need_residual: bool = True,
+                        need_weight: bool = True, need_post_weight: bool = True, need_gate: bool = True):
+    """``(dx, dresidual, dweight, dpost_weight, dgate)`` of ``block_norm_impl``, given the gradients of ``y`` and ``h`` (None: zero).  ``x`` may be None where
+    it is not needed: without ``post_weight``, and with no gradient of the gate."""
+    like = x if x is not None else dy
+    rows_of = h if h is not None else dh
+    rows, k, dtype, stream_dtype, (div, mod, cols) = _block_norm_args(like, rows_of, weight, post_weight, gate)
+    dev = like.device
+    need_weight, need_post_weight, need_gate = need_weight and weight is not None, need_post_weight and post_weight is not None, need_gate and gate is not None
+    if (weight is not None and (dy is None or h is None or rstd is None)) or ((post_weight is not None or need_gate) and x is None):
+        raise ValueError("the gradient needs what the forward kept")
+    for name, t, want in (("dy", dy, like.dtype), ("dh", dh, rows_of.dtype), ("x", x, like.dtype), ("h", h, rows_of.dtype)):
+        if t is not None and (t.dtype != want or t.shape != like.shape or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous, of the forward's type, shape and device")
+    for t in (weight, rstd, post_weight, post_rstd, gate):
+        if t is not None and (not t.is_contiguous() or t.device != dev):
+            raise ValueError("operands must be contiguous, on one device")
+    for t in (rstd, post_rstd):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != rows):
+            raise ValueError("rstd must be float32 [rows]")
+    lib = _lib.load()
+    # one tensor where both gradients are the same
+    same = need_x and need_residual and weight is not None and post_weight is None and gate is None and scale == 1.0 and dtype == stream_dtype
+    with _on(dev), _hooked("block_norm_bwd", rows=rows, k=k):
+        dx = torch.empty_like(like) if need_x and not same else None
+        dres = torch.empty_like(rows_of) if need_residual else None
+        dw = torch.empty_like(weight) if need_weight else None
+        dpw = torch.empty_like(post_weight) if need_post_weight else None
+        dgate = None
+        if need_gate:
+            dgate = torch.empty_like(gate) if rows else torch.zeros_like(gate)
+        ws, nbytes = _workspace(dev, "mxl_block_norm_bwd_workspace_bytes", rows, k, need_weight, need_post_weight, div, mod, cols if need_gate else 0)
+        rc = lib.mxl_block_norm_bwd(None if dy is None else dy.data_ptr(), None if dh is None else dh.data_ptr(), None if x is None else x.data_ptr(),
+                                    None if h is None else h.data_ptr(), rows, k, dtype, stream_dtype, None if post_weight is None else post_weight.data_ptr(),
+                                    None if post_rstd is None else post_rstd.data_ptr(), None if gate is None else gate.data_ptr(), div, mod, cols, scale,
+                                    None if weight is None else weight.data_ptr(), None if rstd is None else rstd.data_ptr(), None if dx is None else dx.data_ptr(),
+                                    None if dres is None else dres.data_ptr(), None if dw is None else dw.data_ptr(), None if dpw is None else dpw.data_ptr(),
+                                    None if dgate is None else dgate.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream())
+    if rc:
+        _lib.check(rc, "mxl_block_norm_bwd")
+    return dres if same else dx, dres, dw, dpw, dgate
+
+
+_NORM_KINDS = {2.0: _lib.NORM_L2, math.inf: _lib.NORM_MAX}
+
+
+def _tensor_list(tensors, what: str):
+    """``(device, addresses, sizes, type codes)`` of tensors on one GPU; the last three as arrays of the C ABI's types."""
+    try:
+        types = array.array("i", [_DT[t.dtype] for t in tensors])
+    except KeyError:
+        for t in tensors:
+            _float_type(t, what)
+        raise
+    devices = {t.device for t in tensors}
+    dev = devices.pop()
+    if devices or dev.type != "cuda":
+        for t in tensors:
+            if not t.is_cuda:
+                _require_cuda(t)
+        raise ValueError(f"{what} must live on one device")
+    if not all([t.is_contiguous() for t in tensors]):
+        raise ValueError(f"{what} must be contiguous")
+    return dev, array.array("Q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]), types
+
+
+def grad_norm_impl(tensors, kind: float = 2.0) -> torch.Tensor:
+    """Norm over all elements of contiguous ``tensors`` (at least one) as a float32 scalar on their device; see ``ops.grad_norm``."""
+    code = _NORM_KINDS.get(float(kind))
+    if code is None:
+        raise ValueError(f"norm_type must be 2 or inf, got {kind!r}")
+    dev, ptrs, sizes, types = _tensor_list(tensors, "gradients")
+    lib = _lib.load()
+    with _on(dev), _hooked("grad_norm", tensors=len(types)):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws, nbytes = _workspace(dev, "mxl_grad_norm_workspace_bytes", len(types))
+        rc = lib.mxl_grad_norm(ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(types), code, norm.data_ptr(), ws.data_ptr(), nbytes, _stream())
+    if rc:
+        _lib.check(rc, "mxl_grad_norm")
+    return norm
+
+
+def clip_grads_impl(tensors, outs, max_norm: float, norm: torch.Tensor) -> None:
+    """``outs[i] = tensors[i] * min(1, max_norm / (norm + 1e-6))`` for contiguous tensors; ``outs`` may be ``tensors``."""
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm!r}")
+    dev, ptrs, sizes, types = _tensor_list(tensors, "gradients")
+    out_ptrs, out_types = ptrs, types
+    if outs is not tensors:
+        out_dev, out_ptrs, out_sizes, out_types = _tensor_list(outs, "out")
+        if out_sizes != sizes or out_dev != dev:
+            raise ValueError("out must hold a tensor of the same size, on the same device, for every gradient")
+    if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != dev:
+        raise ValueError("norm must be a float32 scalar on the device of the gradients")
+    lib = _lib.load()
+    with _on(dev), _hooked("clip_grads", tensors=len(types)):
+        rc = lib.mxl_clip_grads(ptrs.buffer_info()[0], out_ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], out_types.buffer_info()[0],
+                                len(types), max_norm, norm.data_ptr(), _stream())
+    if rc == -1:
+        raise ValueError("a tensor that is written must not overlap another one of the lists (a gradient may be its own output)")
+    if rc:
+        _lib.check(rc, "mxl_clip_grads")
 
 
 # --------------------------------------------------------------------------

@@ -41,7 +41,8 @@ __all__ = ["gemm", "grouped_gemm", "gemm_fp8", "gemm_fp4", "grouped_gemm_fp8", "
            "set_dgrad_reads_rowwise_weight",
            "swiglu_with_probs", "geglu_with_probs", "tokens_per_expert_to_mask", "glu_grouped_gemm_fp8",
            "glu_grouped_gemm_fp4", "manual_sr_seed", "set_kchunk_layout", "rmsnorm", "rmsnorm_gemm_fp8", "rmsnorm_gemm_fp4", "pad_groups", "unpad_groups",
-           "topk_routing", "permute_tokens", "unpermute_tokens", "TokenPermutation", "gemm_bias_act"]
+           "topk_routing", "permute_tokens", "unpermute_tokens", "TokenPermutation", "gemm_bias_act", "add_rmsnorm", "rmsnorm_add",
+           "grad_norm", "clip_grads"]
 
 # dgrad and wgrad of one linear are independent once dY is quantised, so wgrad may run on a second stream, where its
 # workgroups move in as dgrad's last, partial round of tiles drains.  The default is one stream: _overlaps() names the
@@ -855,6 +856,130 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.T
     if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise ValueError("rmsnorm expects bfloat16 input and weight")
     return _RMSNormFunction.apply(x, weight, float(eps))
+
+
+class _BlockNorm(torch.autograd.Function):
+    """``(y, h)`` of ``add_rmsnorm``, or ``h`` alone (``weight`` None)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, post_weight, gate, eps, post_eps, scale, need_grad=True):
+        y, h, rstd, post_rstd = K.block_norm_impl(x, residual, weight, eps, post_weight, post_eps, gate, scale, need_grad)
+        if need_grad:
+            keep_x = post_weight is not None or (gate is not None and ctx.needs_input_grad[4])
+            ctx.save_for_backward(x if keep_x else None, h if weight is not None else None, weight, rstd, post_weight, post_rstd, gate)
+            ctx.scale, ctx.shape = scale, (x.shape, x.dtype, h.dtype, x.device)
+            ctx.set_materialize_grads(False)
+        return h if weight is None else (y, h)
+
+    @staticmethod
+    @_differentiable_once
+    def backward(ctx, *grads):
+        x, h, weight, rstd, post_weight, post_rstd, gate = ctx.saved_tensors
+        shape, dtype, stream_dtype, dev = ctx.shape
+        dy, dh = grads if weight is not None else (None, grads[0])
+        if dy is None and dh is None:
+            return (None,) * 9
+        if weight is not None:
+            dy = torch.zeros(shape, dtype=dtype, device=dev) if dy is None else dy.to(dtype).contiguous()
+        if dh is not None:
+            dh = dh.to(stream_dtype).contiguous()
+        need_x, need_residual, need_weight, need_post, need_gate = ctx.needs_input_grad[:5]
+        if weight is None and not (need_x or need_post or need_gate):
+            return None, dh, None, None, None, None, None, None, None
+        dx, dres, dw, dpw, dgate = K.block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate, ctx.scale, need_x,
+                                                         need_residual and weight is not None, need_weight, need_post, need_gate)
+        return dx, dres if weight is not None else dh if need_residual else None, dw, dpw, dgate, None, None, None, None
+
+
+def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, post_weight: Optional[torch.Tensor] = None,
+                post_eps: Optional[float] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0):
+    """``(y, h)``: the norm before a block together with the residual add in front of it, ``x`` being the previous block's output:
+
+        n = x, or x / sqrt(mean(x^2, -1) + post_eps) * post_weight: the norm after that block
+        h = residual + scale * gate * n
+        y = h / sqrt(mean(h^2, -1) + eps) * weight
+
+    over the last dim, up to 16384 of any size, in fp32 with one rounding of ``h`` and one of ``y`` (the norm of the sums before theirs).  ``x [..., hidden]``,
+    the weights ``[hidden]`` and ``gate`` are of one type, bfloat16, float16 or float32; ``residual`` has it too or is float32 (a residual stream kept
+    in fp32), and ``h`` is of its type.  ``gate`` broadcasts to ``x``: a factor a channel ``[hidden]``, a sequence ``[batch, 1, hidden]`` (with ``[batch, seq,
+    hidden]``) or ``[1, batch, hidden]`` (with ``[seq, batch, hidden]``), a token ``[..., 1]``, or an element; other patterns raise.
+    ``post_eps`` None: ``eps``.  Differentiable in the five tensors; sums over rows are taken in fp32 in a fixed order, and the
+    backward normalises ``h`` as it was rounded."""
+    return _block_norm(x, residual, weight, post_weight, gate, eps, eps if post_eps is None else post_eps, scale)
+
+
+def rmsnorm_add(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, gate: Optional[torch.Tensor] = None,
+                scale: float = 1.0) -> torch.Tensor:
+    """``residual + scale * gate * (x / sqrt(mean(x^2, -1) + eps) * weight)``: the norm after a block, its gate, its residual scale and the add, in
+    fp32 with one rounding; types, sizes and ``gate`` as in ``add_rmsnorm`` (which does this and the next block's norm in one).
+    Differentiable in the four tensors."""
+    return _block_norm(x, residual, None, weight, gate, 0.0, eps, scale)
+
+
+def _block_norm(x, residual, weight, post_weight, gate, eps, post_eps, scale):
+    return _apply(_BlockNorm, x.contiguous(), residual.contiguous(), None if weight is None else weight.contiguous(),
+                  None if post_weight is None else post_weight.contiguous(), None if gate is None else gate.contiguous(), float(eps), float(post_eps),
+                  float(scale))
+
+
+def _grad_list(tensors, what: str):
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+            raise ValueError(f"{what} must be dense tensors")
+    return tensors
+
+
+@torch.no_grad()
+def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all elements of ``grads`` (tensors on one GPU, of any shapes and sizes, bfloat16, float16 and float32 mixed) as a float32 scalar on
+    the device: ``sqrt(sum g^2)``, or ``max |g|`` for ``norm_type`` inf (NaN if there is one).  Squares are summed in fp64 in an order that
+    depends on the sizes alone; they neither overflow nor underflow.  Nothing is read back to the host.  0 for no tensors or no elements."""
+    grads = _grad_list(grads, "gradients")
+    if not grads:
+        if float(norm_type) not in K._NORM_KINDS:
+            raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
+        return torch.zeros((), dtype=torch.float32, device="cuda")
+    return K.grad_norm_impl([g.contiguous() for g in grads], norm_type)
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = None, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``: ``grad_norm(grads, norm_type)`` unless it is given (the norm over all ranks,
+    say), a float32 scalar on the gradients' device, or a number.  In place, or into the tensors of ``out`` (one of the same shape for every gradient, of any of
+    the three types: the optimizer's float32 gradients of bfloat16 ones).  The factor is taken on the device and nothing is read back: within the bound, gradients
+    in place are left untouched.  A norm of NaN makes every element NaN, an infinite one leaves zeros of what is finite.  No tensor that is written may
+    overlap another one."""
+    grads = _grad_list(grads, "gradients")
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm!r}")
+    targets = grads
+    if out is not None:
+        targets = _grad_list(out, "out")
+        if len(targets) != len(grads) or any(o.shape != g.shape for o, g in zip(targets, grads)):
+            raise ValueError("out must hold a tensor of the same shape for every gradient")
+    dense = [g.contiguous() for g in grads]
+    # the kernels write tensors without gaps: others get a copy of theirs
+    if out is None:
+        written = dense
+    else:
+        written = [o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device) for o in targets]
+    gaps = [t for t in targets if not t.is_contiguous()]
+    if len({t.data_ptr() for t in gaps}) < len(gaps) or any(st == 0 and n > 1 for t in gaps for st, n in zip(t.stride(), t.shape)):
+        raise ValueError("a tensor that is written must not overlap itself or another one")
+    if norm is None:
+        norm = grad_norm(dense, norm_type)
+    elif not isinstance(norm, torch.Tensor):
+        norm = torch.full((), float(norm), dtype=torch.float32, device=grads[0].device if grads else "cuda")
+    if not grads:
+        return norm
+    K.clip_grads_impl(dense, written, max_norm, norm)
+    for t, w in zip(targets, written):
+        if w is not t:
+            t.copy_(w)
+    torch.autograd.graph.increment_version(targets)
+    return norm
 
 
 def rmsnorm_gemm_fp8(x, norm_weight, eps: float, b, trans_a: bool = False, trans_b: bool = True,

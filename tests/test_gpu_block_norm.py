@@ -1,0 +1,450 @@
+"""Norms where blocks meet (``ops.add_rmsnorm``, ``ops.rmsnorm_add``) on the GPU against the formulas in float64.
+
+Bars.  u, us: half a step of the type of x and of the residual stream (2^-8 bf16, 2^-11 fp16, 2^-24 fp32), e = 2^-24.  A value is rounded once: u * |v|.
+fp32 work before that: a row's sum in lanes and trees of at most 64 additions, and under 16 operations an element, is 64 e of the magnitudes that are
+added.  The backward normalises h as it was rounded: us of hh, once in hh itself and once through mean(g hh).  Sums over rows are serial in the worst
+case: rows * e more."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+EPS, POST_EPS = 1e-5, 1e-3
+
+
+def _u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _gate_shape(kind, lead, k):
+    return {"": None, "column": (k,), "element": (1,), "scalar": (), "first": (lead[0],) + (1,) * (len(lead) - 1) + (k,), "last": (1,) * (len(lead) - 1) + (lead[-1], k),
+            "token": lead + (1,), "full": lead + (k,), "first_scalar": (lead[0],) + (1,) * len(lead)}[kind]
+
+
+def _inputs(lead, k, dtype, stream, post, gate, seed=0, device="cpu"):
+    g = torch.Generator().manual_seed(seed + 17 * k + sum(lead))
+    n = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    v = {"x": n(*lead, k) * torch.logspace(-1, 1, k)[torch.randperm(k, generator=g)], "residual": 2 * n(*lead, k), "weight": 1 + 0.2 * n(k),
+         "post_weight": 1 + 0.2 * n(k) if post else None, "gate": None if not gate else 0.5 + 0.5 * n(*_gate_shape(gate, lead, k))}
+    v = {name: None if t is None else t.to(stream if name == "residual" else dtype).to(device) for name, t in v.items()}
+    return v, n(*lead, k).to(dtype).to(device), n(*lead, k).to(stream).to(device)
+
+
+def _to(t, shape):
+    """Summed over what ``shape`` broadcasts over."""
+    dims = [d for d in range(t.dim()) if d < t.dim() - len(shape) or shape[d - t.dim() + len(shape)] == 1 != t.shape[d]]
+    return (t.sum(dims) if dims else t).reshape(shape)
+
+
+def _reference(v, dy, dh, scale, dtype, stream, pre=True, eps=EPS, post_eps=POST_EPS):
+    """``{name: (value, bound)}`` in float64 on the CPU."""
+    d = lambda t: None if t is None else t.detach().cpu().double()  # noqa: E731
+    x, res, w, wp, gate = (d(v[n]) for n in ("x", "residual", "weight", "post_weight", "gate"))
+    dy, dh = d(dy), d(dh)
+    u, us = _u(dtype), _u(stream)
+    mean = lambda t: t.mean(-1, keepdim=True)  # noqa: E731
+    rows = x.numel() // x.shape[-1]
+    rp = 1 / torch.sqrt(mean(x * x) + post_eps)
+    xh = x * rp
+    n = xh * wp if wp is not None else x
+    f = scale * gate if gate is not None else torch.tensor(float(scale), dtype=torch.float64)
+    h = res + f * n
+    mag_h = res.abs() + (f * n).abs()
+    out = {"h": (h, us * h.abs() + 64 * E * mag_h)}
+    t, big = (torch.zeros_like(h), torch.zeros_like(h)) if dh is None else (dh, dh.abs())
+    err = torch.zeros_like(h)
+    if pre:
+        r = 1 / torch.sqrt(mean(h * h) + eps)
+        hh = h * r
+        out["y"] = (hh * w, u * (hh * w).abs() + 64 * E * (mag_h * r * w.abs() + (hh * w).abs()))
+        if dy is not None:
+            g = dy * w
+            c1, c1_mag = mean(g * hh), mean((g * hh).abs())
+            t = t + r * (g - hh * c1)
+            big = big + r * (g.abs() + hh.abs() * c1_mag)
+            err = err + 2 * us * r * hh.abs() * c1_mag
+            every = (dy * hh).abs().reshape(rows, -1).sum(0)
+            dw = (dy * hh).reshape(rows, -1).sum(0)
+            out["weight"] = (dw, u * dw.abs() + (us + (64 + rows) * E) * every)
+    err = err + 64 * E * big
+    out["residual"] = (t, us * t.abs() + err)
+    if wp is None:
+        dx, dx_err = f * t, f.abs() * err
+    else:
+        q, a = f * wp * xh, (f * wp * xh).abs()
+        c2 = mean(q * t)
+        dx = rp * (f * t * wp - xh * c2)
+        dx_err = rp * ((f * wp).abs() * err + xh.abs() * mean(a * err)) + 64 * E * rp * ((f * t * wp).abs() + xh.abs() * mean(a * big))
+        dwp = (f * t * xh).reshape(rows, -1).sum(0)
+        out["post_weight"] = (dwp, u * dwp.abs() + ((f * xh).abs() * (err + (64 + rows) * E * big)).reshape(rows, -1).sum(0))
+    out["x"] = (dx, u * dx.abs() + dx_err)
+    if gate is not None:
+        dg = scale * _to(n * t, gate.shape)
+        out["gate"] = (dg, u * dg.abs() + abs(scale) * _to(n.abs() * (err + (64 + rows + x.shape[-1]) * E * big), gate.shape))
+    return out
+
+
+def _close(got, want, name):
+    value, bound = want
+    got = got.detach().cpu().double()
+    assert got.shape == value.shape, (name, got.shape, value.shape)
+    # (subnormal results are off by up to half their own step)
+    tiny = {torch.float16: 2.0 ** -25}.get(name[1], 1e-38)
+    bad = (got - value).abs() > bound + tiny
+    assert not bad.any(), (name, int(bad.sum()), ((got - value).abs() / (bound + tiny)).max().item())
+
+
+def _check(lead, k, dtype, stream, post, gate, scale, pre=True, seed=0):
+    from primus_amd.pytorch import ops
+
+    dev = torch.device("cuda:0")
+    v, dy, dh = _inputs(lead, k, dtype, stream, post or not pre, gate, seed)
+    want = _reference(v, dy if pre else None, dh, scale, dtype, stream, pre)
+    v = {n: None if t is None else t.to(dev).requires_grad_() for n, t in v.items()}
+    if pre:
+        made = list(ops.add_rmsnorm(v["x"], v["residual"], v["weight"], EPS, post_weight=v["post_weight"], post_eps=POST_EPS, gate=v["gate"], scale=scale))
+        given = [dy.to(dev), dh.to(dev)]
+    else:
+        v["weight"] = None
+        made = [ops.rmsnorm_add(v["x"], v["residual"], v["post_weight"], POST_EPS, gate=v["gate"], scale=scale)]
+        given = [dh.to(dev)]
+    assert made[-1].dtype == stream and made[0].dtype == (dtype if pre else stream) and all(m.shape == v["x"].shape for m in made)
+    names = [n for n, t in v.items() if t is not None]
+    grads = dict(zip(names, torch.autograd.grad(made, [v[n] for n in names], given)))
+    for name, got in list(zip(["y", "h"] if pre else ["h"], made)) + list(grads.items()):
+        _close(got, want[name], (name, got.dtype))
+        if name in grads:
+            assert got.dtype == v[name].dtype
+
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+TYPES = [(BF, BF), (BF, FP), (HF, HF), (HF, FP), (FP, FP)]
+# one row and one column; widths around the lanes' eights and the waves' sixty-fours; both kernels (256 and above) and both numbers of chunks (8192)
+WIDTHS = [1, 7, 8, 9, 64, 65, 128, 129, 255, 256, 257, 512, 520, 1601, 4096, 8192, 8193, 16383, 16384]
+
+
+@pytest.mark.parametrize("k", WIDTHS)
+@pytest.mark.parametrize("dtype,stream", TYPES)
+def test_widths(gpu, k, dtype, stream):
+    _check((5, 3), k, dtype, stream, False, "", 1.0)
+    _check((3, 2), k, dtype, stream, True, "full", 0.5)
+    _check((4, 3), k, dtype, stream, True, "column", -1.25, pre=False)
+
+
+@pytest.mark.parametrize("gate", ["", "column", "element", "scalar", "first", "last", "token", "full", "first_scalar"])
+@pytest.mark.parametrize("post,pre", [(False, True), (True, True), (True, False)])
+@pytest.mark.parametrize("k", [40, 333, 1024])
+def test_gates(gpu, gate, post, pre, k):
+    for lead in ((1, 1), (2, 33), (67, 2), (3, 5, 7)):
+        _check(lead, k, BF, FP, post, gate, 0.75, pre)
+        _check(lead, k, HF, HF, post, gate, 1.0, pre)
+
+
+@pytest.mark.parametrize("rows,k", [(1, 4096), (2, 2880), (700, 2880), (5000, 96), (40000, 8), (3001, 257), (530, 7168), (300, 12289)])
+def test_rows(gpu, rows, k):
+    _check((rows,), k, BF, BF, False, "", 1.0)
+    _check((rows,), k, BF, FP, True, "token", 2.0)
+    _check((rows,), k, FP, FP, True, "column", 1.0, pre=False)
+
+
+@pytest.mark.parametrize("batch,seq,k", [(1500, 3, 512), (9000, 2, 64), (700, 1, 4096), (3, 2000, 512)])
+def test_many_gates(gpu, batch, seq, k):
+    """More gates than workers, and a few workers a gate; rows of a gate one after the other, or apart."""
+    for gate in ("first", "last", "first_scalar"):
+        _check((batch, seq), k, BF, BF, True, gate, 1.0)
+        _check((seq, batch), k, HF, HF, False, gate, 1.0)
+
+
+def test_one_dimension(gpu):
+    from primus_amd.pytorch import ops
+
+    x, r, w = (torch.randn(96, device=gpu) for _ in range(3))
+    y, h = ops.add_rmsnorm(x, r, w)
+    y2, h2 = ops.add_rmsnorm(x[None], r[None], w)
+    assert y.shape == (96,) and torch.equal(y, y2[0]) and torch.equal(h, h2[0])
+
+
+def test_no_rows(gpu):
+    from primus_amd.pytorch import ops
+
+    for shape, gate in (((0, 64), (64,)), ((0, 4, 640), (0, 1, 640)), ((2, 0, 64), (2, 1, 1))):
+        x, r = (torch.empty(*shape, dtype=BF, device=gpu, requires_grad=True) for _ in range(2))
+        w, p = (torch.ones(shape[-1], dtype=BF, device=gpu, requires_grad=True) for _ in range(2))
+        g = torch.ones(*gate, dtype=BF, device=gpu, requires_grad=True)
+        y, h = ops.add_rmsnorm(x, r, w, post_weight=p, gate=g)
+        (y.sum() + h.sum()).backward()
+        assert y.shape == h.shape == x.shape and x.grad.shape == x.shape
+        assert not w.grad.any() and not p.grad.any() and not g.grad.any() and g.grad.shape == g.shape
+        h = ops.rmsnorm_add(x, r, w, gate=g)
+        assert h.shape == x.shape
+
+
+def test_zero_rows_and_eps(gpu):
+    """A row of zeros: y = 0, and with eps 0 what the formula has, 0 * inf."""
+    from primus_amd.pytorch import ops
+
+    x = torch.randn(4, 300, dtype=BF, device=gpu)
+    x[1] = 0
+    r = torch.zeros_like(x)
+    w = torch.ones(300, dtype=BF, device=gpu)
+    y, h = ops.add_rmsnorm(x, r, w, 1e-6)
+    assert not y[1].any() and torch.equal(h, x) and torch.isfinite(y).all()
+    y, _ = ops.add_rmsnorm(x, r, w, 0.0)
+    assert y[1].isnan().all() and torch.isfinite(y[[0, 2, 3]]).all()
+
+
+def test_what_is_not_finite_stays_in_its_row(gpu):
+    from primus_amd.pytorch import ops
+
+    for k in (40, 333, 9000):
+        v, dy, dh = _inputs((6,), k, BF, BF, True, "token", device=gpu)
+        bad = {n: None if t is None else t.clone() for n, t in v.items()}
+        bad["x"][1, 3], bad["residual"][2, k - 1], bad["gate"][4, 0] = math.inf, math.nan, math.inf
+        run = lambda a: ops.add_rmsnorm(a["x"], a["residual"], a["weight"], EPS, post_weight=a["post_weight"], gate=a["gate"])  # noqa: E731
+        keep = [0, 3, 5]
+        made, want = [], []
+        for a, to in ((bad, made), (v, want)):
+            a = {n: t.clone().requires_grad_() for n, t in a.items()}
+            y, h = run(a)
+            to += [y, h, *torch.autograd.grad([y, h], [a["x"], a["residual"], a["gate"]], [dy, dh])]
+        for got, ref in zip(made, want):
+            assert torch.equal(got[keep], ref[keep])
+            assert not torch.isfinite(got[2]).all()
+        assert not torch.isfinite(made[0][1]).all() and not torch.isfinite(made[1][4]).all()
+
+
+def test_strides_offsets_and_orders(gpu):
+    """Tensors that are not contiguous, or begin at an odd element: the same bits as their copies."""
+    from primus_amd.pytorch import ops
+
+    g = torch.Generator(device=gpu).manual_seed(5)
+    for k in (24, 333, 1024):
+        wide = torch.randn(4, 6, 2 * k + 1, generator=g, device=gpu).to(BF)
+        x, r = wide[:, ::2, 1:k + 1], wide[:, ::2, k + 1:].transpose(0, 1).contiguous().transpose(0, 1)
+        buf = torch.randn(k * 3 + 7, generator=g, device=gpu).to(BF)
+        w, p, gate = buf[1:k + 1], buf[k + 3:2 * k + 3], buf[2 * k + 5:3 * k + 5].view(1, 1, k)
+        odd = torch.empty(12 * k + 1, dtype=BF, device=gpu)[1:].view(4, 3, k)
+        odd.copy_(x)
+        out = []
+        for a in ((x, r, w, p, gate), tuple(t.clone(memory_format=torch.contiguous_format) for t in (x, r, w, p, gate)), (odd, r, w, p, gate)):
+            a = [t.detach().requires_grad_() for t in a]
+            y, h = ops.add_rmsnorm(a[0], a[1], a[2], post_weight=a[3], gate=a[4], scale=0.5)
+            gy, gh = (torch.ones(3, 4, k, dtype=BF, device=gpu).transpose(0, 1) * s for s in (1.0, 0.5))
+            out.append([y, h, *torch.autograd.grad([y, h], a, [gy, gh])])
+        for got in out[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(got, out[0]))
+
+
+def test_gradients_that_are_not_asked_for(gpu):
+    from primus_amd.pytorch import ops
+
+    for k in (64, 600):
+        v, dy, dh = _inputs((5, 4), k, BF, FP, True, "first", device=gpu)
+        names = list(v)
+
+        def grads(needed, pre=True, given=(True, True)):
+            a = {n: t.detach().clone().requires_grad_(n in needed) for n, t in v.items()}
+            if pre:
+                made = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], EPS, post_weight=a["post_weight"], gate=a["gate"], scale=0.5)
+            else:
+                made = (ops.rmsnorm_add(a["x"], a["residual"], a["post_weight"], EPS, gate=a["gate"], scale=0.5),)
+            use = [(m, d) for m, d, w in zip(made, (dy, dh) if pre else (dh,), given) if w]
+            return dict(zip(needed, torch.autograd.grad([m for m, _ in use], [a[n] for n in needed], [d for _, d in use], allow_unused=True)))
+
+        every = grads(names)
+        for n in names:
+            assert torch.equal(grads([n])[n], every[n]), n
+        post = [n for n in names if n != "weight"]
+        every = grads(post, False)
+        for n in post:
+            assert torch.equal(grads([n], False)[n], every[n]), n
+        assert torch.equal(every["residual"], dh)
+        # y or h alone
+        want = _reference(v, dy, None, 0.5, BF, FP, post_eps=EPS)
+        for n, got in grads(names, given=(True, False)).items():
+            _close(got, want[n], (n, got.dtype))
+        want = _reference(v, None, dh, 0.5, BF, FP, post_eps=EPS)
+        for n, got in grads(names, given=(False, True)).items():
+            if n == "weight":
+                assert not got.any()
+            else:
+                _close(got, want[n], (n, got.dtype))
+
+
+def test_without_gradients(gpu):
+    from primus_amd.pytorch import ops
+
+    v, _, _ = _inputs((5, 4), 96, BF, BF, True, "", device=gpu)
+    a = {n: None if t is None else t.requires_grad_() for n, t in v.items()}
+    y, h = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], post_weight=a["post_weight"])
+    with torch.no_grad():
+        y2, h2 = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], post_weight=a["post_weight"])
+    with torch.inference_mode():
+        y3, h3 = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], post_weight=a["post_weight"])
+    assert y.requires_grad and not y2.requires_grad
+    assert torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(y, y3) and torch.equal(h, h3)
+
+
+def test_second_derivatives_raise(gpu):
+    from primus_amd.pytorch import ops
+
+    x, r, w = (torch.randn(*s, device=gpu, requires_grad=True) for s in ((3, 16), (3, 16), (16,)))
+    y, h = ops.add_rmsnorm(x, r, w)
+    (dx,) = torch.autograd.grad(y.sum() + h.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        dx.sum().backward()
+
+
+def test_differences(gpu):
+    """The gradients against central differences: those of the kernels' float32 outputs within rounding of the float64 formula's, whose distance from the
+    gradient goes with the square of the step."""
+    from primus_amd.pytorch import ops
+
+    k, lead, scale = 129, (3, 5), 0.7
+    v, dy, dh = _inputs(lead, k, FP, FP, True, "first", seed=3)
+    g = torch.Generator().manual_seed(9)
+    names = list(v)
+    way = {n: torch.randn(t.shape, generator=g).double() / math.sqrt(t.numel()) for n, t in v.items()}
+
+    def loss64(a):
+        out = _reference(a, None, None, scale, FP, FP)
+        return out["y"][0], out["h"][0]
+
+    def at(n, step, kernels):
+        a = {m: t.double() for m, t in v.items()}
+        a[n] = a[n] + step * way[n]
+        if kernels:
+            a = {m: t.float() for m, t in a.items()}
+            y, h = ops.add_rmsnorm(*(a[m].to(gpu) for m in ("x", "residual", "weight")), EPS, post_weight=a["post_weight"].to(gpu), post_eps=POST_EPS,
+                                   gate=a["gate"].to(gpu), scale=scale)
+            y, h = y.cpu().double(), h.cpu().double()
+        else:
+            y, h = loss64(a)
+        return (y * dy.double()).sum() + (h * dh.double()).sum(), (y * dy.double()).abs().sum() + (h * dh.double()).abs().sum()
+
+    a = {n: t.to(gpu).requires_grad_() for n, t in v.items()}
+    made = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], EPS, post_weight=a["post_weight"], post_eps=POST_EPS, gate=a["gate"], scale=scale)
+    grads = dict(zip(names, torch.autograd.grad(made, [a[n] for n in names], [dy.to(gpu), dh.to(gpu)])))
+    step = 2.0 ** -6
+    for n in names:
+        d64 = [((at(n, s, False)[0] - at(n, -s, False)[0]) / (2 * s)).item() for s in (step, 2 * step)]
+        plus, minus = at(n, step, True), at(n, -step, True)
+        d32 = ((plus[0] - minus[0]) / (2 * step)).item()
+        # outputs within 64 e of what they are added up of, inputs rounded to fp32 once more
+        rounding = 200 * E * (plus[1] + minus[1]).item() / (2 * step)
+        assert abs(d32 - d64[0]) <= rounding, n
+        slope = (grads[n].cpu().double() * way[n]).sum().item()
+        # the difference at twice the step is four times as far off: a third of their distance, doubled for the higher terms; and the gradient's own rounding
+        assert abs(slope - d64[0]) <= abs(d64[1] - d64[0]) + 200 * E * (plus[1]).item(), n
+
+
+def test_same_bits_each_time(gpu):
+    from primus_amd.pytorch import ops
+
+    for lead, k, gate in (((300, 7), 96, "column"), ((3, 500), 2880, "first"), ((2, 300), 10000, "token")):
+        v, dy, dh = _inputs(lead, k, BF, BF, True, gate, device=gpu)
+        v = {n: t.requires_grad_() for n, t in v.items()}
+        runs = []
+        for _ in range(2):
+            y, h = ops.add_rmsnorm(v["x"], v["residual"], v["weight"], post_weight=v["post_weight"], gate=v["gate"])
+            runs.append([y, h, *torch.autograd.grad([y, h], list(v.values()), [dy, dh])])
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_rows_beyond_32_bit_offsets(gpu):
+    """More than 2^31 elements: the last rows are those of a call on them alone."""
+    from primus_amd.pytorch import ops
+
+    k, rows = 16384, (1 << 17) + 24
+    x = torch.zeros(rows, k, dtype=BF, device=gpu)
+    r = torch.zeros(rows, k, dtype=BF, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    x[-40:] = torch.randn(40, k, generator=g, device=gpu).to(BF)
+    r[-40:] = torch.randn(40, k, generator=g, device=gpu).to(BF)
+    w = torch.randn(k, generator=g, device=gpu).to(BF).requires_grad_()
+    x.requires_grad_()
+    y, h = ops.add_rmsnorm(x, r, w)
+    dy = torch.zeros_like(h)
+    dy[-40:] = torch.randn(40, k, generator=g, device=gpu).to(BF)
+    dx, = torch.autograd.grad(y, x, dy)
+    xs = x.detach()[-40:].clone().requires_grad_()
+    ys, hs = ops.add_rmsnorm(xs, r[-40:], w)
+    dxs, = torch.autograd.grad(ys, xs, dy[-40:].clone())
+    assert torch.equal(y[-40:], ys) and torch.equal(h[-40:], hs) and torch.equal(dx[-40:], dxs)
+    assert not y[:-40].any() and not dx[:-40].any()
+
+
+def test_on_another_stream_and_captured(gpu):
+    """On a side stream, and in a graph replayed on new inputs with eager work between the replays."""
+    from primus_amd.pytorch import ops
+
+    v, dy, dh = _inputs((4, 50), 640, BF, FP, True, "first", device=gpu)
+    names = list(v)
+
+    def run(a, dy, dh):
+        a = {n: t.detach().requires_grad_() for n, t in a.items()}
+        y, h = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], EPS, post_weight=a["post_weight"], gate=a["gate"], scale=0.5)
+        z = ops.rmsnorm_add(y, h, a["post_weight"], EPS, gate=a["gate"])
+        return [y.detach(), h.detach(), z.detach(), *torch.autograd.grad([z, h], list(a.values()), [dh, dh])]
+
+    want = run(v, dy, dh)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(v, dy, dh)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    static = {n: t.clone() for n, t in v.items()}
+    sdy, sdh = dy.clone(), dh.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(static, sdy, sdh)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(static, sdy, sdh)
+    for seed in range(4):
+        new, ndy, ndh = _inputs((4, 50), 640, BF, FP, True, "first", seed=seed, device=gpu)
+        for n in names:
+            static[n].copy_(new[n])
+        sdy.copy_(ndy), sdh.copy_(ndh)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(new, ndy, ndh)
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
+
+
+def test_through_host_memory(gpu):
+    from primus_amd.pytorch import ops
+
+    v, dy, dh = _inputs((4, 5), 96, BF, BF, True, "token", device=gpu)
+    v = {n: t.requires_grad_() for n, t in v.items()}
+    run = lambda: ops.add_rmsnorm(v["x"], v["residual"], v["weight"], post_weight=v["post_weight"], gate=v["gate"])  # noqa: E731
+    want = torch.autograd.grad(run(), list(v.values()), [dy, dh])
+    with torch.autograd.graph.save_on_cpu():
+        made = run()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(made, list(v.values()), [dy, dh]), want))
+
+
+def test_rows_around_the_output_stay(gpu):
+    """The C ABI on views of larger buffers: what is before and behind the rows is not touched."""
+    from primus_amd import _lib
+    from primus_amd.pytorch import kernels as K
+
+    lib = _lib.load()
+    for rows, k, dt in ((3, 33, BF), (5, 700, HF), (2, 8200, FP)):
+        n = rows * k
+        bufs = [torch.full((n + 18,), 7.0, dtype=dt, device=gpu) for _ in range(2)]
+        y, h = (b[9:9 + n].view(rows, k) for b in bufs)
+        x, r = torch.randn(rows, k, device=gpu).to(dt), torch.randn(rows, k, device=gpu).to(dt)
+        w = torch.randn(k, device=gpu).to(dt)
+        rc = lib.mxl_block_norm(x.data_ptr(), r.data_ptr(), rows, k, K._DT[dt], K._DT[dt], None, 0.0, None, 1, 1, 0, 1.0, w.data_ptr(), EPS, y.data_ptr(), h.data_ptr(),
+                                None, None, K._stream())
+        assert rc == 0
+        wy, wh, _, _ = K.block_norm_impl(x, r, w, EPS, None, 0.0, None, 1.0)
+        assert torch.equal(y, wy) and torch.equal(h, wh)
+        assert all((b[:9] == 7).all() and (b[9 + n:] == 7).all() for b in bufs)

@@ -1,0 +1,278 @@
+"""The global gradient norm and clipping (``ops.grad_norm``, ``ops.clip_grads``) on the GPU against float64.
+
+Bars.  The norm is a sum of exact squares in fp64 (2^-53 an addition, at most 2^31 of them in a row of a million), rounded once: 2^-24, and 1e-9 for the sum.
+Clipped gradients: a float is one rounding of g times the fp64 factor, 2^-24 of it; of 16-bit gradients the factor is rounded to fp32 and the product too,
+2^-23 together, before the rounding to the output's type (half a step).  Subnormal results are off by up to half their own step."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def _exact_norm(tensors, kind=2.0):
+    if kind == math.inf:
+        return max((t.detach().cpu().double().abs().max().item() for t in tensors if t.numel()), default=0.0)
+    return math.sqrt(math.fsum(torch.dot(f, f).item() for f in (t.detach().cpu().double().reshape(-1) for t in tensors)))
+
+
+def _tensors(sizes, dtypes, device, seed=0, offsets=(0,)):
+    """Tensors of the sizes; each begins `offset` elements into its storage."""
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for i, n in enumerate(sizes):
+        off = offsets[i % len(offsets)]
+        t = torch.randn(n + off, generator=g) * 10.0 ** -(i % 4)
+        out.append(t.to(dtypes[i % len(dtypes)]).to(device)[off:])
+    return out
+
+
+SIZES = [0, 1, 2, 7, 8, 9, 15, 16, 17, 63, 255, 2047, 2048, 2049, 8191, 8192, 8193, 16384, 16385, 100003]
+
+
+@pytest.mark.parametrize("dtypes", [(FP,), (BF,), (HF,), (FP, BF, HF)])
+@pytest.mark.parametrize("offsets", [(0,), (1, 2, 3, 5, 7, 0, 4)])
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+def test_norm(gpu, dtypes, offsets, kind):
+    from primus_amd.pytorch import ops
+
+    ts = _tensors(SIZES, dtypes, gpu, offsets=offsets)
+    got = ops.grad_norm(ts, kind)
+    want = _exact_norm(ts, kind)
+    assert got.dtype == FP and got.shape == () and got.is_cuda
+    assert abs(got.item() - want) <= (2.0 ** -24 + 1e-9) * want
+    for t in ts:
+        assert abs(ops.grad_norm(t, kind).item() - _exact_norm([t], kind)) <= (2.0 ** -24 + 1e-9) * _exact_norm([t], kind)
+
+
+@pytest.mark.parametrize("count", [1, 159, 160, 161, 320, 321, 700])
+def test_many_tensors(gpu, count):
+    """One launch, its table full, and several."""
+    from primus_amd.pytorch import ops
+
+    ts = _tensors([(37 * i) % 5000 for i in range(count)], (BF, FP), gpu, offsets=(0, 1, 3))
+    for kind in (2.0, math.inf):
+        want = _exact_norm(ts, kind)
+        assert abs(ops.grad_norm(ts, kind).item() - want) <= (2.0 ** -24 + 1e-9) * want
+    outs = [torch.empty_like(t) for t in ts]
+    norm = ops.clip_grads(ts, 0.5 * _exact_norm(ts), out=outs)
+    for o, t in zip(outs, ts):
+        _clipped(o, t, 0.5 * _exact_norm(ts), norm)
+
+
+def test_nothing_to_add(gpu):
+    from primus_amd.pytorch import ops
+
+    empty = torch.empty(0, device=gpu)
+    for ts in ([], [empty], [empty] * 400, [torch.zeros(5, device=gpu), empty]):
+        for kind in (2.0, math.inf):
+            got = ops.grad_norm(ts, kind)
+            assert got.item() == 0.0 and got.dtype == FP and got.is_cuda
+        assert ops.clip_grads(ts, 1.0).item() == 0.0
+
+
+def test_scales_that_fp32_squares_do_not_hold(gpu):
+    from primus_amd.pytorch import ops
+
+    for scale in (1e30, 1e-30, 1e-42):
+        t = torch.linspace(1, 2, 5001, device=gpu) * scale
+        want = _exact_norm([t])
+        # (a subnormal result has steps of 2^-149)
+        assert abs(ops.grad_norm([t]).item() - want) <= (2.0 ** -24 + 1e-9) * want + 2.0 ** -150
+    big = torch.full((4096,), 3e38, device=gpu)
+    assert ops.grad_norm([big]).item() == math.inf and ops.grad_norm([big], math.inf).item() == big[0].item()
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+def test_infinities_and_nans(gpu, dtype):
+    from primus_amd.pytorch import ops
+
+    for n, at in ((5, 2), (100003, 70001)):
+        t = torch.randn(n, device=gpu).to(dtype)
+        other = torch.randn(33, device=gpu).to(dtype)
+        t[at] = -math.inf
+        for kind in (2.0, math.inf):
+            assert ops.grad_norm([other, t], kind).item() == math.inf
+        t[at - 1] = math.nan
+        for kind in (2.0, math.inf):
+            assert math.isnan(ops.grad_norm([other, t], kind).item())
+            assert math.isnan(ops.grad_norm([t, other], kind).item())
+
+
+def _clipped(got, grad, max_norm, norm):
+    c = min(1.0, max_norm / (norm.item() + 1e-6))
+    want = grad.detach().cpu().double() * c
+    bound = (torch.finfo(got.dtype).eps / 2 + (0 if grad.dtype == FP and got.dtype == FP else 2.0 ** -23)) * want.abs()
+    bound += {HF: 2.0 ** -25}.get(got.dtype, 2.0 ** -149)
+    assert got.shape == grad.shape
+    assert ((got.detach().cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("src", [FP, BF, HF])
+@pytest.mark.parametrize("dst", [FP, BF, HF])
+def test_clip_into(gpu, src, dst):
+    from primus_amd.pytorch import ops
+
+    ts = _tensors(SIZES, (src,), gpu, offsets=(0, 1, 3))
+    want = _exact_norm(ts)
+    for max_norm in (0.0, 0.3 * want, 0.999 * want, 2 * want, math.inf):
+        outs = [torch.full((t.numel() + 2,), 7.0, dtype=dst, device=gpu) for t in ts]
+        copies = [t.clone() for t in ts]
+        norm = ops.clip_grads(ts, max_norm, out=[o[1:-1] for o in outs])
+        assert abs(norm.item() - want) <= (2.0 ** -24 + 1e-9) * want
+        for t, c, o in zip(ts, copies, outs):
+            assert torch.equal(t, c) and o[0] == 7 and o[-1] == 7
+            _clipped(o[1:-1], t, max_norm, norm)
+
+
+@pytest.mark.parametrize("dtypes", [(FP,), (BF,), (HF,), (FP, BF, HF)])
+def test_clip_in_place(gpu, dtypes):
+    from primus_amd.pytorch import ops
+
+    ts = _tensors(SIZES, dtypes, gpu, offsets=(0, 1, 3))
+    copies = [t.clone() for t in ts]
+    want = _exact_norm(ts)
+    versions = [t._version for t in ts]
+    norm = ops.clip_grads(ts, 2 * want)
+    assert all(torch.equal(a, b) for a, b in zip(ts, copies))
+    assert torch.equal(norm, ops.grad_norm(ts))
+    norm = ops.clip_grads(ts, 0.25 * want)
+    for t, c, v in zip(ts, copies, versions):
+        _clipped(t, c, 0.25 * want, norm)
+        assert t._version > v
+    # a norm that the caller has: a tensor (of any shape of one element) or a number; the gradients are those of the first pass
+    for given in (norm, norm.view(1), norm.item()):
+        again = [c.clone() for c in copies]
+        assert float(ops.clip_grads(again, 0.25 * want, norm=given)) == norm.item()
+        assert all(torch.equal(a, b) for a, b in zip(again, ts))
+    big = [c.clone() for c in copies]
+    top = ops.clip_grads(big, 1e-3, norm_type=math.inf)
+    for b, c in zip(big, copies):
+        _clipped(b, c, 1e-3, top)
+
+
+def test_norms_that_are_not_finite(gpu):
+    from primus_amd.pytorch import ops
+
+    t = torch.randn(5000, device=gpu)
+    t[7] = math.inf
+    a = t.clone()
+    assert ops.clip_grads([a], 1.0).item() == math.inf
+    assert a[7].isnan() and not a[:7].any() and not a[8:].any()
+    t[8] = math.nan
+    for bound in (1.0, math.inf):
+        b = t.clone()
+        assert ops.clip_grads([b], bound).isnan() and b.isnan().all()
+
+
+def test_strided_gradients(gpu):
+    """Transposed and sliced gradients: written in place too; expanded ones are refused."""
+    from primus_amd.pytorch import ops
+
+    base = torch.randn(40, 60, device=gpu).to(BF)
+    for view in (lambda b: b.t(), lambda b: b[:, 3:50], lambda b: b[::2]):
+        b = base.clone()
+        g = view(b)
+        want = _exact_norm([g])
+        assert abs(ops.grad_norm([g]).item() - want) <= (2.0 ** -24 + 1e-9) * want
+        norm = ops.clip_grads([g], 0.5 * want)
+        _clipped(g, view(base), 0.5 * want, norm)
+        mask = torch.zeros_like(base, dtype=torch.bool)
+        view(mask)[:] = True
+        assert torch.equal(b[~mask], base[~mask])
+        out = view(torch.zeros(40, 60, device=gpu))
+        ops.clip_grads([view(base)], 0.5 * want, out=[out])
+        _clipped(out, view(base), 0.5 * want, norm)
+    e = torch.randn(1, 8, device=gpu).expand(4, 8)
+    assert abs(ops.grad_norm([e]).item() - _exact_norm([e])) <= 2.0 ** -23 * _exact_norm([e])
+    with pytest.raises(ValueError, match="overlap"):
+        ops.clip_grads([e], 1.0)
+
+
+def test_overlaps_are_refused(gpu):
+    from primus_amd.pytorch import ops
+
+    t = torch.randn(100, device=gpu)
+    copy = t.clone()
+    for grads, out in (([t, t], None), ([t[:60], t[50:]], None), ([t[:50]], [t[25:75]]), ([t[:40], t[60:]], [t[:40], t[30:70]]), ([t.view(BF)[:50]], [t[:50]]),
+                       ([t.view(10, 10).t(), t.view(10, 10).t()], None)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.clip_grads(grads, 1e-3, out=out)
+    assert torch.equal(t, copy)
+    # neighbours are no overlap, nor is the same gradient read twice
+    ops.clip_grads([t[:50], t[50:]], 1e-3)
+    o = [torch.empty_like(t), torch.empty_like(t)]
+    ops.clip_grads([copy, copy], 1e-3, out=o)
+    assert torch.equal(*o)
+
+
+def test_beyond_32_bit_offsets(gpu):
+    from primus_amd.pytorch import ops
+
+    n = (1 << 31) + 77
+    t = torch.zeros(n, dtype=BF, device=gpu)
+    t[-3:] = torch.tensor([3.0, -4.0, 12.0], dtype=BF)
+    assert ops.grad_norm([t]).item() == 13.0 and ops.grad_norm([t], math.inf).item() == 12.0
+    norm = ops.clip_grads([t], 6.5)
+    _clipped(t[-3:], torch.tensor([3.0, -4.0, 12.0], dtype=BF), 6.5, norm)
+    assert not t[:-3].any()
+
+
+def test_order_of_sums_is_fixed(gpu):
+    from primus_amd.pytorch import ops
+
+    ts = _tensors([1000003, 77, 500000, 3], (FP, BF), gpu, offsets=(0, 1))
+    first = ops.grad_norm(ts)
+    assert all(torch.equal(ops.grad_norm(ts), first) for _ in range(5))
+
+
+def test_on_another_stream_and_captured(gpu):
+    from primus_amd.pytorch import ops
+
+    sizes = [70001, 5, 200000, 33] * 50
+    ts = _tensors(sizes, (BF, FP), gpu)
+
+    def run(grads, outs):
+        norm = ops.clip_grads(grads, 1.0, out=outs)
+        return [norm] + outs
+
+    fresh = lambda: [torch.empty(n, device=gpu) for n in sizes]  # noqa: E731
+    want = run(ts, fresh())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(ts, fresh())
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    static, outs = [t.clone() for t in ts], fresh()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    made = []
+    for graph in graphs:        # two graphs, replayed in turn
+        with torch.cuda.graph(graph):
+            made.append([ops.grad_norm(static), ops.clip_grads(static, 1.0, out=outs)])
+    for seed in range(4):
+        new = _tensors(sizes, (BF, FP), gpu, seed=seed + 1)
+        for s, n in zip(static, new):
+            s.copy_(n)
+        graphs[seed % 2].replay()
+        torch.cuda.synchronize()
+        want = run(new, fresh())
+        assert torch.equal(made[seed % 2][0], want[0]) and torch.equal(made[seed % 2][1], want[0])
+        assert all(torch.equal(a, b) for a, b in zip(outs, want[1:])), seed
+
+
+def test_parameters_gradients(gpu):
+    """The gradients of a small model, as a training loop hands them over."""
+    from primus_amd.pytorch import ops
+
+    model = torch.nn.Sequential(torch.nn.Linear(24, 40), torch.nn.ReLU(), torch.nn.Linear(40, 3)).to(gpu)
+    model(torch.randn(8, 24, device=gpu)).square().sum().backward()
+    grads = [p.grad for p in model.parameters()]
+    copies = [g.clone() for g in grads]
+    norm = ops.clip_grads((p.grad for p in model.parameters()), 0.1)
+    for g, c in zip(grads, copies):
+        _clipped(g, c, 0.1, norm)
