@@ -658,14 +658,14 @@ int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_b
  * wanted).  k <= 16384, any; at least one of the weights.
  *
  * mxl_block_norm_bwd: gradients given those of y (dy; not looked at without weight) and of h (dh, stream_dtype; NULL: zero).  Any output may be
- * NULL: not wanted.  dresidual is written in stream_dtype; without weight it is dh itself, which is left to the caller (written all the same
- * if asked for).  x is looked at with post_weight or dgate, h with weight.  mxl_block_norm_bwd_workspace_bytes: has_weight, has_post_weight:
- * whether dweight, dpost_weight are wanted, gate_cols 0: dgate is not. */
+ * NULL: not wanted.  dresidual is of stream_dtype; without weight it is dh itself and must be NULL.  dx is the residual's gradient, and is not
+ * written, where it is NULL with weight, without post_weight and without a gate of vectors.  x is looked at with post_weight or dgate, h with weight.
+ * mxl_block_norm_bwd_workspace_bytes: has_weight, has_post_weight: whether dweight, dpost_weight are wanted; gate_cols 0: no gate. */
 int mxl_block_norm(const void* x, const void* residual, int64_t rows, int64_t k, int dtype, int stream_dtype, const void* post_weight,
                    float post_eps, const void* gate, int64_t gate_div, int64_t gate_mod, int64_t gate_cols, float scale, const void* weight,
                    float eps, void* y, void* h, float* post_rstd, float* rstd, void* stream);
 int64_t mxl_block_norm_bwd_workspace_bytes(int64_t rows, int64_t k, int has_weight, int has_post_weight, int64_t gate_div, int64_t gate_mod,
-                                           int64_t gate_cols);
+                                           int64_t gate_cols, int need_dgate);
 int mxl_block_norm_bwd(const void* dy, const void* dh, const void* x, const void* h, int64_t rows, int64_t k, int dtype, int stream_dtype,
                        const void* post_weight, const float* post_rstd, const void* gate, int64_t gate_div, int64_t gate_mod, int64_t gate_cols,
                        float scale, const void* weight, const float* rstd, void* dx, void* dresidual, void* dweight, void* dpost_weight,

@@ -309,7 +309,7 @@ def load() -> ctypes.CDLL:
         lib.mxl_block_norm.restype = i32
         lib.mxl_block_norm.argtypes = [vp, vp, i64, i64, i32, i32, vp, f32, vp, i64, i64, i64, f32, vp, f32, vp, vp, vp, vp, vp]
         lib.mxl_block_norm_bwd_workspace_bytes.restype = i64
-        lib.mxl_block_norm_bwd_workspace_bytes.argtypes = [i64, i64, i32, i32, i64, i64, i64]
+        lib.mxl_block_norm_bwd_workspace_bytes.argtypes = [i64, i64, i32, i32, i64, i64, i64, i32]
         lib.mxl_block_norm_bwd.restype = i32
         lib.mxl_block_norm_bwd.argtypes = [vp, vp, vp, vp, i64, i64, i32, i32, vp, vp, vp, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
         lib.mxl_grad_norm_workspace_bytes.restype = i64

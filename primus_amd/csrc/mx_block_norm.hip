@@ -20,135 +20,126 @@ struct BlockNormArgs {
     float *post_rstd, *rstd;
 };
 
-// T: type of x, y, weights and gate; S: of residual and h.  CH chunks of eight columns a lane.
-template <int T, int S, int CH, bool PRE, bool POST, bool SMALL>
+// T: type of x, y, weights and gate; S: of residual and h.  A workgroup a row (a run of lanes where rows are short), CH chunks of eight
+// columns a lane, all loads asked for at once.
+//
+// Bound by memory: x and residual in, y and h out.  us (TB/s) from memory: [16384, 4096] add and norm 89 (6.0), norm and add 69 (5.8); [8192,
+// 7168] 80 (5.9) and 63 (5.6); both norms [11651, 2880] 50 (5.3).  Against workgroups that stay and ask for their next row while they work on
+// the present one: 96, 69, 85, 69 and 52.
+template <int T, int S, int CH, bool PRE, bool POST, bool SMALL, bool ANY>
 __global__ __launch_bounds__(SMALL ? BN_SMALL_THREADS : BN_MAX_THREADS) void block_norm_kernel(BlockNormArgs p) {
-    __shared__ float part[2][BN_MAX_THREADS / 64][1];
+    __shared__ float part[2][BN_MAX_WAVES][1];
     const int lanes = SMALL ? p.lanes : (int)blockDim.x;
     const int lane = SMALL ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x;
-    const int64_t workers = SMALL ? (int64_t)gridDim.x * (BN_SMALL_THREADS / lanes) : gridDim.x;
-    const int64_t worker = SMALL ? (int64_t)blockIdx.x * (BN_SMALL_THREADS / lanes) + threadIdx.x / lanes : blockIdx.x;
+    const int64_t row = SMALL ? (int64_t)blockIdx.x * (BN_SMALL_THREADS / lanes) + threadIdx.x / lanes : blockIdx.x;
+    if (SMALL && row >= p.rows) return;
     RowSums<1, SMALL> sums(part, lanes);
     const int k = p.k;
     const float inv_k = 1.0f / (float)k;
-    int col[CH], left[CH];
-    Raw8<T> w[CH], wp[CH], gv[CH];
+    typedef RowsOf<T, S, SMALL, ANY> RowsT;
+    typedef RowsOf<S, S, SMALL, ANY> RowsS;
+    const Cols<S> cols = {lanes, lane, k};
+    const bool vec = p.gate.kind == GATE_VECTOR;
+    const int64_t g = p.gate.kind == GATE_NONE ? 0 : (int64_t)((uint32_t)row / p.gate.div % p.gate.mod);
+    const RowsT in_x(p.x, p.rows, row, k), in_g(vec ? p.gate.p : nullptr, p.gate.mod, g, k);
+    const RowsS in_r(p.residual, p.rows, row, k);
+    Raw8<T> xr[CH], gr[CH], wr[CH], wpr[CH];
+    Raw8<S> rr[CH];
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-        col[j] = (j * lanes + lane) * BN_VEC;
-        left[j] = k - col[j];
-        w[j] = wp[j] = gv[j] = none8<T>();
-        if (left[j] > 0) {
-            if (PRE) w[j] = load8<T>(p.weight, col[j], left[j], false);
-            if (POST) wp[j] = load8<T>(p.post_weight, col[j], left[j], false);
-        }
+        xr[j] = in_x.template load<BN_NT>(cols, j);
+        rr[j] = in_r.template load<BN_NT>(cols, j);
+        if (POST) wpr[j] = load_vector<T>(p.post_weight, cols, j);
+        gr[j] = in_g.template load<0>(cols, j);
+        if (PRE) wr[j] = load_vector<T>(p.weight, cols, j);
     }
-    Raw8<T> xn[CH];
-    Raw8<S> rn[CH];
-    auto request = [&](int64_t row) {
+    float factor = p.scale;
+    if (p.gate.kind == GATE_SCALAR) factor *= (float)((const typename DtOf<T>::type*)p.gate.p)[g];
+    float x[CH][BN_VEC], h[CH][BN_VEC];
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            xn[j] = none8<T>();
-            rn[j] = none8<S>();
-            if (left[j] > 0) {
-                xn[j] = load8<T>(p.x, row * k + col[j], left[j], true);
-                rn[j] = load8<S>(p.residual, row * k + col[j], left[j], true);
-            }
-        }
-    };
-    int64_t gate_row = -1;
-    if (worker < p.rows) request(worker);
-    for (int64_t row = worker; row < p.rows; row += workers) {
-        float x[CH][BN_VEC], h[CH][BN_VEC];
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            unpack8<T>(xn[j], x[j]);
-            unpack8<S>(rn[j], h[j]);
-        }
-        float factor = p.scale;
-        if (p.gate.kind != GATE_NONE) {
-            const int64_t g = (uint32_t)row / p.gate.div % p.gate.mod;
-            if (p.gate.kind == GATE_SCALAR) {
-                factor *= (float)((const typename DtOf<T>::type*)p.gate.p)[g];
-            } else if (g != gate_row) {
-#pragma unroll
-                for (int j = 0; j < CH; ++j)
-                    if (left[j] > 0) gv[j] = load8<T>(p.gate.p, g * k + col[j], left[j], false);
-                gate_row = g;
-            }
-        }
-        if (row + workers < p.rows) request(row + workers);
-        if (POST) {
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < CH; ++j)
-#pragma unroll
-                for (int e = 0; e < BN_VEC; ++e) ss += x[j][e] * x[j][e];
-            sums(&ss);
-            const float rp = 1.0f / sqrtf(ss * inv_k + p.post_eps);
-            if (lane == 0 && p.post_rstd) p.post_rstd[row] = rp;
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                float v[BN_VEC];
-                unpack8<T>(wp[j], v);
-#pragma unroll
-                for (int e = 0; e < BN_VEC; ++e) x[j][e] = x[j][e] * rp * v[e];
-            }
-        }
+    for (int j = 0; j < CH; ++j) {
+        unpack8<T>(xr[j], x[j]);
+        unpack8<S>(rr[j], h[j]);
+    }
+    if (POST) {
         float ss = 0.f;
 #pragma unroll
+        for (int j = 0; j < CH; ++j)
+#pragma unroll
+            for (int e = 0; e < BN_VEC; ++e) ss += x[j][e] * x[j][e];
+        sums(&ss);
+        const float rp = 1.0f / sqrtf(ss * inv_k + p.post_eps);
+        if (p.post_rstd && lane == 0) p.post_rstd[row] = rp;
+#pragma unroll
         for (int j = 0; j < CH; ++j) {
-            float f[BN_VEC];
-            if (p.gate.kind == GATE_VECTOR) {
-                unpack8<T>(gv[j], f);
+            float w[BN_VEC];
+            unpack8<T>(wpr[j], w);
 #pragma unroll
-                for (int e = 0; e < BN_VEC; ++e) f[e] *= factor;
-            } else {
-#pragma unroll
-                for (int e = 0; e < BN_VEC; ++e) f[e] = factor;
-            }
-#pragma unroll
-            for (int e = 0; e < BN_VEC; ++e) {
-                h[j][e] += f[e] * x[j][e];
-                if (col[j] + e < k) ss += h[j][e] * h[j][e];    // (past the row: an infinite factor times the zeros there)
-            }
-            if (left[j] > 0) store8<S>(p.h, row * k + col[j], left[j], h[j]);
+            for (int e = 0; e < BN_VEC; ++e) x[j][e] = x[j][e] * rp * w[e];
         }
-        if (PRE) {
-            sums(&ss);
-            const float r = 1.0f / sqrtf(ss * inv_k + p.eps);
-            if (lane == 0 && p.rstd) p.rstd[row] = r;
+    }
+    float ss = 0.f;
+    const RowsS out_h(p.h, p.rows, row, k);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                float v[BN_VEC];
-                unpack8<T>(w[j], v);
+    for (int j = 0; j < CH; ++j) {
+        if (vec) {
+            float f[BN_VEC];
+            unpack8<T>(gr[j], f);
 #pragma unroll
-                for (int e = 0; e < BN_VEC; ++e) v[e] = h[j][e] * r * v[e];
-                if (left[j] > 0) store8<T>(p.y, row * k + col[j], left[j], v);
-            }
+            for (int e = 0; e < BN_VEC; ++e) h[j][e] += factor * f[e] * x[j][e];
+        } else {
+            // (past the row there are zeros, which an infinite factor must not meet)
+#pragma unroll
+            for (int e = 0; e < BN_VEC; ++e) h[j][e] += (cols(j, ANY || k % 2 ? e : e / 2 * 2) < k ? factor : 0.f) * x[j][e];
+        }
+#pragma unroll
+        for (int e = 0; e < BN_VEC; ++e) ss += h[j][e] * h[j][e];
+        out_h.store(cols, j, h[j]);
+    }
+    if (PRE) {
+        sums(&ss);
+        const float r = 1.0f / sqrtf(ss * inv_k + p.eps);
+        if (p.rstd && lane == 0) p.rstd[row] = r;
+        const RowsT out_y(p.y, p.rows, row, k);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            float w[BN_VEC];
+            unpack8<T>(wr[j], w);
+#pragma unroll
+            for (int e = 0; e < BN_VEC; ++e) h[j][e] = h[j][e] * r * w[e];
+            out_y.store(cols, j, h[j]);
         }
     }
 }
 
-template <int T, int S, int CH, bool SMALL>
-static void block_norm_launch(const BlockNormArgs& p, int blocks, int threads, hipStream_t st) {
-    const dim3 g((unsigned)blocks), b((unsigned)threads);
-    if (p.weight && p.post_weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, true, SMALL>), g, b, 0, st, p);
-    else if (p.weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, false, SMALL>), g, b, 0, st, p);
-    else hipLaunchKernelGGL((block_norm_kernel<T, S, CH, false, true, SMALL>), g, b, 0, st, p);
+// Columns a lane.  Two chunks: fewer waves to wait for each other, from 4096 columns on ([8192, 7168] 96 -> 80 us), and of both norms, which
+// wait twice, above 512 ([11651, 2880] 61 -> 50) unless the chip is not full anyway ([64, 4096] 6.5 and 7.0).
+static int block_norm_chunks(const BlockNormArgs& p) {
+    if (p.k > BN_MAX_THREADS * BN_VEC / 2) return 2;
+    return p.weight && p.post_weight && p.k > 512 && p.rows > 512 ? 2 : 1;
 }
-template <int T, int S> static void block_norm_launch(BlockNormArgs& p, hipStream_t st) {
+
+template <int T, int S, int CH, bool SMALL, bool ANY>
+static void block_norm_launch(const BlockNormArgs& p, int64_t blocks, int threads, hipStream_t st) {
+    const dim3 g((unsigned)blocks), b((unsigned)threads);
+    if (p.weight && p.post_weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, true, SMALL, ANY>), g, b, 0, st, p);
+    else if (p.weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, false, SMALL, ANY>), g, b, 0, st, p);
+    else hipLaunchKernelGGL((block_norm_kernel<T, S, CH, false, true, SMALL, ANY>), g, b, 0, st, p);
+}
+template <int T, int S, bool ANY> static void block_norm_launch(BlockNormArgs& p, hipStream_t st) {
     if (p.k <= BN_SMALL_K) {
         p.lanes = bn_lanes(p.k);
-        const int64_t per = BN_SMALL_THREADS / p.lanes, want = (p.rows + per - 1) / per;
-        block_norm_launch<T, S, 1, true>(p, (int)(want < 2048 ? want : 2048), BN_SMALL_THREADS, st);
-        return;
+        const int64_t per = BN_SMALL_THREADS / p.lanes;
+        block_norm_launch<T, S, 1, true, ANY>(p, (p.rows + per - 1) / per, BN_SMALL_THREADS, st);
+    } else if (block_norm_chunks(p) == 1) {
+        block_norm_launch<T, S, 1, false, ANY>(p, p.rows, bn_threads(p.k, 1), st);
+    } else {
+        block_norm_launch<T, S, 2, false, ANY>(p, p.rows, bn_threads(p.k, 2), st);
     }
-    const int threads = bn_threads(p.k);
-    const int64_t cap = 256 * 2048 / threads;
-    const int blocks = (int)(p.rows < cap ? p.rows : cap);
-    if (bn_chunks(p.k) == 1) block_norm_launch<T, S, 1, false>(p, blocks, threads, st);
-    else block_norm_launch<T, S, 2, false>(p, blocks, threads, st);
+}
+template <int T, int S> static void block_norm_launch(BlockNormArgs& p, hipStream_t st) {
+    if (bn_on_dwords(p.rows, p.k, T, {p.x, p.residual, p.gate.kind == GATE_VECTOR ? p.gate.p : nullptr, p.y, p.h})) block_norm_launch<T, S, false>(p, st);
+    else block_norm_launch<T, S, true>(p, st);
 }
 
 }  // namespace mxl

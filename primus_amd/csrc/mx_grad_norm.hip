@@ -61,31 +61,46 @@ template <int DT, bool MAX> __device__ __forceinline__ void add_vec(Stat<MAX>& s
     }
 }
 
-// Elements [lo, hi) of a tensor: up to where 16-byte pieces begin, the pieces, and the rest.
+// Elements [lo, hi) of a tensor: the 16-byte pieces among them, through a buffer descriptor that ends with the last (zeros arrive for
+// pieces past it, which add nothing: no branches, so that all loads are on their way at once), and the elements before and behind.
 template <int DT, bool MAX> __device__ __forceinline__ void chunk_stat(Stat<MAX>& s, const void* base, int64_t lo, int64_t hi) {
     constexpr int SIZE = DT == MXL_DT_F32 ? 4 : 2;
-    const uintptr_t a = (uintptr_t)base + lo * SIZE, z = (uintptr_t)base + hi * SIZE;
-    const uintptr_t a16 = (a + 15) & ~(uintptr_t)15;
-    if (a16 >= z) {         // fewer than 16 bytes
-        const int n = (int)(hi - lo);
-        if ((int)threadIdx.x < n) s.add(load_dt(base, DT, lo + threadIdx.x), 0.f);
-        return;
-    }
-    const int head = (int)(a16 - a) / SIZE, vecs = (int)((z - a16) / 16);
-    const int tail = (int)(z - a16 - (uintptr_t)vecs * 16) / SIZE;
-    if ((int)threadIdx.x < head) s.add(load_dt(base, DT, lo + threadIdx.x), 0.f);
-    const gn_u32x4* v = (const gn_u32x4*)a16;
+    const int64_t bytes = (hi - lo) * SIZE;
+    const uint8_t* a = (const uint8_t*)base + lo * SIZE;
+    int64_t head = -(int64_t)(uintptr_t)a & 15;
+    if (head > bytes) head = bytes;
+    const int vecs = (int)((bytes - head) / 16), tail = (int)(bytes - head - (int64_t)vecs * 16);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a + head), 0, vecs * 16, 0x00020000);
     gn_u32x4 r[GN_LOADS];
 #pragma unroll
-    for (int u = 0; u < GN_LOADS; ++u) {
-        const int i = u * GN_THREADS + (int)threadIdx.x;
-        r[u] = gn_u32x4{0, 0, 0, 0};
-        if (i < vecs) r[u] = __builtin_nontemporal_load(v + i);
+    for (int u = 0; u < GN_LOADS; ++u) r[u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)threadIdx.x * 16, u * GN_THREADS * 16, 2);
+    if (head | tail) {
+        const int i = (int)threadIdx.x;
+        if (i < (int)head / SIZE) s.add(load_dt(base, DT, lo + i), 0.f);
+        else if (i >= 64 && i - 64 < tail / SIZE) s.add(load_dt(base, DT, hi - tail / SIZE + (i - 64)), 0.f);
     }
 #pragma unroll
     for (int u = 0; u < GN_LOADS; ++u) add_vec<DT, MAX>(s, r[u]);
-    if ((int)threadIdx.x < tail) s.add(load_dt(base, DT, hi - tail + threadIdx.x), 0.f);
 }
+
+// Which tensor a chunk belongs to: the number of tensors that end at or before it.  The ends are in registers, some a lane.
+template <int TENSORS> struct TensorOf {
+    static constexpr int PER = (TENSORS + 63) / 64;
+    uint32_t end[PER];
+    __device__ __forceinline__ TensorOf(const uint32_t* ends, int count) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int t = i * 64 + ((int)threadIdx.x & 63);
+            end[i] = t < count ? ends[t] : 0xFFFFFFFFu;
+        }
+    }
+    __device__ __forceinline__ int operator()(uint32_t chunk) const {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) n += __builtin_popcountll(__ballot(end[i] <= chunk));
+        return n;
+    }
+};
 
 __device__ __forceinline__ double lanes_sum_f64(double v) {
 #pragma unroll
@@ -114,9 +129,9 @@ __device__ __forceinline__ float norm_of(double total, bool max) { return max ? 
 template <bool MAX> __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(NormTable t, double* partial, float* out) {
     Stat<MAX> s;
     const uint32_t chunks = t.end[t.count - 1];
-    int at = 0;
+    const TensorOf<GN_TENSORS> tensor_of(t.end, t.count);
     for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        while (t.end[at] <= c) ++at;
+        const int at = tensor_of(c);
         const uint32_t first = at ? t.end[at - 1] : 0;
         const int64_t packed = t.n[at], n = packed & (((int64_t)1 << GN_TYPE_SHIFT) - 1);
         const int type = (int)(packed >> GN_TYPE_SHIFT);
@@ -157,62 +172,69 @@ constexpr int GC_PER = GN_THREADS * 32;     // elements of a chunk
 // The product is rounded once: a float's is made in fp64; of the 16-bit types it is exact but for the coefficient's 24 bits.
 template <int DT> __device__ __forceinline__ float scaled(float g, double c, float cf) { return DT == MXL_DT_F32 ? (float)((double)g * c) : g * cf; }
 
+// Four or eight elements a lane and step (so that a store of a wave writes whole lines: streaming stores of every other sixteen bytes do not
+// combine), through buffer descriptors of the chunk's whole steps' worth (past it nothing is read or written); the rest element by element.
+// Two-byte elements that begin between two dwords: the descriptor begins a dword boundary later, the element in front goes by itself.
 template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void* src, void* dst, int64_t lo, int64_t hi, double c, float cf) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
-    constexpr int IN = DT == MXL_DT_F32 ? 2 : 1, OUT = DO == MXL_DT_F32 ? 2 : 1;    // 16-byte pieces of eight elements
-    constexpr int UNROLL = 4;
-    const uint8_t* s = (const uint8_t*)src + lo * (IN * 2);
-    uint8_t* d = (uint8_t*)dst + lo * (OUT * 2);
-    const int n = (int)(hi - lo), eights = n / 8;
+    constexpr int IN = DT == MXL_DT_F32 ? 4 : 2, OUT = DO == MXL_DT_F32 ? 4 : 2;    // bytes of an element
+    constexpr int PER = IN == 2 && OUT == 2 ? 8 : 4, STEPS = GC_PER / PER / GN_THREADS;
+    constexpr int IW = PER * IN / 4, OW = PER * OUT / 4;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const uint8_t* s = (const uint8_t*)src + lo * IN;
+    uint8_t* d = (uint8_t*)dst + lo * OUT;
+    const bool odd_in = IN == 2 && ((uintptr_t)s & 2), odd_out = OUT == 2 && ((uintptr_t)d & 2);
+    const int n = (int)(hi - lo);
+    if (IN == 2 && OUT == 2 && odd_in != odd_out) {     // one on dwords and the other between them
+        for (int i = (int)threadIdx.x; i < n; i += GN_THREADS) store_dt(dst, DO, lo + i, scaled<DT>(load_dt(src, DT, lo + i), c, cf));
+        return;
+    }
+    const int head = odd_in || odd_out ? 1 : 0, whole = (n - head) / PER;
+    const auto in = __builtin_amdgcn_make_buffer_rsrc((void*)(s + head * IN), 0, whole * PER * IN, 0x00020000);
+    const auto out = __builtin_amdgcn_make_buffer_rsrc(d + head * OUT, 0, whole * PER * OUT, 0x00020000);
+    uint32_t r[STEPS][IW];
 #pragma unroll
-    for (int u0 = 0; u0 < GC_PER / 8 / GN_THREADS; u0 += UNROLL) {
-        uint32_t r[UNROLL][4 * IN];
+    for (int u = 0; u < STEPS; ++u) {
+        if constexpr (IW == 4) {
+            const gn_u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(in, (int)threadIdx.x * 16, u * GN_THREADS * 16, 2);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int i = (u0 + u) * GN_THREADS + (int)threadIdx.x;
-            if (i < eights) {
-#pragma unroll
-                for (int q = 0; q < IN; ++q) {
-                    const u32x4 v = __builtin_nontemporal_load((const u32x4*)(s + (int64_t)i * 16 * IN) + q);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) r[u][4 * q + j] = v[j];
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int i = (u0 + u) * GN_THREADS + (int)threadIdx.x;
-            if (i >= eights) continue;
-            float f[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (DT == MXL_DT_F32) f[j] = __uint_as_float(r[u][j % (4 * IN)]);
-                else if (DT == MXL_DT_BF16) f[j] = j & 1 ? bf16_hi(r[u][j / 2]) : bf16_lo(r[u][j / 2]);
-                else f[j] = j & 1 ? half_hi(r[u][j / 2]) : half_lo(r[u][j / 2]);
-                f[j] = scaled<DT>(f[j], c, cf);
-            }
-            uint32_t o[4 * OUT];
-            if (DO == MXL_DT_F32) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j % (4 * OUT)] = __float_as_uint(f[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (DO == MXL_DT_BF16) o[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
-                    else o[j] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j + 1]) << 16);
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < OUT; ++q) {
-                const u32x4 v = {o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]};
-                __builtin_nontemporal_store(v, (u32x4*)(d + (int64_t)i * 16 * OUT) + q);
-            }
+            for (int j = 0; j < 4; ++j) r[u][j] = v[j];
+        } else {
+            const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(in, (int)threadIdx.x * 8, u * GN_THREADS * 8, 2);
+            r[u][0] = v[0], r[u][1] = v[1];
         }
     }
-    const int rest = n - eights * 8;
-    if ((int)threadIdx.x < rest) {
-        const int64_t i = hi - rest + threadIdx.x;
-        store_dt(dst, DO, i, scaled<DT>(load_dt(src, DT, i), c, cf));
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        float f[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (DT == MXL_DT_F32) f[j] = __uint_as_float(r[u][j % IW]);
+            else if (DT == MXL_DT_BF16) f[j] = j & 1 ? bf16_hi(r[u][j / 2]) : bf16_lo(r[u][j / 2]);
+            else f[j] = j & 1 ? half_hi(r[u][j / 2]) : half_lo(r[u][j / 2]);
+            f[j] = scaled<DT>(f[j], c, cf);
+        }
+        uint32_t o[OW];
+#pragma unroll
+        for (int j = 0; j < OW; ++j) {
+            if (DO == MXL_DT_F32) o[j] = __float_as_uint(f[j % PER]);
+            else if (DO == MXL_DT_BF16) o[j] = pack_bf16(f[2 * j % PER], f[(2 * j + 1) % PER]);
+            else o[j] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j % PER]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[(2 * j + 1) % PER]) << 16);
+        }
+        if constexpr (OW == 4) {
+            const gn_u32x4 t = {o[0], o[1], o[2], o[3]};
+            __builtin_amdgcn_raw_buffer_store_b128(t, out, (int)threadIdx.x * 16, u * GN_THREADS * 16, 2);
+        } else {
+            const u32x2 t = {o[0], o[1]};
+            __builtin_amdgcn_raw_buffer_store_b64(t, out, (int)threadIdx.x * 8, u * GN_THREADS * 8, 2);
+        }
+    }
+    const int rest = n - head - whole * PER;
+    if (head + rest) {
+        const int t = (int)threadIdx.x;
+        if (t < head || (t >= 64 && t - 64 < rest)) {
+            const int64_t i = t < head ? lo : hi - rest + (t - 64);
+            store_dt(dst, DO, i, scaled<DT>(load_dt(src, DT, i), c, cf));
+        }
     }
 }
 
@@ -221,37 +243,34 @@ __global__ __launch_bounds__(GN_THREADS) void clip_kernel(ClipTable t, const flo
     const bool within = raw >= 1.;          // (a NaN is not)
     const double c = within ? 1. : raw;
     const float cf = (float)c;
-    const uint32_t chunks = t.end[t.count - 1];
-    int at = 0;
-    for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
-        while (t.end[at] <= i) ++at;
-        const void* src = t.p[at];
-        void* dst = t.out[at];
-        const int64_t packed = t.n[at], n = packed & (((int64_t)1 << GN_TYPE_SHIFT) - 1);
-        const int types = (int)(packed >> GN_TYPE_SHIFT), in = types & 3, out = types >> 2;
-        if (within && src == dst) continue;
-        const uint32_t first = at ? t.end[at - 1] : 0;
-        const int64_t lo = (int64_t)(i - first) * GC_PER, hi = lo + GC_PER < n ? lo + GC_PER : n;
+    const uint32_t i = blockIdx.x;
+    const int at = TensorOf<GC_TENSORS>(t.end, t.count)(i);
+    const void* src = t.p[at];
+    void* dst = t.out[at];
+    if (within && src == dst) return;
+    const int64_t packed = t.n[at], n = packed & (((int64_t)1 << GN_TYPE_SHIFT) - 1);
+    const int types = (int)(packed >> GN_TYPE_SHIFT), in = types & 3, out = types >> 2;
+    const uint32_t first = at ? t.end[at - 1] : 0;
+    const int64_t lo = (int64_t)(i - first) * GC_PER, hi = lo + GC_PER < n ? lo + GC_PER : n;
 #define MXL_CLIP(DT, DO) clip_chunk<DT, DO>(src, dst, lo, hi, c, cf)
-        switch (in * 4 + out) {
-            case MXL_DT_F32 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_F32, MXL_DT_F32); break;
-            case MXL_DT_F32 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_F32, MXL_DT_BF16); break;
-            case MXL_DT_F32 * 4 + MXL_DT_F16: MXL_CLIP(MXL_DT_F32, MXL_DT_F16); break;
-            case MXL_DT_BF16 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_BF16, MXL_DT_F32); break;
-            case MXL_DT_BF16 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_BF16, MXL_DT_BF16); break;
-            case MXL_DT_BF16 * 4 + MXL_DT_F16: MXL_CLIP(MXL_DT_BF16, MXL_DT_F16); break;
-            case MXL_DT_F16 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_F16, MXL_DT_F32); break;
-            case MXL_DT_F16 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_F16, MXL_DT_BF16); break;
-            default: MXL_CLIP(MXL_DT_F16, MXL_DT_F16); break;
-        }
-#undef MXL_CLIP
+    switch (in * 4 + out) {
+        case MXL_DT_F32 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_F32, MXL_DT_F32); break;
+        case MXL_DT_F32 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_F32, MXL_DT_BF16); break;
+        case MXL_DT_F32 * 4 + MXL_DT_F16: MXL_CLIP(MXL_DT_F32, MXL_DT_F16); break;
+        case MXL_DT_BF16 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_BF16, MXL_DT_F32); break;
+        case MXL_DT_BF16 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_BF16, MXL_DT_BF16); break;
+        case MXL_DT_BF16 * 4 + MXL_DT_F16: MXL_CLIP(MXL_DT_BF16, MXL_DT_F16); break;
+        case MXL_DT_F16 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_F16, MXL_DT_F32); break;
+        case MXL_DT_F16 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_F16, MXL_DT_BF16); break;
+        default: MXL_CLIP(MXL_DT_F16, MXL_DT_F16); break;
     }
+#undef MXL_CLIP
 }
 
 static bool gn_list_ok(const void* const* p, const int64_t* n, const int32_t* dtypes, int count) {
     if (count < 0 || (count > 0 && (!p || !n || !dtypes))) return false;
     for (int i = 0; i < count; ++i)
-        if (n[i] < 0 || n[i] >= ((int64_t)1 << 40) || dtypes[i] < MXL_DT_F32 || dtypes[i] > MXL_DT_F16 || (n[i] > 0 && !p[i])) return false;
+        if (n[i] < 0 || n[i] >= ((int64_t)1 << 36) || dtypes[i] < MXL_DT_F32 || dtypes[i] > MXL_DT_F16 || (n[i] > 0 && !p[i])) return false;
     return true;
 }
 static int gn_size(int dtype) { return dtype == MXL_DT_F32 ? 4 : 2; }
@@ -346,7 +365,7 @@ extern "C" int mxl_clip_grads(const void* const* grads, void* const* outs, const
         for (; i < count && t.count < GC_TENSORS; ++i) {
             if (sizes[i] == 0) continue;
             const int64_t more = (sizes[i] + GC_PER - 1) / GC_PER;
-            if (more + chunks > 0x7FFFFFFF) break;
+            if (more + chunks > 0xFFFFFF) break;        // a launch has fewer than 2^32 threads
             chunks += (uint32_t)more;
             t.p[t.count] = grads[i];
             t.out[t.count] = outs[i];
@@ -354,8 +373,7 @@ extern "C" int mxl_clip_grads(const void* const* grads, void* const* outs, const
             t.end[t.count++] = chunks;
         }
         if (t.count == 0) break;
-        const int blocks = (int)(chunks < (uint32_t)GN_BLOCKS ? chunks : (uint32_t)GN_BLOCKS);
-        hipLaunchKernelGGL(clip_kernel, dim3((unsigned)blocks), dim3(GN_THREADS), 0, st, t, norm, max_norm);
+        hipLaunchKernelGGL(clip_kernel, dim3(chunks), dim3(GN_THREADS), 0, st, t, norm, max_norm);
         if (hipGetLastError() != hipSuccess) return MXL_ELAUNCH;
     }
     return MXL_OK;

@@ -923,11 +923,17 @@ def _block_norm(x, residual, weight, post_weight, gate, eps, post_eps, scale):
 
 
 def _grad_list(tensors, what: str):
+    """``(tensors, those without gaps)``: a copy stands for a tensor that has gaps."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
-            raise ValueError(f"{what} must be dense tensors")
-    return tensors
+    try:
+        if all(map(torch.Tensor.is_contiguous, tensors)):
+            return tensors, tensors
+        return tensors, [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    except (TypeError, RuntimeError):       # (something else in the list, or a layout without strides)
+        for t in tensors:
+            if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+                raise ValueError(f"{what} must be dense tensors") from None
+        raise
 
 
 @torch.no_grad()
@@ -935,12 +941,12 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of ``grads`` (tensors on one GPU, of any shapes and sizes, bfloat16, float16 and float32 mixed) as a float32 scalar on
     the device: ``sqrt(sum g^2)``, or ``max |g|`` for ``norm_type`` inf (NaN if there is one).  Squares are summed in fp64 in an order that
     depends on the sizes alone; they neither overflow nor underflow.  Nothing is read back to the host.  0 for no tensors or no elements."""
-    grads = _grad_list(grads, "gradients")
-    if not grads:
+    _, dense = _grad_list(grads, "gradients")
+    if not dense:
         if float(norm_type) not in K._NORM_KINDS:
             raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
         return torch.zeros((), dtype=torch.float32, device="cuda")
-    return K.grad_norm_impl([g.contiguous() for g in grads], norm_type)
+    return K.grad_norm_impl(dense, norm_type)
 
 
 @torch.no_grad()
@@ -950,34 +956,31 @@ def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = 
     the three types: the optimizer's float32 gradients of bfloat16 ones).  The factor is taken on the device and nothing is read back: within the bound, gradients
     in place are left untouched.  A norm of NaN makes every element NaN, an infinite one leaves zeros of what is finite.  No tensor that is written may
     overlap another one."""
-    grads = _grad_list(grads, "gradients")
+    targets, dense = _grad_list(grads, "gradients")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm!r}")
-    targets = grads
+    written = dense
     if out is not None:
-        targets = _grad_list(out, "out")
+        grads = targets
+        targets, written = _grad_list(out, "out")
         if len(targets) != len(grads) or any(o.shape != g.shape for o, g in zip(targets, grads)):
             raise ValueError("out must hold a tensor of the same shape for every gradient")
-    dense = [g.contiguous() for g in grads]
-    # the kernels write tensors without gaps: others get a copy of theirs
-    if out is None:
-        written = dense
-    else:
-        written = [o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device) for o in targets]
-    gaps = [t for t in targets if not t.is_contiguous()]
-    if len({t.data_ptr() for t in gaps}) < len(gaps) or any(st == 0 and n > 1 for t in gaps for st, n in zip(t.stride(), t.shape)):
-        raise ValueError("a tensor that is written must not overlap itself or another one")
+    if written is not targets:
+        gaps = [t for t, w in zip(targets, written) if w is not t]
+        if len({t.data_ptr() for t in gaps}) < len(gaps) or any(st == 0 and n > 1 for t in gaps for st, n in zip(t.stride(), t.shape)):
+            raise ValueError("a tensor that is written must not overlap itself or another one")
     if norm is None:
         norm = grad_norm(dense, norm_type)
     elif not isinstance(norm, torch.Tensor):
-        norm = torch.full((), float(norm), dtype=torch.float32, device=grads[0].device if grads else "cuda")
-    if not grads:
+        norm = torch.full((), float(norm), dtype=torch.float32, device=dense[0].device if dense else "cuda")
+    if not dense:
         return norm
     K.clip_grads_impl(dense, written, max_norm, norm)
-    for t, w in zip(targets, written):
-        if w is not t:
-            t.copy_(w)
+    if written is not targets:
+        for t, w in zip(targets, written):
+            if w is not t:
+                t.copy_(w)
     torch.autograd.graph.increment_version(targets)
     return norm
 

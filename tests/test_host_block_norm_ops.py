@@ -118,18 +118,20 @@ def test_c_entries_refuse():
                 dict(dtype=3), dict(dtype=0, stream_dtype=1), dict(stream_dtype=2), dict(eps=-1.0), dict(post_eps=math.nan), dict(cols=2), dict(div=3), dict(mod=0), dict(div=0),
                 dict(div=4), dict(mod=3, div=1)):
         assert call(**bad) == -1, bad
-    need = lib.mxl_block_norm_bwd_workspace_bytes(4, 8, 1, 1, 2, 2, 8)
-    assert need > 0 and lib.mxl_block_norm_bwd_workspace_bytes(4, 16385, 1, 1, 1, 1, 0) == -1 and lib.mxl_block_norm_bwd_workspace_bytes(4, 8, 1, 1, 3, 2, 8) == -1
-    assert lib.mxl_block_norm_bwd_workspace_bytes(0, 8, 1, 1, 0, 1, 8) == 0 and lib.mxl_block_norm_bwd_workspace_bytes(4, 8, 0, 0, 1, 1, 0) == 0
+    ws = lib.mxl_block_norm_bwd_workspace_bytes
+    need = ws(4, 8, 1, 1, 2, 2, 8, 1)
+    assert need > 0 and ws(4, 16385, 1, 1, 1, 1, 0, 0) == -1 and ws(4, 8, 1, 1, 3, 2, 8, 1) == -1
+    assert ws(0, 8, 1, 1, 0, 1, 8, 1) == 0 and ws(4, 8, 0, 0, 1, 1, 0, 0) == 0
     names = ("dy", "dh", "x", "h", "rows", "k", "dtype", "stream_dtype", "post_weight", "post_rstd", "gate", "div", "mod", "cols", "scale", "weight", "rstd", "dx", "dres", "dw", "dpw",
              "dgate", "ws", "bytes", "stream")
     right = dict(dy=p, dh=p, x=p, h=p, rows=4, k=8, dtype=1, stream_dtype=1, post_weight=p, post_rstd=p, gate=p, div=2, mod=2, cols=8, scale=1.0, weight=p, rstd=p, dx=p, dres=p, dw=p,
                  dpw=p, dgate=p, ws=p, bytes=need, stream=None)
     call = lambda **k: lib.mxl_block_norm_bwd(*[{**right, **k}[n] for n in names])  # noqa: E731
     assert call() == -3 and call(dh=None) == -3 and call(dx=None, dres=None) == -3 and call(post_weight=None, post_rstd=None, dpw=None) == -3
-    assert call(weight=None, dy=None, h=None, rstd=None, dw=None) == -3 and call(rows=0, dw=None, dpw=None) == 0
+    assert call(weight=None, dy=None, h=None, rstd=None, dw=None, dres=None) == -3 and call(rows=0, dw=None, dpw=None) == 0
     for bad in (dict(dy=None), dict(x=None), dict(h=None), dict(rstd=None), dict(post_rstd=None), dict(gate=None), dict(ws=None), dict(bytes=need - 1), dict(ws=p + 8),
-                dict(weight=None), dict(post_weight=None), dict(weight=None, post_weight=None, dw=None, dpw=None), dict(mod=3), dict(k=0)):
+                dict(weight=None, dres=None), dict(weight=None, dw=None), dict(post_weight=None),
+                dict(weight=None, post_weight=None, dw=None, dpw=None, dres=None), dict(mod=3), dict(k=0)):
         assert call(**bad) == -1, bad
     # lists
     spans = [(p, 10, 0), (p + 64, 7, 1)]
