@@ -1558,41 +1558,50 @@ def block_norm_impl(x, residual, weight, eps: float, post_weight, post_eps: floa
 def block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate, scale: float, need_x: bool = True, need_residual: bool = True,
                         need_weight: bool = True, need_post_weight: bool = True, need_gate: bool = True):
     """``(dx, dresidual, dweight, dpost_weight, dgate)`` of ``block_norm_impl``, given the gradients of ``y`` and ``h`` (None: zero).  ``x`` may be None where
-    it is not needed: without ``post_weight``, and with no gradient of the gate."""
+    it is not needed: without ``post_weight``, and with no gradient of the gate.  Without ``weight`` the residual's gradient is ``dh``, and None here.
+    (What the forward has checked is looked at again only as far as saved tensors may come back changed: this runs on autograd's thread, where a
+    line of Python costs twice what it does on the caller's.)"""
+    pre, post = weight is not None, post_weight is not None
     like = x if x is not None else dy
-    rows_of = h if h is not None else dh
-    rows, k, dtype, stream_dtype, (div, mod, cols) = _block_norm_args(like, rows_of, weight, post_weight, gate)
-    dev = like.device
-    need_weight, need_post_weight, need_gate = need_weight and weight is not None, need_post_weight and post_weight is not None, need_gate and gate is not None
-    if (weight is not None and (dy is None or h is None or rstd is None)) or ((post_weight is not None or need_gate) and x is None):
+    stream = h if pre else dh
+    need_gate = need_gate and gate is not None
+    if like is None or stream is None or (pre and (dy is None or rstd is None)) or (post and (x is None or post_rstd is None)) or (need_gate and x is None) or not (pre or post):
         raise ValueError("the gradient needs what the forward kept")
-    for name, t, want in (("dy", dy, like.dtype), ("dh", dh, rows_of.dtype), ("x", x, like.dtype), ("h", h, rows_of.dtype)):
-        if t is not None and (t.dtype != want or t.shape != like.shape or t.device != dev or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous, of the forward's type, shape and device")
-    for t in (weight, rstd, post_weight, post_rstd, gate):
-        if t is not None and (not t.is_contiguous() or t.device != dev):
-            raise ValueError("operands must be contiguous, on one device")
-    for t in (rstd, post_rstd):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != rows):
-            raise ValueError("rstd must be float32 [rows]")
-    lib = _lib.load()
+    shape, want, stream_want = like.shape, like.dtype, stream.dtype
+    k = shape[-1]
+    rows = like.numel() // k
+    dev = like.device
+    for t in (dy, x):
+        if t is not None and (t.dtype != want or t.shape != shape or t.device != dev or not t.is_contiguous()):
+            raise ValueError("the gradient of y, and x, must be contiguous and of the type, shape and device that the forward's x has")
+    for t in (dh, h):
+        if t is not None and (t.dtype != stream_want or t.shape != shape or t.device != dev or not t.is_contiguous()):
+            raise ValueError("the gradient of h, and h, must be contiguous and of the type, shape and device that the forward's residual has")
+    for t, n in ((weight, k), (post_weight, k), (rstd, rows), (post_rstd, rows)):
+        if t is not None and (t.numel() != n or t.device != dev or not t.is_contiguous() or (t.dtype != want and t.dtype != torch.float32)):
+            raise ValueError("weights and rstd must be contiguous vectors of the rows' and columns' number, on one device")
+    div, mod, cols = 1, 1, 0
+    if gate is not None:
+        if gate.dtype != want or gate.device != dev or not gate.is_contiguous():
+            raise ValueError("gate must be contiguous and of the type and device that the forward's x has")
+        div, mod, cols = _gate_rows(shape, gate.shape)
+    need_weight, need_post_weight = need_weight and pre, need_post_weight and post
+    need_residual = need_residual and pre
     # one tensor where both gradients are the same
-    same = need_x and need_residual and weight is not None and post_weight is None and gate is None and scale == 1.0 and dtype == stream_dtype
+    same = need_x and need_residual and not post and gate is None and scale == 1.0 and want == stream_want
     with _on(dev), _hooked("block_norm_bwd", rows=rows, k=k):
         dx = torch.empty_like(like) if need_x and not same else None
-        dres = torch.empty_like(rows_of) if need_residual and weight is not None else None
+        dres = torch.empty_like(stream) if need_residual else None
         dw = torch.empty_like(weight) if need_weight else None
         dpw = torch.empty_like(post_weight) if need_post_weight else None
-        dgate = None
-        if need_gate:
-            dgate = torch.empty_like(gate) if rows else torch.zeros_like(gate)
+        dgate = (torch.empty_like(gate) if rows else torch.zeros_like(gate)) if need_gate else None
         ws, nbytes = _workspace(dev, "mxl_block_norm_bwd_workspace_bytes", rows, k, need_weight, need_post_weight, div, mod, cols, need_gate)
-        rc = lib.mxl_block_norm_bwd(None if dy is None else dy.data_ptr(), None if dh is None else dh.data_ptr(), None if x is None else x.data_ptr(),
-                                    None if h is None else h.data_ptr(), rows, k, dtype, stream_dtype, None if post_weight is None else post_weight.data_ptr(),
-                                    None if post_rstd is None else post_rstd.data_ptr(), None if gate is None else gate.data_ptr(), div, mod, cols, scale,
-                                    None if weight is None else weight.data_ptr(), None if rstd is None else rstd.data_ptr(), None if dx is None else dx.data_ptr(),
-                                    None if dres is None else dres.data_ptr(), None if dw is None else dw.data_ptr(), None if dpw is None else dpw.data_ptr(),
-                                    None if dgate is None else dgate.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream())
+        rc = _lib.load().mxl_block_norm_bwd(
+            None if dy is None else dy.data_ptr(), None if dh is None else dh.data_ptr(), None if x is None else x.data_ptr(), None if h is None else h.data_ptr(),
+            rows, k, _DT[want], _DT[stream_want], post_weight.data_ptr() if post else None, post_rstd.data_ptr() if post else None,
+            None if gate is None else gate.data_ptr(), div, mod, cols, scale, weight.data_ptr() if pre else None, rstd.data_ptr() if pre else None,
+            None if dx is None else dx.data_ptr(), None if dres is None else dres.data_ptr(), dw.data_ptr() if need_weight else None,
+            dpw.data_ptr() if need_post_weight else None, dgate.data_ptr() if need_gate else None, None if ws is None else ws.data_ptr(), nbytes, _stream())
     if rc:
         _lib.check(rc, "mxl_block_norm_bwd")
     return dres if same else dx, dres, dw, dpw, dgate

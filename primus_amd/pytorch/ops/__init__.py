@@ -867,7 +867,7 @@ class _BlockNorm(torch.autograd.Function):
         if need_grad:
             keep_x = post_weight is not None or (gate is not None and ctx.needs_input_grad[4])
             ctx.save_for_backward(x if keep_x else None, h if weight is not None else None, weight, rstd, post_weight, post_rstd, gate)
-            ctx.scale, ctx.shape = scale, (x.shape, x.dtype, h.dtype, x.device)
+            ctx.scale, ctx.dtypes = scale, (x.dtype, h.dtype)
             ctx.set_materialize_grads(False)
         return h if weight is None else (y, h)
 
@@ -875,19 +875,19 @@ class _BlockNorm(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, *grads):
         x, h, weight, rstd, post_weight, post_rstd, gate = ctx.saved_tensors
-        shape, dtype, stream_dtype, dev = ctx.shape
+        dtype, stream_dtype = ctx.dtypes
         dy, dh = grads if weight is not None else (None, grads[0])
         if dy is None and dh is None:
             return (None,) * 9
         if weight is not None:
-            dy = torch.zeros(shape, dtype=dtype, device=dev) if dy is None else dy.to(dtype).contiguous()
+            dy = torch.zeros(dh.shape, dtype=dtype, device=dh.device) if dy is None else (dy if dy.dtype == dtype else dy.to(dtype)).contiguous()
         if dh is not None:
-            dh = dh.to(stream_dtype).contiguous()
+            dh = (dh if dh.dtype == stream_dtype else dh.to(stream_dtype)).contiguous()
         need_x, need_residual, need_weight, need_post, need_gate = ctx.needs_input_grad[:5]
         if weight is None and not (need_x or need_post or need_gate):
             return None, dh, None, None, None, None, None, None, None
-        dx, dres, dw, dpw, dgate = K.block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate, ctx.scale, need_x,
-                                                         need_residual and weight is not None, need_weight, need_post, need_gate)
+        dx, dres, dw, dpw, dgate = K.block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate, ctx.scale, need_x, need_residual, need_weight,
+                                                         need_post, need_gate)
         return dx, dres if weight is not None else dh if need_residual else None, dw, dpw, dgate, None, None, None, None
 
 
