@@ -658,8 +658,8 @@ int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_b
  * wanted).  k <= 16384, any; at least one of the weights.
  *
  * mxl_block_norm_bwd: gradients given those of y (dy; not looked at without weight) and of h (dh, stream_dtype; NULL: zero).  Any output may be
- * NULL: not wanted.  dresidual is of stream_dtype; without weight it is dh itself and must be NULL.  dx is the residual's gradient, and is not
- * written, where it is NULL with weight, without post_weight and without a gate of vectors.  x is looked at with post_weight or dgate, h with weight.
+ * NULL: not wanted.  dresidual is of stream_dtype; without weight it is dh itself and must be NULL.  Without post_weight and gate and
+ * with a scale of 1, dx has the values of dresidual.  x is looked at with post_weight or dgate, h with weight.
  * mxl_block_norm_bwd_workspace_bytes: has_weight, has_post_weight: whether dweight, dpost_weight are wanted; gate_cols 0: no gate. */
 int mxl_block_norm(const void* x, const void* residual, int64_t rows, int64_t k, int dtype, int stream_dtype, const void* post_weight,
                    float post_eps, const void* gate, int64_t gate_div, int64_t gate_mod, int64_t gate_cols, float scale, const void* weight,

@@ -30,9 +30,15 @@ struct BlockNormBwdArgs {
     float *part_w, *part_p, *part_g;
 };
 
-// SAME: no gradient of x apart from the residual's.  GATEV: the gate is a vector, and groups are its rows.  DEPTH rows are asked for ahead
-// of the one that is worked on.
-template <int T, int S, int CH, bool PRE, bool POST, bool SAME, bool GATEV, bool SMALL, bool ANY, int BOUND, int DEPTH>
+// Whether a lane has the weights and their sums in registers.  Two chunks of both norms, or of a norm and a gate of vectors, do not fit: the
+// weights are loaded again for every row (from the caches) and their sums are in shared memory, 64 bytes a lane each.  us, in registers (spilt)
+// and so, [2730, 12288]: both norms 158 and 109, and a stream in fp32 and a gate 263 and 199, a norm and a gate a row 122 and 111; a norm without
+// one 62 and 69.
+constexpr bool bn_bwd_keeps(int chunks, bool pre, bool post, bool gate) { return chunks == 1 || !pre || !(post || gate); }
+
+// SAME: no gradient of x apart from the residual's.  GATEV: the gate is a vector, and groups are its rows.  AHEAD: the next row is asked for
+// before the present one is worked on.
+template <int T, int S, int CH, bool PRE, bool POST, bool SAME, bool GATEV, bool SMALL, bool ANY, int BOUND, bool AHEAD>
 __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs p) {
     constexpr int NS = PRE && POST ? 4 : 1;
     __shared__ float part[2][BN_MAX_WAVES][NS];
@@ -45,12 +51,27 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
     typedef RowsOf<T, S, SMALL, ANY> RowsT;
     typedef RowsOf<S, S, SMALL, ANY> RowsS;
     const Cols<S> cols = {lanes, lane, k};
-    constexpr bool KEEP = CH == 1;
+    constexpr bool KEEP = bn_bwd_keeps(CH, PRE, POST, GATEV);
     // wq: post_weight times the gate where that is a vector.  au: sum of xh t (x t without post_weight) over the rows of one gate, whose
     // gradient is scale * post_weight times that, and dpost_weight's part of them scale * gate times it.
     float w[CH][BN_VEC], wp[CH][BN_VEC], wq[CH][BN_VEC];
     Raw8<T> gv[CH];
     float aw[CH][BN_VEC], ap[CH][BN_VEC], au[CH][BN_VEC], ags = 0.f;
+    extern __shared__ __attribute__((aligned(16))) uint8_t bn_lds[];
+    float4* const sums_of = (float4*)bn_lds + lane;
+    auto add = [&](float (&reg)[CH][BN_VEC], int which, int j, const float* v) {
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int e = 0; e < BN_VEC; ++e) reg[j][e] += v[e];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float4* s = sums_of + ((which * CH + j) * 2 + q) * lanes;
+                const float4 o = *s;
+                *s = make_float4(o.x + v[4 * q], o.y + v[4 * q + 1], o.z + v[4 * q + 2], o.w + v[4 * q + 3]);
+            }
+        }
+    };
     auto weight = [&](const void* base, int j, float* v) { unpack8<T>(load_vector<T>(base, cols, j), v); };
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
@@ -59,29 +80,32 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
         if (KEEP && POST) weight(p.post_weight, j, wp[j]);
 #pragma unroll
         for (int e = 0; e < BN_VEC; ++e) aw[j][e] = ap[j][e] = au[j][e] = 0.f;
+        if (!KEEP) {        // (a lane has its sums to itself: no barrier)
+#pragma unroll
+            for (int q = 0; q < 2 * (PRE + POST); ++q) sums_of[(q / 2 * CH * 2 + j * 2 + q % 2) * lanes] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
     }
     const bool gate_wanted = p.dgate != nullptr;
     const void* x_in = POST || gate_wanted ? p.x : nullptr;
 
-    // rows that are asked for ahead, as they lie in memory
-    constexpr int BUFS = DEPTH > 1 ? DEPTH : 1;
-    Raw8<T> xn[BUFS][CH], dyn[BUFS][CH];
-    Raw8<S> hn[BUFS][CH], dhn[BUFS][CH];
-    float rn[BUFS], rpn[BUFS];
-    auto request = [&](int b, int64_t row) {
+    // a row as it lies in memory
+    Raw8<T> xn[CH], dyn[CH];
+    Raw8<S> hn[CH], dhn[CH];
+    float rn = 0.f, rpn = 0.f;
+    auto request = [&](int64_t row) {
         const RowsT in_x(x_in, p.rows, row, k), in_dy(p.dy, p.rows, row, k);
         const RowsS in_h(p.h, p.rows, row, k), in_dh(p.dh, p.rows, row, k);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-            xn[b][j] = in_x.template load<BN_NT>(cols, j);
-            dhn[b][j] = in_dh.template load<BN_NT>(cols, j);
+            if (!SAME) xn[j] = in_x.template load<BN_NT>(cols, j);
+            dhn[j] = in_dh.template load<BN_NT>(cols, j);
             if (PRE) {
-                dyn[b][j] = in_dy.template load<BN_NT>(cols, j);
-                hn[b][j] = in_h.template load<BN_NT>(cols, j);
+                dyn[j] = in_dy.template load<BN_NT>(cols, j);
+                hn[j] = in_h.template load<BN_NT>(cols, j);
             }
         }
-        if (PRE) rn[b] = p.rstd[row];
-        if (POST) rpn[b] = p.post_rstd[row];
+        if (PRE) rn = p.rstd[row];
+        if (POST) rpn = p.post_rstd[row];
     };
     // this worker's rows
     struct At {
@@ -109,12 +133,10 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
     At at = {g0, first, 0, worker < p.active && g0 < p.groups && first < p.each}, ahead;
     if (at.live) row_of(at);
     ahead = at;
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-        if (ahead.live) {
-            request(d, ahead.row);
-            advance(ahead);
-        }
+    if (AHEAD && ahead.live) {
+        request(ahead.row);
+        advance(ahead);
+    }
     int64_t gate_row = -1;
     auto gated = [&](int j) {       // wq of a vector gate
         float f[BN_VEC];
@@ -128,23 +150,37 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
         if (!KEEP && POST) weight(p.post_weight, j, wp[j]);
 #pragma unroll
         for (int e = 0; e < BN_VEC; ++e) {
-            if (POST) ap[j][e] += p.scale * f[e] * au[j][e];
+            if (POST) f[e] *= p.scale * au[j][e];
             dgate[e] = p.scale * (POST ? wp[j][e] * au[j][e] : au[j][e]);
             au[j][e] = 0.f;
         }
+        if (POST) add(ap, PRE, j, f);
     };
 
-    auto one_row = [&](int b) {
-        if (DEPTH == 0) request(b, at.row);
+    while (at.live) {
+        if (!AHEAD) request(at.row);
+        // the row's chunks as floats, x (with post_weight) and h normalised
         float x[CH][BN_VEC], t[CH][BN_VEC], dy[CH][BN_VEC], hh[CH][BN_VEC];
-        const float r = PRE ? rn[b] : 0.f, rp = POST ? rpn[b] : 0.f;
+        const float r = rn, rp = rpn;
+        auto weights_again = [&](int j) {
+            const void *pw = p.weight, *pp = p.post_weight;
+            asm volatile("" : "+s"(pw), "+s"(pp));      // (or they are loaded in front of the loop, and kept)
+            if (PRE) weight(pw, j, w[j]);
+            if (POST) weight(pp, j, wp[j]);
+            if (GATEV) gated(j);
+        };
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-            unpack8<S>(dhn[b][j], t[j]);
-            if (POST || GATEV || gate_wanted) unpack8<T>(xn[b][j], x[j]);
+            unpack8<S>(dhn[j], t[j]);
+            if (!SAME) unpack8<T>(xn[j], x[j]);
             if (PRE) {
-                unpack8<T>(dyn[b][j], dy[j]);
-                unpack8<S>(hn[b][j], hh[j]);
+                unpack8<T>(dyn[j], dy[j]);
+                unpack8<S>(hn[j], hh[j]);
+            }
+#pragma unroll
+            for (int e = 0; e < BN_VEC; ++e) {
+                if (POST) x[j][e] *= rp;
+                if (PRE) hh[j][e] *= r;
             }
         }
         const int64_t row = at.row;
@@ -163,8 +199,8 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
             const int64_t gr = gate_wanted ? at.g : (int64_t)((uint32_t)row / p.gate.div % p.gate.mod);
             factor *= (float)((const typename DtOf<T>::type*)p.gate.p)[gr];
         }
-        if (DEPTH > 0 && ahead.live) {
-            request(b, ahead.row);
+        if (AHEAD && ahead.live) {
+            request(ahead.row);
             advance(ahead);
         }
         // The row's sums.  (Columns past the row hold zeros in all that is read, a gate's vector too.  A factor of the whole row, which may
@@ -174,21 +210,15 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
         for (int n = 0; n < NS; ++n) v[n] = 0.f;
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-            if (!KEEP) {
-                if (PRE) weight(p.weight, j, w[j]);
-                if (POST) weight(p.post_weight, j, wp[j]);
-                if (GATEV) gated(j);
-            }
+            if (!KEEP) weights_again(j);
 #pragma unroll
             for (int e = 0; e < BN_VEC; ++e) {
                 float q = 0.f;
                 if (POST) {
-                    x[j][e] *= rp;
                     q = x[j][e] * (GATEV ? wq[j][e] : wp[j][e]);
                 }
                 if (PRE) {
                     const float d = dy[j][e] * w[j][e];
-                    hh[j][e] *= r;
                     v[0] += d * hh[j][e];
                     if (POST) {
                         v[NS - 3] += q * t[j][e];
@@ -212,24 +242,27 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
         const RowsS out_r(p.dres, p.rows, row, k);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-            float o[BN_VEC];
+            float o[BN_VEC], of_w[BN_VEC], of_p[BN_VEC];
+            if (!KEEP) weights_again(j);
 #pragma unroll
             for (int e = 0; e < BN_VEC; ++e) {
                 if (PRE) {
                     t[j][e] += r * (dy[j][e] * w[j][e]);
                     t[j][e] -= hh[j][e] * rc1;
-                    aw[j][e] += dy[j][e] * hh[j][e];
+                    of_w[e] = dy[j][e] * hh[j][e];
                 }
                 if (POST) {
                     o[e] = t[j][e] * (GATEV ? wq[j][e] : wp[j][e]) * rw - x[j][e] * rc2;
                     if (GATEV) au[j][e] += x[j][e] * t[j][e];
-                    else ap[j][e] += x[j][e] * t[j][e] * whole;
+                    else of_p[e] = x[j][e] * t[j][e] * whole;
                 } else {
                     if (GATEV) au[j][e] += x[j][e] * t[j][e];
-                    else if (gate_wanted) nt += x[j][e] * t[j][e];
+                    else if (!SAME) nt += x[j][e] * t[j][e];
                     if (!SAME) o[e] = t[j][e] * (GATEV ? wq[j][e] : factor);
                 }
             }
+            if (PRE) add(aw, 0, j, of_w);
+            if (POST && !GATEV) add(ap, PRE, j, of_p);
             if (!SAME) out_x.store(cols, j, o);
             if (PRE) out_r.store(cols, j, t[j]);
         }
@@ -260,19 +293,21 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
                 ags = 0.f;
             }
         }
-    };
-    while (at.live) {
-        one_row(0);
-        if (DEPTH > 1) {
-            if (!at.live) break;
-            one_row(BUFS - 1);
-        }
     }
     // what several workers share, for the second kernel: a row of a workgroup or, of short rows, of a wave
     float ag[CH][BN_VEC];
     if (GATEV) {
 #pragma unroll
         for (int j = 0; j < CH; ++j) gate_done(j, ag[j]);       // (nothing is left where a worker has its gates to itself)
+    }
+    if (!KEEP) {
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (PRE) *(float4*)&aw[j][4 * q] = sums_of[(j * 2 + q) * lanes];
+                if (POST) *(float4*)&ap[j][4 * q] = sums_of[((PRE * CH + j) * 2 + q) * lanes];
+            }
     }
     int64_t to = blockIdx.x;
     if (SMALL) {
@@ -342,6 +377,6 @@ inline int64_t block_norm_gate_rows(const BlockNormPlan& q) {       // float row
     return q.share > 1 ? q.part_rows : 0;
 }
 
-template <int T, int S> void block_norm_bwd_launch(const BlockNormBwdArgs& p, const BlockNormPlan& q, hipStream_t st);
+template <int T, int S> int block_norm_bwd_launch(const BlockNormBwdArgs& p, const BlockNormPlan& q, hipStream_t st);
 
 }  // namespace mxl

@@ -132,12 +132,13 @@ extern "C" int mxl_block_norm_bwd(const void* dy, const void* dh, const void* x,
     if (rows > 0) {
         BlockNormBwdArgs p = {dy, dh, x, h, post_weight, weight, post_rstd, rstd, bn_gate(gate, rows, gate_div, gate_mod, gate_cols, k), scale, (int)k, q.ldk,
                               q.lanes, rows, q.groups, q.each, q.share, q.gstep, q.gdiv, q.active, dx, dresidual, dgate, part_w, part_p, part_g};
-        if (dtype == MXL_DT_F32) block_norm_bwd_launch<MXL_DT_F32, MXL_DT_F32>(p, q, st);
-        else if (dtype == MXL_DT_BF16 && stream_dtype == MXL_DT_BF16) block_norm_bwd_launch<MXL_DT_BF16, MXL_DT_BF16>(p, q, st);
-        else if (dtype == MXL_DT_BF16) block_norm_bwd_launch<MXL_DT_BF16, MXL_DT_F32>(p, q, st);
-        else if (stream_dtype == MXL_DT_F16) block_norm_bwd_launch<MXL_DT_F16, MXL_DT_F16>(p, q, st);
-        else block_norm_bwd_launch<MXL_DT_F16, MXL_DT_F32>(p, q, st);
-        if (hipGetLastError() != hipSuccess) return MXL_ELAUNCH;
+        int rc;
+        if (dtype == MXL_DT_F32) rc = block_norm_bwd_launch<MXL_DT_F32, MXL_DT_F32>(p, q, st);
+        else if (dtype == MXL_DT_BF16 && stream_dtype == MXL_DT_BF16) rc = block_norm_bwd_launch<MXL_DT_BF16, MXL_DT_BF16>(p, q, st);
+        else if (dtype == MXL_DT_BF16) rc = block_norm_bwd_launch<MXL_DT_BF16, MXL_DT_F32>(p, q, st);
+        else if (stream_dtype == MXL_DT_F16) rc = block_norm_bwd_launch<MXL_DT_F16, MXL_DT_F16>(p, q, st);
+        else rc = block_norm_bwd_launch<MXL_DT_F16, MXL_DT_F32>(p, q, st);
+        if (rc != MXL_OK) return rc;
     }
     BlockNormSumArgs s = {};
     if (dweight) s.part[s.jobs] = part_w, s.out[s.jobs++] = dweight;

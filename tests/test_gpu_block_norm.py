@@ -242,14 +242,16 @@ def test_strides_offsets_and_orders(gpu):
 def test_gradients_that_are_not_asked_for(gpu):
     from primus_amd.pytorch import ops
 
-    for k in (64, 600):
-        v, dy, dh = _inputs((5, 4), k, BF, FP, True, "first", device=gpu)
+    for k, gate, has_post in ((64, "first", True), (600, "first", True), (64, "token", True), (600, "token", True), (600, "token", False), (9000, "token", False),
+                              (600, "column", False), (9001, "element", True)):
+        v, dy, dh = _inputs((5, 4), k, BF, FP, has_post, gate, device=gpu)
+        v = {n: t for n, t in v.items() if t is not None}
         names = list(v)
 
         def grads(needed, pre=True, given=(True, True)):
-            a = {n: t.detach().clone().requires_grad_(n in needed) for n, t in v.items()}
+            a = {n: t.detach().clone().requires_grad_(n in needed) for n, t in v.items() if t is not None}
             if pre:
-                made = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], EPS, post_weight=a["post_weight"], gate=a["gate"], scale=0.5)
+                made = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], EPS, post_weight=a.get("post_weight"), gate=a["gate"], scale=0.5)
             else:
                 made = (ops.rmsnorm_add(a["x"], a["residual"], a["post_weight"], EPS, gate=a["gate"], scale=0.5),)
             use = [(m, d) for m, d, w in zip(made, (dy, dh) if pre else (dh,), given) if w]
@@ -258,11 +260,13 @@ def test_gradients_that_are_not_asked_for(gpu):
         every = grads(names)
         for n in names:
             assert torch.equal(grads([n])[n], every[n]), n
-        post = [n for n in names if n != "weight"]
-        every = grads(post, False)
-        for n in post:
-            assert torch.equal(grads([n], False)[n], every[n]), n
-        assert torch.equal(every["residual"], dh)
+        if has_post:
+            post = [n for n in names if n != "weight"]
+            every = grads(post, False)
+            for n in post:
+                assert torch.equal(grads([n], False)[n], every[n]), n
+            assert torch.equal(every["residual"], dh)
+        v["post_weight"] = v.get("post_weight")
         # y or h alone
         want = _reference(v, dy, None, 0.5, BF, FP, post_eps=EPS)
         for n, got in grads(names, given=(True, False)).items():
