@@ -14,7 +14,7 @@ struct BlockNormArgs {
     const void *x, *residual, *post_weight, *weight;
     Gate gate;
     float scale, post_eps, eps;
-    int64_t rows;
+    int64_t rows, row0;         // this launch's first row
     int k, lanes;
     void *y, *h;
     float *post_rstd, *rstd;
@@ -31,7 +31,7 @@ __global__ __launch_bounds__(SMALL ? BN_SMALL_THREADS : BN_MAX_THREADS) void blo
     __shared__ float part[2][BN_MAX_WAVES][1];
     const int lanes = SMALL ? p.lanes : (int)blockDim.x;
     const int lane = SMALL ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x;
-    const int64_t row = SMALL ? (int64_t)blockIdx.x * (BN_SMALL_THREADS / lanes) + threadIdx.x / lanes : blockIdx.x;
+    const int64_t row = p.row0 + (SMALL ? (int64_t)blockIdx.x * (BN_SMALL_THREADS / lanes) + threadIdx.x / lanes : blockIdx.x);
     if (SMALL && row >= p.rows) return;
     RowSums<1, SMALL> sums(part, lanes);
     const int k = p.k;
@@ -119,22 +119,26 @@ static int block_norm_chunks(const BlockNormArgs& p) {
     return p.weight && p.post_weight && p.k > 512 && p.rows > 512 ? 2 : 1;
 }
 
+// `per` rows a workgroup; a launch has fewer than 2^32 threads
 template <int T, int S, int CH, bool SMALL, bool ANY>
-static void block_norm_launch(const BlockNormArgs& p, int64_t blocks, int threads, hipStream_t st) {
-    const dim3 g((unsigned)blocks), b((unsigned)threads);
-    if (p.weight && p.post_weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, true, SMALL, ANY>), g, b, 0, st, p);
-    else if (p.weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, false, SMALL, ANY>), g, b, 0, st, p);
-    else hipLaunchKernelGGL((block_norm_kernel<T, S, CH, false, true, SMALL, ANY>), g, b, 0, st, p);
+static void block_norm_launch(BlockNormArgs& p, int64_t per, int threads, hipStream_t st) {
+    const int64_t most = 0xFFFFFFFFll / threads * per;
+    for (p.row0 = 0; p.row0 < p.rows; p.row0 += most) {
+        const int64_t rows = p.rows - p.row0 < most ? p.rows - p.row0 : most;
+        const dim3 g((unsigned)((rows + per - 1) / per)), b((unsigned)threads);
+        if (p.weight && p.post_weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, true, SMALL, ANY>), g, b, 0, st, p);
+        else if (p.weight) hipLaunchKernelGGL((block_norm_kernel<T, S, CH, true, false, SMALL, ANY>), g, b, 0, st, p);
+        else hipLaunchKernelGGL((block_norm_kernel<T, S, CH, false, true, SMALL, ANY>), g, b, 0, st, p);
+    }
 }
 template <int T, int S, bool ANY> static void block_norm_launch(BlockNormArgs& p, hipStream_t st) {
     if (p.k <= BN_SMALL_K) {
         p.lanes = bn_lanes(p.k);
-        const int64_t per = BN_SMALL_THREADS / p.lanes;
-        block_norm_launch<T, S, 1, true, ANY>(p, (p.rows + per - 1) / per, BN_SMALL_THREADS, st);
+        block_norm_launch<T, S, 1, true, ANY>(p, BN_SMALL_THREADS / p.lanes, BN_SMALL_THREADS, st);
     } else if (block_norm_chunks(p) == 1) {
-        block_norm_launch<T, S, 1, false, ANY>(p, p.rows, bn_threads(p.k, 1), st);
+        block_norm_launch<T, S, 1, false, ANY>(p, 1, bn_threads(p.k, 1), st);
     } else {
-        block_norm_launch<T, S, 2, false, ANY>(p, p.rows, bn_threads(p.k, 2), st);
+        block_norm_launch<T, S, 2, false, ANY>(p, 1, bn_threads(p.k, 2), st);
     }
 }
 template <int T, int S> static void block_norm_launch(BlockNormArgs& p, hipStream_t st) {
@@ -154,7 +158,7 @@ extern "C" int mxl_block_norm(const void* x, const void* residual, int64_t rows,
     if (rows == 0) return MXL_OK;
     if (!x || !residual || !h || (weight && !y)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
-    BlockNormArgs p = {x, residual, post_weight, weight, bn_gate(gate, rows, gate_div, gate_mod, gate_cols, k), scale, post_eps, eps, rows, (int)k, 0,
+    BlockNormArgs p = {x, residual, post_weight, weight, bn_gate(gate, rows, gate_div, gate_mod, gate_cols, k), scale, post_eps, eps, rows, 0, (int)k, 0,
                        y, h, post_rstd, rstd};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == MXL_DT_F32) block_norm_launch<MXL_DT_F32, MXL_DT_F32>(p, st);

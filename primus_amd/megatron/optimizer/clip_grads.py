@@ -1,0 +1,41 @@
+"""Gradient norm and clipping under the names that Megatron-LM's optimizers import (``megatron.core.optimizer.clip_grads``), on the
+operators of this package: every gradient is read once for the norm and the factor stays on the device, so a step does not
+wait for the host.  ``patches/turbo.py`` installs both with ``use_turbo_clip_grads``.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Iterable, List, Optional, Union
+
+import torch
+
+from ...pytorch import ops
+
+
+@torch.no_grad()
+def get_grad_norm_fp32(grads_for_norm: Union[List[torch.Tensor], torch.Tensor], norm_type: Union[int, float] = 2,
+                       grad_stats_parallel_group: Optional["torch.distributed.ProcessGroup"] = None) -> torch.Tensor:
+    """Norm of the gradients of all ranks of ``grad_stats_parallel_group`` (None: of this one), 2 or inf: a float32 scalar on the device, which
+    formats and compares like the number it stands for.  Between the ranks squares are added in float64."""
+    norm = ops.grad_norm(grads_for_norm, float(norm_type))
+    if grad_stats_parallel_group is None:
+        return norm
+    if float(norm_type) == math.inf:
+        torch.distributed.all_reduce(norm, op=torch.distributed.ReduceOp.MAX, group=grad_stats_parallel_group)
+        return norm
+    total = norm.double().square()
+    torch.distributed.all_reduce(total, op=torch.distributed.ReduceOp.SUM, group=grad_stats_parallel_group)
+    return total.sqrt().float()
+
+
+@torch.no_grad()
+def clip_grad_by_total_norm_fp32(parameters: Union[Iterable[torch.Tensor], torch.Tensor], max_norm: Union[int, float],
+                                 total_norm: Union[torch.Tensor, float], use_decoupled_grad: bool = False) -> None:
+    """Scales the parameters' gradients (``decoupled_grad`` or ``grad``; parameters without one are left out) in place by
+    ``min(1, max_norm / (total_norm + 1e-6))``."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [getattr(p, "decoupled_grad", None) if use_decoupled_grad else p.grad for p in parameters]
+    grads = [g.detach() for g in grads if g is not None]
+    if grads:
+        ops.clip_grads(grads, max_norm, norm=total_norm)

@@ -26,6 +26,8 @@ _SPEC_PROVIDER_TARGETS = (
     "megatron.core.models.gpt.moe_module_specs",
     "megatron.core.transformer.multi_token_prediction",
 )
+# the functions' own module, and the one that has imported them by name
+_CLIP_GRADS_TARGETS = ("megatron.core.optimizer.clip_grads", "megatron.core.optimizer.optimizer")
 
 
 @dataclass
@@ -134,6 +136,18 @@ def patch_te_spec_provider(ctx: PatchContext) -> None:
     for path in _SPEC_PROVIDER_TARGETS:
         ctx.module(path).TESpecProvider = PrimusTurboSpecProvider
         ctx.log.append(f"[Patch:megatron.turbo.te_spec_provider] patched {path}.TESpecProvider")
+
+
+@register_patch("megatron.optimizer.clip_grads", condition=lambda ctx: bool(getattr(ctx.args, "use_turbo_clip_grads", False)) and is_primus_turbo_can_patch(ctx),
+                description="gradient norm and clipping -> the multi-tensor kernels")
+def patch_clip_grads(ctx: PatchContext) -> None:
+    from ..optimizer import clip_grads
+
+    for path in _CLIP_GRADS_TARGETS:
+        module = ctx.module(path)
+        module.get_grad_norm_fp32 = clip_grads.get_grad_norm_fp32
+        module.clip_grad_by_total_norm_fp32 = clip_grads.clip_grad_by_total_norm_fp32
+        ctx.log.append(f"[Patch:megatron.optimizer.clip_grads] patched {path}")
 
 
 def apply_patches(args, targets: Optional[Dict[str, object]] = None) -> PatchContext:

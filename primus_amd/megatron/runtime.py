@@ -35,6 +35,7 @@ _DEFAULT_ARGS = dict(
     patch_zero_bubble=False,
     enable_zero_bubble=False,
     mxfp4_gradient_stochastic_rounding=False,
+    use_turbo_clip_grads=False,     # (this package's own)
 )
 
 _args = SimpleNamespace(**_DEFAULT_ARGS)

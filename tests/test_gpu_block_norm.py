@@ -382,11 +382,70 @@ def test_rows_beyond_32_bit_offsets(gpu):
     assert not y[:-40].any() and not dx[:-40].any()
 
 
-def test_on_another_stream_and_captured(gpu):
+@pytest.mark.parametrize("k,rows", [(64, (1 << 23) + 100), (1, (1 << 29) + (1 << 20)), (4, (1 << 28) + 40)])
+def test_many_short_rows(gpu, k, rows):
+    """Short rows whose tensor passes the descriptors' offsets, and more of them than a launch has threads for: the last rows are those of a
+    call on them alone, forward and backward."""
+    from primus_amd.pytorch import ops
+
+    x, r = (torch.zeros(rows, k, dtype=BF, device=gpu) for _ in range(2))
+    g = torch.Generator(device=gpu).manual_seed(1)
+    x[-70:], r[-70:] = (torch.randn(70, k, generator=g, device=gpu).to(BF) for _ in range(2))
+    w = torch.randn(k, generator=g, device=gpu).to(BF)
+    dy = torch.zeros(rows, k, dtype=BF, device=gpu)
+    dy[-70:] = torch.randn(70, k, generator=g, device=gpu).to(BF)
+    out = []
+    for a in ((x, r, dy), tuple(t[-70:].clone() for t in (x, r, dy))):
+        xs = a[0].requires_grad_()
+        y, h = ops.add_rmsnorm(xs, a[1], w)
+        (dx,) = torch.autograd.grad(y, xs, a[2])
+        out.append([t[-70:].clone() for t in (y, h, dx)])
+        if len(y) > 70:
+            assert not y[:-70].any() and not dx[:-70].any()
+        del y, h, dx
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def test_one_tensor_twice(gpu):
+    """x and the residual one tensor, a weight used by both norms, a gradient handed to several inputs."""
+    from primus_amd.pytorch import ops
+
+    for k in (64, 700):
+        g = torch.Generator().manual_seed(k)
+        x, w, dy, dh = (torch.randn(s, generator=g) for s in ((6, k), (k,), (6, k), (6, k)))
+        a, b = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_()
+        y, h = ops.add_rmsnorm(a, a, b, EPS)
+        got = torch.autograd.grad([y, h], [a, b], [dy.to(gpu), dh.to(gpu)])
+        want = _reference(dict(x=x, residual=x, weight=w, post_weight=None, gate=None), dy, dh, 1.0, FP, FP)
+        _close(got[0], (2 * want["x"][0], 2 * want["x"][1]), ("x twice", FP))
+        _close(got[1], want["weight"], ("weight", FP))
+        y, h = ops.add_rmsnorm(a, a, b, EPS, post_weight=b, post_eps=POST_EPS)
+        got = torch.autograd.grad([y, h], [a, b], [dy.to(gpu), dh.to(gpu)])
+        want = _reference(dict(x=x, residual=x, weight=w, post_weight=w, gate=None), dy, dh, 1.0, FP, FP)
+        for g1, n1, n2 in ((got[0], "x", "residual"), (got[1], "weight", "post_weight")):
+            # (and the sum of the two, half a step)
+            _close(g1, (want[n1][0] + want[n2][0], want[n1][1] + want[n2][1] + E * (want[n1][0] + want[n2][0]).abs()), (n1, FP))
+
+
+def test_saved_tensors_that_come_back_otherwise_are_refused(gpu):
+    from primus_amd.pytorch import ops
+
+    v, dy, dh = _inputs((4, 4), 96, BF, BF, True, "", device=gpu)
+    v = {n: t.requires_grad_() for n, t in v.items() if t is not None}
+    for pack, unpack in ((lambda t: t, lambda t: t.transpose(0, 1) if t.dim() > 1 else t), (lambda t: t, lambda t: t.float() if t.dtype == BF else t.double()),
+                         (lambda t: t, lambda t: t[:1])):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            made = ops.add_rmsnorm(v["x"], v["residual"], v["weight"], post_weight=v["post_weight"])
+        with pytest.raises(ValueError, match="contiguous"):
+            torch.autograd.grad(made, list(v.values()), [dy, dh])
+
+
+@pytest.mark.parametrize("k", [640, 9000])
+def test_on_another_stream_and_captured(gpu, k):
     """On a side stream, and in a graph replayed on new inputs with eager work between the replays."""
     from primus_amd.pytorch import ops
 
-    v, dy, dh = _inputs((4, 50), 640, BF, FP, True, "first", device=gpu)
+    v, dy, dh = _inputs((4, 50), k, BF, FP, True, "first", device=gpu)
     names = list(v)
 
     def run(a, dy, dh):
@@ -412,7 +471,7 @@ def test_on_another_stream_and_captured(gpu):
     with torch.cuda.graph(graph):
         out = run(static, sdy, sdh)
     for seed in range(4):
-        new, ndy, ndh = _inputs((4, 50), 640, BF, FP, True, "first", seed=seed, device=gpu)
+        new, ndy, ndh = _inputs((4, 50), k, BF, FP, True, "first", seed=seed, device=gpu)
         for n in names:
             static[n].copy_(new[n])
         sdy.copy_(ndy), sdh.copy_(ndh)
