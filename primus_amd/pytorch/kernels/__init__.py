@@ -1492,64 +1492,61 @@ def _gate_rows(shape, gate_shape) -> Tuple[int, int, int]:
 
 def _block_norm_args(x, residual, weight, post_weight, gate):
     """``(rows, k, type codes of x and residual, the gate's rows)``."""
-    dtype = _DT.get(x.dtype)
+    want, shape, index = x.dtype, x.shape, x.get_device()
+    dtype = _DT.get(want)
     if dtype is None:
         _float_type(x, "x")
-    if x.dim() < 1 or residual.shape != x.shape:
+    if not shape or residual.shape != shape:
         raise ValueError("x [..., hidden] and residual must have one shape")
-    if residual.dtype != x.dtype and residual.dtype != torch.float32:
+    stream = residual.dtype
+    if stream is not want and stream is not torch.float32:
         raise ValueError("residual must have the type of x or be float32")
-    k = x.shape[-1]
+    k = shape[-1]
     if not 1 <= k <= RMSNORM_MAX_K:
         raise ValueError(f"the normalised dim ({k}) must be in [1, {RMSNORM_MAX_K}]")
-    dev = x.device
-    if not x.is_cuda or residual.device != dev:
+    if index < 0 or residual.get_device() != index:
         _require_cuda(x, residual)
-        _same_device(dev, residual=residual)
+        _same_device(x.device, residual=residual)
     for name, t in (("weight", weight), ("post_weight", post_weight)):
         if t is not None:
-            if t.dtype != x.dtype or t.shape != (k,):
+            if t.dtype is not want or t.dim() != 1 or t.numel() != k:
                 raise ValueError(f"{name} must be a vector of the normalised length, of the type of x")
-            if t.device != dev:
-                _same_device(dev, **{name: t})
+            if t.get_device() != index:
+                _same_device(x.device, **{name: t})
     how = (1, 1, 0)
     if gate is not None:
-        if gate.dtype != x.dtype:
+        if gate.dtype is not want:
             raise ValueError("gate must have the type of x")
-        if gate.device != dev:
-            _same_device(dev, gate=gate)
-        how = _gate_rows(x.shape, gate.shape)
-    return x.numel() // k, k, dtype, _DT[residual.dtype], how
+        if gate.get_device() != index:
+            _same_device(x.device, gate=gate)
+        how = _gate_rows(shape, gate.shape)
+    return x.numel() // k, k, dtype, _DT[stream], how
 
 
 def block_norm_impl(x, residual, weight, eps: float, post_weight, post_eps: float, gate, scale: float, want_rstd: bool = True):
     """``(y, h, rstd, post_rstd)``: ``h = residual + scale * gate * n``, ``n`` = ``x``, normalised with ``post_weight`` if there is one, and
     ``y`` = ``h`` normalised with ``weight`` (None without); see ``ops.add_rmsnorm``."""
     rows, k, dtype, stream_dtype, (div, mod, cols) = _block_norm_args(x, residual, weight, post_weight, gate)
+    pre, post = weight is not None, post_weight is not None
     if rows > 0x7FFFFFFF:
         raise ValueError("at most 2^31 - 1 rows")
-    if weight is None and post_weight is None:
+    if not (pre or post):
         raise ValueError("a norm needs its weight")
     if not (eps >= 0 and post_eps >= 0):
         raise ValueError("eps must not be negative")
-    for t in (x, residual, weight, post_weight, gate):
-        if t is not None and not t.is_contiguous():
-            raise ValueError("operands must be contiguous")
+    if not (x.is_contiguous() and residual.is_contiguous() and (not pre or weight.is_contiguous()) and (not post or post_weight.is_contiguous())
+            and (gate is None or gate.is_contiguous())):
+        raise ValueError("operands must be contiguous")
     dev = x.device
-    lib = _lib.load()
     with _on(dev), _hooked("block_norm", rows=rows, k=k):
         h = torch.empty_like(residual)
-        y = rstd = post_rstd = None
-        if weight is not None:
-            y = torch.empty_like(x)
-            if want_rstd:
-                rstd = torch.empty(rows, dtype=torch.float32, device=dev)
-        if post_weight is not None and want_rstd:
-            post_rstd = torch.empty(rows, dtype=torch.float32, device=dev)
-        rc = lib.mxl_block_norm(x.data_ptr(), residual.data_ptr(), rows, k, dtype, stream_dtype, None if post_weight is None else post_weight.data_ptr(), post_eps,
-                                None if gate is None else gate.data_ptr(), div, mod, cols, scale, None if weight is None else weight.data_ptr(), eps,
-                                None if y is None else y.data_ptr(), h.data_ptr(), None if post_rstd is None else post_rstd.data_ptr(),
-                                None if rstd is None else rstd.data_ptr(), _stream())
+        y = torch.empty_like(x) if pre else None
+        rstd = torch.empty(rows, dtype=torch.float32, device=dev) if pre and want_rstd else None
+        post_rstd = torch.empty(rows, dtype=torch.float32, device=dev) if post and want_rstd else None
+        rc = _lib.load().mxl_block_norm(
+            x.data_ptr(), residual.data_ptr(), rows, k, dtype, stream_dtype, post_weight.data_ptr() if post else None, post_eps,
+            None if gate is None else gate.data_ptr(), div, mod, cols, scale, weight.data_ptr() if pre else None, eps, y.data_ptr() if pre else None,
+            h.data_ptr(), None if post_rstd is None else post_rstd.data_ptr(), None if rstd is None else rstd.data_ptr(), _stream())
     if rc:
         _lib.check(rc, "mxl_block_norm")
     return y, h, rstd, post_rstd
@@ -1567,28 +1564,28 @@ def block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate
     need_gate = need_gate and gate is not None
     if like is None or stream is None or (pre and (dy is None or rstd is None)) or (post and (x is None or post_rstd is None)) or (need_gate and x is None) or not (pre or post):
         raise ValueError("the gradient needs what the forward kept")
-    shape, want, stream_want = like.shape, like.dtype, stream.dtype
+    shape, want, stream_want, index = like.shape, like.dtype, stream.dtype, like.get_device()
     k = shape[-1]
     rows = like.numel() // k
-    dev = like.device
     for t in (dy, x):
-        if t is not None and (t.dtype != want or t.shape != shape or t.device != dev or not t.is_contiguous()):
+        if t is not None and (t.dtype is not want or t.shape != shape or t.get_device() != index or not t.is_contiguous()):
             raise ValueError("the gradient of y, and x, must be contiguous and of the type, shape and device that the forward's x has")
     for t in (dh, h):
-        if t is not None and (t.dtype != stream_want or t.shape != shape or t.device != dev or not t.is_contiguous()):
+        if t is not None and (t.dtype is not stream_want or t.shape != shape or t.get_device() != index or not t.is_contiguous()):
             raise ValueError("the gradient of h, and h, must be contiguous and of the type, shape and device that the forward's residual has")
-    for t, n in ((weight, k), (post_weight, k), (rstd, rows), (post_rstd, rows)):
-        if t is not None and (t.numel() != n or t.device != dev or not t.is_contiguous() or (t.dtype != want and t.dtype != torch.float32)):
-            raise ValueError("weights and rstd must be contiguous vectors of the rows' and columns' number, on one device")
+    for t, n, of in ((weight, k, want), (post_weight, k, want), (rstd, rows, torch.float32), (post_rstd, rows, torch.float32)):
+        if t is not None and (t.numel() != n or t.dtype is not of or t.get_device() != index or not t.is_contiguous()):
+            raise ValueError("weights and rstd must be contiguous vectors of the rows' and columns' number, of the forward's types, on one device")
     div, mod, cols = 1, 1, 0
     if gate is not None:
-        if gate.dtype != want or gate.device != dev or not gate.is_contiguous():
+        if gate.dtype is not want or gate.get_device() != index or not gate.is_contiguous():
             raise ValueError("gate must be contiguous and of the type and device that the forward's x has")
         div, mod, cols = _gate_rows(shape, gate.shape)
+    dev = like.device
     need_weight, need_post_weight = need_weight and pre, need_post_weight and post
     need_residual = need_residual and pre
     # one tensor where both gradients are the same
-    same = need_x and need_residual and not post and gate is None and scale == 1.0 and want == stream_want
+    same = need_x and need_residual and not post and gate is None and scale == 1.0 and want is stream_want
     with _on(dev), _hooked("block_norm_bwd", rows=rows, k=k):
         dx = torch.empty_like(like) if need_x and not same else None
         dres = torch.empty_like(stream) if need_residual else None

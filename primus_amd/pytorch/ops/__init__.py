@@ -917,9 +917,10 @@ def rmsnorm_add(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, e
 
 
 def _block_norm(x, residual, weight, post_weight, gate, eps, post_eps, scale):
-    return _apply(_BlockNorm, x.contiguous(), residual.contiguous(), None if weight is None else weight.contiguous(),
-                  None if post_weight is None else post_weight.contiguous(), None if gate is None else gate.contiguous(), float(eps), float(post_eps),
-                  float(scale))
+    needs = x.requires_grad or residual.requires_grad or any([t is not None and t.requires_grad for t in (weight, post_weight, gate)])
+    return _apply_if(needs, _BlockNorm, x.contiguous(), residual.contiguous(), None if weight is None else weight.contiguous(),
+                     None if post_weight is None else post_weight.contiguous(), None if gate is None else gate.contiguous(), float(eps), float(post_eps),
+                     float(scale))
 
 
 def _grad_list(tensors, what: str):
