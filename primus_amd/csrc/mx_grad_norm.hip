@@ -7,6 +7,9 @@
 //
 // Squares and sums are fp64: a float's square is exact there and neither overflows nor underflows, whatever the gradients' scale.
 // Every workgroup leaves one sum, one workgroup adds them up in their order: the result depends on the sizes alone, and no atomics.
+//
+// Bound by memory.  1.4e9 floats 813 us (6.9 TB/s), 2.2e8 bf16 elements 66 us (6.6); clipping those into floats 237 us (5.5 TB/s).  The fp64 work hides
+// behind the loads.  (With loads behind branches, one after the other: 3520, 100 and, the output's sixteen bytes every 32, 312.)
 #include <math.h>
 #include <stdlib.h>
 
