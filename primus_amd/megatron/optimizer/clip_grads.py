@@ -29,7 +29,6 @@ def get_grad_norm_fp32(grads_for_norm: Union[List[torch.Tensor], torch.Tensor], 
     return total.sqrt().float()
 
 
-@torch.no_grad()
 def clip_grad_by_total_norm_fp32(parameters: Union[Iterable[torch.Tensor], torch.Tensor], max_norm: Union[int, float],
                                  total_norm: Union[torch.Tensor, float], use_decoupled_grad: bool = False) -> None:
     """Scales the parameters' gradients (``decoupled_grad`` or ``grad``; parameters without one are left out) in place by

@@ -929,7 +929,7 @@ def _grad_list(tensors, what: str):
     try:
         if all(map(torch.Tensor.is_contiguous, tensors)):
             return tensors, tensors
-        return tensors, [t if t.is_contiguous() else t.contiguous() for t in tensors]
+        return tensors, [t if t.is_contiguous() else t.detach().contiguous() for t in tensors]
     except (TypeError, RuntimeError):       # (something else in the list, or a layout without strides)
         for t in tensors:
             if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
@@ -937,7 +937,6 @@ def _grad_list(tensors, what: str):
         raise
 
 
-@torch.no_grad()
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of ``grads`` (tensors on one GPU, of any shapes and sizes, bfloat16, float16 and float32 mixed) as a float32 scalar on
     the device: ``sqrt(sum g^2)``, or ``max |g|`` for ``norm_type`` inf (NaN if there is one).  Squares are summed in fp64 in an order that
@@ -950,7 +949,6 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     return K.grad_norm_impl(dense, norm_type)
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = None, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``: ``grad_norm(grads, norm_type)`` unless it is given (the norm over all ranks,
     say), a float32 scalar on the gradients' device, or a number.  In place, or into the tensors of ``out`` (one of the same shape for every gradient, of any of
@@ -979,9 +977,10 @@ def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = 
         return norm
     K.clip_grads_impl(dense, written, max_norm, norm)
     if written is not targets:
-        for t, w in zip(targets, written):
-            if w is not t:
-                t.copy_(w)
+        with torch.no_grad():
+            for t, w in zip(targets, written):
+                if w is not t:
+                    t.copy_(w)
     torch.autograd.graph.increment_version(targets)
     return norm
 
