@@ -90,7 +90,7 @@ __global__ __launch_bounds__(SMALL ? BN_SMALL_THREADS : BN_MAX_THREADS) void blo
         } else {
             // (past the row there are zeros, which an infinite factor must not meet)
 #pragma unroll
-            for (int e = 0; e < BN_VEC; ++e) h[j][e] += (cols(j, ANY || k % 2 ? e : e / 2 * 2) < k ? factor : 0.f) * x[j][e];
+            for (int e = 0; e < BN_VEC; ++e) h[j][e] += (cols(j, e) < k ? factor : 0.f) * x[j][e];
         }
 #pragma unroll
         for (int e = 0; e < BN_VEC; ++e) ss += h[j][e] * h[j][e];
