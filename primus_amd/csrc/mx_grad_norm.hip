@@ -293,11 +293,13 @@ static int span_order(const void* a, const void* b) {
     const Span *x = (const Span*)a, *y = (const Span*)b;
     return x->lo < y->lo ? -1 : x->lo > y->lo;
 }
-// Whether what is written shares no byte with anything else that is read or written (a gradient that is its own output is one span).
-static int clip_spans_apart(const void* const* p, void* const* out, const int64_t* n, const int32_t* dtypes, const int32_t* out_dtypes, int count) {
+// Whether what is written shares no byte with anything else that is read, the norm too, or written (a gradient that is its own output is one span).
+static int clip_spans_apart(const void* const* p, void* const* out, const int64_t* n, const int32_t* dtypes, const int32_t* out_dtypes, int count,
+                            const float* norm) {
     Span* s = (Span*)malloc((size_t)(2 * (int64_t)count + 1) * sizeof(Span));
     if (!s) return 0;
     int64_t m = 0;
+    s[m++] = {(uintptr_t)norm, (uintptr_t)norm + sizeof(float), 0};
     for (int i = 0; i < count; ++i) {
         if (n[i] == 0) continue;
         const bool same = p[i] == out[i] && dtypes[i] == out_dtypes[i];
@@ -364,7 +366,7 @@ extern "C" int mxl_grad_norm(const void* const* grads, const int64_t* sizes, con
 extern "C" int mxl_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* dtypes, const int32_t* out_dtypes,
                               int count, double max_norm, const float* norm, void* stream) {
     if (!gn_list_ok(grads, sizes, dtypes, count) || !gn_list_ok(outs, sizes, out_dtypes, count) || !norm || !(max_norm >= 0.)) return MXL_EINVAL;
-    if (!clip_spans_apart(grads, outs, sizes, dtypes, out_dtypes, count)) return MXL_EINVAL;
+    if (!clip_spans_apart(grads, outs, sizes, dtypes, out_dtypes, count, norm)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     hipStream_t st = (hipStream_t)stream;
     int i = 0;

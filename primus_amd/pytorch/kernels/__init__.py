@@ -1666,7 +1666,7 @@ def clip_grads_impl(tensors, outs, max_norm: float, norm: torch.Tensor) -> None:
         rc = lib.mxl_clip_grads(ptrs.buffer_info()[0], out_ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], out_types.buffer_info()[0],
                                 len(types), max_norm, norm.data_ptr(), _stream())
     if rc == -1:
-        raise ValueError("a tensor that is written must not overlap another one of the lists (a gradient may be its own output)")
+        raise ValueError("a tensor that is written must not overlap the norm or another one of the lists (a gradient may be its own output)")
     if rc:
         _lib.check(rc, "mxl_clip_grads")
 

@@ -954,7 +954,7 @@ def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = 
     say), a float32 scalar on the gradients' device, or a number.  In place, or into the tensors of ``out`` (one of the same shape for every gradient, of any of
     the three types: the optimizer's float32 gradients of bfloat16 ones).  The factor is taken on the device and nothing is read back: within the bound, gradients
     in place are left untouched.  A norm of NaN makes every element NaN, an infinite one leaves zeros of what is finite.  No tensor that is written may
-    overlap another one."""
+    overlap another one or ``norm``."""
     targets, dense = _grad_list(grads, "gradients")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

@@ -1,0 +1,35 @@
+"""What the C entries of the gradient norm and clipping refuse about addresses, before anything is launched: checked without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from primus_amd import _lib
+
+FP, BF, HF = 0, 1, 2
+
+
+@pytest.fixture()
+def memory():
+    if torch.cuda.device_count() > 0:
+        pytest.skip("a GPU is present: calls that are right would be real launches")
+    buf = ctypes.create_string_buffer(1 << 16)
+    yield ctypes.addressof(buf) // 16 * 16 + 16
+
+
+def _clip(ins, outs, norm):
+    arrays = [[(ctypes.c_uint64 * len(s))(*[t[0] for t in s]), (ctypes.c_int64 * len(s))(*[t[1] for t in s]), (ctypes.c_int32 * len(s))(*[t[2] for t in s])] for s in (ins, outs)]
+    return _lib.load().mxl_clip_grads(arrays[0][0], arrays[1][0], arrays[0][1], arrays[0][2], arrays[1][2], len(ins), 1.0, norm, None)
+
+
+def test_norm_inside_what_is_written(memory):
+    """Workgroups read the norm while others write: it may lie in no tensor that is written.  (-3: right, but no device here.)"""
+    a, b = (memory, 10, FP), (memory + 4096, 10, BF)
+    for norm in (memory, memory + 36):
+        assert _clip([a], [a], norm) == -1
+    for norm in (memory + 4096, memory + 4112):
+        assert _clip([a], [b], norm) == -1
+    assert _clip([a, (memory + 64, 0, FP)], [b, (memory + 64, 0, FP)], memory + 64) == -3
+    for norm in (memory, memory + 36, memory + 40, memory + 4092, memory + 4116):      # in a gradient that is read, and beside both
+        assert _clip([a], [b], norm) == -3
