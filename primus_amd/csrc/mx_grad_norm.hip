@@ -277,13 +277,14 @@ __global__ __launch_bounds__(GN_THREADS) void clip_kernel(ClipTable t, const flo
     }
 }
 
+static int gn_size(int dtype) { return dtype == MXL_DT_F32 ? 4 : 2; }
 static bool gn_list_ok(const void* const* p, const int64_t* n, const int32_t* dtypes, int count) {
     if (count < 0 || (count > 0 && (!p || !n || !dtypes))) return false;
     for (int i = 0; i < count; ++i)
-        if (n[i] < 0 || n[i] >= ((int64_t)1 << 36) || dtypes[i] < MXL_DT_F32 || dtypes[i] > MXL_DT_F16 || (n[i] > 0 && !p[i])) return false;
+        if (n[i] < 0 || n[i] >= ((int64_t)1 << 36) || dtypes[i] < MXL_DT_F32 || dtypes[i] > MXL_DT_F16 ||
+            (n[i] > 0 && (!p[i] || (uintptr_t)p[i] % gn_size(dtypes[i])))) return false;
     return true;
 }
-static int gn_size(int dtype) { return dtype == MXL_DT_F32 ? 4 : 2; }
 
 struct Span {
     uintptr_t lo, hi;
@@ -329,7 +330,7 @@ extern "C" int64_t mxl_grad_norm_workspace_bytes(int count) {
 
 extern "C" int mxl_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int count, int kind, float* norm, void* workspace,
                              int64_t workspace_bytes, void* stream) {
-    if (!gn_list_ok(grads, sizes, dtypes, count) || (kind != MXL_NORM_L2 && kind != MXL_NORM_MAX) || !norm) return MXL_EINVAL;
+    if (!gn_list_ok(grads, sizes, dtypes, count) || (kind != MXL_NORM_L2 && kind != MXL_NORM_MAX) || !norm || ((uintptr_t)norm & 3)) return MXL_EINVAL;
     if (workspace_bytes < mxl_grad_norm_workspace_bytes(count) || (count > 0 && (!workspace || ((uintptr_t)workspace & 7) != 0))) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     hipStream_t st = (hipStream_t)stream;
@@ -365,7 +366,7 @@ extern "C" int mxl_grad_norm(const void* const* grads, const int64_t* sizes, con
 
 extern "C" int mxl_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* dtypes, const int32_t* out_dtypes,
                               int count, double max_norm, const float* norm, void* stream) {
-    if (!gn_list_ok(grads, sizes, dtypes, count) || !gn_list_ok(outs, sizes, out_dtypes, count) || !norm || !(max_norm >= 0.)) return MXL_EINVAL;
+    if (!gn_list_ok(grads, sizes, dtypes, count) || !gn_list_ok(outs, sizes, out_dtypes, count) || !norm || ((uintptr_t)norm & 3) || !(max_norm >= 0.)) return MXL_EINVAL;
     if (!clip_spans_apart(grads, outs, sizes, dtypes, out_dtypes, count, norm)) return MXL_EINVAL;
     if (!device_is_gfx950()) return MXL_ENODEV;
     hipStream_t st = (hipStream_t)stream;

@@ -33,3 +33,23 @@ def test_norm_inside_what_is_written(memory):
     assert _clip([a, (memory + 64, 0, FP)], [b, (memory + 64, 0, FP)], memory + 64) == -3
     for norm in (memory, memory + 36, memory + 40, memory + 4092, memory + 4116):      # in a gradient that is read, and beside both
         assert _clip([a], [b], norm) == -3
+
+
+def _norm(spans, out, workspace):
+    lib = _lib.load()
+    a = [(ctypes.c_uint64 * len(spans))(*[t[0] for t in spans]), (ctypes.c_int64 * len(spans))(*[t[1] for t in spans]), (ctypes.c_int32 * len(spans))(*[t[2] for t in spans])]
+    return lib.mxl_grad_norm(a[0], a[1], a[2], len(spans), 0, out, workspace, lib.mxl_grad_norm_workspace_bytes(len(spans)), None)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+def test_addresses_between_elements(memory, dtype):
+    """Sixteen-byte pieces are counted in elements from a tensor's address: it has to be an element's.  Of a tensor without elements it is not looked at."""
+    size, norm = 4 if dtype == FP else 2, memory + 32768
+    for off in range(1, 8):
+        want = -3 if off % size == 0 else -1
+        at = (memory + off, 10, dtype)
+        assert _norm([at], norm, memory + 1024) == want
+        assert _clip([at], [at], norm) == want and _clip([at], [(memory + 4096, 10, FP)], norm) == want and _clip([(memory + 4096, 10, FP)], [at], norm) == want
+    assert _norm([(memory + 1, 0, dtype)], norm, memory + 1024) == -3 and _clip([(memory + 1, 0, dtype)] * 2, [(memory + 1, 0, dtype)] * 2, norm) == -3
+    for off in (1, 2, 3):
+        assert _norm([(memory, 10, dtype)], norm + off, memory + 1024) == -1 and _clip([(memory, 10, dtype)], [(memory, 10, dtype)], norm + off) == -1
