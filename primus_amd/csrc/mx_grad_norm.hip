@@ -226,9 +226,11 @@ template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void*
             else if (DO == MXL_DT_BF16) o[j] = pack_bf16(f[2 * j % PER], f[(2 * j + 1) % PER]);
             else o[j] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j % PER]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[(2 * j + 1) % PER]) << 16);
         }
+        // (No scalar offset: a store of more than 8 bytes fetches its data after it has issued, and only without one does the compiler keep two wait states
+        // in front of an instruction that writes those registers.)
         if constexpr (OW == 4) {
             const gn_u32x4 t = {o[0], o[1], o[2], o[3]};
-            __builtin_amdgcn_raw_buffer_store_b128(t, out, (int)threadIdx.x * 16, u * GN_THREADS * 16, 2);
+            __builtin_amdgcn_raw_buffer_store_b128(t, out, (int)threadIdx.x * 16 + u * GN_THREADS * 16, 0, 2);
         } else {
             const u32x2 t = {o[0], o[1]};
             __builtin_amdgcn_raw_buffer_store_b64(t, out, (int)threadIdx.x * 8, u * GN_THREADS * 8, 2);
