@@ -8,7 +8,7 @@
 // Squares and sums are fp64: a float's square is exact there and neither overflows nor underflows, whatever the gradients' scale.
 // Every workgroup leaves one sum, one workgroup adds them up in their order: the result depends on the sizes alone, and no atomics.
 //
-// Bound by memory.  1.4e9 floats 813 us (6.9 TB/s), 2.2e8 bf16 elements 66 us (6.6); clipping those into floats 237 us (5.5 TB/s).  The fp64 work hides
+// Bound by memory.  1.4e9 floats 813 us (6.9 TB/s), 2.2e8 bf16 elements 66 us (6.6); clipping those into floats 220 us (6.0 TB/s).  The fp64 work hides
 // behind the loads.  (With loads behind branches, one after the other: 3520, 100 and, the output's sixteen bytes every 32, 312.)
 #include <math.h>
 #include <stdlib.h>
@@ -175,13 +175,19 @@ constexpr int GC_PER = GN_THREADS * 32;     // elements of a chunk
 // 2048 2192), but all of them have to come and go where the norm is within the bound (79, 36 and 31 us), the common case.
 constexpr uint32_t GC_BLOCKS = 32768;
 
-// The product is rounded once: a float's is made in fp64; of the 16-bit types it is exact but for the coefficient's 24 bits.
-template <int DT> __device__ __forceinline__ float scaled(float g, double c, float cf) { return DT == MXL_DT_F32 ? (float)((double)g * c) : g * cf; }
+// The product is made in fp64 and rounded to fp32 (of a 16-bit type it is exact till then but for the factor's 53 bits), and once more to a 16-bit output.
+// The factor as a float would lose bits, and all of them in the end, below 2^-126.
+// us for 2.2e8 elements, with 16-bit ones scaled in fp32 and so: bf16 to bf16 139 and 138, to fp16 138 and 138, to fp32 238 and 220.
+template <int DO> __device__ __forceinline__ float scaled(float g, double c) {
+    float f = (float)((double)g * c);
+    if (DO != MXL_DT_F32) asm("" : "+v"(f));    // (or both roundings become one from fp64, many instructions: bf16 to fp16 209 us)
+    return f;
+}
 
 // Four or eight elements a lane and step (so that a store of a wave writes whole lines: streaming stores of every other sixteen bytes do not
 // combine), through buffer descriptors of the chunk's whole steps' worth (past it nothing is read or written); the rest element by element.
 // Two-byte elements that begin between two dwords: the descriptor begins a dword boundary later, the element in front goes by itself.
-template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void* src, void* dst, int64_t lo, int64_t hi, double c, float cf) {
+template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void* src, void* dst, int64_t lo, int64_t hi, double c) {
     constexpr int IN = DT == MXL_DT_F32 ? 4 : 2, OUT = DO == MXL_DT_F32 ? 4 : 2;    // bytes of an element
     constexpr int PER = IN == 2 && OUT == 2 ? 8 : 4, STEPS = GC_PER / PER / GN_THREADS;
     constexpr int IW = PER * IN / 4, OW = PER * OUT / 4;
@@ -191,7 +197,7 @@ template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void*
     const bool odd_in = IN == 2 && ((uintptr_t)s & 2), odd_out = OUT == 2 && ((uintptr_t)d & 2);
     const int n = (int)(hi - lo);
     if (IN == 2 && OUT == 2 && odd_in != odd_out) {     // one on dwords and the other between them
-        for (int i = (int)threadIdx.x; i < n; i += GN_THREADS) store_dt(dst, DO, lo + i, scaled<DT>(load_dt(src, DT, lo + i), c, cf));
+        for (int i = (int)threadIdx.x; i < n; i += GN_THREADS) store_dt(dst, DO, lo + i, scaled<DO>(load_dt(src, DT, lo + i), c));
         return;
     }
     const int head = odd_in || odd_out ? 1 : 0, whole = (n - head) / PER;
@@ -217,7 +223,7 @@ template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void*
             if (DT == MXL_DT_F32) f[j] = __uint_as_float(r[u][j % IW]);
             else if (DT == MXL_DT_BF16) f[j] = j & 1 ? bf16_hi(r[u][j / 2]) : bf16_lo(r[u][j / 2]);
             else f[j] = j & 1 ? half_hi(r[u][j / 2]) : half_lo(r[u][j / 2]);
-            f[j] = scaled<DT>(f[j], c, cf);
+            f[j] = scaled<DO>(f[j], c);
         }
         uint32_t o[OW];
 #pragma unroll
@@ -241,7 +247,7 @@ template <int DT, int DO> __device__ __forceinline__ void clip_chunk(const void*
         const int t = (int)threadIdx.x;
         if (t < head || (t >= 64 && t - 64 < rest)) {
             const int64_t i = t < head ? lo : hi - rest + (t - 64);
-            store_dt(dst, DO, i, scaled<DT>(load_dt(src, DT, i), c, cf));
+            store_dt(dst, DO, i, scaled<DO>(load_dt(src, DT, i), c));
         }
     }
 }
@@ -250,7 +256,6 @@ __global__ __launch_bounds__(GN_THREADS) void clip_kernel(ClipTable t, const flo
     const double raw = max_norm / ((double)*norm + 1e-6);
     const bool within = raw >= 1.;          // (a NaN is not)
     const double c = within ? 1. : raw;
-    const float cf = (float)c;
     if (within && t.in_place) return;
     const uint32_t chunks = t.end[t.count - 1];
     const TensorOf<GC_TENSORS> tensor_of(t.end, t.count);
@@ -263,7 +268,7 @@ __global__ __launch_bounds__(GN_THREADS) void clip_kernel(ClipTable t, const flo
         const int types = (int)(packed >> GN_TYPE_SHIFT), in = types & 3, out = types >> 2;
         const uint32_t first = at ? t.end[at - 1] : 0;
         const int64_t lo = (int64_t)(i - first) * GC_PER, hi = lo + GC_PER < n ? lo + GC_PER : n;
-#define MXL_CLIP(DT, DO) clip_chunk<DT, DO>(src, dst, lo, hi, c, cf)
+#define MXL_CLIP(DT, DO) clip_chunk<DT, DO>(src, dst, lo, hi, c)
         switch (in * 4 + out) {
             case MXL_DT_F32 * 4 + MXL_DT_F32: MXL_CLIP(MXL_DT_F32, MXL_DT_F32); break;
             case MXL_DT_F32 * 4 + MXL_DT_BF16: MXL_CLIP(MXL_DT_F32, MXL_DT_BF16); break;

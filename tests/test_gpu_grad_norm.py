@@ -276,3 +276,25 @@ def test_parameters_gradients(gpu):
     norm = ops.clip_grads((p.grad for p in model.parameters()), 0.1)
     for g, c in zip(grads, copies):
         _clipped(g, c, 0.1, norm)
+
+
+@pytest.mark.parametrize("src", [FP, BF, HF])
+@pytest.mark.parametrize("dst", [FP, BF, HF])
+def test_factors_below_the_normal_range(gpu, src, dst):
+    """A norm so large, and a bound so small, that fp32 holds a few bits of the factor at most, while most results are normal numbers.  Of those that are
+    not, a bf16's are multiples of 2^-133, so that rounding to one is off by up to 2^-134, which is more than ``_clipped`` allows for; an fp32's of
+    2^-149, an fp16's of 2^-24.  The product is rounded to fp32 first."""
+    from primus_amd.pytorch import ops
+
+    g = torch.Generator().manual_seed(3)
+    top = 6e4 if src == HF else 1e37
+    ts = [(torch.rand(n, generator=g) * 2 - 1).mul(top).to(src).to(gpu) for n in (5, 8192, 9001)]
+    for norm, max_norm in ((1e38, 1e-3), (1e38, 1e-6), (3e38, 1e-7)):
+        norm = torch.tensor(norm, device=gpu)
+        outs = [torch.empty(t.shape, dtype=dst, device=gpu) for t in ts]
+        ops.clip_grads(ts, max_norm, norm=norm, out=outs)
+        half = {HF: 2.0 ** -25, BF: 2.0 ** -134, FP: 0.0}[dst] + 2.0 ** -150
+        for t, o in zip(ts, outs):
+            want = t.cpu().double() * (max_norm / (norm.item() + 1e-6))
+            bound = (torch.finfo(dst).eps / 2 + (0 if dst == FP else 2.0 ** -23)) * want.abs() + half
+            assert ((o.cpu().double() - want).abs() <= bound).all(), max_norm
