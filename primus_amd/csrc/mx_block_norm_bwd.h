@@ -303,8 +303,16 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
     // what several workers share, for the second kernel: a row of a workgroup or, of short rows, of a wave
     float ag[CH][BN_VEC];
     if (GATEV) {
+        // (a worker that has its gates to itself is done with each of them; once more, with sums of zero, an infinite gate would add NaN)
 #pragma unroll
-        for (int j = 0; j < CH; ++j) gate_done(j, ag[j]);       // (nothing is left where a worker has its gates to itself)
+        for (int j = 0; j < CH; ++j) {
+            if (p.share > 1) {
+                gate_done(j, ag[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < BN_VEC; ++e) ag[j][e] = 0.f;
+            }
+        }
     }
     if (!KEEP) {
 #pragma unroll

@@ -511,3 +511,22 @@ def test_rows_around_the_output_stay(gpu):
         wy, wh, _, _ = K.block_norm_impl(x, r, w, EPS, None, 0.0, None, 1.0)
         assert torch.equal(y, wy) and torch.equal(h, wh)
         assert all((b[:9] == 7).all() and (b[9 + n:] == 7).all() for b in bufs)
+
+
+@pytest.mark.parametrize("k", [40, 333, 1024, 9000])
+def test_an_infinite_gate_leaves_its_own_sums(gpu, k):
+    """An element of a gate that is infinite: the post weight's gradient is infinite in its column, as the formula's is, and the other columns' finite."""
+    from primus_amd.pytorch import ops
+
+    rows, column = 6, 3
+    for dtype, stream in ((BF, FP), (HF, HF)):
+        v, _, dh = _inputs((rows,), k, dtype, stream, True, "full", device=gpu)
+        for row in (0, rows - 1):
+            gate = v["gate"].clone()
+            gate[row, column] = math.inf
+            wp = v["post_weight"].clone().requires_grad_()
+            (got,) = torch.autograd.grad(ops.rmsnorm_add(v["x"], v["residual"], wp, POST_EPS, gate=gate), wp, dh)
+            want = math.copysign(math.inf, (dh[row, column].double() * v["x"][row, column].double()).item())
+            assert got[column].item() == want, (dtype, row)
+            rest = [c for c in range(k) if c != column]
+            assert torch.isfinite(got[rest]).all()
