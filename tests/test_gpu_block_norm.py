@@ -530,3 +530,80 @@ def test_an_infinite_gate_leaves_its_own_sums(gpu, k):
             assert got[column].item() == want, (dtype, row)
             rest = [c for c in range(k) if c != column]
             assert torch.isfinite(got[rest]).all()
+
+
+def _signs(shape, g, dtype, device):
+    return (2 * torch.randint(0, 2, shape, generator=g) - 1).to(dtype).to(device)
+
+
+def _few(rows, k, g):
+    """[rows, k] of -1, 0 and 1, something in every row, and about 2500 (at least rows / k) a column, 2500 a row, that are not 0: sums stay below 256."""
+    each = max(1, min(k, 2500 * k // rows, 2500))
+    at = (torch.randint(0, k, (rows, 1), generator=g) + torch.arange(each) * (k // each)) % k
+    return torch.zeros(rows, k).scatter_(1, at, _signs((rows, each), g, torch.float32, "cpu"))
+
+
+@pytest.mark.parametrize("lead,k", [((40000,), 8), ((5000,), 96), ((9000, 2), 64), ((2, 9000), 64), ((3001,), 257), ((70, 43), 257), ((530,), 7168), ((300,), 12289), ((1500, 3), 512),
+                                    ((33, 31), 129), ((1023,), 1601)])
+@pytest.mark.parametrize("gate", ["", "column", "first", "last", "token", "full"])
+def test_every_row_counts(gpu, lead, k, gate):
+    """Sums over rows that are whole numbers: a row, a worker or a wave that is left out changes them by one at least.  x and gate are 1 or -1, so a row's
+    normalised values are too, but for the rounding of 1 / k and of the root: below 2^-22 in all, rows * 2^-22 in a sum, which is under 1 / 4.  Whole numbers
+    up to 256 are a bf16's, and what is so close to one rounds to it."""
+    from primus_amd.pytorch import ops
+
+    rows = math.prod(lead)
+    g = torch.Generator().manual_seed(k + rows)
+    one = torch.ones(k)
+    whole = lambda t, w, name: _whole(t, w, name + (gate,))  # noqa: E731
+    for dtype, stream in ((BF, BF), (HF, FP), (FP, FP)):
+        x = _signs(lead + (k,), g, dtype, gpu)
+        shape = _gate_shape(gate, lead, k)
+        a = {"x": x, "residual": torch.zeros(lead + (k,), dtype=stream, device=gpu), "weight": one.to(dtype).to(gpu), "post_weight": one.to(dtype).to(gpu),
+             "gate": None if shape is None else _signs(shape, g, dtype, gpu)}
+        d = _few(rows, k, g).view(lead + (k,))
+        n = x.cpu().float() * d
+        f = n if shape is None else n * a["gate"].cpu().float()
+        want = {"weight": f.reshape(rows, k).sum(0), "post_weight": f.reshape(rows, k).sum(0), "gate": None if shape is None else _to(n, shape)}
+        assert want["weight"].abs().max() <= 256 and (shape is None or want["gate"].abs().max() <= 256)     # (of the data, by its seed)
+        a = {name: None if t is None else t.requires_grad_() for name, t in a.items()}
+        for post in (False, True):
+            y, h = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], 0.0, post_weight=a["post_weight"] if post else None, gate=a["gate"])
+            (dw,) = torch.autograd.grad(y, a["weight"], d.to(dtype).to(gpu), retain_graph=True)
+            whole(dw, want["weight"], ("weight", post, dtype))
+            names = [m for m in ("post_weight", "gate") if (post or m == "gate") and a[m] is not None]
+            if names:
+                for m, got in zip(names, torch.autograd.grad(h, [a[m] for m in names], d.to(stream).to(gpu))):
+                    whole(got, want[m], (m, post, dtype))
+        h = ops.rmsnorm_add(a["x"], a["residual"], a["post_weight"], 0.0, gate=a["gate"])
+        names = [m for m in ("post_weight", "gate") if a[m] is not None]
+        for m, got in zip(names, torch.autograd.grad(h, [a[m] for m in names], d.to(stream).to(gpu))):
+            whole(got, want[m], (m, "alone", dtype))
+
+
+def _whole(got, want, name):
+    off = (got.detach().cpu().float() - want).abs()
+    assert got.shape == want.shape and (off <= 0.25).all(), (name, int((off > 0.25).sum()), off.max().item())
+
+
+@pytest.mark.parametrize("k,rows", [(16384, (1 << 17) + 24), (64, (1 << 23) + 100), (4, (1 << 28) + 40)])
+def test_weight_gradients_beyond_32_bit_offsets(gpu, k, rows):
+    """The weights' gradients of more rows than 31 bits of offsets reach, of which the first, the last and some between are not zero: whole numbers, as above."""
+    from primus_amd.pytorch import ops
+
+    g = torch.Generator().manual_seed(k)
+    at = sorted({0, 1, rows // 2, rows - 65, *range(rows - 40, rows)} | set(torch.randint(0, rows, (60,), generator=g).tolist()))
+    x, dy = (torch.zeros(rows, k, dtype=BF, device=gpu) for _ in range(2))
+    r = torch.zeros(rows, k, dtype=BF, device=gpu)
+    sx, sd = (_signs((len(at), k), g, BF, gpu) for _ in range(2))
+    where = torch.tensor(at, device=gpu)
+    x[where], dy[where] = sx, sd
+    want = (sx.float() * sd.float()).sum(0).cpu()
+    w = torch.ones(k, dtype=BF, device=gpu, requires_grad=True)
+    y, h = ops.add_rmsnorm(x, r, w, 1e-6)       # (1 / sqrt(1 + 1e-6): 1e-6 * 110 rows off)
+    (dw,) = torch.autograd.grad(y, w, dy)
+    _whole(dw, want, ("weight", k))
+    del y, h
+    h = ops.rmsnorm_add(x, r, w, 1e-6)
+    (dw,) = torch.autograd.grad(h, w, dy)
+    _whole(dw, want, ("post_weight", k))
