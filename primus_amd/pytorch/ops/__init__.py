@@ -21,6 +21,8 @@ Activations and gradients use 1-D blocks of 32, weights 2-D 32x32 blocks.
 from __future__ import annotations
 
 import contextlib
+import itertools
+import operator
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -949,12 +951,60 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     return K.grad_norm_impl(dense, norm_type)
 
 
+def _span(t, written: bool):
+    """``(first byte, end, (stride in bytes, length) of every dimension, from the shortest stride on, bytes that stand together, written)``"""
+    lo = t.data_ptr()
+    if t.is_contiguous():
+        return lo, lo + t.nbytes, (), t.nbytes, written
+    size = t.element_size()
+    dims = sorted((st * size, n) for st, n in zip(t.stride(), t.shape) if n > 1)
+    return lo, lo + sum(st * (n - 1) for st, n in dims) + size, dims, size, written
+
+
+def _apart(spans) -> bool:
+    """Whether spans can be seen to share no byte: by their positions modulo one of their strides, where dimensions whose strides are multiples of it fall
+    together and the others reach from the first element on.  That tells slices of one tensor apart."""
+    for step in {st for span in spans for st, _ in span[2] if st}:
+        at = sorted([(lo % step, size + sum([st * (n - 1) for st, n in dims if st % step])) for lo, _, dims, size, _ in spans])
+        if all([a + reach <= b for (a, reach), (b, _) in zip(at, at[1:])]) and sum(at[-1]) <= at[0][0] + step:
+            return True
+    return False
+
+
+def _refuse_overlaps(targets, grads, norm) -> None:
+    """What the C entry refuses of tensors without gaps, for pairs in which one has them: the kernels have a copy in its place."""
+    spans = [_span(t, True) for t in targets if t.numel()]
+    for _, _, dims, reach, _ in spans:
+        for stride, n in dims:
+            if stride < reach:
+                raise ValueError("a tensor that is written must not overlap itself")
+            reach += stride * (n - 1)
+    if grads is not targets:
+        spans += [_span(g, False) for g, t in zip(grads, targets) if g.numel() and (g.data_ptr() != t.data_ptr() or g.stride() != t.stride() or g.dtype != t.dtype)]
+    if isinstance(norm, torch.Tensor) and norm.numel():
+        spans.append(_span(norm, False))
+    spans.sort(key=operator.itemgetter(0))
+    first, end = 0, 0
+    for i in range(len(spans) + 1):
+        if i < len(spans) and spans[i][0] < end:
+            end = max(end, spans[i][1])
+            continue
+        # (spans first .. i - 1 reach into one another, and into no others)
+        near = spans[first:i]
+        if len(near) > 1 and any([s[2] for s in near]) and not _apart(near):
+            for a, b in itertools.combinations(near, 2):
+                if (a[4] or b[4]) and (a[2] or b[2]) and b[0] < a[1] and not _apart((a, b)):
+                    raise ValueError("a tensor that is written must not overlap the norm or another one of the lists (a gradient may be its own output)")
+        if i < len(spans):
+            first, end = i, spans[i][1]
+
+
 def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = None, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``: ``grad_norm(grads, norm_type)`` unless it is given (the norm over all ranks,
     say), a float32 scalar on the gradients' device, or a number.  In place, or into the tensors of ``out`` (one of the same shape for every gradient, of any of
     the three types: the optimizer's float32 gradients of bfloat16 ones).  The factor is taken on the device and nothing is read back: within the bound, gradients
     in place are left untouched.  A norm of NaN makes every element NaN, an infinite one leaves zeros of what is finite.  No tensor that is written may
-    overlap another one or ``norm``."""
+    overlap itself, another one or ``norm``; slices of one tensor that lie between each other's rows or columns do not."""
     targets, dense = _grad_list(grads, "gradients")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -965,10 +1015,8 @@ def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = 
         targets, written = _grad_list(out, "out")
         if len(targets) != len(grads) or any(o.shape != g.shape for o, g in zip(targets, grads)):
             raise ValueError("out must hold a tensor of the same shape for every gradient")
-    if written is not targets:
-        gaps = [t for t, w in zip(targets, written) if w is not t]
-        if len({t.data_ptr() for t in gaps}) < len(gaps) or any(st == 0 and n > 1 for t in gaps for st, n in zip(t.stride(), t.shape)):
-            raise ValueError("a tensor that is written must not overlap itself or another one")
+    if written is not targets or (out is not None and dense is not grads):
+        _refuse_overlaps(targets, targets if out is None else grads, norm)
     if norm is None:
         norm = grad_norm(dense, norm_type)
     elif not isinstance(norm, torch.Tensor):
