@@ -34,6 +34,7 @@ extern "C" {
 #define MXL_ENODEV (-3)  /* current device is not gfx950 */
 #define MXL_ESCRATCH (-4) /* the problem needs more scratch memory than an allocation-free entry point owns */
 #define MXL_ESTREAM (-5)  /* an allocation-free entry point was called on a stream it is not bound to */
+#define MXL_ENOMEM (-6) /* the host has no memory for what a call keeps while it checks its lists */
 
 #define MXL_FMT_E4M3 0
 #define MXL_FMT_E2M1 1

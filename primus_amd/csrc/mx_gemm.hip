@@ -1737,6 +1737,7 @@ extern "C" const char* mxl_error_string(int code) {
         case MXL_ENODEV: return "device is not gfx950";
         case MXL_ESCRATCH: return "the problem needs more scratch memory than this allocation-free entry point owns";
         case MXL_ESTREAM: return "the allocation-free entry point is bound to another stream on this device (or unbound while capturing)";
+        case MXL_ENOMEM: return "the host has no memory for what the call keeps while it checks its lists";
         default: return "unknown error";
     }
 }

@@ -301,11 +301,11 @@ static int span_order(const void* a, const void* b) {
     const Span *x = (const Span*)a, *y = (const Span*)b;
     return x->lo < y->lo ? -1 : x->lo > y->lo;
 }
-// Whether what is written shares no byte with anything else that is read, the norm too, or written (a gradient that is its own output is one span).
+// MXL_OK if what is written shares no byte with anything else that is read, the norm too, or written (a gradient that is its own output is one span).
 static int clip_spans_apart(const void* const* p, void* const* out, const int64_t* n, const int32_t* dtypes, const int32_t* out_dtypes, int count,
                             const float* norm) {
     Span* s = (Span*)malloc((size_t)(2 * (int64_t)count + 1) * sizeof(Span));
-    if (!s) return 0;
+    if (!s) return MXL_ENOMEM;
     int64_t m = 0;
     s[m++] = {(uintptr_t)norm, (uintptr_t)norm + sizeof(float), 0};
     for (int i = 0; i < count; ++i) {
@@ -323,7 +323,7 @@ static int clip_spans_apart(const void* const* p, void* const* out, const int64_
         if (s[i].hi > end) end = s[i].hi;
     }
     free(s);
-    return apart;
+    return apart ? MXL_OK : MXL_EINVAL;
 }
 
 }  // namespace mxl
@@ -374,7 +374,8 @@ extern "C" int mxl_grad_norm(const void* const* grads, const int64_t* sizes, con
 extern "C" int mxl_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* dtypes, const int32_t* out_dtypes,
                               int count, double max_norm, const float* norm, void* stream) {
     if (!gn_list_ok(grads, sizes, dtypes, count) || !gn_list_ok(outs, sizes, out_dtypes, count) || !norm || ((uintptr_t)norm & 3) || !(max_norm >= 0.)) return MXL_EINVAL;
-    if (!clip_spans_apart(grads, outs, sizes, dtypes, out_dtypes, count, norm)) return MXL_EINVAL;
+    const int apart = clip_spans_apart(grads, outs, sizes, dtypes, out_dtypes, count, norm);
+    if (apart != MXL_OK) return apart;
     if (!device_is_gfx950()) return MXL_ENODEV;
     hipStream_t st = (hipStream_t)stream;
     int i = 0;

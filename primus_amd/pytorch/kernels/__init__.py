@@ -1632,6 +1632,14 @@ def _tensor_list(tensors, what: str):
     return devices.pop(), array.array("Q", map(torch.Tensor.data_ptr, tensors)), array.array("q", map(torch.Tensor.numel, tensors)), types
 
 
+def _why_refused(ptrs, sizes, what: str) -> None:
+    """Raises for what the C entries refuse of a single tensor."""
+    if any(n and not p for p, n in zip(ptrs, sizes)):
+        raise ValueError(f"{what} must be plain tensors with memory of their own (of a sharded one, its local part)")
+    if any(n >= 1 << 36 for n in sizes):
+        raise ValueError(f"{what} must have less than 2^36 elements each")
+
+
 def grad_norm_impl(tensors, kind: float = 2.0) -> torch.Tensor:
     """Norm over all elements of contiguous ``tensors`` (at least one) as a float32 scalar on their device; see ``ops.grad_norm``."""
     code = _NORM_KINDS.get(float(kind))
@@ -1644,6 +1652,8 @@ def grad_norm_impl(tensors, kind: float = 2.0) -> torch.Tensor:
         norm = torch.empty((), dtype=torch.float32, device=dev)
         ws, nbytes = _workspace(dev, "mxl_grad_norm_workspace_bytes", len(types))
         rc = lib.mxl_grad_norm(ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(types), code, norm.data_ptr(), ws.data_ptr(), nbytes, _stream())
+    if rc == -1:
+        _why_refused(ptrs, sizes, "gradients")
     if rc:
         _lib.check(rc, "mxl_grad_norm")
     return norm
@@ -1666,6 +1676,8 @@ def clip_grads_impl(tensors, outs, max_norm: float, norm: torch.Tensor) -> None:
         rc = lib.mxl_clip_grads(ptrs.buffer_info()[0], out_ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], out_types.buffer_info()[0],
                                 len(types), max_norm, norm.data_ptr(), _stream())
     if rc == -1:
+        _why_refused(ptrs, sizes, "gradients")
+        _why_refused(out_ptrs, sizes, "out")
         raise ValueError("a tensor that is written must not overlap the norm or another one of the lists (a gradient may be its own output)")
     if rc:
         _lib.check(rc, "mxl_clip_grads")

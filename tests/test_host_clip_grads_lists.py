@@ -53,3 +53,62 @@ def test_addresses_between_elements(memory, dtype):
     assert _norm([(memory + 1, 0, dtype)], norm, memory + 1024) == -3 and _clip([(memory + 1, 0, dtype)] * 2, [(memory + 1, 0, dtype)] * 2, norm) == -3
     for off in (1, 2, 3):
         assert _norm([(memory, 10, dtype)], norm + off, memory + 1024) == -1 and _clip([(memory, 10, dtype)], [(memory, 10, dtype)], norm + off) == -1
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor on the GPU by its looks, without memory of its own, as a sharded parameter's gradient is one."""
+
+    @staticmethod
+    def __new__(cls, shape):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=torch.float32, device="cuda:0")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+def test_a_tensor_without_memory_is_no_overlap(memory, monkeypatch):
+    from contextlib import nullcontext
+
+    from primus_amd.pytorch import kernels as K
+
+    monkeypatch.setattr(K, "_on", lambda device: nullcontext())
+    monkeypatch.setattr(K, "_stream", lambda: None)
+    w, norm = [_Wrapped((3, 5))], _Wrapped(())
+    with pytest.raises(ValueError, match="memory of their own"):
+        K.clip_grads_impl(w, w, 1.0, norm)
+    for sizes, ptrs, why in (([0, 4], [0, 16], None), ([1 << 36], [16], "2\\^36"), ([3, 1], [16, 0], "memory of their own")):
+        if why is None:
+            K._why_refused(ptrs, sizes, "gradients")
+            continue
+        with pytest.raises(ValueError, match=why):
+            K._why_refused(ptrs, sizes, "gradients")
+
+
+_NO_MEMORY = """
+import ctypes, resource, sys
+sys.path.insert(0, {root!r})
+from primus_amd import _lib
+lib = _lib.load()
+n = 1 << 22
+ptr, size, kind = (ctypes.c_uint64 * n)(), (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
+norm = ctypes.c_float(1.0)
+call = lambda: lib.mxl_clip_grads(ptr, ptr, size, kind, kind, n, 1.0, ctypes.byref(norm), None)
+with open("/proc/self/statm") as f:
+    now = int(f.read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (now + (32 << 20), resource.RLIM_INFINITY))      # (the spans take 24 bytes a tensor and direction: 201 MB)
+first = call()
+resource.setrlimit(resource.RLIMIT_AS, (resource.RLIM_INFINITY, resource.RLIM_INFINITY))
+print(first, call(), lib.mxl_error_string(first).decode())
+"""
+
+
+def test_no_host_memory_is_no_overlap(memory):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", _NO_MEMORY.format(root=root)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stderr[-2000:]
+    assert out.stdout.split()[:2] == ["-6", "-3"] and "memory" in out.stdout
