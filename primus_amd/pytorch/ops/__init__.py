@@ -939,11 +939,25 @@ def _grad_list(tensors, what: str):
         raise
 
 
+def _not_recorded(what: str, *lists) -> None:
+    """For operators that autograd does not know of: refuses tensors with a tangent, which would be dropped, and ``torch.jit.trace``, which would record the
+    allocations and none of the launches."""
+    if torch._C._get_tracing_state() is not None:
+        raise NotImplementedError(f"{what} cannot be traced")
+    if torch.autograd.forward_ad._current_level >= 0:
+        for tensors in lists:
+            for t in [tensors] if isinstance(tensors, torch.Tensor) else tensors or ():
+                if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                    raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of ``grads`` (tensors on one GPU, of any shapes and sizes, bfloat16, float16 and float32 mixed) as a float32 scalar on
     the device: ``sqrt(sum g^2)``, or ``max |g|`` for ``norm_type`` inf (NaN if there is one).  Squares are summed in fp64 in an order that
-    depends on the sizes alone; they neither overflow nor underflow.  Nothing is read back to the host.  0 for no tensors or no elements."""
-    _, dense = _grad_list(grads, "gradients")
+    depends on the sizes alone; they neither overflow nor underflow.  Nothing is read back to the host.  0 for no tensors or no elements.  Not differentiable:
+    the norm is a new tensor without a graph, as under ``torch.no_grad``; tensors with a forward-mode tangent and ``torch.jit.trace`` are refused."""
+    listed, dense = _grad_list(grads, "gradients")
+    _not_recorded("grad_norm", listed)
     if not dense:
         if float(norm_type) not in K._NORM_KINDS:
             raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
@@ -1004,7 +1018,8 @@ def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = 
     say), a float32 scalar on the gradients' device, or a number.  In place, or into the tensors of ``out`` (one of the same shape for every gradient, of any of
     the three types: the optimizer's float32 gradients of bfloat16 ones).  The factor is taken on the device and nothing is read back: within the bound, gradients
     in place are left untouched.  A norm of NaN makes every element NaN, an infinite one leaves zeros of what is finite.  No tensor that is written may
-    overlap itself, another one or ``norm``; slices of one tensor that lie between each other's rows or columns do not."""
+    overlap itself, another one or ``norm``; slices of one tensor that lie between each other's rows or columns do not.
+    Not differentiable: it works as under ``torch.no_grad``, and refuses what ``grad_norm`` refuses."""
     targets, dense = _grad_list(grads, "gradients")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -1015,6 +1030,7 @@ def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = 
         targets, written = _grad_list(out, "out")
         if len(targets) != len(grads) or any(o.shape != g.shape for o, g in zip(targets, grads)):
             raise ValueError("out must hold a tensor of the same shape for every gradient")
+    _not_recorded("clip_grads", targets, grads if out is not None else (), norm if isinstance(norm, torch.Tensor) else ())
     if written is not targets or (out is not None and dense is not grads):
         _refuse_overlaps(targets, targets if out is None else grads, norm)
     if norm is None:
