@@ -17,12 +17,13 @@ from ...pytorch import ops
 def get_grad_norm_fp32(grads_for_norm: Union[List[torch.Tensor], torch.Tensor], norm_type: Union[int, float] = 2,
                        grad_stats_parallel_group: Optional["torch.distributed.ProcessGroup"] = None) -> torch.Tensor:
     """Norm of the gradients of all ranks of ``grad_stats_parallel_group`` (None: of this one), 2 or inf: a float32 scalar on the device, which
-    formats and compares like the number it stands for.  Between the ranks squares are added in float64."""
+    formats and compares like the number it stands for.  Between the ranks squares are added in float64; the largest magnitude is NaN if any rank's is."""
     norm = ops.grad_norm(grads_for_norm, float(norm_type))
     if grad_stats_parallel_group is None:
         return norm
     if float(norm_type) == math.inf:
-        torch.distributed.all_reduce(norm, op=torch.distributed.ReduceOp.MAX, group=grad_stats_parallel_group)
+        # (of numbers that are not negative the bits are ordered as they are, and a NaN's are above all; a maximum of floats may lose it)
+        torch.distributed.all_reduce(norm.view(torch.int32), op=torch.distributed.ReduceOp.MAX, group=grad_stats_parallel_group)
         return norm
     total = norm.double().square()
     torch.distributed.all_reduce(total, op=torch.distributed.ReduceOp.SUM, group=grad_stats_parallel_group)
