@@ -1,4 +1,4 @@
-"""The largest magnitude over ranks: a NaN of one rank, whatever its place.  Two processes over gloo."""
+"""The norm over ranks: a NaN of one rank, whatever its place, and which ranks a group of None means.  Two processes over gloo."""
 
 import math
 import os
@@ -20,13 +20,15 @@ def _rank(rank, world, port, out):
     for values in CASES:
         grads = [torch.tensor([values[rank]])]
         top = clip_grads.get_grad_norm_fp32(grads, math.inf, group)
-        out.put((rank, top.item(), top.dtype == torch.float32 and top.dim() == 0))
+        out.put((rank, top.item(), clip_grads.get_grad_norm_fp32(grads, 2, group).item(), clip_grads.get_grad_norm_fp32(grads, math.inf, grad_stats_parallel_group=None).item(),
+                 clip_grads.get_grad_norm_fp32(grads, grad_stats_parallel_group=None).item(), clip_grads.get_grad_norm_fp32(grads).item(),
+                 top.dtype == torch.float32 and top.dim() == 0))
     torch.distributed.destroy_process_group()
 
 
 @pytest.fixture(scope="module")
 def norms():
-    """``{rank: [(largest magnitude, whether it is a float32 scalar), ...]}``"""
+    """``{rank: [(largest, 2-norm, and both for a group of None, of the rank alone), ...]}``"""
     ctx = torch.multiprocessing.get_context("spawn")
     out = ctx.SimpleQueue()
     port = 29950 + os.getpid() % 300
@@ -43,10 +45,34 @@ def norms():
     return got
 
 
+def _same(a, b):
+    return math.isnan(a) and math.isnan(b) or a == b or abs(a - b) <= 2 * 2.0 ** -24 * abs(b)
+
+
 @pytest.mark.parametrize("at", range(len(CASES)))
 def test_largest_magnitude(norms, at):
     """NaN where any rank has one."""
     want = math.nan if any(map(math.isnan, CASES[at])) else torch.tensor(max(CASES[at])).item()
     for rank in (0, 1):
-        top, scalar = norms[rank][at]
+        top, *_, scalar = norms[rank][at]
         assert scalar and (top == want or math.isnan(top) and math.isnan(want)), (rank, top)
+
+
+def _of_all(values):
+    return math.nan if any(map(math.isnan, values)) else torch.tensor(math.hypot(*torch.tensor(values).tolist())).item()
+
+
+@pytest.mark.parametrize("at", range(len(CASES)))
+def test_which_ranks(norms, at):
+    """A group, None for all ranks, and the rank alone where none is named."""
+    for rank in (0, 1):
+        top, two, every_top, every_two, alone, _ = norms[rank][at]
+        assert _same(two, _of_all(CASES[at])) and _same(every_two, two) and _same(every_top, top)
+        assert _same(alone, torch.tensor(CASES[at][rank]).item())
+
+
+def test_without_ranks(monkeypatch):
+    assert not torch.distributed.is_initialized()
+    monkeypatch.setattr(ops, "grad_norm", lambda grads, kind=2.0: grads[0].abs().max())
+    for kind in (2, math.inf):
+        assert clip_grads.get_grad_norm_fp32([torch.tensor([-3.0])], kind, None).item() == 3.0
