@@ -660,8 +660,11 @@ int mxl_linear_bf16_bwd(const void* dy_bf16, const void* a_bf16, const void* b_b
  *
  * mxl_block_norm_bwd: gradients given those of y (dy; not looked at without weight) and of h (dh, stream_dtype; NULL: zero).  Any output may be
  * NULL: not wanted.  dresidual is of stream_dtype; without weight it is dh itself and must be NULL.  Without post_weight and gate and
- * with a scale of 1, dx has the values of dresidual.  x is looked at with post_weight or dgate, h with weight.
+ * with a scale of 1, dx has the values of dresidual.  x is looked at with post_weight or dgate, h with weight.  stream_dtype | MXL_NORM_SUMMED (with
+ * weight, a stream of 16 bits): h is the residual that the forward was given, and x is looked at; h is summed again as the forward had it, where
+ * otherwise dweight has the rounding of h.  Without rows dgate is not written.
  * mxl_block_norm_bwd_workspace_bytes: has_weight, has_post_weight: whether dweight, dpost_weight are wanted; gate_cols 0: no gate. */
+#define MXL_NORM_SUMMED 0x100
 int mxl_block_norm(const void* x, const void* residual, int64_t rows, int64_t k, int dtype, int stream_dtype, const void* post_weight,
                    float post_eps, const void* gate, int64_t gate_div, int64_t gate_mod, int64_t gate_cols, float scale, const void* weight,
                    float eps, void* y, void* h, float* post_rstd, float* rstd, void* stream);

@@ -37,6 +37,7 @@ GF_B_TRANSPOSED = 8                         # forward / dgrad: b's codes are tho
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2           # element types of logits, rows and probabilities around the expert MLP
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 NORM_L2, NORM_MAX = 0, 1
+NORM_SUMMED = 0x100                         # flag of the block norm's backward, on the stream's type: h is the residual
 BF_B_KN, BF_ACCUM_F32, BF_TILE_128, BF_TILE_256 = 1, 2, 4, 8    # flags of the bf16 grouped GEMMs
 
 EXPORTS = (

@@ -7,16 +7,20 @@
 //   dx = rp * (f * t * post_weight - xh * mean(f * n * t))            dpost_weight = sum_rows f * t * xh        (dx = f * t without)
 //
 // mean(f n t) needs t and t needs mean(g hh), but sum q t = sum q dh + r * (sum q g - mean(g hh) * sum q hh): all four sums of a
-// row go through one reduction.  hh is made from h as it was stored.
+// row go through one reduction.
+//
+// hh is made from h as it was stored where that is in fp32, and where dweight is not wanted.  Otherwise h is summed again from x and the residual: the
+// rounding of h to 16 bits in every hh is as large as dweight's own, [16384, 4096] bf16 2.4e-3 of its norm off, 1.8e-3 so.  Nothing more is read with
+// post_weight or a gate's gradient, x is read for those anyway; without them a tensor more, us from h and so: [16384, 4096] 90 and 113, [8192, 7168] 78 and 99.
 //
 // Workers (workgroups, or runs of lanes where rows are short) each own rows of one gate after the other, so that the gate's gradient
 // is a sum in registers like the weights'.  Sums that several workers share go through float rows in the workspace, which a second
 // kernel adds up in their order: no atomics.
 //
 // Bound by memory, and near to it by instructions: a row's floats are made once and stay in registers over the reduction, and what a whole row
-// multiplies is applied to the sums.  us (TB/s) from memory: add and norm [16384, 4096] 91 (5.9); norm and add with a gate a channel [8192, 7168]
+// multiplies is applied to the sums.  us (TB/s) from memory: add and norm [16384, 4096] 113 (5.9); norm and add with a gate a channel [8192, 7168]
 // 63 (5.6); both norms, a gate a sequence, the stream in fp32 [5403, 2880] 57 (4.9).  A row ahead pays where a CU holds one workgroup (over 512
-// threads: [8192, 7168] 93 -> 78 us), and costs where it holds more ([16384, 4096] 90 -> 96): others' loads are on their way then anyway.
+// threads: [8192, 7168] from h 93 -> 78 us), and costs where it holds more ([16384, 4096] 90 -> 96): others' loads are on their way then anyway.
 #pragma once
 #include "mx_block_norm.h"
 
@@ -32,6 +36,7 @@ struct BlockNormBwdArgs {
     // rows of group g: (i / gdiv) * groups * gdiv + g * gdiv + i % gdiv, i < each; worker w has i = w % share, + share, ... of group
     // w / share, then of the groups gstep further on
     int64_t groups, each, share, gstep, gdiv, active;
+    bool summed;        // h is the residual: with x it makes h as the forward had it (16-bit streams)
     void *dx, *dres, *dgate;
     float *part_w, *part_p, *part_g;
 };
@@ -47,6 +52,7 @@ constexpr bool bn_bwd_keeps(int chunks, bool pre, bool post, bool gate) { return
 template <int T, int S, int CH, bool PRE, bool POST, bool SAME, bool GATEV, bool SMALL, bool ANY, int BOUND, bool AHEAD>
 __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs p) {
     constexpr int NS = PRE && POST ? 4 : 1;
+    constexpr bool SUM = PRE && S != MXL_DT_F32;        // h may have to be summed again
     __shared__ float part[2][BN_MAX_WAVES][NS];
     const int lanes = SMALL ? p.lanes : (int)blockDim.x;
     const int lane = SMALL ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x;
@@ -92,7 +98,8 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
         }
     }
     const bool gate_wanted = p.dgate != nullptr;
-    const void* x_in = POST || gate_wanted ? p.x : nullptr;
+    const bool summed = SUM && p.summed;
+    const void* x_in = POST || gate_wanted || summed ? p.x : nullptr;
 
     // a row as it lies in memory
     Raw8<T> xn[CH], dyn[CH];
@@ -103,7 +110,7 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
         const RowsS in_h(p.h, p.rows, row, k), in_dh(p.dh, p.rows, row, k);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-            if (!SAME) xn[j] = in_x.template load<BN_NT>(cols, j);
+            if (!SAME || SUM) xn[j] = in_x.template load<BN_NT>(cols, j);
             dhn[j] = in_dh.template load<BN_NT>(cols, j);
             if (PRE) {
                 dyn[j] = in_dy.template load<BN_NT>(cols, j);
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
             unpack8<S>(dhn[j], t[j]);
-            if (!SAME) unpack8<T>(xn[j], x[j]);
+            if (!SAME || SUM) unpack8<T>(xn[j], x[j]);
             if (PRE) {
                 unpack8<T>(dyn[j], dy[j]);
                 unpack8<S>(hn[j], hh[j]);
@@ -186,7 +193,7 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
 #pragma unroll
             for (int e = 0; e < BN_VEC; ++e) {
                 if (POST) x[j][e] *= rp;
-                if (PRE) hh[j][e] *= r;
+                if (PRE && !SUM) hh[j][e] *= r;
             }
         }
         const int64_t row = at.row;
@@ -209,6 +216,7 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
             request(ahead.row);
             advance(ahead);
         }
+        const float whole = GATEV ? 1.f : factor;       // of f: what wq does not have
         // The row's sums.  (Columns past the row hold zeros in all that is read, a gate's vector too.  A factor of the whole row, which may
         // be infinite, is applied behind the sums; r and rp are infinite for a row of zeros without eps alone, whose gradients are NaN.)
         float v[NS];
@@ -222,6 +230,10 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
                 float q = 0.f;
                 if (POST) {
                     q = x[j][e] * (GATEV ? wq[j][e] : wp[j][e]);
+                }
+                if (SUM) {
+                    const float n = POST ? q : GATEV ? x[j][e] * wq[j][e] : x[j][e];
+                    hh[j][e] = (summed ? hh[j][e] + n * whole : hh[j][e]) * r;
                 }
                 if (PRE) {
                     const float d = dy[j][e] * w[j][e];
@@ -241,7 +253,6 @@ __global__ __launch_bounds__(BOUND) void block_norm_bwd_kernel(BlockNormBwdArgs 
         const float c1 = PRE ? v[0] * inv_k : 0.f;
         float qt = 0.f;
         if (POST) qt = PRE ? v[NS - 3] + r * (v[NS - 2] - c1 * v[NS - 1]) : v[0];
-        const float whole = GATEV ? 1.f : factor;       // of f: what wq does not have
         const float rc1 = r * c1, rw = rp * whole, rc2 = rw * (qt * inv_k);
         float nt = 0.f;
         const RowsT out_x(p.dx, p.rows, row, k);

@@ -103,7 +103,10 @@ extern "C" int mxl_block_norm_bwd(const void* dy, const void* dh, const void* x,
                                   const void* post_weight, const float* post_rstd, const void* gate, int64_t gate_div, int64_t gate_mod,
                                   int64_t gate_cols, float scale, const void* weight, const float* rstd, void* dx, void* dresidual, void* dweight,
                                   void* dpost_weight, void* dgate, void* workspace, int64_t workspace_bytes, void* stream) {
+    const bool summed = (stream_dtype & MXL_NORM_SUMMED) != 0;
+    stream_dtype &= ~MXL_NORM_SUMMED;
     if (!bn_shape_ok(rows, k, dtype, stream_dtype) || (!weight && !post_weight) || (dgate && !gate) || (dresidual && !weight)) return MXL_EINVAL;
+    if (summed && (!weight || stream_dtype == MXL_DT_F32)) return MXL_EINVAL;
     if (!bn_gate_ok(rows, k, gate, gate_div, gate_mod, gate_cols)) return MXL_EINVAL;
     if ((dweight && !weight) || (dpost_weight && !post_weight)) return MXL_EINVAL;
     if (rows == 0) {
@@ -114,7 +117,7 @@ extern "C" int mxl_block_norm_bwd(const void* dy, const void* dh, const void* x,
     BlockNormPlan q;
     const int64_t need = mxl_block_norm_bwd_workspace_bytes(rows, k, dweight != nullptr, dpost_weight != nullptr, gate_div, gate_mod, gate ? gate_cols : 0, dgate != nullptr);
     if (rows > 0) {
-        if ((weight && (!dy || !h || !rstd)) || (post_weight && (!x || !post_rstd)) || (dgate && !x)) return MXL_EINVAL;
+        if ((weight && (!dy || !h || !rstd)) || (post_weight && (!x || !post_rstd)) || ((dgate || summed) && !x)) return MXL_EINVAL;
         if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)) return MXL_EINVAL;
         if (!device_is_gfx950()) return MXL_ENODEV;
         q = block_norm_plan(rows, k, dgate || (gate && gate_cols == k), gate_div, gate_mod);
@@ -131,7 +134,7 @@ extern "C" int mxl_block_norm_bwd(const void* dy, const void* dh, const void* x,
     if (gate_joined) part_g = ws;
     if (rows > 0) {
         BlockNormBwdArgs p = {dy, dh, x, h, post_weight, weight, post_rstd, rstd, bn_gate(gate, rows, gate_div, gate_mod, gate_cols, k), scale, (int)k, q.ldk,
-                              q.lanes, rows, q.groups, q.each, q.share, q.gstep, q.gdiv, q.active, dx, dresidual, dgate, part_w, part_p, part_g};
+                              q.lanes, rows, q.groups, q.each, q.share, q.gstep, q.gdiv, q.active, summed, dx, dresidual, dgate, part_w, part_p, part_g};
         int rc;
         if (dtype == MXL_DT_F32) rc = block_norm_bwd_launch<MXL_DT_F32, MXL_DT_F32>(p, q, st);
         else if (dtype == MXL_DT_BF16 && stream_dtype == MXL_DT_BF16) rc = block_norm_bwd_launch<MXL_DT_BF16, MXL_DT_BF16>(p, q, st);

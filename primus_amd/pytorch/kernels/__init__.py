@@ -1553,16 +1553,17 @@ def block_norm_impl(x, residual, weight, eps: float, post_weight, post_eps: floa
 
 
 def block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate, scale: float, need_x: bool = True, need_residual: bool = True,
-                        need_weight: bool = True, need_post_weight: bool = True, need_gate: bool = True):
+                        need_weight: bool = True, need_post_weight: bool = True, need_gate: bool = True, summed: bool = False):
     """``(dx, dresidual, dweight, dpost_weight, dgate)`` of ``block_norm_impl``, given the gradients of ``y`` and ``h`` (None: zero).  ``x`` may be None where
     it is not needed: without ``post_weight``, and with no gradient of the gate.  Without ``weight`` the residual's gradient is ``dh``, and None here.
+    ``summed``: ``h`` is the residual of the forward, in 16 bits, and ``x`` is there: they are summed again, and ``dweight`` has no rounding of ``h``.
     (What the forward has checked is looked at again only as far as saved tensors may come back changed: this runs on autograd's thread, where a
     line of Python costs twice what it does on the caller's.)"""
     pre, post = weight is not None, post_weight is not None
     like = x if x is not None else dy
     stream = h if pre else dh
     need_gate = need_gate and gate is not None
-    if like is None or stream is None or (pre and (dy is None or rstd is None)) or (post and (x is None or post_rstd is None)) or (need_gate and x is None) or not (pre or post):
+    if like is None or stream is None or (pre and (dy is None or rstd is None)) or (post and (x is None or post_rstd is None)) or ((need_gate or summed) and x is None) or not (pre or post):
         raise ValueError("the gradient needs what the forward kept")
     shape, want, stream_want, index = like.shape, like.dtype, stream.dtype, like.get_device()
     k = shape[-1]
@@ -1595,7 +1596,7 @@ def block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate
         ws, nbytes = _workspace(dev, "mxl_block_norm_bwd_workspace_bytes", rows, k, need_weight, need_post_weight, div, mod, cols, need_gate)
         rc = _lib.load().mxl_block_norm_bwd(
             None if dy is None else dy.data_ptr(), None if dh is None else dh.data_ptr(), None if x is None else x.data_ptr(), None if h is None else h.data_ptr(),
-            rows, k, _DT[want], _DT[stream_want], post_weight.data_ptr() if post else None, post_rstd.data_ptr() if post else None,
+            rows, k, _DT[want], _DT[stream_want] | (_lib.NORM_SUMMED if summed else 0), post_weight.data_ptr() if post else None, post_rstd.data_ptr() if post else None,
             None if gate is None else gate.data_ptr(), div, mod, cols, scale, weight.data_ptr() if pre else None, rstd.data_ptr() if pre else None,
             None if dx is None else dx.data_ptr(), None if dres is None else dres.data_ptr(), dw.data_ptr() if need_weight else None,
             dpw.data_ptr() if need_post_weight else None, dgate.data_ptr() if need_gate else None, None if ws is None else ws.data_ptr(), nbytes, _stream())

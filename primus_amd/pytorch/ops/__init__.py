@@ -868,7 +868,8 @@ class _BlockNorm(torch.autograd.Function):
         y, h, rstd, post_rstd = K.block_norm_impl(x, residual, weight, eps, post_weight, post_eps, gate, scale, need_grad)
         if need_grad:
             keep_x = post_weight is not None or (gate is not None and ctx.needs_input_grad[4])
-            ctx.save_for_backward(x if keep_x else None, h if weight is not None else None, weight, rstd, post_weight, post_rstd, gate)
+            ctx.summed = weight is not None and h.dtype is not torch.float32 and ctx.needs_input_grad[2]
+            ctx.save_for_backward(x if keep_x or ctx.summed else None, None if weight is None else residual if ctx.summed else h, weight, rstd, post_weight, post_rstd, gate)
             ctx.scale, ctx.dtypes = scale, (x.dtype, h.dtype)
             ctx.set_materialize_grads(False)
         return h if weight is None else (y, h)
@@ -889,7 +890,7 @@ class _BlockNorm(torch.autograd.Function):
         if weight is None and not (need_x or need_post or need_gate):
             return None, dh, None, None, None, None, None, None, None
         dx, dres, dw, dpw, dgate = K.block_norm_bwd_impl(dy, dh, x, h, weight, rstd, post_weight, post_rstd, gate, ctx.scale, need_x, need_residual, need_weight,
-                                                         need_post, need_gate)
+                                                         need_post, need_gate, ctx.summed)
         return dx, dres if weight is not None else dh if need_residual else None, dw, dpw, dgate, None, None, None, None
 
 
@@ -905,8 +906,9 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, e
     the weights ``[hidden]`` and ``gate`` are of one type, bfloat16, float16 or float32; ``residual`` has it too or is float32 (a residual stream kept
     in fp32), and ``h`` is of its type.  ``gate`` broadcasts to ``x``: a factor a channel ``[hidden]``, a sequence ``[batch, 1, hidden]`` (with ``[batch, seq,
     hidden]``) or ``[1, batch, hidden]`` (with ``[seq, batch, hidden]``), a token ``[..., 1]``, or an element; other patterns raise.
-    ``post_eps`` None: ``eps``.  Differentiable in the five tensors; sums over rows are taken in fp32 in a fixed order, and the
-    backward normalises ``h`` as it was rounded."""
+    ``post_eps`` None: ``eps``.  Differentiable in the five tensors; sums over rows are taken in fp32 in a fixed order.  For the
+    gradient of ``weight`` with a 16-bit ``residual``, ``x`` and ``residual`` are kept, from which ``h`` is summed again; otherwise ``h`` is kept, and ``x`` only
+    with ``post_weight`` or for the gradient of ``gate``."""
     return _block_norm(x, residual, weight, post_weight, gate, eps, eps if post_eps is None else post_eps, scale)
 
 

@@ -615,3 +615,29 @@ def test_weight_gradients_beyond_32_bit_offsets(gpu, released, k, rows):
     h = ops.rmsnorm_add(x, r, w, 1e-6)
     (dw,) = torch.autograd.grad(h, w, dy)
     _whole(dw, want, ("post_weight", k))
+
+
+@pytest.mark.parametrize("k", [40, 333, 1024, 9000])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_weight_gradient_of_the_sums_before_their_rounding(gpu, dtype, k):
+    """With a stream of 16 bits dweight = sum dy * hh has hh of the sums that y was made of, not of h as it was rounded.  hh is off by the fp32 work on what
+    is added up in h, 64 e of its magnitudes; then the bars of the sum and of its one rounding."""
+    from primus_amd.pytorch import ops
+
+    for lead, post, gate, scale in (((3, 67), False, "", 1.0), ((201,), False, "", -0.75), ((3, 67), True, "", 0.5), ((3, 67), True, "first", 1.0), ((67, 3), False, "last", 1.0),
+                                    ((201,), True, "token", 1.0), ((3, 67), False, "full", 1.25), ((201,), False, "element", 1.0)):
+        v, dy, _ = _inputs(lead, k, dtype, dtype, post, gate)
+        d = {n: None if t is None else t.double() for n, t in v.items()}
+        x = d["x"] if not post else d["x"] / torch.sqrt((d["x"] ** 2).mean(-1, keepdim=True) + POST_EPS) * d["post_weight"]
+        add = scale * x * (1 if d["gate"] is None else d["gate"])
+        h = d["residual"] + add
+        r = 1 / torch.sqrt((h * h).mean(-1, keepdim=True) + EPS)
+        rows = math.prod(lead)
+        total = lambda t: t.reshape(rows, k).sum(0)  # noqa: E731
+        want = total(dy.double() * h * r)
+        bar = _u(dtype) * want.abs() + total(dy.double().abs() * (64 * E * (d["residual"].abs() + add.abs()) * r + (64 + rows) * E * (h * r).abs()))
+        a = {n: None if t is None else t.to(gpu).requires_grad_() for n, t in v.items()}
+        for wanted in ([n for n in a if a[n] is not None], ["weight"]):
+            y, _ = ops.add_rmsnorm(a["x"], a["residual"], a["weight"], EPS, post_weight=a["post_weight"], post_eps=POST_EPS, gate=a["gate"], scale=scale)
+            got = torch.autograd.grad(y, [a[n] for n in wanted], dy.to(gpu))[wanted.index("weight")]
+            _close(got, (want, bar), ("weight", dtype))

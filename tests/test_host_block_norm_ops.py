@@ -154,3 +154,21 @@ def test_c_entries_refuse():
     for ins, outs in (([(p, 10, 0)] * 2, [(p, 10, 0)] * 2), ([(p, 10, 0), (p + 36, 10, 0)],) * 2, ([(p, 10, 0)], [(p + 4, 10, 0)]), ([(p, 10, 1)], [(p, 10, 0)]),
                       (spans, [(p + 4096, 10, 0), (p + 4100, 7, 0)]), (spans, [(p + 4096, 10, 0), (p + 36, 7, 0)])):
         assert clip(ins, outs) == -1, (ins, outs)
+
+
+def test_c_entry_refuses_to_sum_what_it_has_not():
+    """A backward that sums h again: with a weight, x and a stream of 16 bits."""
+    if torch.cuda.device_count() > 0:
+        pytest.skip("a GPU is present: these calls would be real launches")
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = ctypes.addressof(buf) // 16 * 16 + 16
+    need = lib.mxl_block_norm_bwd_workspace_bytes(4, 8, 1, 1, 1, 1, 0, 0)
+
+    def call(x=p, dtype=1, stream=1, weight=p, post=None):
+        pre = None if weight is None else p
+        return lib.mxl_block_norm_bwd(pre, p, x, pre, 4, 8, dtype, stream | _lib.NORM_SUMMED, post, post, None, 1, 1, 0, 1.0, weight, pre, p, pre, pre, post, None, p, need, None)
+
+    assert call() == -3 and call(dtype=2, stream=2) == -3 and call(post=p) == -3
+    for bad in (dict(x=None), dict(stream=0), dict(dtype=0, stream=0), dict(weight=None, post=p), dict(stream=1 | 0x200), dict(stream=2)):
+        assert call(**bad) == -1, bad
