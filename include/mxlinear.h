@@ -678,7 +678,7 @@ int mxl_block_norm_bwd(const void* dy, const void* dh, const void* x, const void
 /* ---- the global norm of many gradients, and clipping ----
  * grads, sizes (elements), dtypes (MXL_DT_*): host arrays of `count` tensors, each a run of elements without gaps; its address is a multiple of the element's size.
  * mxl_grad_norm: *norm (device) = sqrt of the sum of all squares (MXL_NORM_L2) or the largest magnitude (MXL_NORM_MAX; NaN if there is one);
- * fp64 sums in an order that the sizes decide; 0 for no elements.
+ * fp64 sums in an order that the sizes, the types and the addresses modulo 16 decide; 0 for no elements.
  * mxl_clip_grads: out = grad * min(1, max_norm / (*norm + 1e-6)), NaN for a norm of NaN; outs[i] may be grads[i] (same type): with a factor of 1 those
  * are left untouched.  No byte that is written may belong to another tensor of the lists or to *norm. */
 #define MXL_NORM_L2 0

@@ -44,7 +44,8 @@ struct BlockNormBwdArgs {
 // Whether a lane has the weights and their sums in registers.  Two chunks of both norms, or of a norm and a gate of vectors, do not fit: the
 // weights are loaded again for every row (from the caches) and their sums are in shared memory, 64 bytes a lane each.  us, in registers (spilt)
 // and so, [2730, 12288]: both norms 158 and 109, and a stream in fp32 and a gate 263 and 199, a norm and a gate a row 122 and 111; a norm without
-// one 62 and 69.
+// one 62 and 69.  Two chunks use scratch all the same, by the compiler's report, bytes a lane: both norms and a gate of vectors 100 to 264, both norms without one
+// up to 84, one norm up to 88.
 constexpr bool bn_bwd_keeps(int chunks, bool pre, bool post, bool gate) { return chunks == 1 || !pre || !(post || gate); }
 
 // SAME: no gradient of x apart from the residual's.  GATEV: the gate is a vector, and groups are its rows.  AHEAD: the next row is asked for

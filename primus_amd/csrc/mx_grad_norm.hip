@@ -6,7 +6,8 @@
 // captured launch keeps its own table.  A launch's tensors are cut into chunks, which its workgroups take in turn.
 //
 // Squares and sums are fp64: a float's square is exact there and neither overflows nor underflows, whatever the gradients' scale.
-// Every workgroup leaves one sum, one workgroup adds them up in their order: the result depends on the sizes alone, and no atomics.
+// Every workgroup leaves one sum, one workgroup adds them up in their order, and no atomics: which sums an element goes through depends on the sizes, the types and
+// the addresses modulo 16 (a chunk's elements in front of its first whole sixteen bytes go by themselves), on nothing else.
 //
 // Bound by memory.  1.4e9 floats 813 us (6.9 TB/s), 2.2e8 bf16 elements 66 us (6.6); clipping those into floats 220 us (6.0 TB/s).  The fp64 work hides
 // behind the loads.  (With loads behind branches, one after the other: 3520, 100 and, the output's sixteen bytes every 32, 312.)
@@ -171,8 +172,8 @@ struct ClipTable {
 };
 static_assert(sizeof(ClipTable) <= 4032, "kernel arguments");
 constexpr int GC_PER = GN_THREADS * 32;     // elements of a chunk
-// Workgroups of a launch.  As many as there are chunks is fastest where something is written (1.4e9 floats in place 2068 us; 32768 workgroups 2124,
-// 2048 2192), but all of them have to come and go where the norm is within the bound (79, 36 and 31 us), the common case.
+// Workgroups of a launch.  As many as there are chunks is fastest where something is written (1.4e9 floats in place, launch after launch, 2057 us; 32768
+// workgroups 2101, 2048 2152), but all of them have to come and go where the norm is within the bound (39, 9 and 5 us), the common case.
 constexpr uint32_t GC_BLOCKS = 32768;
 
 // The product is made in fp64 and rounded to fp32 (of a 16-bit type it is exact till then but for the factor's 53 bits), and once more to a 16-bit output.

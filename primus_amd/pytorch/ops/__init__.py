@@ -956,7 +956,7 @@ def _not_recorded(what: str, *lists) -> None:
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of ``grads`` (tensors on one GPU, of any shapes and sizes, bfloat16, float16 and float32 mixed) as a float32 scalar on
     the device: ``sqrt(sum g^2)``, or ``max |g|`` for ``norm_type`` inf (NaN if there is one).  Squares are summed in fp64 in an order that
-    depends on the sizes alone; they neither overflow nor underflow.  Nothing is read back to the host.  0 for no tensors or no elements.  Not differentiable:
+    depends on sizes, types and addresses modulo 16; they neither overflow nor underflow.  Nothing is read back to the host.  0 for no tensors or no elements.  Not differentiable:
     the norm is a new tensor without a graph, as under ``torch.no_grad``; tensors with a forward-mode tangent and ``torch.jit.trace`` are refused."""
     listed, dense = _grad_list(grads, "gradients")
     _not_recorded("grad_norm", listed)
@@ -1019,7 +1019,7 @@ def clip_grads(grads, max_norm: float, norm: Union[torch.Tensor, float, None] = 
     """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``: ``grad_norm(grads, norm_type)`` unless it is given (the norm over all ranks,
     say), a float32 scalar on the gradients' device, or a number.  In place, or into the tensors of ``out`` (one of the same shape for every gradient, of any of
     the three types: the optimizer's float32 gradients of bfloat16 ones).  The factor is taken on the device and nothing is read back: within the bound, gradients
-    in place are left untouched.  A norm of NaN makes every element NaN, an infinite one leaves zeros of what is finite.  No tensor that is written may
+    in place are left untouched.  A norm of NaN makes every element NaN, an infinite one leaves zeros of what is finite (NaN with an infinite ``max_norm``).  No tensor that is written may
     overlap itself, another one or ``norm``; slices of one tensor that lie between each other's rows or columns do not.
     Not differentiable: it works as under ``torch.no_grad``, and refuses what ``grad_norm`` refuses."""
     targets, dense = _grad_list(grads, "gradients")
